@@ -15,6 +15,7 @@ LIB_PATH = pathlib.Path(__file__).resolve().parent / "libtttj_amd.so"
 
 TT_OK, TT_ERR_INVALID, TT_ERR_HIP = 0, 1, 2
 PLAN_AUTO, PLAN_LAYERWISE, PLAN_MEGAKERNEL, PLAN_FUSED_LN = 0, 1, 2, 3
+FP16, BF16 = 0, 1
 EPILOGUES = {"bias": 0, "gelu": 1, "resid_masked": 2, "masked_resid": 3, "qkv": 4}
 
 _P = ctypes.c_void_p
@@ -50,6 +51,10 @@ SIGNATURES = {
     "tt_attention_fwd": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "tt_attention_masked_fwd": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "tt_attention_fwd_prescaled": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "tt_packed_attention_fwd": (_I, [_P] * 5 + [_I] * 5 + [_I64] * 6 + [_F, _I, _I, _P]),
+    "tt_cache_append": (_I, [_P] * 7 + [_I] * 7 + [_I64] * 11 + [_P]),
+    "tt_cache_attention_workspace_bytes": (_I, [_I] * 7 + [ctypes.POINTER(_I64)]),
+    "tt_cache_attention_fwd": (_I, [_P] * 8 + [_I64] + [_I] * 9 + [_I64] * 9 + [_F, _I, _P]),
     "tt_transformer_fwd": (_I, [_P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "tt_noalloc_scratch_bytes": (_I, [ctypes.POINTER(_I64)]),
     "tt_transformer_fwd_noalloc": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
@@ -115,6 +120,15 @@ def workspace_bytes(batch: int, seq: int, d_model: int, heads: int, ffn_dim: int
     out = _I64()
     check(load().tt_workspace_bytes(batch, seq, d_model, heads, ffn_dim, num_layers, plan,
                                     ctypes.byref(out)), "tt_workspace_bytes")
+    return out.value
+
+
+def cache_attention_workspace_bytes(tokens: int, batch: int, heads: int, kv_heads: int,
+                                    head_dim: int, max_length: int, single: bool) -> int:
+    out = _I64()
+    check(load().tt_cache_attention_workspace_bytes(tokens, batch, heads, kv_heads, head_dim,
+                                                    max_length, int(single), ctypes.byref(out)),
+          "tt_cache_attention_workspace_bytes")
     return out.value
 
 

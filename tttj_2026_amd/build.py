@@ -41,6 +41,7 @@ SOURCE_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attention_small.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "rowchain.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "seq_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "megakernel.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

@@ -1,0 +1,275 @@
+// Launches of the attention of ragged token rows (seq_attention.hpp): whole prompts, and new tokens over a paged
+// cache; the merge of key ranges; the write of new keys and values into the cache.
+#include "seq_attention.hpp"
+#include "seq_launch.hpp"
+
+namespace tt {
+
+// out = sum_s w_s O_s / sum_s w_s l_s over the key ranges s of a row, w_s = 2^(m_s - max m).  One wave per
+// (token, head); rows whose keys lie in one range were written by their block.
+template <typename T>
+__global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t nrows = (int64_t)a.tokens * a.heads;
+  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= nrows) return;
+  const int token = (int)(row / a.heads);
+  int seq = token, i = 0, count = 1;
+  if (a.starts != nullptr) {
+    seq = seq_search(a.batch, token, [&](int b) { return seq_start(a.starts, b, a.tokens); });
+    const int first = seq_start(a.starts, seq, a.tokens);
+    i = token - first;
+    count = seq_start(a.starts, seq + 1, a.tokens) - first;
+    if (i < 0 || i >= count) return;  // a row of no sequence
+  }
+  const int lim = seq_limit(a, i, count, seq_keys<true>(a, seq, count));
+  if (lim <= a.chunk) return;
+  const int parts = min((lim + a.chunk - 1) / a.chunk, a.splits);
+  float m = -INFINITY;
+  for (int s = lane; s < parts; s += 64) m = fmaxf(m, a.part_ml[s * nrows + row].x);
+  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+  float l = 0.f;
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  const bool live = 4 * lane < a.head_dim;
+  for (int s = 0; s < parts; ++s) {
+    const float2 ml = a.part_ml[s * nrows + row];
+    const float w = ml.x == -INFINITY ? ml.y : __builtin_amdgcn_exp2f(ml.x - m);
+    l = fmaf(w, ml.y, l);
+    if (live) {
+      const floatx4 x = *reinterpret_cast<const floatx4*>(a.part_o + (s * nrows + row) * a.head_dim + 4 * lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[e], o[e]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  if (live)
+    *reinterpret_cast<v4*>(static_cast<T*>(a.out) + row * a.head_dim + 4 * lane) =
+        v4{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+}
+
+struct AppendArgs {
+  const uint16_t *k, *v;
+  uint16_t *k_cache, *v_cache;
+  const int32_t *starts, *lengths, *table;
+  int64_t k_row, k_head, v_row, v_head, kc_page, kc_row, kc_head, vc_page, vc_row, vc_head, table_row;
+  int tokens, batch, heads, chunks;  // per token: `heads` runs of `chunks` 16-byte pieces
+  int pages, table_pages, page_shift;
+};
+
+// One wave per token: its K and V rows go to their place in the cache.
+__global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int token = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (token >= a.tokens) return;
+  int seq = token, i = 0, count = 1;
+  if (a.starts != nullptr) {
+    seq = seq_search(a.batch, token, [&](int b) { return seq_start(a.starts, b, a.tokens); });
+    const int first = seq_start(a.starts, seq, a.tokens);
+    i = token - first;
+    count = seq_start(a.starts, seq + 1, a.tokens) - first;
+    if (i < 0 || i >= count) return;
+  }
+  const int64_t at = (int64_t)a.lengths[seq] - count + i;
+  if (at < 0 || (at >> a.page_shift) >= a.table_pages) return;
+  const int page = a.table[seq * a.table_row + (at >> a.page_shift)];
+  if ((uint32_t)page >= (uint32_t)a.pages) return;
+  const int in = (int)at & ((1 << a.page_shift) - 1);
+  const uint16_t* k = a.k + token * a.k_row;
+  const uint16_t* v = a.v + token * a.v_row;
+  uint16_t* kc = a.k_cache + page * a.kc_page + in * a.kc_row;
+  uint16_t* vc = a.v_cache + page * a.vc_page + in * a.vc_row;
+  for (int c = lane; c < a.heads * a.chunks; c += 64) {
+    const int h = a.heads == 1 ? 0 : c / a.chunks, e = (c - h * a.chunks) * 8;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(k + h * a.k_head + e);
+    const u32x4 y = *reinterpret_cast<const u32x4*>(v + h * a.v_head + e);
+    *reinterpret_cast<u32x4*>(kc + h * a.kc_head + e) = x;
+    *reinterpret_cast<u32x4*>(vc + h * a.vc_head + e) = y;
+  }
+}
+
+int launch_seq_attention(const SeqAttnArgs& a, bool paged, bool narrow, int dtype, hipStream_t stream) {
+  if (a.head_dim > 128) return launch_seq_attention_wide(a, paged, narrow, dtype, stream);
+  if (a.head_dim > 64) return launch_seq_hd<128>(a, paged, narrow, dtype, stream);
+  if (a.head_dim > 32) return launch_seq_hd<64>(a, paged, narrow, dtype, stream);
+  return launch_seq_hd<32>(a, paged, narrow, dtype, stream);
+}
+
+// How the keys of a call over the cache are split.
+struct SeqPlan {
+  bool narrow;  // 32 rows per block
+  int slots, splits, chunk;
+};
+
+SeqPlan seq_cache_plan(int64_t tokens, int batch, int heads, int kv_heads, int head_dim, int max_length, bool single) {
+  SeqPlan p;
+  const int64_t G = heads / kv_heads;
+  p.narrow = single ? G <= 32 : tokens * G <= 32 * (int64_t)batch;
+  const int R = p.narrow ? 32 : 128;
+  p.slots = (int)(single ? tokens * ((G + R - 1) / R) : tokens * G / R + batch);
+  const int64_t blocks = (int64_t)p.slots * kv_heads;
+  const int64_t want = 4L * device_cus();
+  const int step = 256;
+  int64_t splits = blocks >= want ? 1 : want / blocks;
+  int64_t chunk = (max_length + splits - 1) / splits;
+  chunk = (chunk + step - 1) / step * step;
+  p.splits = (int)((max_length + chunk - 1) / chunk);
+  p.chunk = (int)chunk;
+  if (p.splits <= 1) {
+    p.splits = 1;
+    p.chunk = INT32_MAX;
+  }
+  return p;
+}
+
+static int64_t part_floats(const SeqPlan& p, int64_t tokens, int heads, int head_dim) {
+  return p.splits == 1 ? 0 : p.splits * tokens * heads * (head_dim + 2);
+}
+
+static int check_heads(const char* what, int tokens, int batch, int heads, int kv_heads, int head_dim, int dtype) {
+  TT_REQUIRE(tokens >= 0 && batch >= 0, "%s: bad shape (tokens %d, batch %d)", what, tokens, batch);
+  TT_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: heads %d are no multiple of kv_heads %d", what,
+             heads, kv_heads);
+  TT_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "%s: head_dim %d is no multiple of 8 up to 256",
+             what, head_dim);
+  TT_REQUIRE((int64_t)tokens * heads < (1LL << 31), "%s: %d rows of %d heads", what, tokens, heads);
+  TT_REQUIRE(dtype == TT_FP16 || dtype == TT_BF16, "%s: bad dtype %d", what, dtype);
+  return TT_OK;
+}
+
+// Rows and heads are read 16 bytes at a time, and 16 rows at an offset of 32 bits.
+static int check_rows(const char* what, const void* p, int64_t row, int64_t head) {
+  TT_REQUIRE(((uintptr_t)p & 15) == 0 && row % 8 == 0 && head % 8 == 0, "%s: not aligned to 16 bytes", what);
+  TT_REQUIRE(row >= 0 && head >= 0 && row < (1LL << 26), "%s: row stride of %lld elements", what, (long long)row);
+  return TT_OK;
+}
+
+static int check_pages(const char* what, int pages, int page_size, int table_pages) {
+  TT_REQUIRE(pages > 0 && table_pages > 0, "%s: no pages (%d in the cache, %d per sequence)", what, pages, table_pages);
+  TT_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "%s: page_size %d is no power of two from 16 on",
+             what, page_size);
+  TT_REQUIRE((int64_t)page_size * table_pages <= (1LL << 30), "%s: %d pages of %d per sequence", what, table_pages,
+             page_size);
+  return TT_OK;
+}
+
+}  // namespace tt
+
+#define TT_CHECK(call)            \
+  do {                            \
+    const int rc_ = (call);       \
+    if (rc_ != TT_OK) return rc_; \
+  } while (0)
+
+extern "C" int tt_packed_attention_fwd(const void* q, const void* k, const void* v, const int32_t* starts, void* out,
+                                       int tokens, int batch, int heads, int kv_heads, int head_dim, int64_t q_row,
+                                       int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
+                                       float scale, int causal, int dtype, void* stream) {
+  using namespace tt;
+  TT_CHECK(check_heads("packed_attention", tokens, batch, heads, kv_heads, head_dim, dtype));
+  TT_REQUIRE(scale > 0.f && scale < 3e38f, "packed_attention: scale %g is not positive and finite", scale);
+  if (tokens == 0 || batch == 0) return TT_OK;
+  TT_REQUIRE(q && k && v && starts && out, "packed_attention: null pointer");
+  TT_CHECK(check_rows("packed_attention: q", q, q_row, q_head));
+  TT_CHECK(check_rows("packed_attention: k", k, k_row, k_head));
+  TT_CHECK(check_rows("packed_attention: v", v, v_row, v_head));
+  TT_CHECK(check_rows("packed_attention: out", out, 0, 0));
+  SeqAttnArgs a{};
+  a.q = q, a.k = k, a.v = v, a.out = out, a.starts = starts;
+  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  a.tokens = tokens, a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
+  a.head_dim = head_dim, a.causal = causal != 0, a.scale_log2 = scale * 1.4426950408889634f;
+  a.slots = (int)((int64_t)tokens * a.group / 128 + batch), a.splits = 1, a.chunk = INT32_MAX;
+  return launch_seq_attention(a, false, false, dtype, (hipStream_t)stream);
+}
+
+extern "C" int tt_cache_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int head_dim,
+                                                  int max_length, int single, int64_t* bytes) {
+  using namespace tt;
+  TT_CHECK(check_heads("cache_attention", tokens, batch, heads, kv_heads, head_dim, TT_FP16));
+  TT_REQUIRE(max_length >= 0 && max_length <= (1 << 30) && bytes != nullptr, "cache_attention: max_length %d",
+             max_length);
+  *bytes = 0;
+  if (tokens == 0 || batch == 0) return TT_OK;
+  *bytes = 4 * part_floats(seq_cache_plan(tokens, batch, heads, kv_heads, head_dim, max_length, single != 0), tokens,
+                           heads, head_dim);
+  return TT_OK;
+}
+
+extern "C" int tt_cache_attention_fwd(const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
+                                      const int32_t* lengths, const int32_t* starts, void* out, void* workspace,
+                                      int64_t workspace_bytes, int tokens, int batch, int heads, int kv_heads,
+                                      int head_dim, int pages, int page_size, int table_pages, int max_length,
+                                      int64_t q_row, int64_t q_head, int64_t k_page, int64_t k_row, int64_t k_head,
+                                      int64_t v_page, int64_t v_row, int64_t v_head, int64_t table_row, float scale,
+                                      int dtype, void* stream) {
+  using namespace tt;
+  TT_CHECK(check_heads("cache_attention", tokens, batch, heads, kv_heads, head_dim, dtype));
+  TT_CHECK(check_pages("cache_attention", pages, page_size, table_pages));
+  TT_REQUIRE(scale > 0.f && scale < 3e38f, "cache_attention: scale %g is not positive and finite", scale);
+  TT_REQUIRE(max_length >= 0 && max_length <= (1 << 30), "cache_attention: max_length %d", max_length);
+  if (tokens == 0 || batch == 0) return TT_OK;
+  TT_REQUIRE(q && k_cache && v_cache && table && lengths && out, "cache_attention: null pointer");
+  TT_REQUIRE(starts != nullptr || tokens == batch, "cache_attention: %d tokens for %d sequences without starts", tokens,
+             batch);
+  TT_CHECK(check_rows("cache_attention: q", q, q_row, q_head));
+  TT_CHECK(check_rows("cache_attention: k_cache", k_cache, k_row, k_head));
+  TT_CHECK(check_rows("cache_attention: v_cache", v_cache, v_row, v_head));
+  TT_REQUIRE(k_page % 8 == 0 && v_page % 8 == 0 && k_page >= 0 && v_page >= 0 && table_row >= 0,
+             "cache_attention: page strides %lld, %lld", (long long)k_page, (long long)v_page);
+  TT_CHECK(check_rows("cache_attention: out", out, 0, 0));
+  const SeqPlan p = seq_cache_plan(tokens, batch, heads, kv_heads, head_dim, max_length, starts == nullptr);
+  const int64_t parts = part_floats(p, tokens, heads, head_dim);
+  TT_REQUIRE(parts == 0 || (workspace != nullptr && workspace_bytes >= 4 * parts && ((uintptr_t)workspace & 15) == 0),
+             "cache_attention: a workspace of %lld bytes is needed, %lld given", (long long)(4 * parts),
+             (long long)workspace_bytes);
+  SeqAttnArgs a{};
+  a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.starts = starts, a.lengths = lengths, a.table = table;
+  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  a.k_page = k_page, a.v_page = v_page, a.table_row = table_row;
+  a.tokens = tokens, a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
+  a.head_dim = head_dim, a.pages = pages, a.table_pages = table_pages, a.page_shift = __builtin_ctz(page_size);
+  a.causal = 1, a.scale_log2 = scale * 1.4426950408889634f;
+  a.slots = p.slots, a.splits = p.splits, a.chunk = p.chunk;
+  a.part_o = static_cast<float*>(workspace);
+  if (parts > 0) a.part_ml = reinterpret_cast<float2*>(a.part_o + p.splits * (int64_t)tokens * heads * head_dim);
+  TT_CHECK(launch_seq_attention(a, true, p.narrow, dtype, (hipStream_t)stream));
+  if (p.splits == 1) return TT_OK;
+  const unsigned blocks = (unsigned)(((int64_t)tokens * heads + 3) / 4);
+  if (dtype == TT_FP16) hipLaunchKernelGGL(seq_merge_kernel<half>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(seq_merge_kernel<bf16>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
+  return launch_status("seq_merge_kernel");
+}
+
+extern "C" int tt_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int32_t* table,
+                               const int32_t* lengths, const int32_t* starts, int tokens, int batch, int kv_heads,
+                               int head_dim, int pages, int page_size, int table_pages, int64_t k_row, int64_t k_head,
+                               int64_t v_row, int64_t v_head, int64_t kc_page, int64_t kc_row, int64_t kc_head,
+                               int64_t vc_page, int64_t vc_row, int64_t vc_head, int64_t table_row, void* stream) {
+  using namespace tt;
+  TT_CHECK(check_heads("cache_append", tokens, batch, kv_heads, kv_heads, head_dim, TT_FP16));
+  TT_CHECK(check_pages("cache_append", pages, page_size, table_pages));
+  if (tokens == 0 || batch == 0) return TT_OK;
+  TT_REQUIRE(k && v && k_cache && v_cache && table && lengths, "cache_append: null pointer");
+  TT_REQUIRE(starts != nullptr || tokens == batch, "cache_append: %d tokens for %d sequences without starts", tokens,
+             batch);
+  TT_CHECK(check_rows("cache_append: k", k, k_row, k_head));
+  TT_CHECK(check_rows("cache_append: v", v, v_row, v_head));
+  TT_CHECK(check_rows("cache_append: k_cache", k_cache, kc_row, kc_head));
+  TT_CHECK(check_rows("cache_append: v_cache", v_cache, vc_row, vc_head));
+  TT_REQUIRE(kc_page % 8 == 0 && vc_page % 8 == 0 && kc_page >= 0 && vc_page >= 0 && table_row >= 0,
+             "cache_append: page strides %lld, %lld", (long long)kc_page, (long long)vc_page);
+  AppendArgs a{};
+  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.k_cache = static_cast<uint16_t*>(k_cache), a.v_cache = static_cast<uint16_t*>(v_cache);
+  a.starts = starts, a.lengths = lengths, a.table = table;
+  a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  a.kc_page = kc_page, a.kc_row = kc_row, a.kc_head = kc_head;
+  a.vc_page = vc_page, a.vc_row = vc_row, a.vc_head = vc_head, a.table_row = table_row;
+  a.tokens = tokens, a.batch = batch, a.heads = kv_heads, a.chunks = head_dim / 8;
+  if (k_head == head_dim && v_head == head_dim && kc_head == head_dim && vc_head == head_dim)
+    a.heads = 1, a.chunks = kv_heads * (head_dim / 8);  // the heads of a token lie side by side everywhere
+  a.pages = pages, a.table_pages = table_pages, a.page_shift = __builtin_ctz(page_size);
+  hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
+  return launch_status("cache_append_kernel");
+}

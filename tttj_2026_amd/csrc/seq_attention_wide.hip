@@ -1,0 +1,11 @@
+// seq_attention_kernel for head_dim above 128: 128 accumulator floats per lane, which are left in AGPRs here (this
+// file is built without the VGPR-form MFMA flag).
+#include "seq_launch.hpp"
+
+namespace tt {
+
+int launch_seq_attention_wide(const SeqAttnArgs& a, bool paged, bool narrow, int dtype, hipStream_t stream) {
+  return launch_seq_hd<256>(a, paged, narrow, dtype, stream);
+}
+
+}  // namespace tt

@@ -1,0 +1,48 @@
+// Host side of seq_attention.hpp: the launch of one instantiation, shared by seq_attention.hip (head_dim up to
+// 128) and seq_attention_wide.hip (up to 256).
+#pragma once
+
+#include "seq_attention.hpp"
+
+#include <atomic>
+
+namespace tt {
+
+template <typename T, int HD, int RW, int KW, int KT, bool PAGED>
+int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
+  constexpr int lds = 2 * 2 * KW * KT * HD * (int)sizeof(T);  // K and V, two tiles deep
+  static_assert(lds >= (KW - 1) * RW * (HD / 2 + 2) * 256, "the groups are merged in the tiles' LDS");
+  static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic LDS is raised
+  int dev = 0;
+  TT_HIP(hipGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
+    TT_HIP(hipFuncSetAttribute((const void*)seq_attention_kernel<T, HD, RW, KW, KT, PAGED>,
+                               hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const int64_t blocks = (int64_t)a.slots * a.kv_heads * a.splits;
+  constexpr int threads = 64 * RW * KW;
+  TT_REQUIRE(blocks * threads < (1LL << 32), "attention: %lld blocks are more than one launch takes",
+             (long long)blocks);
+  hipLaunchKernelGGL((seq_attention_kernel<T, HD, RW, KW, KT, PAGED>), dim3((unsigned)blocks), dim3(threads), lds,
+                     stream, a);
+  return launch_status("seq_attention_kernel");
+}
+
+template <int HD, typename T>
+int launch_seq_type(const SeqAttnArgs& a, bool paged, bool narrow, hipStream_t stream) {
+  if (!paged) return launch_seq<T, HD, 4, 1, 64, false>(a, stream);
+  if (narrow) return launch_seq<T, HD, 1, (HD <= 128 ? 4 : 2), 32, true>(a, stream);
+  return launch_seq<T, HD, 4, 1, 64, true>(a, stream);
+}
+
+template <int HD>
+int launch_seq_hd(const SeqAttnArgs& a, bool paged, bool narrow, int dtype, hipStream_t stream) {
+  return dtype == TT_FP16 ? launch_seq_type<HD, half>(a, paged, narrow, stream)
+                          : launch_seq_type<HD, bf16>(a, paged, narrow, stream);
+}
+
+int launch_seq_attention_wide(const SeqAttnArgs& a, bool paged, bool narrow, int dtype, hipStream_t stream);
+
+}  // namespace tt
