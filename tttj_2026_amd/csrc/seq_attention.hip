@@ -5,13 +5,16 @@
 
 namespace tt {
 
-// out = sum_s w_s O_s / sum_s w_s l_s over the key ranges s of a row, w_s = 2^(m_s - max m).  One wave per
-// (token, head); rows whose keys lie in one range were written by their block.
-template <typename T>
-__global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a) {
-  const int lane = threadIdx.x & 63;
+// out = sum_s w_s O_s / sum_s w_s l_s over the key ranges s of a row, w_s = 2^(m_s - max m).  W waves per
+// (token, head): head_dim / 4 lanes (rounded up to a power of two) take a part, the parts are dealt to 64 W / that
+// many groups of lanes, four loads of each in flight, and the groups are added up at the end.  Rows whose keys lie in
+// one range were written by their block.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int lanes) {
+  __shared__ float s_sum[W > 1 ? W : 1][W > 1 ? 64 : 1][5];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t nrows = (int64_t)a.tokens * a.heads;
-  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   if (row >= nrows) return;
   const int token = (int)(row / a.heads);
   int seq = token, i = 0, count = 1;
@@ -24,28 +27,71 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a) {
   }
   const int lim = seq_limit(a, i, count, seq_keys<true>(a, seq, count));
   if (lim <= a.chunk) return;
-  const int parts = min((lim + a.chunk - 1) / a.chunk, a.splits);
+  const int parts = min((int)(((int64_t)lim + a.chunk - 1) / a.chunk), a.splits);
+  const float2* const ml = a.part_ml + row;
   float m = -INFINITY;
-  for (int s = lane; s < parts; s += 64) m = fmaxf(m, a.part_ml[s * nrows + row].x);
+  for (int s = lane; s < parts; s += 64) m = fmaxf(m, ml[s * nrows].x);
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+  const int in = lane & (lanes - 1), d = 4 * in;
+  const int groups = 64 / lanes * W, group = (W > 1 ? wave * (64 / lanes) : 0) + lane / lanes;
+  const bool live = d < a.head_dim;
+  const float* const o_part = a.part_o + row * a.head_dim + (live ? d : 0);
   float l = 0.f;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  const bool live = 4 * lane < a.head_dim;
-  for (int s = 0; s < parts; ++s) {
-    const float2 ml = a.part_ml[s * nrows + row];
-    const float w = ml.x == -INFINITY ? ml.y : __builtin_amdgcn_exp2f(ml.x - m);
-    l = fmaf(w, ml.y, l);
-    if (live) {
-      const floatx4 x = *reinterpret_cast<const floatx4*>(a.part_o + (s * nrows + row) * a.head_dim + 4 * lane);
+  for (int s0 = group; s0 < parts; s0 += 4 * groups) {
+    float2 y[4];
+    floatx4 x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[e], o[e]);
+    for (int u = 0; u < 4; ++u) {
+      const int s = min(s0 + u * groups, parts - 1);
+      y[u] = ml[s * nrows];
+      x[u] = *reinterpret_cast<const floatx4*>(o_part + s * nrows * a.head_dim);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (s0 + u * groups >= parts) break;
+      const float w = y[u].x == -INFINITY ? y[u].y : __builtin_amdgcn_exp2f(y[u].x - m);
+      l = fmaf(w, y[u].y, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[u][e], o[e]);
+    }
+  }
+  for (int off = lanes; off < 64; off <<= 1) {
+    l += __shfl_xor(l, off);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off);
+  }
+  if constexpr (W > 1) {
+    s_sum[wave][lane][4] = l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s_sum[wave][lane][e] = o[e];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      l += s_sum[w][lane][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += s_sum[w][lane][e];
     }
   }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   typedef T v4 __attribute__((ext_vector_type(4)));
-  if (live)
-    *reinterpret_cast<v4*>(static_cast<T*>(a.out) + row * a.head_dim + 4 * lane) =
+  if (live && lane < lanes)
+    *reinterpret_cast<v4*>(static_cast<T*>(a.out) + row * a.head_dim + d) =
         v4{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+}
+
+template <typename T>
+static int launch_seq_merge(const SeqAttnArgs& a, hipStream_t stream) {
+  int lanes = 2;
+  while (4 * lanes < a.head_dim) lanes *= 2;
+  const int64_t rows = (int64_t)a.tokens * a.heads;
+  // Few rows of many parts take a block each; otherwise a wave each.
+  if (a.splits > 8 && rows < (1 << 16))
+    hipLaunchKernelGGL((seq_merge_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a, lanes);
+  else
+    hipLaunchKernelGGL((seq_merge_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, lanes);
+  return launch_status("seq_merge_kernel");
 }
 
 struct AppendArgs {
@@ -235,10 +281,7 @@ extern "C" int tt_cache_attention_fwd(const void* q, const void* k_cache, const 
   if (parts > 0) a.part_ml = reinterpret_cast<float2*>(a.part_o + p.splits * (int64_t)tokens * heads * head_dim);
   TT_CHECK(launch_seq_attention(a, true, p.narrow, dtype, (hipStream_t)stream));
   if (p.splits == 1) return TT_OK;
-  const unsigned blocks = (unsigned)(((int64_t)tokens * heads + 3) / 4);
-  if (dtype == TT_FP16) hipLaunchKernelGGL(seq_merge_kernel<half>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL(seq_merge_kernel<bf16>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);
-  return launch_status("seq_merge_kernel");
+  return dtype == TT_FP16 ? launch_seq_merge<half>(a, (hipStream_t)stream) : launch_seq_merge<bf16>(a, (hipStream_t)stream);
 }
 
 extern "C" int tt_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int32_t* table,
