@@ -287,7 +287,8 @@ int tt_cache_append(const void* k, const void* v, void* k_cache, void* v_cache,
  * tt_cache_attention_workspace_bytes gives for the same arguments (single: starts == NULL); 0 needs
  * none.  No counterpart in the reference. */
 int tt_cache_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int head_dim,
-                                       int max_length, int single, int64_t* bytes);
+                                       int page_size, int table_pages, int max_length, int single,
+                                       int64_t* bytes);
 int tt_cache_attention_fwd(const void* q, const void* k_cache, const void* v_cache,
                            const int32_t* table, const int32_t* lengths, const int32_t* starts,
                            void* out, void* workspace, int64_t workspace_bytes, int tokens,

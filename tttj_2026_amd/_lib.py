@@ -53,7 +53,7 @@ SIGNATURES = {
     "tt_attention_fwd_prescaled": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "tt_packed_attention_fwd": (_I, [_P] * 5 + [_I] * 5 + [_I64] * 6 + [_F, _I, _I, _P]),
     "tt_cache_append": (_I, [_P] * 7 + [_I] * 7 + [_I64] * 11 + [_P]),
-    "tt_cache_attention_workspace_bytes": (_I, [_I] * 7 + [ctypes.POINTER(_I64)]),
+    "tt_cache_attention_workspace_bytes": (_I, [_I] * 9 + [ctypes.POINTER(_I64)]),
     "tt_cache_attention_fwd": (_I, [_P] * 8 + [_I64] + [_I] * 9 + [_I64] * 9 + [_F, _I, _P]),
     "tt_transformer_fwd": (_I, [_P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "tt_noalloc_scratch_bytes": (_I, [ctypes.POINTER(_I64)]),
@@ -124,10 +124,12 @@ def workspace_bytes(batch: int, seq: int, d_model: int, heads: int, ffn_dim: int
 
 
 def cache_attention_workspace_bytes(tokens: int, batch: int, heads: int, kv_heads: int,
-                                    head_dim: int, max_length: int, single: bool) -> int:
+                                    head_dim: int, page_size: int, table_pages: int,
+                                    max_length: int, single: bool) -> int:
     out = _I64()
     check(load().tt_cache_attention_workspace_bytes(tokens, batch, heads, kv_heads, head_dim,
-                                                    max_length, int(single), ctypes.byref(out)),
+                                                    page_size, table_pages, max_length, int(single),
+                                                    ctypes.byref(out)),
           "tt_cache_attention_workspace_bytes")
     return out.value
 

@@ -42,6 +42,7 @@ SOURCE_FLAGS = {
     "attention_small.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "rowchain.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "seq_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "seq_attention_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "megakernel.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

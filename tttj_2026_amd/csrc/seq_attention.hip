@@ -5,55 +5,59 @@
 
 namespace tt {
 
-// out = sum_s w_s O_s / sum_s w_s l_s over the key ranges s of a row, w_s = 2^(m_s - max m).  W waves per
+// out = sum_s w_s O_s / sum_s w_s l_s over the shares s that a row's keys lie in, w_s = 2^(m_s - max m).  W waves per
 // (token, head): head_dim / 4 lanes (rounded up to a power of two) take a part, the parts are dealt to 64 W / that
-// many groups of lanes, four loads of each in flight, and the groups are added up at the end.  Rows whose keys lie in
-// one range were written by their block.
+// many groups of lanes, four loads of each in flight, and the groups are added up at the end.  Rows of tiles that lie
+// in one share were written by its block.
 template <typename T, int W>
-__global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int lanes) {
+__global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int rows_per_tile, int lanes) {
   __shared__ float s_sum[W > 1 ? W : 1][W > 1 ? 64 : 1][5];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t nrows = (int64_t)a.tokens * a.heads;
-  const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-  if (row >= nrows) return;
-  const int token = (int)(row / a.heads);
-  int seq = token, i = 0, count = 1;
+  const int row = W > 1 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
+  if (row >= a.tokens * a.heads) return;
+  const int token = row / a.heads, head = row - token * a.heads;
+  int seq = token;
   if (a.starts != nullptr) {
     seq = seq_search(a.batch, token, [&](int b) { return seq_start(a.starts, b, a.tokens); });
-    const int first = seq_start(a.starts, seq, a.tokens);
-    i = token - first;
-    count = seq_start(a.starts, seq + 1, a.tokens) - first;
-    if (i < 0 || i >= count) return;  // a row of no sequence
+    const int2 own = seq_rows(a, seq);
+    if (token < own.x || token >= own.x + own.y) return;  // a row of no sequence
   }
-  const int lim = seq_limit(a, i, count, seq_keys<true>(a, seq, count));
-  if (lim <= a.chunk) return;
-  const int parts = min((int)(((int64_t)lim + a.chunk - 1) / a.chunk), a.splits);
-  const float2* const ml = a.part_ml + row;
+  const SeqUnits u = seq_units(a, seq, rows_per_tile);
+  const int hkv = head / a.group;
+  const int r = (token - u.first) * a.group + head - hkv * a.group;
+  const int tile = r / rows_per_tile;
+  const SeqShare sh = seq_share(a, 0, seq, rows_per_tile);
+  const int share = sh.share, begin = sh.base + tile * u.units;
+  const int first = begin / share, parts = (begin + u.units - 1) / share - first + 1;
+  if (parts == 1) return;
+  // part p of the tile belongs to slot first + p: its second entry where the tile begins there, its first otherwise
+  const int64_t place = (int64_t)hkv * rows_per_tile + r - tile * rows_per_tile, step = 2 * (int64_t)a.kv_heads * rows_per_tile;
+  const auto at = [&](int p) -> int64_t { return (first + p) * step + (p == 0 ? step / 2 : 0) + place; };
   float m = -INFINITY;
-  for (int s = lane; s < parts; s += 64) m = fmaxf(m, ml[s * nrows].x);
+  for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.part_ml[at(p)].x);
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
   const int in = lane & (lanes - 1), d = 4 * in;
   const int groups = 64 / lanes * W, group = (W > 1 ? wave * (64 / lanes) : 0) + lane / lanes;
   const bool live = d < a.head_dim;
-  const float* const o_part = a.part_o + row * a.head_dim + (live ? d : 0);
   float l = 0.f;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = group; s0 < parts; s0 += 4 * groups) {
+  for (int p0 = group; p0 < parts; p0 += 4 * groups) {
     float2 y[4];
-    floatx4 x[4];
+    floatx4 v[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int s = min(s0 + u * groups, parts - 1);
-      y[u] = ml[s * nrows];
-      x[u] = *reinterpret_cast<const floatx4*>(o_part + s * nrows * a.head_dim);
+    for (int i = 0; i < 4; ++i) {
+      const int64_t e = at(min(p0 + i * groups, parts - 1));
+      y[i] = a.part_ml[e];
+      v[i] = *reinterpret_cast<const floatx4*>(a.part_o + e * a.head_dim + (live ? d : 0));
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (s0 + u * groups >= parts) break;
-      const float w = y[u].x == -INFINITY ? y[u].y : __builtin_amdgcn_exp2f(y[u].x - m);
-      l = fmaf(w, y[u].y, l);
+    for (int i = 0; i < 4; ++i) {
+      if (p0 + i * groups >= parts) break;
+      // a part without a maximum saw no key (its sum, 0, is its weight) or only NaN (NaN is)
+      const float w = y[i].x == -INFINITY ? y[i].y : __builtin_amdgcn_exp2f(y[i].x - m);
+      l = fmaf(w, y[i].y, l);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[u][e], o[e]);
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, v[i][e], o[e]);
     }
   }
   for (int off = lanes; off < 64; off <<= 1) {
@@ -77,20 +81,19 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int lanes
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   typedef T v4 __attribute__((ext_vector_type(4)));
   if (live && lane < lanes)
-    *reinterpret_cast<v4*>(static_cast<T*>(a.out) + row * a.head_dim + d) =
+    *reinterpret_cast<v4*>(static_cast<T*>(a.out) + (int64_t)row * a.head_dim + d) =
         v4{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
 }
 
 template <typename T>
-static int launch_seq_merge(const SeqAttnArgs& a, hipStream_t stream) {
+static int launch_seq_merge(const SeqAttnArgs& a, int rows_per_tile, bool many_parts, hipStream_t stream) {
   int lanes = 2;
   while (4 * lanes < a.head_dim) lanes *= 2;
-  const int64_t rows = (int64_t)a.tokens * a.heads;
-  // Few rows of many parts take a block each; otherwise a wave each.
-  if (a.splits > 8 && rows < (1 << 16))
-    hipLaunchKernelGGL((seq_merge_kernel<T, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a, lanes);
+  const int rows = a.tokens * a.heads;
+  if (many_parts)  // a block per row, else a wave
+    hipLaunchKernelGGL((seq_merge_kernel<T, 4>), dim3(rows), dim3(256), 0, stream, a, rows_per_tile, lanes);
   else
-    hipLaunchKernelGGL((seq_merge_kernel<T, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, lanes);
+    hipLaunchKernelGGL((seq_merge_kernel<T, 1>), dim3(rows / 4 + 1), dim3(256), 0, stream, a, rows_per_tile, lanes);
   return launch_status("seq_merge_kernel");
 }
 
@@ -141,35 +144,44 @@ int launch_seq_attention(const SeqAttnArgs& a, bool paged, bool narrow, int dtyp
   return launch_seq_hd<32>(a, paged, narrow, dtype, stream);
 }
 
-// How the keys of a call over the cache are split.
-struct SeqPlan {
-  bool narrow;  // 32 rows per block
-  int slots, splits, chunk;
-};
-
-SeqPlan seq_cache_plan(int64_t tokens, int batch, int heads, int kv_heads, int head_dim, int max_length, bool single) {
-  SeqPlan p;
-  const int64_t G = heads / kv_heads;
-  p.narrow = single ? G <= 32 : tokens * G <= 32 * (int64_t)batch;
-  const int R = p.narrow ? 32 : 128;
-  p.slots = (int)(single ? tokens * ((G + R - 1) / R) : tokens * G / R + batch);
-  const int64_t blocks = (int64_t)p.slots * kv_heads;
-  const int64_t want = 4L * device_cus();
-  const int step = 256;
-  int64_t splits = blocks >= want ? 1 : want / blocks;
-  int64_t chunk = (max_length + splits - 1) / splits;
-  chunk = (chunk + step - 1) / step * step;
-  p.splits = (int)((max_length + chunk - 1) / chunk);
-  p.chunk = (int)chunk;
-  if (p.splits <= 1) {
-    p.splits = 1;
-    p.chunk = INT32_MAX;
-  }
-  return p;
+// Blocks of a kernel that a CU holds (its registers and LDS).
+static int seq_resident(bool narrow, int head_dim) {
+  if (narrow) return head_dim <= 32 ? 6 : head_dim <= 64 ? 5 : 2;
+  return head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1;
 }
 
-static int64_t part_floats(const SeqPlan& p, int64_t tokens, int heads, int head_dim) {
-  return p.splits == 1 ? 0 : p.splits * tokens * heads * (head_dim + 2);
+// How a call is given to blocks.
+struct SeqPlan {
+  bool narrow;  // 32 rows per block, for single tokens and few drafted ones; otherwise 128
+  int rows;     // of a block
+  int slots, mode;
+  int64_t part_rows;  // rows of the workspace
+  bool many_parts;
+};
+
+// max_length < 0: packed sequences (no keys but their own).
+static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int head_dim, int64_t held, int max_length, bool single) {
+  SeqPlan p{};
+  const int64_t G = heads / kv_heads;
+  const bool paged = max_length >= 0;
+  p.narrow = paged && (single ? G <= 32 : tokens * G <= 32 * (int64_t)batch);
+  p.rows = p.narrow ? 32 : 128;
+  const int64_t tiles = single ? tokens * ((G + p.rows - 1) / p.rows) : tokens * G / p.rows + batch;
+  const int64_t blocks = tiles * kv_heads, held_blocks = (int64_t)seq_resident(p.narrow, head_dim) * device_cus();
+  p.slots = (int)tiles;
+  p.mode = kSeqInOrder;
+  if (paged && max_length > 512 && batch <= 512 && blocks < (p.narrow ? 4 : 1) * held_blocks && tiles * (held / kSeqUnit + 1) < (1LL << 31)) {
+    p.mode = kSeqShares;
+    const int64_t units = tiles * ((max_length + kSeqUnit - 1) / kSeqUnit);
+    int64_t slots = held_blocks / kv_heads;
+    if (slots > (units + kSeqMinShare - 1) / kSeqMinShare) slots = (units + kSeqMinShare - 1) / kSeqMinShare;
+    p.slots = (int)(slots > 1 ? slots : 1);
+    p.part_rows = 2 * (int64_t)p.slots * kv_heads * p.rows;
+    p.many_parts = p.slots > 8 * tiles;
+  } else if (!single && batch <= 64 && blocks > held_blocks && tokens * G < (1LL << 30)) {
+    p.mode = kSeqHeaviest;
+  }
+  return p;
 }
 
 static int check_heads(const char* what, int tokens, int batch, int heads, int kv_heads, int head_dim, int dtype) {
@@ -225,20 +237,22 @@ extern "C" int tt_packed_attention_fwd(const void* q, const void* k, const void*
   a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
   a.tokens = tokens, a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
   a.head_dim = head_dim, a.causal = causal != 0, a.scale_log2 = scale * 1.4426950408889634f;
-  a.slots = (int)((int64_t)tokens * a.group / 128 + batch), a.splits = 1, a.chunk = INT32_MAX;
+  const SeqPlan p = seq_plan(tokens, batch, heads, kv_heads, head_dim, 0, -1, false);
+  a.slots = p.slots, a.mode = p.mode;
   return launch_seq_attention(a, false, false, dtype, (hipStream_t)stream);
 }
 
 extern "C" int tt_cache_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int head_dim,
-                                                  int max_length, int single, int64_t* bytes) {
+                                                  int page_size, int table_pages, int max_length, int single,
+                                                  int64_t* bytes) {
   using namespace tt;
   TT_CHECK(check_heads("cache_attention", tokens, batch, heads, kv_heads, head_dim, TT_FP16));
-  TT_REQUIRE(max_length >= 0 && max_length <= (1 << 30) && bytes != nullptr, "cache_attention: max_length %d",
-             max_length);
+  TT_CHECK(check_pages("cache_attention", 1, page_size, table_pages));
+  TT_REQUIRE(max_length >= 0 && bytes != nullptr, "cache_attention: max_length %d", max_length);
   *bytes = 0;
   if (tokens == 0 || batch == 0) return TT_OK;
-  *bytes = 4 * part_floats(seq_cache_plan(tokens, batch, heads, kv_heads, head_dim, max_length, single != 0), tokens,
-                           heads, head_dim);
+  *bytes = 4 * (head_dim + 2) * seq_plan(tokens, batch, heads, kv_heads, head_dim, (int64_t)page_size * table_pages,
+                                         max_length, single != 0).part_rows;
   return TT_OK;
 }
 
@@ -253,7 +267,7 @@ extern "C" int tt_cache_attention_fwd(const void* q, const void* k_cache, const 
   TT_CHECK(check_heads("cache_attention", tokens, batch, heads, kv_heads, head_dim, dtype));
   TT_CHECK(check_pages("cache_attention", pages, page_size, table_pages));
   TT_REQUIRE(scale > 0.f && scale < 3e38f, "cache_attention: scale %g is not positive and finite", scale);
-  TT_REQUIRE(max_length >= 0 && max_length <= (1 << 30), "cache_attention: max_length %d", max_length);
+  TT_REQUIRE(max_length >= 0, "cache_attention: max_length %d", max_length);
   if (tokens == 0 || batch == 0) return TT_OK;
   TT_REQUIRE(q && k_cache && v_cache && table && lengths && out, "cache_attention: null pointer");
   TT_REQUIRE(starts != nullptr || tokens == batch, "cache_attention: %d tokens for %d sequences without starts", tokens,
@@ -264,10 +278,11 @@ extern "C" int tt_cache_attention_fwd(const void* q, const void* k_cache, const 
   TT_REQUIRE(k_page % 8 == 0 && v_page % 8 == 0 && k_page >= 0 && v_page >= 0 && table_row >= 0,
              "cache_attention: page strides %lld, %lld", (long long)k_page, (long long)v_page);
   TT_CHECK(check_rows("cache_attention: out", out, 0, 0));
-  const SeqPlan p = seq_cache_plan(tokens, batch, heads, kv_heads, head_dim, max_length, starts == nullptr);
-  const int64_t parts = part_floats(p, tokens, heads, head_dim);
-  TT_REQUIRE(parts == 0 || (workspace != nullptr && workspace_bytes >= 4 * parts && ((uintptr_t)workspace & 15) == 0),
-             "cache_attention: a workspace of %lld bytes is needed, %lld given", (long long)(4 * parts),
+  const SeqPlan p = seq_plan(tokens, batch, heads, kv_heads, head_dim, (int64_t)page_size * table_pages, max_length,
+                             starts == nullptr);
+  const int64_t bytes = 4 * (head_dim + 2) * p.part_rows;
+  TT_REQUIRE(bytes == 0 || (workspace != nullptr && workspace_bytes >= bytes && ((uintptr_t)workspace & 15) == 0),
+             "cache_attention: a workspace of %lld bytes is needed, %lld given", (long long)bytes,
              (long long)workspace_bytes);
   SeqAttnArgs a{};
   a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.starts = starts, a.lengths = lengths, a.table = table;
@@ -276,12 +291,13 @@ extern "C" int tt_cache_attention_fwd(const void* q, const void* k_cache, const 
   a.tokens = tokens, a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
   a.head_dim = head_dim, a.pages = pages, a.table_pages = table_pages, a.page_shift = __builtin_ctz(page_size);
   a.causal = 1, a.scale_log2 = scale * 1.4426950408889634f;
-  a.slots = p.slots, a.splits = p.splits, a.chunk = p.chunk;
+  a.slots = p.slots, a.mode = p.mode;
   a.part_o = static_cast<float*>(workspace);
-  if (parts > 0) a.part_ml = reinterpret_cast<float2*>(a.part_o + p.splits * (int64_t)tokens * heads * head_dim);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + p.part_rows * head_dim);
   TT_CHECK(launch_seq_attention(a, true, p.narrow, dtype, (hipStream_t)stream));
-  if (p.splits == 1) return TT_OK;
-  return dtype == TT_FP16 ? launch_seq_merge<half>(a, (hipStream_t)stream) : launch_seq_merge<bf16>(a, (hipStream_t)stream);
+  if (p.mode != kSeqShares) return TT_OK;
+  return dtype == TT_FP16 ? launch_seq_merge<half>(a, p.rows, p.many_parts, (hipStream_t)stream)
+                          : launch_seq_merge<bf16>(a, p.rows, p.many_parts, (hipStream_t)stream);
 }
 
 extern "C" int tt_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int32_t* table,

@@ -74,6 +74,11 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const lds_short*)p;
 }
 
+__device__ __forceinline__ void lds_done() {  // this wave's LDS accesses, its copies in flight apart
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  asm volatile("" ::: "memory");
+}
+
 struct SeqAttnArgs {
   const void *q, *k, *v;   // q rows [tokens, heads, head_dim]; k, v the same with kv_heads, or a paged cache
   void* out;               // [tokens, heads * head_dim]
@@ -86,11 +91,18 @@ struct SeqAttnArgs {
   int pages, table_pages, page_shift;
   int causal;
   float scale_log2;        // c log2(e)
-  int slots;               // row tiles of the launch per kv head
-  int splits, chunk;       // key ranges of `chunk` keys, `splits` of them at most
-  float* part_o;           // [splits][tokens * heads][head_dim] where splits > 1
-  float2* part_ml;         // [splits][tokens * heads]: maximum (log2 domain) and sum
+  int slots;               // blocks of the launch per kv head
+  int mode;                // kSeqInOrder, kSeqHeaviest or kSeqShares
+  float* part_o;           // kSeqShares: [2 slots][kv_heads][R][head_dim], the rows of tiles that lie in several shares
+  float2* part_ml;         // ... [2 slots][kv_heads][R], their maximum (log2 domain) and sum
 };
+
+// How row tiles are given to blocks.
+constexpr int kSeqInOrder = 0;   // a tile each, the last sequence's last tile first
+constexpr int kSeqHeaviest = 1;  // a tile each, those with most keys first, over all sequences (batch <= 64)
+constexpr int kSeqShares = 2;    // all (tile, 64 keys) units of a kv head in equal shares, one per block
+constexpr int kSeqUnit = 64;
+constexpr int kSeqMinShare = 4;  // units: a smaller share does not pay for joining it
 
 constexpr float kSeqLazy = 8.0f;   // log2 growth of a row's maximum that moves its reference
 constexpr float kSeqShift = 7.0f;  // log2 of the factor on the probabilities: 2^(8 + 7) < 65504
@@ -146,6 +158,13 @@ __device__ __forceinline__ SeqTile seq_tile(const SeqAttnArgs& a, int slot, int 
   return s;
 }
 
+// First row and rows of sequence b.
+__device__ __forceinline__ int2 seq_rows(const SeqAttnArgs& a, int b) {
+  if (a.starts == nullptr) return make_int2(b, 1);
+  const int first = seq_start(a.starts, b, a.tokens);
+  return make_int2(first, max(seq_start(a.starts, b + 1, a.tokens) - first, 0));
+}
+
 // Keys that sequence `seq` of `count` rows holds.
 template <bool PAGED>
 __device__ __forceinline__ int seq_keys(const SeqAttnArgs& a, int seq, int count) {
@@ -156,6 +175,124 @@ __device__ __forceinline__ int seq_keys(const SeqAttnArgs& a, int seq, int count
 // Keys that token i of `count` may see, of `keys`.
 __device__ __forceinline__ int seq_limit(const SeqAttnArgs& a, int i, int count, int keys) {
   return a.causal ? max(keys - count + i + 1, 0) : keys;
+}
+
+// Sum over the lanes up to this one, by DPP: shifts by 1, 2, 4 and 8 within rows of 16 lanes, then the last lane of
+// row 0 (2) to row 1 (3) and that of row 1 to rows 2 and 3.
+__device__ __forceinline__ int wave_scan_int(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+__device__ __forceinline__ int wave_sum_int(int v) { return __builtin_amdgcn_readlane(wave_scan_int(v), 63); }
+
+__device__ __forceinline__ int wave_max_int(int v) {  // of values >= 0
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The tile of rank `rank` by its number of keys, in units of 64 (kSeqHeaviest; lane b holds sequence b): the tiles of a
+// sequence that see more than 64 w keys are those from a certain one on, so their number over all sequences follows
+// from w without a list, and a bisection over w finds the rank's level.  tile < 0: no such tile.
+template <bool PAGED>
+__device__ __forceinline__ SeqTile seq_ranked(const SeqAttnArgs& a, int rank, int rows_per_tile) {
+  const int lane = threadIdx.x & 63, G = a.group;
+  int2 own = make_int2(0, 0);
+  int keys = 0;
+  if (lane < a.batch) {
+    own = seq_rows(a, lane);
+    keys = seq_keys<PAGED>(a, lane, own.y);
+  }
+  const int tiles = (own.y * G + rows_per_tile - 1) / rows_per_tile;
+  // The first tile with a row that sees more than 64 w keys (w < 0: any row).
+  const auto from = [&](int w) -> int {
+    if (w < 0) return 0;
+    if (!a.causal) return keys > kSeqUnit * w ? 0 : tiles;
+    const int token = kSeqUnit * w - (keys - own.y);
+    return token <= 0 ? 0 : token >= own.y ? tiles : token * G / rows_per_tile;
+  };
+  SeqTile s{0, -1, 0, 0};
+  if (rank >= wave_sum_int(tiles)) return s;
+  int lo = -1, hi = wave_max_int((keys + kSeqUnit - 1) / kSeqUnit);  // more than `rank` tiles above lo, not above hi
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (wave_sum_int(tiles - from(mid)) > rank) lo = mid;
+    else hi = mid;
+  }
+  const int at = rank - wave_sum_int(tiles - from(lo + 1));  // among the tiles of this level
+  const int here = from(lo + 1) - from(lo);
+  const int upto = wave_scan_int(here);
+  const int b = __ffsll((unsigned long long)__ballot(upto > at)) - 1;
+  s.seq = __builtin_amdgcn_readfirstlane(b);
+  s.tile = __builtin_amdgcn_readlane(from(lo) + at - (upto - here), s.seq);
+  s.first = __builtin_amdgcn_readlane(own.x, s.seq);
+  s.count = __builtin_amdgcn_readlane(own.y, s.seq);
+  return s;
+}
+
+// kSeqShares.  A sequence counts tiles x units units, its keys in units of 64 (at least one), whether or not all rows
+// of a tile see them: its new tokens are few against its keys wherever keys are shared out.
+struct SeqUnits {
+  int first, count, keys, tiles, units;
+};
+
+__device__ __forceinline__ SeqUnits seq_units(const SeqAttnArgs& a, int b, int rows_per_tile) {
+  SeqUnits u;
+  const int2 own = seq_rows(a, b);
+  u.first = own.x;
+  u.count = own.y;
+  u.keys = seq_keys<true>(a, b, own.y);
+  u.tiles = (own.y * a.group + rows_per_tile - 1) / rows_per_tile;
+  u.units = max((u.keys + kSeqUnit - 1) / kSeqUnit, 1);
+  return u;
+}
+
+struct SeqShare {
+  int total, share;  // units of a kv head, and those of one block
+  int seq, base;     // the sequence asked for, and its first unit
+};
+
+// The shares of a launch, and the sequence that holds the first unit of block `slot` (seq < 0), or sequence `seq`.
+__device__ __forceinline__ SeqShare seq_share(const SeqAttnArgs& a, int slot, int seq, int rows_per_tile) {
+  const int lane = threadIdx.x & 63;
+  const auto units_of = [&](int b) -> int {
+    if (b >= a.batch) return 0;
+    const SeqUnits u = seq_units(a, b, rows_per_tile);
+    return u.tiles * u.units;
+  };
+  SeqShare s;
+  int upto = wave_scan_int(units_of(lane));
+  s.total = __builtin_amdgcn_readlane(upto, 63);
+  if (a.batch > 64) {
+    int n = 0;
+    for (int b = 64 + lane; b < a.batch; b += 64) n += units_of(b);
+    s.total += wave_sum_int(n);
+  }
+  s.share = max((s.total + a.slots - 1) / a.slots, kSeqMinShare);
+  const int64_t x = (int64_t)slot * s.share;
+  s.base = 0;
+  for (int b0 = 0;;) {
+    const int all = __builtin_amdgcn_readlane(upto, 63);
+    if (b0 + 64 >= a.batch || (seq >= 0 ? seq < b0 + 64 : s.base + all > x)) {
+      const int l = seq >= 0 ? seq - b0 : __popcll(__ballot(s.base + upto <= x));
+      s.seq = b0 + min(l, 63);
+      if (l > 0) s.base += __builtin_amdgcn_readlane(upto, min(l, 64) - 1);
+      return s;
+    }
+    s.base += all;
+    b0 += 64;
+    upto = wave_scan_int(units_of(b0 + lane));
+  }
 }
 
 template <typename T, int HD, int CB, int RW, int KW, int KT, bool PAGED, int WPE = (HD <= 64 ? 3 : HD <= 128 ? 2 : 1)>
@@ -179,43 +316,33 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   extern __shared__ __align__(16) char seq_lds[];
 
   const int hkv = blockIdx.x % a.kv_heads;
-  const int rest = blockIdx.x / a.kv_heads;
-  const int split = rest / a.slots;
-  int slot = rest - split * a.slots;
-  if (a.causal) slot = a.slots - 1 - slot;  // the heaviest tiles of a sequence first
-  const SeqTile sq = seq_tile(a, slot, R);
+  const int slot = blockIdx.x / a.kv_heads;
   const int G = a.group;
-  const int rows = sq.count * G;
-  const int r0 = sq.tile * R;
-  if (sq.tile < 0 || r0 >= rows) return;
-  const int keys = seq_keys<PAGED>(a, sq.seq, sq.count);
-  const int kbeg = split * a.chunk;
-  const int block_end = seq_limit(a, min(r0 + R - 1, rows - 1) / G, sq.count, keys);
-  if (split > 0 && kbeg >= block_end) return;
-  // the last range takes what is left, should a sequence be longer than the launch was sized for
-  const int kend = split == a.splits - 1 ? block_end : min(block_end, kbeg + a.chunk);
-  const int ntiles = (kend - kbeg + KT - 1) / KT;
-
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x;
+  int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = RW == 1 ? 0 : wave % RW, grp = RW == 1 ? wave : wave / RW;
-  const int hf = lane >> 5, col = lane & 31;
+  int hf = lane >> 5, col = lane & 31;
   T* const sk = reinterpret_cast<T*>(seq_lds) + (size_t)grp * 2 * TILE;
   T* const sv = reinterpret_cast<T*>(seq_lds) + (size_t)KW * 2 * TILE + (size_t)grp * 2 * TILE;
 
-  // Rows of this wave; those behind the last repeat it and are not stored, so limits rise along the rows.
-  const int wr0 = r0 + rw * WR;
-  const bool wave_active = wr0 < rows;
-  const int block_lo = seq_limit(a, r0 / G, sq.count, keys);  // the first row's
-  const int lim_lo = seq_limit(a, min(wr0, rows - 1) / G, sq.count, keys);
-  const int lim_hi = min(seq_limit(a, min(wr0 + WR - 1, rows - 1) / G, sq.count, keys), kend);
-  int tok[CB], head[CB], lim[CB];
-#pragma unroll
-  for (int b = 0; b < CB; ++b) {
-    const int r = min(wr0 + 32 * b + col, rows - 1);
-    tok[b] = r / G;
-    head[b] = hkv * G + r - tok[b] * G;
-    lim[b] = seq_limit(a, tok[b], sq.count, keys);
+  // What this block does: a row tile with all its keys, or (kSeqShares) units x ... share_end - 1, tile after tile.
+  SeqTile sq;
+  const bool shares = PAGED && a.mode == kSeqShares;
+  int x = 0, share_end = 0, base = 0;
+  SeqUnits su{};
+  if (shares) {
+    const SeqShare sh = seq_share(a, slot, -1, R);
+    if ((int64_t)slot * sh.share >= sh.total) return;
+    x = slot * sh.share;
+    share_end = min(sh.total - x, sh.share) + x;
+    sq.seq = sh.seq;
+    base = sh.base;
+    su = seq_units(a, sq.seq, R);
+  } else {
+    if (a.mode == kSeqHeaviest) sq = seq_ranked<PAGED>(a, slot, R);
+    else sq = seq_tile(a, a.slots - 1 - slot, R);
+    if (sq.tile < 0 || sq.tile * R >= sq.count * G) return;
   }
 
   // Copy sources: lane l of copy c of a group fetches row c RPC + l / CH of the group into the next 16 bytes of
@@ -233,6 +360,71 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   const T* const kh = static_cast<const T*>(a.k) + hkv * a.k_head;
   const T* const vh = static_cast<const T*>(a.v) + hkv * a.v_head;
 
+  if (hd < HD) {
+    for (int e = tid; e < 4 * KW * TILE / 8; e += 64 * RW * KW)
+      reinterpret_cast<u32x4*>(seq_lds)[e] = u32x4{0u, 0u, 0u, 0u};
+    __syncthreads();
+  }
+
+  const float c2 = a.scale_log2, lazy = kSeqLazy / a.scale_log2;
+  // LDS addresses of this lane's pieces of the first K and V block of a stage; the others lie at constant distances.
+  // (The empty asm keeps each in one register: the compiler would spread the sums over many.)
+  uint32_t kread[KSTEPS], vread[DB];
+#pragma unroll
+  for (int kk = 0; kk < KSTEPS; ++kk) {
+    kread[kk] = lds_address(sk + col * HD + kswz<HD>(col, 2 * kk + hf) * 8);
+    asm volatile("" : "+v"(kread[kk]));
+  }
+  const int vrow = 4 * hf + ((lane >> 2) & 3);
+#pragma unroll
+  for (int i = 0; i < DB; ++i) {
+    const int c = vseg<HD>(vrow, 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1));
+    vread[i] = lds_address(sv + vrow * HD + c * 8 + 4 * (lane & 1));
+    asm volatile("" : "+v"(vread[i]));
+  }
+  for (;;) {
+  // (What follows from these is worked out again for each tile instead of being held in registers throughout.)
+  asm volatile("" : "+v"(lane), "+v"(hf), "+v"(col));
+  int keys, kbeg = 0, kend = INT32_MAX, part = -1;
+  if (shares) {
+    while (x >= base + su.tiles * su.units) {  // the next sequence that has rows
+      if (sq.seq + 1 >= a.batch) return;
+      base += su.tiles * su.units;
+      su = seq_units(a, ++sq.seq, R);
+    }
+    sq.first = su.first;
+    sq.count = su.count;
+    sq.tile = (x - base) / su.units;
+    keys = su.keys;
+    const int begin = x - base - sq.tile * su.units, end = min(begin + share_end - x, su.units);
+    kbeg = begin * kSeqUnit;
+    if (end < su.units) kend = end * kSeqUnit;
+    if (end - begin < su.units) part = 2 * slot + (begin == 0 ? 1 : 0);
+    x += end - begin;
+  } else {
+    keys = seq_keys<PAGED>(a, sq.seq, sq.count);
+  }
+  const int rows = sq.count * G;
+  const int r0 = sq.tile * R;
+  const int block_end = seq_limit(a, min(r0 + R - 1, rows - 1) / G, sq.count, keys);
+  kend = min(kend, block_end);
+  const int ntiles = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
+
+  // Rows of this wave; those behind the last repeat it and are not stored, so limits rise along the rows.
+  const int wr0 = r0 + rw * WR;
+  const bool wave_active = wr0 < rows;
+  const int block_lo = seq_limit(a, r0 / G, sq.count, keys);  // the first row's
+  const int lim_lo = seq_limit(a, min(wr0, rows - 1) / G, sq.count, keys);
+  const int lim_hi = min(seq_limit(a, min(wr0 + WR - 1, rows - 1) / G, sq.count, keys), kend);
+  int tok[CB], head[CB], lim[CB];
+#pragma unroll
+  for (int b = 0; b < CB; ++b) {
+    const int r = min(wr0 + 32 * b + col, rows - 1);
+    tok[b] = r / G;
+    head[b] = hkv * G + r - tok[b] * G;
+    lim[b] = seq_limit(a, tok[b], sq.count, keys);
+  }
+
   // Paged: lane l holds the page of the 16-key group l behind key t0 (of the first 8).
   auto tile_pages = [&](int t0) TT_INLINE -> int {
     const int key = min(t0 + 16 * (lane & 7), max(keys - 1, 0));
@@ -242,44 +434,71 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   auto bad_groups = [&](int pe, int t0) TT_INLINE -> uint32_t {
     return (uint32_t)__ballot((uint32_t)pe >= (uint32_t)a.pages && t0 + 16 * lane < keys) & 0xffu;
   };
-  auto issue_half = [&](const T* h, int64_t page_stride, int64_t row_stride, const uint32_t (&off)[CPG], T* tile, int t0,
-                        int pe, int pe_lane) TT_INLINE {
+  // Where those groups lie in K and V (bytes), and how many bytes there belong to keys; worked out by the lanes for
+  // pages, whose numbers they hold, and by the scalar unit otherwise.
+  struct Places {
+    uint64_t k, v;
+    uint32_t k_bytes, v_bytes;
+  };
+  auto place = [&](int t, int pe) TT_INLINE -> Places {
+    const int n = min(max(keys - t, 0), 16);
+    Places p;
+    if constexpr (PAGED) {
+      const uint32_t page = (uint32_t)pe < (uint32_t)a.pages ? pe : 0, in = t & ((1 << a.page_shift) - 1);
+      p.k = 2 * (page * (uint64_t)a.k_page + in * (uint64_t)a.k_row);
+      p.v = 2 * (page * (uint64_t)a.v_page + in * (uint64_t)a.v_row);
+    } else {
+      const uint32_t row = sq.first + min(t, keys - 1);
+      p.k = 2 * (row * (uint64_t)a.k_row);
+      p.v = 2 * (row * (uint64_t)a.v_row);
+    }
+    p.k_bytes = n == 0 ? 0 : 2 * ((n - 1) * (uint32_t)a.k_row + hd);
+    p.v_bytes = n == 0 ? 0 : 2 * ((n - 1) * (uint32_t)a.v_row + hd);
+    return p;
+  };
+  auto places = [&](int pe, int t0) TT_INLINE -> Places {
+    if constexpr (PAGED) return place(t0 + 16 * (lane & 7), pe);
+    else return Places{(uint64_t)t0, 0, 0, 0};
+  };
+  // Copies of this wave's rows of a K (V) tile whose first 16 keys are group `group` of `at`.
+  auto issue_half = [&](bool is_k, const Places& at, T* tile, int group) TT_INLINE {
 #pragma unroll
     for (int p = 0; p < PG; ++p) {
-      const int g0 = rw * WROWS + p * 16;
-      const int t = t0 + g0;
-      const int n = t < kbeg ? 0 : min(max(keys - t, 0), 16);
-      const T* src;
+      const int g = rw * PG + p;
+      if (group + g < 0) continue;
+      uint64_t where;
+      uint32_t bytes;
       if constexpr (PAGED) {
-        const int e = __builtin_amdgcn_readlane(pe, max(pe_lane + g0 / 16, 0));
-        const int page = (uint32_t)e < (uint32_t)a.pages ? e : 0;
-        src = h + page * page_stride + (t & ((1 << a.page_shift) - 1)) * row_stride;
+        const uint64_t w = is_k ? at.k : at.v;
+        where = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), group + g) << 32 |
+                (uint32_t)__builtin_amdgcn_readlane((int)w, group + g);
+        bytes = __builtin_amdgcn_readlane((int)(is_k ? at.k_bytes : at.v_bytes), group + g);
       } else {
-        src = h + (int64_t)(sq.first + max(min(t, keys - 1), 0)) * row_stride;
+        const Places q = place((int)at.k + 16 * (group + g), 0);
+        where = is_k ? q.k : q.v;
+        bytes = is_k ? q.k_bytes : q.v_bytes;
       }
-      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(src, n == 0 ? 0 : (uint32_t)((n - 1) * (int)row_stride + hd) * 2);
+      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(reinterpret_cast<const char*>(is_k ? kh : vh) + where, bytes);
 #pragma unroll
       for (int c = 0; c < CPG; ++c)
-        lds_copy16_buf(r, off[c], reinterpret_cast<half*>(tile + (g0 + c * RPC) * HD));
+        lds_copy16_buf(r, is_k ? koff[c] : voff[c], reinterpret_cast<half*>(tile + (g * 16 + c * RPC) * HD));
     }
   };
-  // The K tile staged with a V tile from key t0 begins KLEAD keys later: the scores run that far ahead.
+  // The K tile staged with a V tile begins KLEAD keys later: the scores run that far ahead.
   constexpr int KLEAD = PIPE ? 32 : 0;
-  auto issue_k = [&](int t0, int st, int pe) TT_INLINE {
-    issue_half(kh, a.k_page, a.k_row, koff, sk + st * TILE, t0 + KLEAD, pe, KLEAD / 16);
+  auto issue_k = [&](const Places& p, int st) TT_INLINE {
+    issue_half(true, p, sk + st * TILE, KLEAD / 16);
   };
-  auto issue_v = [&](int t0, int st, int pe) TT_INLINE {
-    issue_half(vh, a.v_page, a.v_row, voff, sv + st * TILE, t0, pe, 0);
+  auto issue_v = [&](const Places& p, int st) TT_INLINE {
+    issue_half(false, p, sv + st * TILE, 0);
   };
-  // This wave's copies have landed, and the waves of the block meet.  Before that, V rows of keys behind the last are
-  // cleared (0 times whatever lay there would not be 0), and where some rows of the block see keys that others do
-  // not, infinities and NaN are taken out of V: 0 times those would reach the rows that do not see them.  Such values
-  // are added to the rows that do see them at the end (restore_odd).
+  // After the copies of this wave's V rows have landed: rows of keys behind the last are cleared (0 times whatever lay
+  // there would not be 0), and where some rows of the block see keys that others do not, infinities and NaN are taken
+  // out of V: 0 times those would reach the rows that do not see them.  Such values are added to the rows that do see
+  // them at the end (restore_odd).
   const bool mixed = block_lo < block_end;
   bool odd = false;
-  auto land_v = [&](int t0, int st) TT_INLINE {
-    __builtin_amdgcn_s_waitcnt(0);
-    asm volatile("" ::: "memory");
+  auto settle_v = [&](int t0, int st) TT_INLINE {
     const int g0 = rw * WROWS;
     u32x4* const tile = reinterpret_cast<u32x4*>(sv + st * TILE + g0 * HD);
     const int n = min(max(keys - (t0 + g0), 0), WROWS);
@@ -302,55 +521,48 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     }
     if (n < WROWS)
       for (int e = n * CH + lane; e < WROWS * CH; e += 64) tile[e] = u32x4{0u, 0u, 0u, 0u};
-    __builtin_amdgcn_s_waitcnt(0xC07F);
+    lds_done();
+  };
+  auto land_v = [&](int t0, int st) TT_INLINE {
+    __builtin_amdgcn_s_waitcnt(0);
     asm volatile("" ::: "memory");
+    settle_v(t0, st);
     if constexpr (RW > 1) raw_barrier();
   };
 
-  if (hd < HD) {
-    for (int e = tid; e < 4 * KW * TILE / 8; e += 64 * RW * KW)
-      reinterpret_cast<u32x4*>(seq_lds)[e] = u32x4{0u, 0u, 0u, 0u};
-    __syncthreads();
-  }
-
-  v8 qf[CB][KSTEPS];
-#pragma unroll
-  for (int b = 0; b < CB; ++b) {
-    const T* qp = static_cast<const T*>(a.q) + (int64_t)(sq.first + tok[b]) * a.q_row + head[b] * a.q_head;
-#pragma unroll
-    for (int kk = 0; kk < KSTEPS; ++kk) {
-      if (16 * kk + 8 * hf < hd) qf[b][kk] = *reinterpret_cast<const v8*>(qp + 16 * kk + 8 * hf);
-      else qf[b][kk] = __builtin_bit_cast(v8, u32x4{0u, 0u, 0u, 0u});
-    }
-  }
-
-  const float c2 = a.scale_log2, lazy = kSeqLazy / a.scale_log2;
-  // LDS addresses of this lane's pieces of the first K and V block of a stage; the others lie at constant distances.
-  // (The empty asm keeps each in one register: the compiler would spread the sums over many.)
-  uint32_t kread[KSTEPS], vread[DB];
-#pragma unroll
-  for (int kk = 0; kk < KSTEPS; ++kk) {
-    kread[kk] = lds_address(sk + col * HD + kswz<HD>(col, 2 * kk + hf) * 8);
-    asm volatile("" : "+v"(kread[kk]));
-  }
-  const int vrow = 4 * hf + ((lane >> 2) & 3);
-#pragma unroll
-  for (int i = 0; i < DB; ++i) {
-    const int c = vseg<HD>(vrow, 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1));
-    vread[i] = lds_address(sv + vrow * HD + c * 8 + 4 * (lane & 1));
-    asm volatile("" : "+v"(vread[i]));
-  }
   floatx16 o[CB][DB];
   float m_ref[CB], l_run[CB], mc[CB], thr[CB];
 
+  // Asked for after the first copies, which need addresses of their own first.
+  v8 qf[CB][KSTEPS];
+  auto load_q = [&]() TT_INLINE {
+#pragma unroll
+    for (int b = 0; b < CB; ++b) {
+      const T* qp = static_cast<const T*>(a.q) + (int64_t)(sq.first + tok[b]) * a.q_row + head[b] * a.q_head;
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk) {
+        if (16 * kk + 8 * hf < hd) qf[b][kk] = *reinterpret_cast<const v8*>(qp + 16 * kk + 8 * hf);
+        else qf[b][kk] = __builtin_bit_cast(v8, u32x4{0u, 0u, 0u, 0u});
+      }
+    }
+  };
   using Scores = floatx16[CB][SB];
   using Probs = v8[CB][SB][2];
+  auto read_k = [&](int kk, int st, int kb) TT_INLINE -> v8 {  // 32 keys, features 16 kk + 8 hf + {0..7}
+    return *(const __attribute__((address_space(3))) v8*)(kread[kk] + 2 * (st * TILE + kb * 32 * HD));
+  };
+  auto read_v = [&](int i, int st, int kc) TT_INLINE -> v8 {
+    // features 32 i + l % 32; keys 16 kc + 4 hf + {0..3} and 8 further: the order of the lane's probabilities
+    const uint32_t at = vread[i] + 2 * (st * TILE + kc * 16 * HD);
+    const shortx4 x0 = read_tr16((const lds_short*)at), x1 = read_tr16((const lds_short*)(at + 16 * HD));
+    return __builtin_bit_cast(v8, shortx8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]});
+  };
   auto scores = [&](Scores& s, int st, int kb0) TT_INLINE {
 #pragma unroll
     for (int kb = 0; kb < SB; ++kb)
 #pragma unroll
       for (int kk = 0; kk < KSTEPS; ++kk) {
-        const v8 x = *(const __attribute__((address_space(3))) v8*)(kread[kk] + 2 * (st * TILE + (kb0 + kb) * 32 * HD));
+        const v8 x = read_k(kk, st, kb0 + kb);
 #pragma unroll
         for (int b = 0; b < CB; ++b) {
           if (kk == 0) {
@@ -444,13 +656,9 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int i = 0; i < DB; ++i) {
-          // keys 32 kb + 16 c + 4 hf + {0..3} and 8 further: the order of the lane's probabilities
-          const uint32_t at = vread[i] + 2 * (st * TILE + (32 * (kb0 + kb) + 16 * c) * HD);
-          const shortx4 x0 = read_tr16((const lds_short*)at);
-          const shortx4 x1 = read_tr16((const lds_short*)(at + 16 * HD));
-          const shortx8 x = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+          const v8 x = read_v(i, st, 2 * (kb0 + kb) + c);
 #pragma unroll
-          for (int b = 0; b < CB; ++b) o[b][i] = Num<T>::mfma(__builtin_bit_cast(v8, x), p16[b][kb][c], o[b][i]);
+          for (int b = 0; b < CB; ++b) o[b][i] = Num<T>::mfma(x, p16[b][kb][c], o[b][i]);
         }
   };
   {
@@ -466,11 +674,6 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       thr[b] = -INFINITY;    // a tile maximum above this moves m_ref
     }
 
-    // Tiles of this wave's group, and those of them that its rows see.
-    [[maybe_unused]] const int rounds = RW == 1 ? (ntiles - grp + KW - 1) / KW : (ntiles + KW - 1) / KW;
-    const int tiles_w = wave_active && lim_hi > kbeg ? (lim_hi - kbeg + KT - 1) / KT : 0;
-    [[maybe_unused]] const int rounds_w = (tiles_w - grp + KW - 1) / KW;
-    [[maybe_unused]] const int t_first = kbeg + grp * KT;  // first key of the group's first tile
     if constexpr (PIPE) {
       static_assert(KW == 1 && KT == 64, "two steps of 32 keys per tile");
       const int steps = wave_active && lim_hi > kbeg ? (lim_hi - kbeg + 31) / 32 : 0;  // of this wave
@@ -482,11 +685,13 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           pe = tile_pages(kbeg);
           pe_next = tile_pages(kbeg + KT);
         }
+        const Places at = places(pe, kbeg);
         // the first 32 keys go where the second half of a K tile before the first would lie
-        issue_half(kh, a.k_page, a.k_row, koff, sk + TILE, kbeg - 32, pe, -2);
-        issue_k(kbeg, 0, pe);
-        issue_v(kbeg, 0, pe);
+        issue_half(true, at, sk + TILE, -2);
+        issue_k(at, 0);
+        issue_v(at, 0);
       }
+      load_q();
       land_v(kbeg, 0);
       if (steps > 0) {
         scores(sa, 1, 1);
@@ -494,6 +699,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         row_max(sa, mt);
         move_max(mt);
       }
+      lds_done();
+      raw_barrier();  // the second tile's copies go where those first 32 keys lie
       // A step of 32 keys: the exps of its scores s run beside the products of the next 32 keys, and its P V beside
       // their maximum.
       auto step = [&](int t0, int st, int h, uint32_t bad, Scores& s, Scores& sn) TT_INLINE {
@@ -525,8 +732,9 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         if (r + 1 >= ntiles) return;
         pe = pe_next;
         if constexpr (PAGED) pe_next = tile_pages(t0 + 2 * KT);
-        issue_k(t0 + KT, st ^ 1, pe);
-        issue_v(t0 + KT, st ^ 1, pe);
+        const Places at = places(pe, t0 + KT);
+        issue_k(at, st ^ 1);
+        issue_v(at, st ^ 1);
       };
       auto whole_tile = [&](int r, int st) TT_INLINE {
         const int t0 = kbeg + r * KT;
@@ -535,15 +743,20 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         step(t0, st, 1, bad, sb, sa);
         land_v(t0 + KT, st ^ 1);
       };
-      // Tiles both of whose steps have a next one, two per pass so that their stages are constants; then this wave's
-      // last tile; then those that only other waves of the block need.
+      // Tiles both of whose steps have a next one, up to head_dim 128 two per pass so that their stages are constants
+      // (beyond, the code would not fit the instruction cache); then this wave's last tile; then those that only
+      // other waves of the block need.
       const int whole = max(steps - 1, 0) / 2;
       int r = 0;
-      for (; r + 1 < whole; r += 2) {
-        whole_tile(r, 0);
-        whole_tile(r + 1, 1);
+      if constexpr (HD <= 128) {
+        for (; r + 1 < whole; r += 2) {
+          whole_tile(r, 0);
+          whole_tile(r + 1, 1);
+        }
+        if (r < whole) whole_tile(r++, 0);
+      } else {
+        for (; r < whole; ++r) whole_tile(r, r & 1);
       }
-      if (r < whole) whole_tile(r++, 0);
       if (r < ntiles) {
         const int t0 = kbeg + r * KT;
         const int st = r & 1;
@@ -560,48 +773,83 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         }
       }
     } else {
-      int pe = 0, pe_next = 0;
-      if (grp < ntiles) {
+      // Tiles grp, grp + KW, ... by this wave alone.  The tile after the next is asked for as soon as this one's
+      // fragments are in registers, so that close to two tiles are in flight all the time.
+      static_assert(RW == 1 && CB == 1 && SB == 1, "a wave's own tiles of 32 keys");
+      constexpr int COPIES = 2 * PG * CPG;  // of a tile
+      const int rounds = (ntiles - grp + KW - 1) / KW;
+      const int t_first = kbeg + grp * KT;
+      int pe0 = 0, pe1 = 0, pe2 = 0;  // pages of this tile, the next and the one after it
+      if (rounds > 0) {
         if constexpr (PAGED) {
-          pe = tile_pages(t_first);
-          pe_next = tile_pages(t_first + KW * KT);
+          pe0 = tile_pages(t_first);
+          pe1 = tile_pages(t_first + KW * KT);
+          pe2 = tile_pages(t_first + 2 * KW * KT);
         }
-        issue_k(t_first, 0, pe);
-        issue_v(t_first, 0, pe);
+        const Places at = places(pe0, t_first);
+        issue_k(at, 0);
+        issue_v(at, 0);
+        if (rounds > 1) {
+          const Places next = places(pe1, t_first + KW * KT);
+          issue_k(next, 1);
+          issue_v(next, 1);
+        }
       }
-      land_v(t_first, 0);
+      load_q();
       for (int r = 0; r < rounds; ++r) {
-        const int t = r * KW + grp;
-        const int t0 = kbeg + t * KT;
+        const int t0 = t_first + r * KW * KT;
         const int st = r & 1;
-        const uint32_t bad = PAGED ? bad_groups(pe, t0) : 0;
-        if (t + KW < ntiles) {
-          pe = pe_next;
-          if constexpr (PAGED) pe_next = tile_pages(t0 + 2 * KW * KT);
-          issue_k(t0 + KW * KT, st ^ 1, pe);
-          issue_v(t0 + KW * KT, st ^ 1, pe);
+        // All but the next tile's copies, which were the last to be issued, have landed.
+        if (r + 1 < rounds) wait_vmcnt<COPIES>();
+        else wait_vmcnt<0>();
+        asm volatile("" ::: "memory");
+        settle_v(t0, st);
+        // A wave has its SIMD to itself: all fragments are read before the first product, and only the first waits.
+        v8 kf[KSTEPS], vf[2][DB];
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) kf[kk] = read_k(kk, st, 0);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < DB; ++i) vf[c][i] = read_v(i, st, c);
+        __builtin_amdgcn_sched_barrier(0);
+        Scores s;
+        Probs p16;
+        float mt[CB];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[0][0][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) s[0][0] = Num<T>::mfma(kf[kk], qf[0][kk], s[0][0]);
+        const uint32_t bad = PAGED ? bad_groups(pe0, t0) : 0;
+        const int pn = pe2;
+        if constexpr (PAGED) {
+          pe0 = pe1;
+          pe1 = pe2;
+          pe2 = tile_pages(t0 + 3 * KW * KT);
         }
-        if (r < rounds_w) {
-          Scores s;
-          Probs p16;
-          float mt[CB];
-          scores(s, st, 0);
-          mask_scores(s, t0, bad);
-          row_max(s, mt);
-          move_max(mt);
-          probabilities(s, p16);
-          add_sums(p16);
-          add_values(p16, st, 0);
+        if (r + 2 < rounds) {
+          lds_done();
+          const Places at = places(pn, t0 + 2 * KW * KT);
+          issue_k(at, st);
+          issue_v(at, st);
         }
-        if (r + 1 < rounds) land_v(t0 + KW * KT, st ^ 1);
+        mask_scores(s, t0, bad);
+        row_max(s, mt);
+        move_max(mt);
+        probabilities(s, p16);
+        add_sums(p16);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < DB; ++i) o[0][i] = Num<T>::mfma(vf[c][i], p16[0][0][c], o[0][i]);
       }
     }
   }
-  if (RW * KW > 1 && mixed) odd = __syncthreads_or(odd);
+  if (RW * KW > 1 && mixed) odd = __syncthreads_or(odd) != 0;
 
   if constexpr (KW > 1) {
     static_assert(CB == 1, "groups of waves hold one block of rows");
-    // [group - 1][wave of the group][value][lane]: O, the maximum in log2 units and this lane's half of the sum
+    // [group - 1][wave of the group][value][lane]: O, the maximum and this lane's half of the sum
     constexpr int NV = DB * 16 + 2;
     float* const mrg = reinterpret_cast<float*>(seq_lds);
     __syncthreads();
@@ -615,80 +863,90 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       p[(NV - 1) * 64] = l_run[0];
     }
     __syncthreads();
-    if (grp > 0) return;
+    if (grp == 0) {
 #pragma unroll 1
-    for (int g = 0; g < KW - 1; ++g) {
-      const float* p = mrg + (size_t)(g * RW + rw) * NV * 64 + lane;
-      const float m_g = p[(NV - 2) * 64], l_g = p[(NV - 1) * 64];
-      const float m_new = fmaxf(m_ref[0], m_g);
-      // a part without a maximum saw no key (its sum, 0, is then its weight) or only NaN (NaN is)
-      const float c0 = m_ref[0] == -INFINITY ? l_run[0] : __builtin_amdgcn_exp2f((m_ref[0] - m_new) * c2);
-      const float c1 = m_g == -INFINITY ? l_g : __builtin_amdgcn_exp2f((m_g - m_new) * c2);
-      l_run[0] = l_run[0] * c0 + l_g * c1;
-      m_ref[0] = m_new;
+      for (int g = 0; g < KW - 1; ++g) {
+        const float* p = mrg + (size_t)(g * RW + rw) * NV * 64 + lane;
+        const float m_g = p[(NV - 2) * 64], l_g = p[(NV - 1) * 64];
+        const float m_new = fmaxf(m_ref[0], m_g);
+        // a part without a maximum saw no key (its sum, 0, is then its weight) or only NaN (NaN is)
+        const float c0 = m_ref[0] == -INFINITY ? l_run[0] : __builtin_amdgcn_exp2f((m_ref[0] - m_new) * c2);
+        const float c1 = m_g == -INFINITY ? l_g : __builtin_amdgcn_exp2f((m_g - m_new) * c2);
+        l_run[0] = l_run[0] * c0 + l_g * c1;
+        m_ref[0] = m_new;
 #pragma unroll
-      for (int i = 0; i < DB; ++i)
+        for (int i = 0; i < DB; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[0][i][e] = o[0][i][e] * c0 + p[(i * 16 + e) * 64] * c1;
+          for (int e = 0; e < 16; ++e) o[0][i][e] = o[0][i][e] * c0 + p[(i * 16 + e) * 64] * c1;
+      }
     }
   }
 
+  // Output rows, or a part's sums: O in units of exp2(m - 7), the maximum in log2 units, the sum.
+  const int64_t part0 = ((int64_t)part * a.kv_heads + hkv) * R - r0;  // + row
+  if (grp == 0) {
 #pragma unroll
-  for (int b = 0; b < CB; ++b) {
-    const float l = xhalf_sum(l_run[b]);
-    if (wr0 + 32 * b + col >= rows) continue;
-    const int64_t orow = (int64_t)(sq.first + tok[b]) * a.heads + head[b];
-    if (lim[b] > a.chunk) {  // this row's keys lie in several parts
-      float* dst = a.part_o + ((int64_t)split * a.tokens * a.heads + orow) * hd;
+    for (int b = 0; b < CB; ++b) {
+      const float l = xhalf_sum(l_run[b]);
+      const int r = wr0 + 32 * b + col;
+      if (r >= rows) continue;
+      if (part >= 0) {
+        float* dst = a.part_o + (part0 + r) * hd;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if (32 * i + 8 * g < hd)
+              *reinterpret_cast<floatx4*>(dst + 32 * i + 8 * g + 4 * hf) =
+                  floatx4{o[b][i][4 * g], o[b][i][4 * g + 1], o[b][i][4 * g + 2], o[b][i][4 * g + 3]};
+        if (hf == 0) a.part_ml[part0 + r] = make_float2(m_ref[b] * c2, l);
+        continue;
+      }
+      const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key: zeros
+      T* dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + tok[b]) * a.heads + head[b]) * hd;
 #pragma unroll
       for (int i = 0; i < DB; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          if (32 * i + 8 * g < hd)
-            *reinterpret_cast<floatx4*>(dst + 32 * i + 8 * g + 4 * hf) =
-                floatx4{o[b][i][4 * g], o[b][i][4 * g + 1], o[b][i][4 * g + 2], o[b][i][4 * g + 3]};
-      if (hf == 0) a.part_ml[(int64_t)split * a.tokens * a.heads + orow] = make_float2(m_ref[b] * c2, l);
-      continue;
+          if (32 * i + 8 * g < hd) {
+            typedef T v4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<v4*>(dst + 32 * i + 8 * g + 4 * hf) =
+                v4{(T)(o[b][i][4 * g] * inv), (T)(o[b][i][4 * g + 1] * inv), (T)(o[b][i][4 * g + 2] * inv),
+                   (T)(o[b][i][4 * g + 3] * inv)};
+          }
     }
-    if (split > 0) continue;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key: zeros
-    T* dst = static_cast<T*>(a.out) + orow * hd;
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (32 * i + 8 * g < hd) {
-          typedef T v4 __attribute__((ext_vector_type(4)));
-          *reinterpret_cast<v4*>(dst + 32 * i + 8 * g + 4 * hf) =
-              v4{(T)(o[b][i][4 * g] * inv), (T)(o[b][i][4 * g + 1] * inv), (T)(o[b][i][4 * g + 2] * inv),
-                 (T)(o[b][i][4 * g + 3] * inv)};
+    if (mixed && __builtin_amdgcn_ballot_w64(odd) != 0) {
+      // restore_odd: the wave adds the infinities and NaN of V that were taken out to those of its rows that see them.
+      __threadfence_block();
+      const int from = kbeg + max(block_lo - kbeg, 0) / KT * KT;
+      for (int key = from; key < lim_hi; ++key) {
+        const T* vp = vh;
+        if constexpr (PAGED) {
+          const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
+          if ((uint32_t)page >= (uint32_t)a.pages) continue;
+          vp += page * a.v_page + (key & ((1 << a.page_shift) - 1)) * a.v_row;
+        } else {
+          vp += (int64_t)(sq.first + key) * a.v_row;
         }
-  }
-
-  if (!mixed || __builtin_amdgcn_ballot_w64(odd) == 0) return;
-  // restore_odd: a wave adds the infinities and NaN of V that were taken out to those of its rows that see them.
-  __threadfence_block();
-  const int from = kbeg + max(block_lo - kbeg, 0) / KT * KT;
-  for (int key = from; key < lim_hi; ++key) {
-    const T* vp = vh;
-    if constexpr (PAGED) {
-      const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
-      if ((uint32_t)page >= (uint32_t)a.pages) continue;
-      vp += page * a.v_page + (key & ((1 << a.page_shift) - 1)) * a.v_row;
-    } else {
-      vp += (int64_t)(sq.first + key) * a.v_row;
-    }
-    for (int d = lane; d < hd; d += 64) {
-      const T x = vp[d];
-      if ((__builtin_bit_cast(uint16_t, x) & Num<T>::kExp) != Num<T>::kExp) continue;
-      for (int r = wr0; r < min(wr0 + WR, rows); ++r) {
-        const int token = r / G, seen = seq_limit(a, token, sq.count, keys);
-        if (key >= seen || (split > 0 && seen <= a.chunk)) continue;
-        const int64_t orow = (int64_t)(sq.first + token) * a.heads + hkv * G + r - token * G;
-        if (seen > a.chunk) a.part_o[((int64_t)split * a.tokens * a.heads + orow) * hd + d] += (float)x;
-        else static_cast<T*>(a.out)[orow * hd + d] = (T)((float)static_cast<T*>(a.out)[orow * hd + d] + (float)x);
+        for (int d = lane; d < hd; d += 64) {
+          const T y = vp[d];
+          if ((__builtin_bit_cast(uint16_t, y) & Num<T>::kExp) != Num<T>::kExp) continue;
+          for (int r = wr0; r < min(wr0 + WR, rows); ++r) {
+            const int token = r / G;
+            if (key >= seq_limit(a, token, sq.count, keys)) continue;
+            if (part >= 0) {
+              a.part_o[(part0 + r) * hd + d] += (float)y;
+            } else {
+              T* const dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + token) * a.heads + hkv * G + r - token * G) * hd + d;
+              *dst = (T)((float)*dst + (float)y);
+            }
+          }
+        }
       }
     }
+  }
+  if (!shares || x >= share_end) return;
+  __syncthreads();  // the next tile's copies go where this one's may still be read
   }
 }
 

@@ -1,5 +1,5 @@
-// seq_attention_kernel for head_dim above 128: 128 accumulator floats per lane, which are left in AGPRs here (this
-// file is built without the VGPR-form MFMA flag).
+// seq_attention_kernel for head_dim above 128 (one wave per SIMD; of its 512 registers the compiler keeps 128
+// accumulator floats per lane in AGPRs).
 #include "seq_launch.hpp"
 
 namespace tt {

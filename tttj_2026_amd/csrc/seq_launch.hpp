@@ -21,7 +21,7 @@ int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
                                hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int64_t blocks = (int64_t)a.slots * a.kv_heads * a.splits;
+  const int64_t blocks = (int64_t)a.slots * a.kv_heads;
   constexpr int threads = 64 * RW * KW;
   TT_REQUIRE(blocks * threads < (1LL << 32), "attention: %lld blocks are more than one launch takes",
              (long long)blocks);
@@ -33,7 +33,7 @@ int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
 template <int HD, typename T>
 int launch_seq_type(const SeqAttnArgs& a, bool paged, bool narrow, hipStream_t stream) {
   if (!paged) return launch_seq<T, HD, 1, 4, 1, 64, false>(a, stream);
-  if (narrow) return launch_seq<T, HD, 1, 1, (HD <= 128 ? 4 : 2), 32, true>(a, stream);
+  if (narrow) return launch_seq<T, HD, 1, 1, (HD <= 128 ? 2 : 1), 32, true>(a, stream);
   return launch_seq<T, HD, 1, 4, 1, 64, true>(a, stream);
 }
 

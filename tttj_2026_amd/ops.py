@@ -314,7 +314,8 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     batch = lengths.shape[0]
     held = table.shape[1] * page
     max_length = held if max_length is None else min(int(max_length), held)
-    nbytes = _lib.cache_attention_workspace_bytes(tokens, batch, heads, kv_heads, hd, max_length, starts is None)
+    nbytes = _lib.cache_attention_workspace_bytes(tokens, batch, heads, kv_heads, hd, page, table.shape[1], max_length,
+                                                  starts is None)
     work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     with _on_device(q):
         rc = _lib.load().tt_cache_attention_fwd(
