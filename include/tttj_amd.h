@@ -246,6 +246,9 @@ int tt_attention_fwd_prescaled(const void* q, const void* k, const void* vt, con
 #define TT_FP16 0
 #define TT_BF16 1
 
+/* The calls below take their many arguments in a structure, whose `size` is sizeof the structure
+ * (checked, so that a caller built for another layout is refused). */
+
 /* Attention of whole sequences packed one behind the other, without padding: q rows
  * [tokens, heads, head_dim], k and v rows [tokens, kv_heads, head_dim] -> out [tokens, heads * head_dim]
  * (contiguous).  starts [batch + 1] (device, int32, rising) holds the first row of each sequence and
@@ -256,47 +259,59 @@ int tt_attention_fwd_prescaled(const void* q, const void* k, const void* vt, con
  * are not written.  Values of `starts` outside [0, tokens] are taken as the nearest in it.  No
  * counterpart in the reference, whose attention takes padded batches with as many key heads as query
  * heads (kernels/case8_attention.py:48-206). */
-int tt_packed_attention_fwd(const void* q, const void* k, const void* v, const int32_t* starts,
-                            void* out, int tokens, int batch, int heads, int kv_heads, int head_dim,
-                            int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
-                            int64_t v_row, int64_t v_head, float scale, int causal, int dtype,
-                            void* stream);
+typedef struct {
+  int64_t size;
+  const void *q, *k, *v;
+  const int32_t* starts;
+  void* out;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  int32_t tokens, batch, heads, kv_heads, head_dim, causal, dtype;
+  float scale;
+} tt_packed_attention;
+int tt_packed_attention_fwd(const tt_packed_attention* args, void* stream);
 
-/* Write the keys and values of new tokens (rows as in tt_packed_attention_fwd, 16-bit elements of
- * either type) into a paged cache: halves k_cache and v_cache of `pages` pages of `page_size` (a power
- * of two from 16 on) tokens of kv_heads heads, with page, token and head strides in elements (`kc_*`,
- * `vc_*`; aligned to 16 bytes).  Position t of sequence b lies in page table[b * table_row +
- * t / page_size] at t % page_size; lengths [batch] counts the keys of each sequence with the new ones,
- * so that the n rows of sequence b take positions lengths[b] - n ... lengths[b] - 1.  starts as above,
- * or NULL: row b is the one new token of sequence b (tokens == batch).  A token whose position is
- * negative or past table_pages pages, or whose page number is not in [0, pages), is not written.  No
- * counterpart in the reference, which keeps no keys between calls. */
-int tt_cache_append(const void* k, const void* v, void* k_cache, void* v_cache,
-                    const int32_t* table, const int32_t* lengths, const int32_t* starts, int tokens,
-                    int batch, int kv_heads, int head_dim, int pages, int page_size,
-                    int table_pages, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
-                    int64_t kc_page, int64_t kc_row, int64_t kc_head, int64_t vc_page,
-                    int64_t vc_row, int64_t vc_head, int64_t table_row, void* stream);
+/* Write the keys and values of new tokens (rows as above, 16-bit elements of either type) into a paged
+ * cache: halves k_cache and v_cache of `pages` pages of `page_size` (a power of two from 16 on) tokens
+ * of kv_heads heads, with page, token and head strides in elements (`kc_*`, `vc_*`; aligned to 16
+ * bytes).  Position t of sequence b lies in page table[b * table_row + t / page_size] at t % page_size;
+ * lengths [batch] counts the keys of each sequence with the new ones, so that the n rows of sequence b
+ * take positions lengths[b] - n ... lengths[b] - 1.  starts as above, or NULL: row b is the one new
+ * token of sequence b (tokens == batch).  A token whose position is negative or past table_pages
+ * pages, or whose page number is not in [0, pages), is not written.  No counterpart in the reference,
+ * which keeps no keys between calls. */
+typedef struct {
+  int64_t size;
+  const void *k, *v;
+  void *k_cache, *v_cache;
+  const int32_t *table, *lengths, *starts;
+  int64_t k_row, k_head, v_row, v_head, kc_page, kc_row, kc_head, vc_page, vc_row, vc_head, table_row;
+  int32_t tokens, batch, kv_heads, head_dim, pages, page_size, table_pages, reserved;
+} tt_cache_rows;
+int tt_cache_append(const tt_cache_rows* args, void* stream);
 
 /* Attention of new tokens over such a cache, which holds their own keys already: token i of the n new
  * ones of sequence b sees the keys at positions 0 ... lengths[b] - n + i (none: its row is +0.0).
- * max_length is the longest length the caller expects; it decides how keys are split over blocks, and
- * a longer sequence costs time only.  Lengths beyond table_pages pages are cut to them.  Keys in a page
- * whose number is not in [0, pages) are not read and count as NaN.  `workspace` (aligned to 16 bytes,
- * any contents, used by this call alone until it is done) has the bytes that
+ * max_length is the longest length the caller expects; it decides how the work is split, and a longer
+ * sequence costs time only.  Lengths beyond table_pages pages are cut to them.  Keys in a page whose
+ * number is not in [0, pages) are not read and count as NaN.  `workspace` (aligned to 16 bytes, any
+ * contents, used by this call alone until it is done) has the bytes that
  * tt_cache_attention_workspace_bytes gives for the same arguments (single: starts == NULL); 0 needs
  * none.  No counterpart in the reference. */
+typedef struct {
+  int64_t size;
+  const void *q, *k_cache, *v_cache;
+  const int32_t *table, *lengths, *starts;
+  void *out, *workspace;
+  int64_t workspace_bytes;
+  int64_t q_row, q_head, k_page, k_row, k_head, v_page, v_row, v_head, table_row;
+  int32_t tokens, batch, heads, kv_heads, head_dim, pages, page_size, table_pages, max_length, dtype;
+  float scale;
+  int32_t reserved;
+} tt_cache_attention;
 int tt_cache_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int head_dim,
                                        int page_size, int table_pages, int max_length, int single,
                                        int64_t* bytes);
-int tt_cache_attention_fwd(const void* q, const void* k_cache, const void* v_cache,
-                           const int32_t* table, const int32_t* lengths, const int32_t* starts,
-                           void* out, void* workspace, int64_t workspace_bytes, int tokens,
-                           int batch, int heads, int kv_heads, int head_dim, int pages,
-                           int page_size, int table_pages, int max_length, int64_t q_row,
-                           int64_t q_head, int64_t k_page, int64_t k_row, int64_t k_head,
-                           int64_t v_page, int64_t v_row, int64_t v_head, int64_t table_row,
-                           float scale, int dtype, void* stream);
+int tt_cache_attention_fwd(const tt_cache_attention* args, void* stream);
 
 /* Where a forward's intermediates of its LAST layer are left in the workspace, for per-stage checks
  * of the fused plans (the megakernel's tasks and the fused-LN tiles never materialise LN1 / LN2 or

@@ -22,11 +22,11 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int rows_
     const int2 own = seq_rows(a, seq);
     if (token < own.x || token >= own.x + own.y) return;  // a row of no sequence
   }
-  const SeqUnits u = seq_units(a, seq, rows_per_tile);
+  const SeqShare sh = seq_share(a, 0, seq, rows_per_tile);
+  const SeqUnits u = sh.units;
   const int hkv = head / a.group;
   const int r = (token - u.first) * a.group + head - hkv * a.group;
   const int tile = r / rows_per_tile;
-  const SeqShare sh = seq_share(a, 0, seq, rows_per_tile);
   const int share = sh.share, begin = sh.base + tile * u.units;
   const int first = begin / share, parts = (begin + u.units - 1) / share - first + 1;
   if (parts == 1) return;
@@ -137,47 +137,56 @@ __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
   }
 }
 
-int launch_seq_attention(const SeqAttnArgs& a, bool paged, bool narrow, int dtype, hipStream_t stream) {
-  if (a.head_dim > 128) return launch_seq_attention_wide(a, paged, narrow, dtype, stream);
-  if (a.head_dim > 64) return launch_seq_hd<128>(a, paged, narrow, dtype, stream);
-  if (a.head_dim > 32) return launch_seq_hd<64>(a, paged, narrow, dtype, stream);
-  return launch_seq_hd<32>(a, paged, narrow, dtype, stream);
+int launch_seq_attention(const SeqAttnArgs& a, bool paged, SeqShape shape, int dtype, hipStream_t stream) {
+  if (a.head_dim > 128) return launch_seq_attention_wide(a, paged, shape, dtype, stream);
+  if (a.head_dim > 64) return launch_seq_hd<128>(a, paged, shape, dtype, stream);
+  if (a.head_dim > 32) return launch_seq_hd<64>(a, paged, shape, dtype, stream);
+  return launch_seq_hd<32>(a, paged, shape, dtype, stream);
 }
 
 // Blocks of a kernel that a CU holds (its registers and LDS).
-static int seq_resident(bool narrow, int head_dim) {
-  if (narrow) return head_dim <= 32 ? 6 : head_dim <= 64 ? 5 : 2;
-  return head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1;
+static int seq_resident(bool wide, int head_dim) {
+  if (wide) return head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1;
+  return head_dim <= 32 ? 6 : head_dim <= 64 ? 5 : 2;
 }
 
 // How a call is given to blocks.
 struct SeqPlan {
-  bool narrow;  // 32 rows per block, for single tokens and few drafted ones; otherwise 128
-  int rows;     // of a block
+  SeqShape shape;
+  int rows;  // of a block
   int slots, mode;
   int64_t part_rows;  // rows of the workspace
   bool many_parts;
 };
 
 // max_length < 0: packed sequences (no keys but their own).
-static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int head_dim, int64_t held, int max_length, bool single) {
+static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int head_dim, int64_t held, int max_length,
+                        bool single) {
   SeqPlan p{};
   const int64_t G = heads / kv_heads;
+  const int cus = device_cus();
   const bool paged = max_length >= 0;
-  p.narrow = paged && (single ? G <= 32 : tokens * G <= 32 * (int64_t)batch);
-  p.rows = p.narrow ? 32 : 128;
+  const bool wide = !paged || (single ? G > 32 : tokens * G > 32 * (int64_t)batch);
+  p.rows = wide ? 128 : 32;
   const int64_t tiles = single ? tokens * ((G + p.rows - 1) / p.rows) : tokens * G / p.rows + batch;
-  const int64_t blocks = tiles * kv_heads, held_blocks = (int64_t)seq_resident(p.narrow, head_dim) * device_cus();
+  const int64_t blocks = tiles * kv_heads, held_blocks = (int64_t)seq_resident(wide, head_dim) * cus;
+  p.shape = wide ? SeqShape::kWide : blocks <= cus ? SeqShape::kDeep : SeqShape::kNarrow;
   p.slots = (int)tiles;
   p.mode = kSeqInOrder;
-  if (paged && max_length > 512 && batch <= 512 && blocks < (p.narrow ? 4 : 1) * held_blocks && tiles * (held / kSeqUnit + 1) < (1LL << 31)) {
+  // Keys up to which a block takes a tile alone: dealing them out costs a second launch and its parts.  Measured on
+  // MI355X per call, alone -> in shares: 16 heads of 64, 1000 keys 9.3 -> 11.0 us, 2000 12.9 -> 11.5; 8 of 128, 500
+  // keys 9.9 -> 12.4, 1000 14.1 -> 12.7; 2 of 256, 300 keys 15.5 -> 23.4, 1000 31 -> 22.  Six rounds of the block.
+  const int alone = 6 * 32 * (p.shape == SeqShape::kDeep ? (head_dim <= 64 ? 8 : head_dim <= 128 ? 4 : 2) : 2);
+  if (paged && max_length > alone && batch <= 512 && blocks < (wide ? 1 : 4) * held_blocks &&
+      tiles * (held / kSeqUnit + 1) < (1LL << 31)) {
     p.mode = kSeqShares;
+    if (!wide) p.shape = SeqShape::kNarrow;
     const int64_t units = tiles * ((max_length + kSeqUnit - 1) / kSeqUnit);
     int64_t slots = held_blocks / kv_heads;
     if (slots > (units + kSeqMinShare - 1) / kSeqMinShare) slots = (units + kSeqMinShare - 1) / kSeqMinShare;
     p.slots = (int)(slots > 1 ? slots : 1);
     p.part_rows = 2 * (int64_t)p.slots * kv_heads * p.rows;
-    p.many_parts = p.slots > 8 * tiles;
+    p.many_parts = p.slots > 8 * tiles && tokens * heads <= 2048;
   } else if (!single && batch <= 64 && blocks > held_blocks && tokens * G < (1LL << 30)) {
     p.mode = kSeqHeaviest;
   }
@@ -219,27 +228,30 @@ static int check_pages(const char* what, int pages, int page_size, int table_pag
     if (rc_ != TT_OK) return rc_; \
   } while (0)
 
-extern "C" int tt_packed_attention_fwd(const void* q, const void* k, const void* v, const int32_t* starts, void* out,
-                                       int tokens, int batch, int heads, int kv_heads, int head_dim, int64_t q_row,
-                                       int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
-                                       float scale, int causal, int dtype, void* stream) {
+// The structure is the caller's: its size first.
+#define TT_ARGS(type, what)                                                                             \
+  TT_REQUIRE(args != nullptr && args->size == (int64_t)sizeof(type), what ": not a " #type " structure"); \
+  const type& c = *args
+
+extern "C" int tt_packed_attention_fwd(const tt_packed_attention* args, void* stream) {
   using namespace tt;
-  TT_CHECK(check_heads("packed_attention", tokens, batch, heads, kv_heads, head_dim, dtype));
-  TT_REQUIRE(scale > 0.f && scale < 3e38f, "packed_attention: scale %g is not positive and finite", scale);
-  if (tokens == 0 || batch == 0) return TT_OK;
-  TT_REQUIRE(q && k && v && starts && out, "packed_attention: null pointer");
-  TT_CHECK(check_rows("packed_attention: q", q, q_row, q_head));
-  TT_CHECK(check_rows("packed_attention: k", k, k_row, k_head));
-  TT_CHECK(check_rows("packed_attention: v", v, v_row, v_head));
-  TT_CHECK(check_rows("packed_attention: out", out, 0, 0));
+  TT_ARGS(tt_packed_attention, "packed_attention");
+  TT_CHECK(check_heads("packed_attention", c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, c.dtype));
+  TT_REQUIRE(c.scale > 0.f && c.scale < 3e38f, "packed_attention: scale %g is not positive and finite", c.scale);
+  if (c.tokens == 0 || c.batch == 0) return TT_OK;
+  TT_REQUIRE(c.q && c.k && c.v && c.starts && c.out, "packed_attention: null pointer");
+  TT_CHECK(check_rows("packed_attention: q", c.q, c.q_row, c.q_head));
+  TT_CHECK(check_rows("packed_attention: k", c.k, c.k_row, c.k_head));
+  TT_CHECK(check_rows("packed_attention: v", c.v, c.v_row, c.v_head));
+  TT_CHECK(check_rows("packed_attention: out", c.out, 0, 0));
   SeqAttnArgs a{};
-  a.q = q, a.k = k, a.v = v, a.out = out, a.starts = starts;
-  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
-  a.tokens = tokens, a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
-  a.head_dim = head_dim, a.causal = causal != 0, a.scale_log2 = scale * 1.4426950408889634f;
-  const SeqPlan p = seq_plan(tokens, batch, heads, kv_heads, head_dim, 0, -1, false);
+  a.q = c.q, a.k = c.k, a.v = c.v, a.out = c.out, a.starts = c.starts;
+  a.q_row = c.q_row, a.q_head = c.q_head, a.k_row = c.k_row, a.k_head = c.k_head, a.v_row = c.v_row, a.v_head = c.v_head;
+  a.tokens = c.tokens, a.batch = c.batch, a.heads = c.heads, a.kv_heads = c.kv_heads, a.group = c.heads / c.kv_heads;
+  a.head_dim = c.head_dim, a.causal = c.causal != 0, a.scale_log2 = c.scale * 1.4426950408889634f;
+  const SeqPlan p = seq_plan(c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, 0, -1, false);
   a.slots = p.slots, a.mode = p.mode;
-  return launch_seq_attention(a, false, false, dtype, (hipStream_t)stream);
+  return launch_seq_attention(a, false, SeqShape::kWide, c.dtype, (hipStream_t)stream);
 }
 
 extern "C" int tt_cache_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int head_dim,
@@ -256,79 +268,72 @@ extern "C" int tt_cache_attention_workspace_bytes(int tokens, int batch, int hea
   return TT_OK;
 }
 
-extern "C" int tt_cache_attention_fwd(const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
-                                      const int32_t* lengths, const int32_t* starts, void* out, void* workspace,
-                                      int64_t workspace_bytes, int tokens, int batch, int heads, int kv_heads,
-                                      int head_dim, int pages, int page_size, int table_pages, int max_length,
-                                      int64_t q_row, int64_t q_head, int64_t k_page, int64_t k_row, int64_t k_head,
-                                      int64_t v_page, int64_t v_row, int64_t v_head, int64_t table_row, float scale,
-                                      int dtype, void* stream) {
+extern "C" int tt_cache_attention_fwd(const tt_cache_attention* args, void* stream) {
   using namespace tt;
-  TT_CHECK(check_heads("cache_attention", tokens, batch, heads, kv_heads, head_dim, dtype));
-  TT_CHECK(check_pages("cache_attention", pages, page_size, table_pages));
-  TT_REQUIRE(scale > 0.f && scale < 3e38f, "cache_attention: scale %g is not positive and finite", scale);
-  TT_REQUIRE(max_length >= 0, "cache_attention: max_length %d", max_length);
-  if (tokens == 0 || batch == 0) return TT_OK;
-  TT_REQUIRE(q && k_cache && v_cache && table && lengths && out, "cache_attention: null pointer");
-  TT_REQUIRE(starts != nullptr || tokens == batch, "cache_attention: %d tokens for %d sequences without starts", tokens,
-             batch);
-  TT_CHECK(check_rows("cache_attention: q", q, q_row, q_head));
-  TT_CHECK(check_rows("cache_attention: k_cache", k_cache, k_row, k_head));
-  TT_CHECK(check_rows("cache_attention: v_cache", v_cache, v_row, v_head));
-  TT_REQUIRE(k_page % 8 == 0 && v_page % 8 == 0 && k_page >= 0 && v_page >= 0 && table_row >= 0,
-             "cache_attention: page strides %lld, %lld", (long long)k_page, (long long)v_page);
-  TT_CHECK(check_rows("cache_attention: out", out, 0, 0));
-  const SeqPlan p = seq_plan(tokens, batch, heads, kv_heads, head_dim, (int64_t)page_size * table_pages, max_length,
-                             starts == nullptr);
-  const int64_t bytes = 4 * (head_dim + 2) * p.part_rows;
-  TT_REQUIRE(bytes == 0 || (workspace != nullptr && workspace_bytes >= bytes && ((uintptr_t)workspace & 15) == 0),
+  TT_ARGS(tt_cache_attention, "cache_attention");
+  TT_CHECK(check_heads("cache_attention", c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, c.dtype));
+  TT_CHECK(check_pages("cache_attention", c.pages, c.page_size, c.table_pages));
+  TT_REQUIRE(c.scale > 0.f && c.scale < 3e38f, "cache_attention: scale %g is not positive and finite", c.scale);
+  TT_REQUIRE(c.max_length >= 0, "cache_attention: max_length %d", c.max_length);
+  if (c.tokens == 0 || c.batch == 0) return TT_OK;
+  TT_REQUIRE(c.q && c.k_cache && c.v_cache && c.table && c.lengths && c.out, "cache_attention: null pointer");
+  TT_REQUIRE(c.starts != nullptr || c.tokens == c.batch, "cache_attention: %d tokens for %d sequences without starts",
+             c.tokens, c.batch);
+  TT_CHECK(check_rows("cache_attention: q", c.q, c.q_row, c.q_head));
+  TT_CHECK(check_rows("cache_attention: k_cache", c.k_cache, c.k_row, c.k_head));
+  TT_CHECK(check_rows("cache_attention: v_cache", c.v_cache, c.v_row, c.v_head));
+  TT_REQUIRE(c.k_page % 8 == 0 && c.v_page % 8 == 0 && c.k_page >= 0 && c.v_page >= 0 && c.table_row >= 0,
+             "cache_attention: page strides %lld, %lld", (long long)c.k_page, (long long)c.v_page);
+  TT_CHECK(check_rows("cache_attention: out", c.out, 0, 0));
+  const SeqPlan p = seq_plan(c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, (int64_t)c.page_size * c.table_pages, c.max_length,
+                             c.starts == nullptr);
+  const int64_t bytes = 4 * (c.head_dim + 2) * p.part_rows;
+  TT_REQUIRE(bytes == 0 || (c.workspace != nullptr && c.workspace_bytes >= bytes && ((uintptr_t)c.workspace & 15) == 0),
              "cache_attention: a workspace of %lld bytes is needed, %lld given", (long long)bytes,
-             (long long)workspace_bytes);
+             (long long)c.workspace_bytes);
   SeqAttnArgs a{};
-  a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.starts = starts, a.lengths = lengths, a.table = table;
-  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
-  a.k_page = k_page, a.v_page = v_page, a.table_row = table_row;
-  a.tokens = tokens, a.batch = batch, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads;
-  a.head_dim = head_dim, a.pages = pages, a.table_pages = table_pages, a.page_shift = __builtin_ctz(page_size);
-  a.causal = 1, a.scale_log2 = scale * 1.4426950408889634f;
+  a.q = c.q, a.k = c.k_cache, a.v = c.v_cache, a.out = c.out, a.starts = c.starts, a.lengths = c.lengths, a.table = c.table;
+  a.q_row = c.q_row, a.q_head = c.q_head, a.k_row = c.k_row, a.k_head = c.k_head, a.v_row = c.v_row, a.v_head = c.v_head;
+  a.k_page = c.k_page, a.v_page = c.v_page, a.table_row = c.table_row;
+  a.tokens = c.tokens, a.batch = c.batch, a.heads = c.heads, a.kv_heads = c.kv_heads, a.group = c.heads / c.kv_heads;
+  a.head_dim = c.head_dim, a.pages = c.pages, a.table_pages = c.table_pages, a.page_shift = __builtin_ctz(c.page_size);
+  a.causal = 1, a.scale_log2 = c.scale * 1.4426950408889634f;
   a.slots = p.slots, a.mode = p.mode;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + p.part_rows * head_dim);
-  TT_CHECK(launch_seq_attention(a, true, p.narrow, dtype, (hipStream_t)stream));
+  a.part_o = static_cast<float*>(c.workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + p.part_rows * c.head_dim);
+  TT_CHECK(launch_seq_attention(a, true, p.shape, c.dtype, (hipStream_t)stream));
   if (p.mode != kSeqShares) return TT_OK;
-  return dtype == TT_FP16 ? launch_seq_merge<half>(a, p.rows, p.many_parts, (hipStream_t)stream)
+  return c.dtype == TT_FP16 ? launch_seq_merge<half>(a, p.rows, p.many_parts, (hipStream_t)stream)
                           : launch_seq_merge<bf16>(a, p.rows, p.many_parts, (hipStream_t)stream);
 }
 
-extern "C" int tt_cache_append(const void* k, const void* v, void* k_cache, void* v_cache, const int32_t* table,
-                               const int32_t* lengths, const int32_t* starts, int tokens, int batch, int kv_heads,
-                               int head_dim, int pages, int page_size, int table_pages, int64_t k_row, int64_t k_head,
-                               int64_t v_row, int64_t v_head, int64_t kc_page, int64_t kc_row, int64_t kc_head,
-                               int64_t vc_page, int64_t vc_row, int64_t vc_head, int64_t table_row, void* stream) {
+extern "C" int tt_cache_append(const tt_cache_rows* args, void* stream) {
   using namespace tt;
-  TT_CHECK(check_heads("cache_append", tokens, batch, kv_heads, kv_heads, head_dim, TT_FP16));
-  TT_CHECK(check_pages("cache_append", pages, page_size, table_pages));
-  if (tokens == 0 || batch == 0) return TT_OK;
-  TT_REQUIRE(k && v && k_cache && v_cache && table && lengths, "cache_append: null pointer");
-  TT_REQUIRE(starts != nullptr || tokens == batch, "cache_append: %d tokens for %d sequences without starts", tokens,
-             batch);
-  TT_CHECK(check_rows("cache_append: k", k, k_row, k_head));
-  TT_CHECK(check_rows("cache_append: v", v, v_row, v_head));
-  TT_CHECK(check_rows("cache_append: k_cache", k_cache, kc_row, kc_head));
-  TT_CHECK(check_rows("cache_append: v_cache", v_cache, vc_row, vc_head));
-  TT_REQUIRE(kc_page % 8 == 0 && vc_page % 8 == 0 && kc_page >= 0 && vc_page >= 0 && table_row >= 0,
-             "cache_append: page strides %lld, %lld", (long long)kc_page, (long long)vc_page);
+  TT_ARGS(tt_cache_rows, "cache_append");
+  TT_CHECK(check_heads("cache_append", c.tokens, c.batch, c.kv_heads, c.kv_heads, c.head_dim, TT_FP16));
+  TT_CHECK(check_pages("cache_append", c.pages, c.page_size, c.table_pages));
+  TT_REQUIRE(c.tokens < (1 << 26), "cache_append: %d tokens are more than one launch takes", c.tokens);
+  if (c.tokens == 0 || c.batch == 0) return TT_OK;
+  TT_REQUIRE(c.k && c.v && c.k_cache && c.v_cache && c.table && c.lengths, "cache_append: null pointer");
+  TT_REQUIRE(c.starts != nullptr || c.tokens == c.batch, "cache_append: %d tokens for %d sequences without starts",
+             c.tokens, c.batch);
+  TT_CHECK(check_rows("cache_append: k", c.k, c.k_row, c.k_head));
+  TT_CHECK(check_rows("cache_append: v", c.v, c.v_row, c.v_head));
+  TT_CHECK(check_rows("cache_append: k_cache", c.k_cache, c.kc_row, c.kc_head));
+  TT_CHECK(check_rows("cache_append: v_cache", c.v_cache, c.vc_row, c.vc_head));
+  TT_REQUIRE(c.kc_page % 8 == 0 && c.vc_page % 8 == 0 && c.kc_page >= 0 && c.vc_page >= 0 && c.table_row >= 0,
+             "cache_append: page strides %lld, %lld", (long long)c.kc_page, (long long)c.vc_page);
   AppendArgs a{};
-  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
-  a.k_cache = static_cast<uint16_t*>(k_cache), a.v_cache = static_cast<uint16_t*>(v_cache);
-  a.starts = starts, a.lengths = lengths, a.table = table;
-  a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
-  a.kc_page = kc_page, a.kc_row = kc_row, a.kc_head = kc_head;
-  a.vc_page = vc_page, a.vc_row = vc_row, a.vc_head = vc_head, a.table_row = table_row;
-  a.tokens = tokens, a.batch = batch, a.heads = kv_heads, a.chunks = head_dim / 8;
-  if (k_head == head_dim && v_head == head_dim && kc_head == head_dim && vc_head == head_dim)
-    a.heads = 1, a.chunks = kv_heads * (head_dim / 8);  // the heads of a token lie side by side everywhere
-  a.pages = pages, a.table_pages = table_pages, a.page_shift = __builtin_ctz(page_size);
-  hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
+  a.k = static_cast<const uint16_t*>(c.k), a.v = static_cast<const uint16_t*>(c.v);
+  a.k_cache = static_cast<uint16_t*>(c.k_cache), a.v_cache = static_cast<uint16_t*>(c.v_cache);
+  a.starts = c.starts, a.lengths = c.lengths, a.table = c.table;
+  a.k_row = c.k_row, a.k_head = c.k_head, a.v_row = c.v_row, a.v_head = c.v_head;
+  a.kc_page = c.kc_page, a.kc_row = c.kc_row, a.kc_head = c.kc_head;
+  a.vc_page = c.vc_page, a.vc_row = c.vc_row, a.vc_head = c.vc_head, a.table_row = c.table_row;
+  a.tokens = c.tokens, a.batch = c.batch, a.heads = c.kv_heads, a.chunks = c.head_dim / 8;
+  if (c.k_head == c.head_dim && c.v_head == c.head_dim && c.kc_head == c.head_dim && c.vc_head == c.head_dim)
+    a.heads = 1, a.chunks = c.kv_heads * (c.head_dim / 8);  // the heads of a token lie side by side everywhere
+  a.pages = c.pages, a.table_pages = c.table_pages, a.page_shift = __builtin_ctz(c.page_size);
+  hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)((c.tokens + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
   return launch_status("cache_append_kernel");
 }

@@ -260,22 +260,25 @@ __device__ __forceinline__ SeqUnits seq_units(const SeqAttnArgs& a, int b, int r
 struct SeqShare {
   int total, share;  // units of a kv head, and those of one block
   int seq, base;     // the sequence asked for, and its first unit
+  SeqUnits units;
 };
 
 // The shares of a launch, and the sequence that holds the first unit of block `slot` (seq < 0), or sequence `seq`.
 __device__ __forceinline__ SeqShare seq_share(const SeqAttnArgs& a, int slot, int seq, int rows_per_tile) {
   const int lane = threadIdx.x & 63;
-  const auto units_of = [&](int b) -> int {
-    if (b >= a.batch) return 0;
-    const SeqUnits u = seq_units(a, b, rows_per_tile);
-    return u.tiles * u.units;
+  const auto units_of = [&](int b) -> SeqUnits {
+    return b < a.batch ? seq_units(a, b, rows_per_tile) : SeqUnits{0, 0, 0, 0, 1};
   };
   SeqShare s;
-  int upto = wave_scan_int(units_of(lane));
+  SeqUnits u = units_of(lane);
+  int upto = wave_scan_int(u.tiles * u.units);
   s.total = __builtin_amdgcn_readlane(upto, 63);
   if (a.batch > 64) {
     int n = 0;
-    for (int b = 64 + lane; b < a.batch; b += 64) n += units_of(b);
+    for (int b = 64 + lane; b < a.batch; b += 64) {
+      const SeqUnits v = units_of(b);
+      n += v.tiles * v.units;
+    }
     s.total += wave_sum_int(n);
   }
   s.share = max((s.total + a.slots - 1) / a.slots, kSeqMinShare);
@@ -284,14 +287,18 @@ __device__ __forceinline__ SeqShare seq_share(const SeqAttnArgs& a, int slot, in
   for (int b0 = 0;;) {
     const int all = __builtin_amdgcn_readlane(upto, 63);
     if (b0 + 64 >= a.batch || (seq >= 0 ? seq < b0 + 64 : s.base + all > x)) {
-      const int l = seq >= 0 ? seq - b0 : __popcll(__ballot(s.base + upto <= x));
-      s.seq = b0 + min(l, 63);
-      if (l > 0) s.base += __builtin_amdgcn_readlane(upto, min(l, 64) - 1);
+      const int l = min(seq >= 0 ? seq - b0 : __popcll(__ballot(s.base + upto <= x)), 63);
+      s.seq = b0 + l;
+      if (l > 0) s.base += __builtin_amdgcn_readlane(upto, l - 1);
+      s.units = SeqUnits{__builtin_amdgcn_readlane(u.first, l), __builtin_amdgcn_readlane(u.count, l),
+                         __builtin_amdgcn_readlane(u.keys, l), __builtin_amdgcn_readlane(u.tiles, l),
+                         __builtin_amdgcn_readlane(u.units, l)};
       return s;
     }
     s.base += all;
     b0 += 64;
-    upto = wave_scan_int(units_of(b0 + lane));
+    u = units_of(b0 + lane);
+    upto = wave_scan_int(u.tiles * u.units);
   }
 }
 
@@ -338,7 +345,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     share_end = min(sh.total - x, sh.share) + x;
     sq.seq = sh.seq;
     base = sh.base;
-    su = seq_units(a, sq.seq, R);
+    su = sh.units;
   } else {
     if (a.mode == kSeqHeaviest) sq = seq_ranked<PAGED>(a, slot, R);
     else sq = seq_tile(a, a.slots - 1 - slot, R);
@@ -847,99 +854,113 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   }
   if (RW * KW > 1 && mixed) odd = __syncthreads_or(odd) != 0;
 
+  // Sums of this wave's rows over both halves of the wave; then, over the groups, by all of them: group g joins the
+  // g-th, (g + KW)-th, ... of the 4-feature pieces that a lane holds, from [group][piece][lane] and (maximum, sum) in LDS.
+  float l_row[CB];
+#pragma unroll
+  for (int b = 0; b < CB; ++b) l_row[b] = xhalf_sum(l_run[b]);
   if constexpr (KW > 1) {
-    static_assert(CB == 1, "groups of waves hold one block of rows");
-    // [group - 1][wave of the group][value][lane]: O, the maximum and this lane's half of the sum
-    constexpr int NV = DB * 16 + 2;
-    float* const mrg = reinterpret_cast<float*>(seq_lds);
+    static_assert(CB == 1 && RW == 1, "groups are waves with one block of rows");
+    floatx4* const pieces = reinterpret_cast<floatx4*>(seq_lds);
+    float2* const sums = reinterpret_cast<float2*>(pieces + KW * DB * 4 * 64);
     __syncthreads();
-    if (grp > 0) {
-      float* p = mrg + (size_t)((grp - 1) * RW + rw) * NV * 64 + lane;
 #pragma unroll
-      for (int i = 0; i < DB; ++i)
+    for (int i = 0; i < DB; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) p[(i * 16 + e) * 64] = o[0][i][e];
-      p[(NV - 2) * 64] = m_ref[0];
-      p[(NV - 1) * 64] = l_run[0];
+      for (int g = 0; g < 4; ++g)
+        pieces[(grp * DB * 4 + i * 4 + g) * 64 + lane] =
+            floatx4{o[0][i][4 * g], o[0][i][4 * g + 1], o[0][i][4 * g + 2], o[0][i][4 * g + 3]};
+    if (hf == 0) sums[grp * 32 + col] = make_float2(m_ref[0], l_row[0]);
+    __syncthreads();
+    float2 ml[KW];
+    float m = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < KW; ++g) {
+      ml[g] = sums[g * 32 + col];
+      m = fmaxf(m, ml[g].x);
     }
-    __syncthreads();
-    if (grp == 0) {
-#pragma unroll 1
-      for (int g = 0; g < KW - 1; ++g) {
-        const float* p = mrg + (size_t)(g * RW + rw) * NV * 64 + lane;
-        const float m_g = p[(NV - 2) * 64], l_g = p[(NV - 1) * 64];
-        const float m_new = fmaxf(m_ref[0], m_g);
-        // a part without a maximum saw no key (its sum, 0, is then its weight) or only NaN (NaN is)
-        const float c0 = m_ref[0] == -INFINITY ? l_run[0] : __builtin_amdgcn_exp2f((m_ref[0] - m_new) * c2);
-        const float c1 = m_g == -INFINITY ? l_g : __builtin_amdgcn_exp2f((m_g - m_new) * c2);
-        l_run[0] = l_run[0] * c0 + l_g * c1;
-        m_ref[0] = m_new;
+    float w[KW], l = 0.f;
 #pragma unroll
-        for (int i = 0; i < DB; ++i)
+    for (int g = 0; g < KW; ++g) {
+      // a group without a maximum saw no key (its sum, 0, is its weight) or only NaN (NaN is)
+      w[g] = ml[g].x == -INFINITY ? ml[g].y : __builtin_amdgcn_exp2f((ml[g].x - m) * c2);
+      l = fmaf(w[g], ml[g].y, l);
+    }
+    m_ref[0] = m;
+    l_row[0] = l;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[0][i][e] = o[0][i][e] * c0 + p[(i * 16 + e) * 64] * c1;
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if ((i * 4 + g) % KW != grp) continue;
+        floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+          const floatx4 y = pieces[(k * DB * 4 + i * 4 + g) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[e] = fmaf(w[k], y[e], sum[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][i][4 * g + e] = sum[e];
       }
-    }
   }
 
   // Output rows, or a part's sums: O in units of exp2(m - 7), the maximum in log2 units, the sum.
   const int64_t part0 = ((int64_t)part * a.kv_heads + hkv) * R - r0;  // + row
-  if (grp == 0) {
 #pragma unroll
-    for (int b = 0; b < CB; ++b) {
-      const float l = xhalf_sum(l_run[b]);
-      const int r = wr0 + 32 * b + col;
-      if (r >= rows) continue;
-      if (part >= 0) {
-        float* dst = a.part_o + (part0 + r) * hd;
-#pragma unroll
-        for (int i = 0; i < DB; ++i)
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            if (32 * i + 8 * g < hd)
-              *reinterpret_cast<floatx4*>(dst + 32 * i + 8 * g + 4 * hf) =
-                  floatx4{o[b][i][4 * g], o[b][i][4 * g + 1], o[b][i][4 * g + 2], o[b][i][4 * g + 3]};
-        if (hf == 0) a.part_ml[part0 + r] = make_float2(m_ref[b] * c2, l);
-        continue;
-      }
-      const float inv = l == 0.f ? 0.f : 1.0f / l;  // no key: zeros
-      T* dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + tok[b]) * a.heads + head[b]) * hd;
+  for (int b = 0; b < CB; ++b) {
+    const int r = wr0 + 32 * b + col;
+    if (r >= rows) continue;
+    if (part >= 0) {
+      float* dst = a.part_o + (part0 + r) * hd;
 #pragma unroll
       for (int i = 0; i < DB; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          if (32 * i + 8 * g < hd) {
-            typedef T v4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<v4*>(dst + 32 * i + 8 * g + 4 * hf) =
-                v4{(T)(o[b][i][4 * g] * inv), (T)(o[b][i][4 * g + 1] * inv), (T)(o[b][i][4 * g + 2] * inv),
-                   (T)(o[b][i][4 * g + 3] * inv)};
-          }
+          if (32 * i + 8 * g < hd && (i * 4 + g) % KW == grp)
+            *reinterpret_cast<floatx4*>(dst + 32 * i + 8 * g + 4 * hf) =
+                floatx4{o[b][i][4 * g], o[b][i][4 * g + 1], o[b][i][4 * g + 2], o[b][i][4 * g + 3]};
+      if (hf == 0 && grp == 0) a.part_ml[part0 + r] = make_float2(m_ref[b] * c2, l_row[b]);
+      continue;
     }
-    if (mixed && __builtin_amdgcn_ballot_w64(odd) != 0) {
-      // restore_odd: the wave adds the infinities and NaN of V that were taken out to those of its rows that see them.
-      __threadfence_block();
-      const int from = kbeg + max(block_lo - kbeg, 0) / KT * KT;
-      for (int key = from; key < lim_hi; ++key) {
-        const T* vp = vh;
-        if constexpr (PAGED) {
-          const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
-          if ((uint32_t)page >= (uint32_t)a.pages) continue;
-          vp += page * a.v_page + (key & ((1 << a.page_shift) - 1)) * a.v_row;
-        } else {
-          vp += (int64_t)(sq.first + key) * a.v_row;
+    const float inv = l_row[b] == 0.f ? 0.f : 1.0f / l_row[b];  // no key: zeros
+    T* dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + tok[b]) * a.heads + head[b]) * hd;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (32 * i + 8 * g < hd && (i * 4 + g) % KW == grp) {
+          typedef T v4 __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<v4*>(dst + 32 * i + 8 * g + 4 * hf) =
+              v4{(T)(o[b][i][4 * g] * inv), (T)(o[b][i][4 * g + 1] * inv), (T)(o[b][i][4 * g + 2] * inv),
+                 (T)(o[b][i][4 * g + 3] * inv)};
         }
-        for (int d = lane; d < hd; d += 64) {
-          const T y = vp[d];
-          if ((__builtin_bit_cast(uint16_t, y) & Num<T>::kExp) != Num<T>::kExp) continue;
-          for (int r = wr0; r < min(wr0 + WR, rows); ++r) {
-            const int token = r / G;
-            if (key >= seq_limit(a, token, sq.count, keys)) continue;
-            if (part >= 0) {
-              a.part_o[(part0 + r) * hd + d] += (float)y;
-            } else {
-              T* const dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + token) * a.heads + hkv * G + r - token * G) * hd + d;
-              *dst = (T)((float)*dst + (float)y);
-            }
+  }
+  if (mixed && __builtin_amdgcn_ballot_w64(odd) != 0) {
+    // restore_odd: a wave adds the infinities and NaN of V that were taken out to those of its rows that see them.
+    __threadfence_block();
+    if constexpr (KW > 1) __syncthreads();
+    const int from = kbeg + max(block_lo - kbeg, 0) / KT * KT;
+    for (int key = from; grp == 0 && key < lim_hi; ++key) {
+      const T* vp = vh;
+      if constexpr (PAGED) {
+        const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
+        if ((uint32_t)page >= (uint32_t)a.pages) continue;
+        vp += page * a.v_page + (key & ((1 << a.page_shift) - 1)) * a.v_row;
+      } else {
+        vp += (int64_t)(sq.first + key) * a.v_row;
+      }
+      for (int d = lane; d < hd; d += 64) {
+        const T y = vp[d];
+        if ((__builtin_bit_cast(uint16_t, y) & Num<T>::kExp) != Num<T>::kExp) continue;
+        for (int r = wr0; r < min(wr0 + WR, rows); ++r) {
+          const int token = r / G;
+          if (key >= seq_limit(a, token, sq.count, keys)) continue;
+          if (part >= 0) {
+            a.part_o[(part0 + r) * hd + d] += (float)y;
+          } else {
+            T* const dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + token) * a.heads + hkv * G + r - token * G) * hd + d;
+            *dst = (T)((float)*dst + (float)y);
           }
         }
       }

@@ -4,8 +4,8 @@
 
 namespace tt {
 
-int launch_seq_attention_wide(const SeqAttnArgs& a, bool paged, bool narrow, int dtype, hipStream_t stream) {
-  return launch_seq_hd<256>(a, paged, narrow, dtype, stream);
+int launch_seq_attention_wide(const SeqAttnArgs& a, bool paged, SeqShape shape, int dtype, hipStream_t stream) {
+  return launch_seq_hd<256>(a, paged, shape, dtype, stream);
 }
 
 }  // namespace tt

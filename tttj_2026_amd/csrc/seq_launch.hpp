@@ -8,10 +8,14 @@
 
 namespace tt {
 
+// Blocks of 128 rows on four waves; of 32 rows, for single tokens and few drafted ones, whose keys are shared by one
+// or two waves; and of 32 rows with as many waves as the LDS holds tiles for, where blocks are few.
+enum class SeqShape { kWide, kNarrow, kDeep };
+
 template <typename T, int HD, int CB, int RW, int KW, int KT, bool PAGED>
 int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
   constexpr int lds = 2 * 2 * KW * KT * HD * (int)sizeof(T);  // K and V, two tiles deep
-  static_assert(lds >= (KW - 1) * RW * (HD / 2 + 2) * 256, "the groups are merged in the tiles' LDS");
+  static_assert(KW == 1 || lds >= KW * (HD / 8 * 64 * 16 + 32 * 8), "the groups are joined in the tiles' LDS");
   static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic LDS is raised
   int dev = 0;
   TT_HIP(hipGetDevice(&dev));
@@ -31,18 +35,19 @@ int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
 }
 
 template <int HD, typename T>
-int launch_seq_type(const SeqAttnArgs& a, bool paged, bool narrow, hipStream_t stream) {
+int launch_seq_type(const SeqAttnArgs& a, bool paged, SeqShape shape, hipStream_t stream) {
   if (!paged) return launch_seq<T, HD, 1, 4, 1, 64, false>(a, stream);
-  if (narrow) return launch_seq<T, HD, 1, 1, (HD <= 128 ? 2 : 1), 32, true>(a, stream);
+  if (shape == SeqShape::kDeep) return launch_seq<T, HD, 1, 1, (HD <= 64 ? 8 : HD <= 128 ? 4 : 2), 32, true>(a, stream);
+  if (shape == SeqShape::kNarrow) return launch_seq<T, HD, 1, 1, (HD <= 128 ? 2 : 1), 32, true>(a, stream);
   return launch_seq<T, HD, 1, 4, 1, 64, true>(a, stream);
 }
 
 template <int HD>
-int launch_seq_hd(const SeqAttnArgs& a, bool paged, bool narrow, int dtype, hipStream_t stream) {
-  return dtype == TT_FP16 ? launch_seq_type<HD, half>(a, paged, narrow, stream)
-                          : launch_seq_type<HD, bf16>(a, paged, narrow, stream);
+int launch_seq_hd(const SeqAttnArgs& a, bool paged, SeqShape shape, int dtype, hipStream_t stream) {
+  return dtype == TT_FP16 ? launch_seq_type<HD, half>(a, paged, shape, stream)
+                          : launch_seq_type<HD, bf16>(a, paged, shape, stream);
 }
 
-int launch_seq_attention_wide(const SeqAttnArgs& a, bool paged, bool narrow, int dtype, hipStream_t stream);
+int launch_seq_attention_wide(const SeqAttnArgs& a, bool paged, SeqShape shape, int dtype, hipStream_t stream);
 
 }  // namespace tt

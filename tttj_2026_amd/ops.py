@@ -155,68 +155,92 @@ def attention(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, mask: Optional
 
 _SEQ_DTYPES = {torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16}
 
+# The current stream of a device as an integer, without a Stream object (0.1 us instead of 2).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-def _rows(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
+
+def _call(name: str, args: bytes, device: torch.device) -> None:
+    """One library call with packed arguments, on the current stream of ``device``."""
+    index, before = device.index, torch.cuda.current_device()
+    fn = getattr(_lib.load(), name)
+    if index == before:
+        rc = fn(args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     """``t`` [T, heads, head_dim] in a form the kernels read: adjacent features, rows and heads 16 bytes aligned
     (a column slice of a fused projection's output is; anything else is copied)."""
-    if t.dim() != 3 or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be a [tokens, heads, head_dim] tensor of {like.dtype} on {like.device}")
+    if t.dim() != 3 or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be a [tokens, heads, head_dim] tensor of {dtype} on {device}")
     row, head, feature = t.stride()
     if feature != 1 or (row | head) & 7 or t.data_ptr() & 15 or row >= 1 << 26:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _int32(t: torch.Tensor, name: str, like: torch.Tensor, *shape: int) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.device != like.device or t.shape != shape:
-        raise ValueError(f"{name} must be an int32 tensor of shape {list(shape)} on {like.device}")
+def _int32(t: torch.Tensor, name: str, size: int, device: torch.device) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != size:
+        raise ValueError(f"{name} must be an int32 tensor of {size} elements on {device}")
     return t.contiguous()
 
 
-def _query(q: torch.Tensor, kv_heads: int, scale: Optional[float], out: Optional[torch.Tensor]):
-    """Checks of a query tensor [T, heads, head_dim]; (q, out, scale)."""
-    if q.dim() != 3 or q.dtype not in _SEQ_DTYPES or q.device.type != "cuda":
-        raise ValueError("q must be a CUDA [tokens, heads, head_dim] tensor of float16 or bfloat16")
-    tokens, heads, hd = q.shape
+def _heads(heads: int, kv_heads: int, hd: int) -> None:
     if kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise ValueError(f"{heads} query heads cannot share {kv_heads} key / value heads evenly")
     if hd % 8 or not 8 <= hd <= 256:
         raise ValueError(f"head_dim {hd} is not a multiple of 8 from 8 to 256")
+
+
+def _typed(t: torch.Tensor, name: str):
+    """(dtype, device) of a tensor that the others of a call have to match."""
+    dtype, device = t.dtype, t.device
+    if dtype not in _SEQ_DTYPES or device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor of float16 or bfloat16")
+    return dtype, device
+
+
+def _context(out: Optional[torch.Tensor], tokens: int, width: int, dtype: torch.dtype,
+             device: torch.device) -> torch.Tensor:
     if out is None:
-        out = torch.empty(tokens, heads * hd, dtype=q.dtype, device=q.device)
-    elif (out.shape != (tokens, heads * hd) or out.dtype != q.dtype or out.device != q.device
-          or not out.is_contiguous() or out.data_ptr() & 15):
-        raise ValueError("out must be a contiguous, 16-byte aligned [tokens, heads * head_dim] tensor like q")
-    return _rows(q, "q", q), out, hd ** -0.5 if scale is None else float(scale)
+        return torch.empty((tokens, width), dtype=dtype, device=device)
+    if (out.shape != (tokens, width) or out.dtype != dtype or out.device != device or not out.is_contiguous()
+            or out.data_ptr() & 15):
+        raise ValueError(f"out must be a contiguous, 16-byte aligned [{tokens}, {width}] tensor of {dtype} on {device}")
+    return out
 
 
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, kv_heads: int, hd: int) -> int:
-    """Checks of a cache's halves [pages, page_size, kv_heads, head_dim] (used in place, so never copied)."""
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dim() != 4 or t.dtype != like.dtype or t.device != like.device or t.shape[2:] != (kv_heads, hd):
-            raise ValueError(f"{name} must be a [pages, page_size, {kv_heads}, {hd}] tensor of {like.dtype} on "
-                             f"{like.device}")
-        page, row, head, feature = t.stride()
-        if feature != 1 or (page | row | head) & 7 or t.data_ptr() & 15:
-            raise ValueError(f"{name} needs adjacent features, and pages, tokens and heads 16 bytes aligned")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError("k_cache and v_cache must have one shape")
-    return k_cache.shape[1]
+def _cache(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device: torch.device):
+    """Strides of one half of a cache, [pages, page_size, kv_heads, head_dim] (used in place, so never copied)."""
+    if t.dim() != 4 or t.shape[1:] != shape[1:] or t.shape[0] != shape[0] or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be a [pages, page_size, kv_heads, head_dim] tensor of shape {list(shape)} and "
+                         f"{dtype} on {device}")
+    page, row, head, feature = t.stride()
+    if feature != 1 or (page | row | head) & 7 or t.data_ptr() & 15:
+        raise ValueError(f"{name} needs adjacent features, and pages, tokens and heads 16 bytes aligned")
+    return page, row, head
 
 
-class _on_device:
-    """The device of ``t`` is the current one inside."""
-
-    def __init__(self, t: torch.Tensor):
-        self.index, self.before = t.device.index, torch.cuda.current_device()
-
-    def __enter__(self):
-        if self.index != self.before:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.index != self.before:
-            torch.cuda.set_device(self.before)
+def _sequences(tokens: int, page_table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor],
+               device: torch.device):
+    """Checks of the description of a batch over a cache; (page_table, lengths, starts)."""
+    batch = lengths.shape[0] if lengths.dim() == 1 else -1
+    lengths = _int32(lengths, "lengths", batch, device)
+    if (page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != device
+            or page_table.shape[0] != batch or page_table.shape[1] == 0):
+        raise ValueError(f"page_table must be an int32 tensor [{batch}, pages per sequence] on {device}")
+    if page_table.stride(1) != 1:
+        page_table = page_table.contiguous()
+    if starts is not None:
+        starts = _int32(starts, "starts", batch + 1, device)
+    elif tokens != batch:
+        raise ValueError(f"{tokens} tokens for {batch} sequences need starts")
+    return page_table, lengths, starts
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, *,
@@ -230,42 +254,24 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     up to itself).  Query head h reads key / value head h // (heads // kv_heads).  ``scale`` defaults to
     head_dim^-1/2.  float16 or bfloat16, head_dim a multiple of 8 up to 256; q, k, v may be column slices of one
     projection's output.  Rows outside every sequence are left as they are in ``out`` (arbitrary in a new tensor)."""
-    if k.dim() != 3 or k.shape != v.shape:
-        raise ValueError("k and v must have one shape [tokens, kv_heads, head_dim]")
-    q, out, scale = _query(q, k.shape[1], scale, out)
-    k, v = _rows(k, "k", q), _rows(v, "v", q)
-    if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-        raise ValueError("q, k and v must have one number of tokens and one head_dim")
-    if starts.dim() != 1 or starts.shape[0] == 0:
-        raise ValueError("starts must be an int32 tensor of shape [B + 1]")
-    starts = _int32(starts, "starts", q, starts.shape[0])
+    dtype, device = _typed(q, "q")
+    q, k, v = _rows(q, "q", dtype, device), _rows(k, "k", dtype, device), _rows(v, "v", dtype, device)
     tokens, heads, hd = q.shape
-    with _on_device(q):
-        rc = _lib.load().tt_packed_attention_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), starts.data_ptr(), out.data_ptr(), tokens, starts.shape[0] - 1,
-            heads, k.shape[1], hd, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-            scale, int(causal), _SEQ_DTYPES[q.dtype], _stream(q))
-    _lib.check(rc, "tt_packed_attention_fwd")
+    kv_heads = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != hd:
+        raise ValueError("k and v must have one shape, and q's number of tokens and head_dim")
+    _heads(heads, kv_heads, hd)
+    batch = starts.shape[0] - 1 if starts.dim() == 1 else -1
+    if batch < 0:
+        raise ValueError("starts must be an int32 tensor of B + 1 elements")
+    starts = _int32(starts, "starts", batch + 1, device)
+    out = _context(out, tokens, heads * hd, dtype, device)
+    args = _lib.PACKED_ATTENTION
+    _call("tt_packed_attention_fwd", args.pack(
+        args.size, q.data_ptr(), k.data_ptr(), v.data_ptr(), starts.data_ptr(), out.data_ptr(), *q.stride()[:2],
+        *k.stride()[:2], *v.stride()[:2], tokens, batch, heads, kv_heads, hd, causal, _SEQ_DTYPES[dtype],
+        hd ** -0.5 if scale is None else scale), device)
     return out
-
-
-def _sequences(tokens: int, page_table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor],
-               like: torch.Tensor):
-    """Checks of the description of a batch over a cache; (page_table, lengths, starts)."""
-    if lengths.dim() != 1 or page_table.dim() != 2:
-        raise ValueError("lengths must be [B] and page_table [B, pages per sequence]")
-    batch = lengths.shape[0]
-    lengths = _int32(lengths, "lengths", like, batch)
-    if (page_table.dtype != torch.int32 or page_table.device != like.device or page_table.shape[0] != batch
-            or page_table.shape[1] == 0):
-        raise ValueError(f"page_table must be an int32 tensor [{batch}, pages per sequence] on {like.device}")
-    if page_table.stride(1) != 1:
-        page_table = page_table.contiguous()
-    if starts is not None:
-        starts = _int32(starts, "starts", like, batch + 1)
-    elif tokens != batch:
-        raise ValueError(f"{tokens} tokens for {batch} sequences need starts")
-    return page_table, lengths, starts
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -279,19 +285,21 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     the n tokens of sequence b, rows starts[b] ... starts[b + 1] - 1 (or row b alone without ``starts``), take
     positions lengths[b] - n ... lengths[b] - 1.  Tokens whose position is negative or beyond the table, or whose
     page is no page of the cache, are not written."""
-    if k.dim() != 3 or k.shape != v.shape or k.dtype not in _SEQ_DTYPES or k.device.type != "cuda":
-        raise ValueError("k and v must be CUDA [tokens, kv_heads, head_dim] tensors of float16 or bfloat16")
-    k, v = _rows(k, "k", k), _rows(v, "v", k)
+    dtype, device = _typed(k, "k")
+    k, v = _rows(k, "k", dtype, device), _rows(v, "v", dtype, device)
     tokens, kv_heads, hd = k.shape
-    page = _cache(k_cache, v_cache, k, kv_heads, hd)
-    table, lengths, starts = _sequences(tokens, page_table, lengths, starts, k)
-    with _on_device(k):
-        rc = _lib.load().tt_cache_append(
-            k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(),
-            _ptr(starts), tokens, lengths.shape[0], kv_heads, hd, k_cache.shape[0], page, table.shape[1], k.stride(0),
-            k.stride(1), v.stride(0), v.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3], table.stride(0),
-            _stream(k))
-    _lib.check(rc, "tt_cache_append")
+    if k.shape != v.shape:
+        raise ValueError("k and v must have one shape")
+    _heads(kv_heads, kv_heads, hd)
+    shape = (k_cache.shape[0], k_cache.shape[1], kv_heads, hd) if k_cache.dim() == 4 else ()
+    kc = _cache(k_cache, "k_cache", shape, dtype, device)
+    vc = _cache(v_cache, "v_cache", shape, dtype, device)
+    table, lengths, starts = _sequences(tokens, page_table, lengths, starts, device)
+    args = _lib.CACHE_ROWS
+    _call("tt_cache_append", args.pack(
+        args.size, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
+        lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), *k.stride()[:2], *v.stride()[:2], *kc, *vc,
+        table.stride(0), tokens, lengths.shape[0], kv_heads, hd, shape[0], shape[1], table.shape[1], 0), device)
 
 
 def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -304,24 +312,26 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (a length of 0 in a padded batch) gets zeros.  Without ``starts`` every sequence has one new token.
     ``max_length`` (default: what the table can hold) is the longest length the caller expects; it only decides how
     the work is split.  Keys in a page whose number is no page of the cache are not read and count as NaN."""
-    if k_cache.dim() != 4:
-        raise ValueError("k_cache must be [pages, page_size, kv_heads, head_dim]")
-    kv_heads = k_cache.shape[2]
-    q, out, scale = _query(q, kv_heads, scale, out)
+    dtype, device = _typed(q, "q")
+    q = _rows(q, "q", dtype, device)
     tokens, heads, hd = q.shape
-    page = _cache(k_cache, v_cache, q, kv_heads, hd)
-    table, lengths, starts = _sequences(tokens, page_table, lengths, starts, q)
-    batch = lengths.shape[0]
-    held = table.shape[1] * page
+    shape = (*k_cache.shape[:3], hd) if k_cache.dim() == 4 else ()
+    kc = _cache(k_cache, "k_cache", shape, dtype, device)
+    vc = _cache(v_cache, "v_cache", shape, dtype, device)
+    pages, page, kv_heads, _ = shape
+    _heads(heads, kv_heads, hd)
+    table, lengths, starts = _sequences(tokens, page_table, lengths, starts, device)
+    out = _context(out, tokens, heads * hd, dtype, device)
+    batch, table_pages = table.shape
+    held = table_pages * page
     max_length = held if max_length is None else min(int(max_length), held)
-    nbytes = _lib.cache_attention_workspace_bytes(tokens, batch, heads, kv_heads, hd, page, table.shape[1], max_length,
+    nbytes = _lib.cache_attention_workspace_bytes(tokens, batch, heads, kv_heads, hd, page, table_pages, max_length,
                                                   starts is None)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    with _on_device(q):
-        rc = _lib.load().tt_cache_attention_fwd(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), _ptr(starts),
-            out.data_ptr(), _ptr(work), nbytes, tokens, batch, heads, kv_heads, hd, k_cache.shape[0], page,
-            table.shape[1], max_length, q.stride(0), q.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3],
-            table.stride(0), scale, _SEQ_DTYPES[q.dtype], _stream(q))
-    _lib.check(rc, "tt_cache_attention_fwd")
+    work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    args = _lib.CACHE_ATTENTION
+    _call("tt_cache_attention_fwd", args.pack(
+        args.size, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+        0 if starts is None else starts.data_ptr(), out.data_ptr(), 0 if work is None else work.data_ptr(), nbytes,
+        *q.stride()[:2], *kc, *vc, table.stride(0), tokens, batch, heads, kv_heads, hd, pages, page, table_pages,
+        max_length, _SEQ_DTYPES[dtype], hd ** -0.5 if scale is None else scale, 0), device)
     return out
