@@ -1,0 +1,442 @@
+"""Packed prompts and the paged cache where they can go wrong: masked infinities and NaN, bad pages, rows outside
+sequences, strides, offsets past 32 bits, large and tiny scores, batches beyond the lanes of a wave, captured graphs,
+other streams, refusals, and a run of all three as a program makes it.  Bounds as in test_gpu_seq_attention.py."""
+
+import pytest
+import torch
+
+from tttj_2026_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _i32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _starts(counts, first=0):
+    return _i32([first, *(first + torch.tensor(counts).cumsum(0)).tolist()])
+
+
+def _randn(seed, *shape, dtype=F16):
+    return torch.randn(*shape, generator=torch.Generator("cuda").manual_seed(seed), device="cuda").to(dtype)
+
+
+def _attend(q, k, v, limits, scale=None):
+    """Row i of q [n, H, hd] over the first limits[i] rows of k, v [L, Hkv, hd]: (o, sum p |v|) in float64.  Keys that a
+    row does not see are left out of its sums whatever they hold."""
+    n, h, hd = q.shape
+    g = h // k.shape[1]
+    q, k, v = q.double(), k.double(), v.double()
+    hidden = torch.arange(k.shape[0], device=q.device)[None, :] >= torch.as_tensor(limits, device=q.device)[:, None]
+    zero = torch.zeros((), dtype=torch.float64, device=q.device)
+    out, mag = (torch.zeros(n, h, hd, dtype=torch.float64, device=q.device) for _ in range(2))
+    for i in range(h):
+        s = q[:, i] @ k[:, i // g].T.contiguous() * (hd ** -0.5 if scale is None else scale)
+        p = torch.softmax(s.masked_fill(hidden, float("-inf")), -1)
+        p = torch.where(hidden, zero, p)
+        x = v[:, i // g]
+        fine = torch.isfinite(x)
+        out[:, i] = p @ torch.where(fine, x, zero)
+        mag[:, i] = p @ torch.where(fine, x, zero).abs()
+        for j in (~fine).any(1).nonzero().flatten().tolist():
+            seen = ~hidden[:, j]
+            out[seen, i] += torch.where(fine[j], zero, x[j])
+    return out.view(n, h * hd), mag.view(n, h * hd)
+
+
+def _check(y, ref, mag):
+    u = torch.finfo(y.dtype).eps / 2
+    y = y.double()
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(y), torch.isnan(ref))
+    assert torch.equal(y[~fine].nan_to_num(7.0), ref[~fine].nan_to_num(7.0))
+    err = (y - ref)[fine].abs()
+    assert bool((err <= 4 * u * mag[fine] + 2.0 ** -25).all()), (err - 4 * u * mag[fine]).max().item()
+
+
+def _store(lengths, hkv, hd, page, dtype=F16, seed=0):
+    """A cache with random K and V for every sequence, its pages in random order; (k_cache, v_cache, table, k, v)."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // page) for n in lengths]
+    order = torch.randperm(sum(need) + 2, generator=g).tolist()
+    table = torch.full((len(lengths), max(need) + 1), 1 << 30, dtype=torch.int32)
+    kc, vc = (torch.full((sum(need) + 2, page, hkv, hd), float("nan"), dtype=dtype, device="cuda") for _ in range(2))
+    k, v, at = [], [], 0
+    for b, n in enumerate(lengths):
+        table[b, :need[b]] = torch.tensor(order[at:at + need[b]], dtype=torch.int32)
+        at += need[b]
+        k.append(_randn(seed + 7 * b + 1, n, hkv, hd, dtype=dtype))
+        v.append(_randn(seed + 7 * b + 2, n, hkv, hd, dtype=dtype))
+        _write(kc, vc, table, b, 0, k[b], v[b])
+    return kc, vc, table.cuda(), k, v
+
+
+def _write(kc, vc, table, b, first, k, v):
+    t = torch.arange(first, first + len(k))
+    where = table[b, t // kc.shape[1]].long().to(kc.device), (t % kc.shape[1]).to(kc.device)
+    kc[where], vc[where] = k, v
+
+
+def _over_cache(q, k, v, counts, lengths, scale=None):
+    refs, first = [], 0
+    for b, n in enumerate(counts):
+        limits = (lengths[b] - n + torch.arange(1, n + 1)).clamp(min=0)
+        refs.append(_attend(q[first:first + n], k[b], v[b], limits, scale))
+        first += n
+    return [torch.cat(x) for x in zip(*refs)]
+
+
+def _over_prompts(q, k, v, counts, causal=True, scale=None):
+    refs, first = [], 0
+    for n in counts:
+        limits = torch.arange(1, n + 1) if causal else torch.full((n,), n)
+        refs.append(_attend(q[first:first + n], k[first:first + n], v[first:first + n], limits, scale))
+        first += n
+    return [torch.cat(x) for x in zip(*refs)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [32, 80, 128, 256])
+@pytest.mark.parametrize("h,hkv", [(4, 4), (8, 2)])
+def test_packed_masked_values(dtype, hd, h, hkv):
+    """Infinities and NaN in V, and NaN in K of the last token of the first sequence, reach exactly the rows that see
+    them; a NaN sequence leaves its neighbours alone."""
+    counts = [150, 40, 9]
+    q, k, v = (_randn(s, sum(counts), n, hd, dtype=dtype) for s, n in ((1, h), (2, hkv), (3, hkv)))
+    v[20, 0, 3], v[70, hkv - 1, 5], v[130, 0, hd - 1] = float("inf"), float("nan"), float("-inf")
+    v[131, 0, hd - 1] = float("inf")
+    y = ops.packed_attention(q, k, v, _starts(counts))
+    _check(y, *_over_prompts(q, k, v, counts))
+    k[149], v[150:190], k[150:190] = float("nan"), float("nan"), float("nan")
+    y = ops.packed_attention(q, k, v, _starts(counts)).double()
+    ref, mag = _over_prompts(q, k, v, counts)
+    keep = [*range(149), *range(190, 199)]
+    assert torch.isnan(y[149:190]).all()
+    _check(y[keep].to(dtype), ref[keep], mag[keep])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("counts,lengths", [([5, 1, 7], [2000, 40, 7]), ([70, 100], [70, 1500])])
+def test_cache_masked_values(dtype, hd, counts, lengths):
+    """The same over a cache, for drafted tokens and chunks, keys in one block or dealt to many."""
+    kc, vc, table, k, v = _store(lengths, 2, hd, 32, dtype)
+    for b, n in enumerate(counts):
+        if n > 2:
+            v[b][lengths[b] - 2, 1, 4] = float("inf")
+            v[b][lengths[b] - 1, 0, 9] = float("nan")
+            _write(kc, vc, table.cpu(), b, 0, k[b], v[b])
+    q = _randn(9, sum(counts), 6, hd, dtype=dtype)
+    ref = _over_cache(q, k, v, counts, lengths)
+    for most in (None, max(lengths), 10):
+        _check(ops.cache_attention(q, kc, vc, table, _i32(lengths), _starts(counts), max_length=most), *ref)
+
+
+@pytest.mark.parametrize("number", [-1, 1 << 30])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_bad_pages(number, hd):
+    """Keys in a page that is no page of the cache count as NaN for the rows that see them, and nothing is written
+    there; the sequence beside is not touched."""
+    counts, lengths = [40, 3], [150, 90]
+    kc, vc, table, k, v = _store(lengths, 2, hd, 32)
+    table[0, 4] = number  # positions 128 ... 159
+    q = _randn(4, 43, 4, hd)
+    y = ops.cache_attention(q, kc, vc, table, _i32(lengths), _starts(counts))
+    assert torch.isnan(y[18:40]).all()
+    ref, mag = _over_cache(q, k, v, counts, lengths)
+    keep = [*range(18), 40, 41, 42]
+    _check(y[keep], ref[keep], mag[keep])
+    one = ops.cache_attention(q[:2].contiguous(), kc, vc, table, _i32(lengths))
+    assert torch.isnan(one[0]).all() and torch.isfinite(one[1]).all()
+    before = kc.clone(), vc.clone()
+    new = _randn(5, 43, 2, hd)
+    ops.cache_append(new, new, kc, vc, table, _i32(lengths), _starts(counts))
+    for b, n in ((0, 18), (1, 3)):
+        for i in range(n):
+            t = lengths[b] - counts[b] + i
+            for c in before:
+                c[table[b, t // 32].item(), t % 32] = new[(0, 40)[b] + i]
+    for c, want in zip((kc, vc), before):
+        assert torch.equal(c.view(torch.int16), want.view(torch.int16))
+
+
+def test_rows_outside_sequences():
+    """Rows before the first sequence and behind the last are left as they are; starts beyond the rows are cut."""
+    q, k, v = _randn(1, 200, 4, 64), _randn(2, 200, 2, 64), _randn(3, 200, 2, 64)
+    out = torch.full((200, 256), 3.0, dtype=F16, device="cuda")
+    assert ops.packed_attention(q, k, v, _starts([50, 0, 60], 17), out=out) is out
+    _check(out[17:127], *_over_prompts(q[17:127], k[17:127], v[17:127], [50, 0, 60]))
+    assert bool((out[:17] == 3).all()) and bool((out[127:] == 3).all())
+    y = ops.packed_attention(q, k, v, _i32([-5, 150, 1 << 30]))
+    _check(y, *_over_prompts(q, k, v, [150, 50]))
+    kc, vc, table, k, v = _store([70, 900], 2, 64, 16)
+    out.fill_(3.0)
+    ops.cache_attention(q, kc, vc, table, _i32([70, 900]), _starts([30, 90], 5), out=out)
+    _check(out[5:125], *_over_cache(q[5:125], k, v, [30, 90], [70, 900]))
+    assert bool((out[:5] == 3).all()) and bool((out[125:] == 3).all())
+    kept = kc.clone()
+    ops.cache_append(kc[0, :1].expand(4, 2, 64), kc[0, :1].expand(4, 2, 64), kc, vc, table, _i32([0, -3]), _starts([0, 0], 2))
+    assert torch.equal(kept.view(torch.int16), kc.view(torch.int16))
+
+
+def test_lengths_are_cut_to_the_table():
+    kc, vc, table, k, v = _store([64, 32], 2, 64, 16)
+    q = _randn(1, 2, 4, 64)
+    y = ops.cache_attention(q, kc, vc, table[:, :2].contiguous(), _i32([1 << 30, -4]))
+    _check(y, *[torch.cat(x) for x in zip(_attend(q[:1], k[0][:32], v[0][:32], [32]), _attend(q[1:], k[1], v[1], [0]))])
+
+
+def test_strides():
+    """Any strides of q, k, v (copied where the kernels cannot read them) and of the cache."""
+    t, h, hkv, hd = 90, 4, 2, 64
+    base = _randn(1, h, t, hd)
+    q = base.transpose(0, 1)                                        # heads outermost
+    k = _randn(2, t, hkv, 2 * hd)[..., ::2]                         # features not adjacent
+    v = _randn(3, t * hkv * hd + 4)[4:].view(t, hkv, hd)            # not aligned
+    y = ops.packed_attention(q, k, v, _starts([t]))
+    _check(y, *_over_prompts(q, k, v, [t]))
+    shared = _randn(4, t, 1, hd).expand(t, hkv, hd)                 # one key head for all groups
+    _check(ops.packed_attention(q, shared, v, _starts([t])), *_over_prompts(q, shared, v, [t]))
+    kc, vc, table, ks, vs = _store([t, 700], hkv, hd, 32)
+    pages = kc.shape[0]
+    both = torch.empty(pages, 2, hkv, 32, hd, dtype=F16, device="cuda")  # halves of one tensor, heads before tokens
+    k2, v2 = both[:, 0].permute(0, 2, 1, 3), both[:, 1].permute(0, 2, 1, 3)
+    k2.copy_(kc), v2.copy_(vc)
+    wide = torch.zeros(2, 3 * table.shape[1], dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    args = table, _i32([t, 700]), _starts([20, 70])
+    ref = _over_cache(q, ks, vs, [20, 70], [t, 700])
+    _check(ops.cache_attention(q, k2, v2, wide[:, :table.shape[1]], *args[1:]), *ref)
+    _check(ops.cache_attention(q, kc, vc, *args), *ref)
+    new = _randn(6, hkv, t, hd).transpose(0, 1)
+    ops.cache_append(new, v, k2, v2, *args)
+    ops.cache_append(new, v, kc, vc, *args)
+    assert torch.equal(k2.contiguous().view(torch.int16), kc.view(torch.int16))
+    assert torch.equal(v2.contiguous().view(torch.int16), vc.view(torch.int16))
+
+
+def test_offsets_past_32_bits():
+    """Pages and rows whose byte offsets do not fit 32 bits."""
+    page, hkv, hd = 64, 8, 128
+    pages = (5 << 30) // (page * hkv * hd * 2)
+    kc, vc = (torch.empty(pages, page, hkv, hd, dtype=F16, device="cuda") for _ in range(2))
+    table = torch.tensor([[pages - 1, 3, pages - 5], [pages - 2, pages - 3, 0]], dtype=torch.int32)
+    k, v = ([_randn(s + b, 150 - 40 * b, hkv, hd) for b in range(2)] for s in (1, 5))
+    counts, lengths = [150, 110], [150, 110]
+    ops.cache_append(torch.cat(k), torch.cat(v), kc, vc, table.cuda(), _i32(lengths), _starts(counts))
+    for b in range(2):
+        t = torch.arange(lengths[b])
+        where = table[b, t // page].long().cuda(), (t % page).cuda()
+        assert torch.equal(kc[where], k[b]) and torch.equal(vc[where], v[b])
+    q = _randn(9, 2, 16, hd)
+    _check(ops.cache_attention(q, kc, vc, table.cuda(), _i32(lengths)), *_over_cache(q, k, v, [1, 1], lengths))
+    del kc, vc
+    rows = torch.empty(300000, 8192, dtype=F16, device="cuda")  # 4.9 GB: rows of a wide projection
+    rows[-100:] = _randn(3, 100, 8192)
+    q, k, v = (rows[:, 1000 * i + 8:1000 * i + 136].unflatten(1, (2, 64)) for i in range(3))
+    y = ops.packed_attention(q, k, v, _i32([299900, 300000]))
+    _check(y[-100:], *_over_prompts(q[-100:], k[-100:], v[-100:], [100]))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_rising_and_large_scores(dtype, hd):
+    """Scores that rise along the keys, so that the running maximum moves all the time, up to several hundred; the
+    error of a score of that size (2^-24 of the sum of 256 products' magnitudes, far below u) stays within the bound."""
+    n = 700
+    k = _randn(1, n, 1, hd, dtype=dtype)
+    q = k.float().mean(0, keepdim=True).expand(n, 1, hd).to(dtype) * 0 + 1
+    k = (torch.ones(n, 1, hd, device="cuda") * torch.linspace(-2, 2, n, device="cuda")[:, None, None]).to(dtype)
+    v = _randn(2, n, 1, hd, dtype=dtype)
+    y = ops.packed_attention(q, k, v, _starts([n]), scale=0.5)
+    _check(y, *_over_prompts(q, k, v, [n], scale=0.5))
+    kc, vc, table, _, _ = _store([n], 1, hd, 16, dtype)
+    _write(kc, vc, table.cpu(), 0, 0, k, v)
+    one = ops.cache_attention(q[-1:], kc, vc, table, _i32([n]), scale=0.5)
+    _check(one, *_attend(q[-1:], k, v, [n], 0.5))
+
+
+def test_many_small_probabilities():
+    """60000 keys of 2^-25 of the largest probability each: together 0.0018, which fp16 probabilities would lose."""
+    n, hd = 60000, 64
+    k = torch.zeros(n, 1, hd, dtype=F16, device="cuda")
+    k[123, 0, 0] = 25.0
+    v = torch.ones(n, 1, hd, dtype=F16, device="cuda")
+    v[123] = 0
+    kc, vc, table, _, _ = _store([n], 1, hd, 256)
+    _write(kc, vc, table.cpu(), 0, 0, k, v)
+    q = torch.zeros(1, 1, hd, dtype=F16, device="cuda")
+    q[0, 0, 0] = 1.0
+    y = ops.cache_attention(q, kc, vc, table, _i32([n]), scale=0.6931471805599453)
+    _check(y, *_attend(q, k, v, [n], 0.6931471805599453))
+
+
+@pytest.mark.parametrize("batch,hkv,longest", [(1, 1, 3000), (65, 2, 1500), (200, 1, 1200), (512, 1, 900), (600, 1, 900)])
+def test_single_token_batches(batch, hkv, longest):
+    """Batches whose lengths take several steps of a wave to add up, dealt to blocks in shares or not."""
+    lengths = [longest - (longest * b * 37) % longest if b % 5 else b % 3 for b in range(batch)]
+    kc, vc, table, k, v = _store(lengths, hkv, 64, 16)
+    q = _randn(4, batch, 3 * hkv, 64)
+    y = ops.cache_attention(q, kc, vc, table, _i32(lengths))
+    _check(y, *_over_cache(q, k, v, [1] * batch, lengths))
+    assert torch.equal(y, ops.cache_attention(q, kc, vc, table, _i32(lengths)))
+
+
+@pytest.mark.parametrize("counts", [[64] * 40, [20] * 70, [900, 0, 3, 500, 1, 129, 700, 64]])
+def test_many_tiles(counts):
+    """More tiles than blocks fit the chip: heaviest first up to 64 sequences, in order beyond."""
+    h, hkv, hd = 32, 8, 64
+    lengths = [n + (b * 61) % 300 for b, n in enumerate(counts)]
+    kc, vc, table, k, v = _store(lengths, hkv, hd, 64)
+    q = _randn(3, sum(counts), h, hd)
+    y = ops.cache_attention(q, kc, vc, table, _i32(lengths), _starts(counts))
+    _check(y, *_over_cache(q, k, v, counts, lengths))
+    for causal in (True, False):
+        k1, v1 = _randn(5, sum(counts), h, hd), _randn(6, sum(counts), h, hd)
+        _check(ops.packed_attention(q, k1, v1, _starts(counts), causal=causal), *_over_prompts(q, k1, v1, counts, causal))
+
+
+@pytest.mark.parametrize("h", [1, 33, 128])
+def test_one_head_for_all(h):
+    kc, vc, table, k, v = _store([500, 3], 1, 128, 128)
+    for counts in ([1, 1], [4, 2]):
+        q = _randn(2, sum(counts), h, 128)
+        starts = None if counts == [1, 1] else _starts(counts)
+        _check(ops.cache_attention(q, kc, vc, table, _i32([500, 3]), starts), *_over_cache(q, k, v, counts, [500, 3]))
+
+
+def test_nothing_to_do():
+    kc, vc, table, _, _ = _store([5], 2, 64, 16)
+    none = torch.empty(0, 2, 64, dtype=F16, device="cuda")
+    assert ops.packed_attention(none, none, none, _i32([0])).shape == (0, 128)
+    assert ops.packed_attention(none, none, none, _i32([0, 0, 0])).shape == (0, 128)
+    assert ops.cache_attention(none, kc, vc, table, _i32([5]), _i32([0, 0])).shape == (0, 128)
+    assert ops.cache_attention(none, kc, vc, table[:0], _i32([]), _i32([0])).shape == (0, 128)
+    ops.cache_append(none, none, kc, vc, table, _i32([5]), _i32([0, 0]))
+
+
+def test_graphs_and_streams():
+    """A captured step (append and attention, keys in shares) is replayed with other tokens and growing lengths, other
+    work between the replays; two graphs and an eager call on another stream give what eager calls give."""
+    lengths, h, hkv, hd = [1000, 1, 3000], 8, 2, 128
+    kc, vc, table, _, _ = _store([n + 20 for n in lengths], hkv, hd, 16)
+    n = _i32(lengths)
+    qkv = torch.zeros(3, (h + 2 * hkv) * hd, dtype=F16, device="cuda")
+
+    def step():
+        q, k, v = qkv.split([h * hd, hkv * hd, hkv * hd], 1)
+        k, v = k.view(3, hkv, hd), v.view(3, hkv, hd)
+        ops.cache_append(k, v, kc, vc, table, n)
+        return ops.cache_attention(q.view(3, h, hd), kc, vc, table, n)
+
+    step()
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g, pool=graphs[0].pool() if i else None):
+            outs.append(step())
+    side = torch.cuda.Stream()
+    for i in range(4):
+        n.add_(1)
+        qkv.copy_(_randn(10 + i, *qkv.shape))
+        want = step()
+        junk = torch.full((1 << 22,), float("nan"), device="cuda").sum()  # other work, in memory freed meanwhile
+        for g, y in zip(graphs, outs):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            y = step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(y, want) and torch.isnan(junk)
+
+
+def test_prompt_chunks_and_tokens():
+    """A program's run: ragged prompts through a fused projection, whole and in chunks over the cache, then single
+    tokens, each against the attention of the whole sequences in float64."""
+    d, h, hkv, hd, page = 256, 8, 2, 64, 32
+    prompts, new = [50, 200, 7], 4
+    w, b = _randn(1, (h + 2 * hkv) * hd, d) / 16, torch.zeros((h + 2 * hkv) * hd, dtype=F16, device="cuda")
+    total = [n + new for n in prompts]
+    x = [_randn(20 + i, n, d) for i, n in enumerate(total)]
+
+    def project(rows):
+        qkv = ops.linear(rows, w, b)
+        q, k, v = qkv.split([h * hd, hkv * hd, hkv * hd], 1)
+        t = len(rows)
+        return q.view(t, h, hd), k.view(t, hkv, hd), v.view(t, hkv, hd)
+
+    full = [project(s) for s in x]
+    refs = [_attend(q, k, v, torch.arange(1, len(q) + 1)) for q, k, v in full]
+    pages = [-(-n // page) for n in total]
+    table = torch.zeros(3, max(pages), dtype=torch.int32)
+    for i, n in enumerate(pages):
+        table[i, :n] = torch.arange(n, dtype=torch.int32) * 3 + i
+    table = table.cuda()
+    caches = torch.full((2, 3 * max(pages), page, hkv, hd), float("nan"), dtype=F16, device="cuda")
+
+    q, k, v = project(torch.cat([s[:n] for s, n in zip(x, prompts)]))
+    starts, lengths = _starts(prompts), _i32(prompts)
+    y = ops.packed_attention(q, k, v, starts)
+    ops.cache_append(k, v, *caches, table, lengths, starts)
+    again = ops.cache_attention(q, *caches, table, lengths, starts)
+    for whole in (y, again):
+        _check(whole, *[torch.cat([r[i][:n] for r, n in zip(refs, prompts)]) for i in range(2)])
+
+    caches.fill_(float("nan"))  # the same prompts in chunks of 64
+    for first in range(0, max(prompts), 64):
+        counts = [min(max(n - first, 0), 64) for n in prompts]
+        q, k, v = project(torch.cat([s[first:first + c] for s, c in zip(x, counts)]))
+        starts, lengths = _starts(counts), _i32([min(n, first + 64) for n in prompts])
+        ops.cache_append(k, v, *caches, table, lengths, starts)
+        y = ops.cache_attention(q, *caches, table, lengths, starts)
+        _check(y, *[torch.cat([r[i][first:first + c] for r, c in zip(refs, counts)]) for i in range(2)])
+
+    lengths = _i32(prompts)
+    for i in range(new):
+        lengths.add_(1)
+        q, k, v = project(torch.stack([s[n + i] for s, n in zip(x, prompts)]))
+        ops.cache_append(k, v, *caches, table, lengths)
+        y = ops.cache_attention(q, *caches, table, lengths)
+        _check(y, *[torch.stack([r[j][n + i] for r, n in zip(refs, prompts)]) for j in range(2)])
+
+
+def test_refusals():
+    q, k = _randn(1, 8, 4, 64), _randn(2, 8, 2, 64)
+    starts = _starts([8])
+    kc, vc, table, _, _ = _store([8], 2, 64, 16)
+    n = _i32([8])
+    for args in ((q.float(), k.float(), k.float(), starts), (q, k.bfloat16(), k, starts), (q, k, k[:7], starts),
+                 (q[:, :3], k, k, starts), (q, k[..., :32], k[..., :32], starts), (q, k, k, starts.long()),
+                 (q, k, k, starts.cpu()), (q.cpu(), k, k, starts), (q, k, k, starts[:0]), (q, k, k, starts.view(1, 2)),
+                 (q[..., :12], k[..., :12], k[..., :12], starts), (q[0], k, k, starts)):
+        with pytest.raises(ValueError):
+            ops.packed_attention(*args)
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            ops.packed_attention(q, k, k, starts, scale=scale)
+    for out in (torch.empty(8, 255, dtype=F16, device="cuda"), torch.empty(8, 256, device="cuda"),
+                torch.empty(256, 8, dtype=F16, device="cuda").T, torch.empty(8, 256, dtype=F16)):
+        with pytest.raises(ValueError):
+            ops.packed_attention(q, k, k, starts, out=out)
+    for args in ((kc, vc[:1], table, n, starts), (kc, vc, table.long(), n, starts), (kc, vc, table, n.long(), starts),
+                 (kc, vc, table, n, None), (kc, vc, table[:, :0], n, starts), (kc, vc, table, _i32([8, 8]), starts),
+                 (kc[:, :12], vc[:, :12], table, n, starts), (kc[:, :8], vc[:, :8], table, n, starts),
+                 (kc.bfloat16(), vc.bfloat16(), table, n, starts), (kc[:0], vc[:0], table, n, starts),
+                 (kc[..., :32], vc[..., :32], table, n, starts), (kc.transpose(2, 3), vc.transpose(2, 3), table, n, starts)):
+        with pytest.raises(ValueError):
+            ops.cache_attention(q, *args)
+        with pytest.raises(ValueError):
+            ops.cache_append(k, k, *args)
+    odd = torch.empty(kc.numel() + 4, dtype=F16, device="cuda")[4:].view(kc.shape)  # used in place: never copied
+    with pytest.raises(ValueError):
+        ops.cache_attention(q, odd, vc, table, n, starts)
+    with pytest.raises(ValueError):
+        ops.cache_append(k, k, kc, odd, table, n, starts)
+    with pytest.raises(ValueError):
+        ops.cache_attention(q, kc, vc, table, n, starts, max_length=-1)

@@ -28,9 +28,9 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int rows_
   const int r = (token - u.first) * a.group + head - hkv * a.group;
   const int tile = r / rows_per_tile;
   const int share = sh.share, begin = sh.base + tile * u.units;
-  const int first = begin / share, parts = (begin + u.units - 1) / share - first + 1;
+  const int first = (begin + kSeqTileCost) / share, parts = (begin + u.units - 1) / share - first + 1;
   if (parts == 1) return;
-  // part p of the tile belongs to slot first + p: its second entry where the tile begins there, its first otherwise
+  // part p of the tile belongs to slot first + p: its second entry where the keys begin there, its first otherwise
   const int64_t place = (int64_t)hkv * rows_per_tile + r - tile * rows_per_tile, step = 2 * (int64_t)a.kv_heads * rows_per_tile;
   const auto at = [&](int p) -> int64_t { return (first + p) * step + (p == 0 ? step / 2 : 0) + place; };
   float m = -INFINITY;
@@ -178,10 +178,10 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   // keys 9.9 -> 12.4, 1000 14.1 -> 12.7; 2 of 256, 300 keys 15.5 -> 23.4, 1000 31 -> 22.  Six rounds of the block.
   const int alone = 6 * 32 * (p.shape == SeqShape::kDeep ? (head_dim <= 64 ? 8 : head_dim <= 128 ? 4 : 2) : 2);
   if (paged && max_length > alone && batch <= 512 && blocks < (wide ? 1 : 4) * held_blocks &&
-      tiles * (held / kSeqUnit + 1) < (1LL << 31)) {
+      tiles * (held / kSeqUnit + 1 + kSeqTileCost) < (1LL << 31)) {
     p.mode = kSeqShares;
     if (!wide) p.shape = SeqShape::kNarrow;
-    const int64_t units = tiles * ((max_length + kSeqUnit - 1) / kSeqUnit);
+    const int64_t units = tiles * ((max_length + kSeqUnit - 1) / kSeqUnit + kSeqTileCost);
     int64_t slots = held_blocks / kv_heads;
     if (slots > (units + kSeqMinShare - 1) / kSeqMinShare) slots = (units + kSeqMinShare - 1) / kSeqMinShare;
     p.slots = (int)(slots > 1 ? slots : 1);

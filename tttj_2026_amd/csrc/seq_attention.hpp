@@ -102,7 +102,9 @@ constexpr int kSeqInOrder = 0;   // a tile each, the last sequence's last tile f
 constexpr int kSeqHeaviest = 1;  // a tile each, those with most keys first, over all sequences (batch <= 64)
 constexpr int kSeqShares = 2;    // all (tile, 64 keys) units of a kv head in equal shares, one per block
 constexpr int kSeqUnit = 64;
+constexpr int kSeqLevels = 32;
 constexpr int kSeqMinShare = 4;  // units: a smaller share does not pay for joining it
+constexpr int kSeqTileCost = 2;  // units that beginning and ending a tile takes the time of
 
 constexpr float kSeqLazy = 8.0f;   // log2 growth of a row's maximum that moves its reference
 constexpr float kSeqShift = 7.0f;  // log2 of the factor on the probabilities: 2^(8 + 7) < 65504
@@ -201,9 +203,10 @@ __device__ __forceinline__ int wave_max_int(int v) {  // of values >= 0
   return __builtin_amdgcn_readlane(v, 63);
 }
 
-// The tile of rank `rank` by its number of keys, in units of 64 (kSeqHeaviest; lane b holds sequence b): the tiles of a
-// sequence that see more than 64 w keys are those from a certain one on, so their number over all sequences follows
-// from w without a list, and a bisection over w finds the rank's level.  tile < 0: no such tile.
+// The tile of rank `rank` by its number of keys (kSeqHeaviest; lane b holds sequence b): the tiles of a sequence that
+// see more than w units of keys are those from a certain one on, so their number over all sequences follows from w
+// without a list, and a bisection over w finds the rank's level.  A unit is a 32nd of the most keys; within a
+// level, tiles go sequence by sequence.  tile < 0: no such tile.
 template <bool PAGED>
 __device__ __forceinline__ SeqTile seq_ranked(const SeqAttnArgs& a, int rank, int rows_per_tile) {
   const int lane = threadIdx.x & 63, G = a.group;
@@ -214,16 +217,17 @@ __device__ __forceinline__ SeqTile seq_ranked(const SeqAttnArgs& a, int rank, in
     keys = seq_keys<PAGED>(a, lane, own.y);
   }
   const int tiles = (own.y * G + rows_per_tile - 1) / rows_per_tile;
-  // The first tile with a row that sees more than 64 w keys (w < 0: any row).
+  const int unit = (wave_max_int(keys) + kSeqLevels - 1) / kSeqLevels;
+  // The first tile with a row that sees more than w units of keys (w < 0: any row).
   const auto from = [&](int w) -> int {
     if (w < 0) return 0;
-    if (!a.causal) return keys > kSeqUnit * w ? 0 : tiles;
-    const int token = kSeqUnit * w - (keys - own.y);
+    if (!a.causal) return keys > unit * w ? 0 : tiles;
+    const int token = unit * w - (keys - own.y);
     return token <= 0 ? 0 : token >= own.y ? tiles : token * G / rows_per_tile;
   };
   SeqTile s{0, -1, 0, 0};
   if (rank >= wave_sum_int(tiles)) return s;
-  int lo = -1, hi = wave_max_int((keys + kSeqUnit - 1) / kSeqUnit);  // more than `rank` tiles above lo, not above hi
+  int lo = -1, hi = kSeqLevels;  // more than `rank` tiles above lo, not above hi
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (wave_sum_int(tiles - from(mid)) > rank) lo = mid;
@@ -240,8 +244,9 @@ __device__ __forceinline__ SeqTile seq_ranked(const SeqAttnArgs& a, int rank, in
   return s;
 }
 
-// kSeqShares.  A sequence counts tiles x units units, its keys in units of 64 (at least one), whether or not all rows
-// of a tile see them: its new tokens are few against its keys wherever keys are shared out.
+// kSeqShares.  A sequence counts tiles x units units: kSeqTileCost, which hold no keys, and its keys in units of 64 (at
+// least one), whether or not all rows of a tile see them (its new tokens are few against its keys wherever keys are
+// shared out).  A tile's parts are the shares that hold keys of it.
 struct SeqUnits {
   int first, count, keys, tiles, units;
 };
@@ -253,7 +258,7 @@ __device__ __forceinline__ SeqUnits seq_units(const SeqAttnArgs& a, int b, int r
   u.count = own.y;
   u.keys = seq_keys<true>(a, b, own.y);
   u.tiles = (own.y * a.group + rows_per_tile - 1) / rows_per_tile;
-  u.units = max((u.keys + kSeqUnit - 1) / kSeqUnit, 1);
+  u.units = max((u.keys + kSeqUnit - 1) / kSeqUnit, 1) + kSeqTileCost;
   return u;
 }
 
@@ -404,10 +409,12 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     sq.tile = (x - base) / su.units;
     keys = su.keys;
     const int begin = x - base - sq.tile * su.units, end = min(begin + share_end - x, su.units);
-    kbeg = begin * kSeqUnit;
-    if (end < su.units) kend = end * kSeqUnit;
-    if (end - begin < su.units) part = 2 * slot + (begin == 0 ? 1 : 0);
     x += end - begin;
+    if (end <= kSeqTileCost) return;  // nothing but a tile's beginning was left of the share
+    const bool first = begin <= kSeqTileCost;
+    if (!first) kbeg = (begin - kSeqTileCost) * kSeqUnit;
+    if (end < su.units) kend = (end - kSeqTileCost) * kSeqUnit;
+    if (!first || end < su.units) part = 2 * slot + (first ? 1 : 0);
   } else {
     keys = seq_keys<PAGED>(a, sq.seq, sq.count);
   }
