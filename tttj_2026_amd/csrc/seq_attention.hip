@@ -144,10 +144,10 @@ int launch_seq_attention(const SeqAttnArgs& a, bool paged, SeqShape shape, int d
   return launch_seq_hd<32>(a, paged, shape, dtype, stream);
 }
 
-// Blocks of a kernel that a CU holds (its registers and LDS).
+// Blocks of a kernel that a CU holds (its registers, and its LDS: 16, 32, 64 or 128 KiB and a little more each).
 static int seq_resident(bool wide, int head_dim) {
   if (wide) return head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1;
-  return head_dim <= 32 ? 6 : head_dim <= 64 ? 5 : 2;
+  return head_dim <= 32 ? 6 : head_dim <= 64 ? 4 : 2;
 }
 
 // How a call is given to blocks.
@@ -173,10 +173,14 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   p.shape = wide ? SeqShape::kWide : blocks <= cus ? SeqShape::kDeep : SeqShape::kNarrow;
   p.slots = (int)tiles;
   p.mode = kSeqInOrder;
-  // Keys up to which a block takes a tile alone: dealing them out costs a second launch and its parts.  Measured on
-  // MI355X per call, alone -> in shares: 16 heads of 64, 1000 keys 9.3 -> 11.0 us, 2000 12.9 -> 11.5; 8 of 128, 500
-  // keys 9.9 -> 12.4, 1000 14.1 -> 12.7; 2 of 256, 300 keys 15.5 -> 23.4, 1000 31 -> 22.  Six rounds of the block.
-  const int alone = 6 * 32 * (p.shape == SeqShape::kDeep ? (head_dim <= 64 ? 8 : head_dim <= 128 ? 4 : 2) : 2);
+  // Keys up to which a block takes a tile alone, in rounds of the block's waves: dealing keys out costs a second launch,
+  // and parts that are written and read.  Measured on MI355X per call, alone -> in shares: 16 blocks of 8 waves on
+  // heads of 64, 1000 keys (4 rounds) 9.3 -> 11.0 us, 2000 12.9 -> 11.5; 8 blocks of 4 on heads of 128, 500 keys 9.9 ->
+  // 12.4, 1000 (8 rounds) 14.1 -> 12.7.  Blocks that fill a good part of the chip gain less: 256 on heads of 64, 4000
+  // keys (16 rounds) 46 -> 50, 8000 99 -> 105; 128 on heads of 128, 2000 (16) 27 -> 30, 4000 49 -> 48, and with lengths
+  // from 1 to 4000 39 -> 32; 512 of two waves on heads of 128, 1000 keys (16) 43 -> 47, lengths to 4000 125 -> 107.
+  const int keys_per_round = 32 * (p.shape == SeqShape::kDeep ? (head_dim <= 64 ? 8 : head_dim <= 128 ? 4 : 2) : 2);
+  const int alone = (blocks <= cus / 4 ? 6 : 16) * keys_per_round;
   if (paged && max_length > alone && batch <= 512 && blocks < (wide ? 1 : 4) * held_blocks &&
       tiles * (held / kSeqUnit + 1 + kSeqTileCost) < (1LL << 31)) {
     p.mode = kSeqShares;
