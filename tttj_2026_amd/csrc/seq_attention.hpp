@@ -740,15 +740,42 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         add_values(p16, st, h);
       };
       uint32_t bad = 0;
+      // Packed keys: this wave's rows of the next tile, moved on by a tile at a time (working every tile's place out
+      // from its number took the scalar unit some forty instructions more).
+      const char *k_next = nullptr, *v_next = nullptr;
+      if constexpr (!PAGED) {
+        const int64_t row = sq.first + KT + rw * WROWS;
+        k_next = reinterpret_cast<const char*>(kh) + 2 * (row + KLEAD) * a.k_row;
+        v_next = reinterpret_cast<const char*>(vh) + 2 * row * a.v_row;
+      }
+      const auto bytes_of = [&](int left, int row) TT_INLINE -> uint32_t {  // of `left` rows, 16 at most
+        const int n = min(left, 16);
+        return n > 0 ? 2 * ((n - 1) * (uint32_t)row + hd) : 0;
+      };
       auto fetch = [&](int r, int st) TT_INLINE {
         const int t0 = kbeg + r * KT;
         if constexpr (PAGED) bad = bad_groups(pe, t0);
         if (r + 1 >= ntiles) return;
-        pe = pe_next;
-        if constexpr (PAGED) pe_next = tile_pages(t0 + 2 * KT);
-        const Places at = places(pe, t0 + KT);
-        issue_k(at, st ^ 1);
-        issue_v(at, st ^ 1);
+        if constexpr (PAGED) {
+          pe = pe_next;
+          pe_next = tile_pages(t0 + 2 * KT);
+          const Places at = places(pe, t0 + KT);
+          issue_k(at, st ^ 1);
+          issue_v(at, st ^ 1);
+        } else {
+          static_assert(PG == 1, "16 rows of a tile per wave");
+          const int left = keys - (t0 + KT + rw * WROWS);
+          const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(k_next, bytes_of(left - KLEAD, (int)a.k_row));
+          const __amdgpu_buffer_rsrc_t vr = buffer_rsrc(v_next, bytes_of(left, (int)a.v_row));
+          T* const kt = sk + (st ^ 1) * TILE + rw * WROWS * HD;
+          T* const vt = sv + (st ^ 1) * TILE + rw * WROWS * HD;
+#pragma unroll
+          for (int c = 0; c < CPG; ++c) lds_copy16_buf(kr, koff[c], reinterpret_cast<half*>(kt + c * RPC * HD));
+#pragma unroll
+          for (int c = 0; c < CPG; ++c) lds_copy16_buf(vr, voff[c], reinterpret_cast<half*>(vt + c * RPC * HD));
+          k_next += 2 * KT * a.k_row;
+          v_next += 2 * KT * a.v_row;
+        }
       };
       auto whole_tile = [&](int r, int st) TT_INLINE {
         const int t0 = kbeg + r * KT;
@@ -912,7 +939,39 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       }
   }
 
-  // Output rows, or a part's sums: O in units of exp2(m - 7), the maximum in log2 units, the sum.
+  // Whole rows of a wide block go out through LDS, 16 bytes per lane and rows side by side: straight from the
+  // accumulators a store would touch 32 rows, 16 bytes of each.  (16-byte pieces are exchanged within their row by its
+  // number, against bank conflicts.)
+  if constexpr (RW > 1) {
+    if (part < 0) {
+      static_assert(CB == 1, "one block of rows per wave");
+      constexpr int SW = CH < 16 ? CH - 1 : 15;
+      T* const tile = reinterpret_cast<T*>(seq_lds) + rw * 32 * HD;
+      __syncthreads();
+      const float inv = l_row[0] == 0.f ? 0.f : 1.0f / l_row[0];  // no key: zeros
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          typedef T v4 __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<v4*>(tile + col * HD + (((4 * i + g) ^ (col & SW)) * 8 + 4 * hf)) =
+              v4{(T)(o[0][i][4 * g] * inv), (T)(o[0][i][4 * g + 1] * inv), (T)(o[0][i][4 * g + 2] * inv),
+                 (T)(o[0][i][4 * g + 3] * inv)};
+        }
+      lds_done();
+      const int place = tok[0] * a.heads + head[0];  // lane r holds row r's
+      T* const out = static_cast<T*>(a.out) + (int64_t)sq.first * a.heads * hd;
+#pragma unroll
+      for (int e = 0; e < 32 * CH / 64; ++e) {
+        const int r = e * RPC + lane / CH, c = lane % CH;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(tile + r * HD + ((c ^ (r & SW)) * 8));
+        const int to = __shfl(place, r);
+        if (wr0 + r < rows && 8 * c < hd) *reinterpret_cast<u32x4*>(out + (int64_t)to * hd + 8 * c) = x;
+      }
+    }
+  }
+
+  // Other output rows, or a part's sums: O in units of exp2(m - 7), the maximum in log2 units, the sum.
   const int64_t part0 = ((int64_t)part * a.kv_heads + hkv) * R - r0;  // + row
 #pragma unroll
   for (int b = 0; b < CB; ++b) {
@@ -930,7 +989,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       if (hf == 0 && grp == 0) a.part_ml[part0 + r] = make_float2(m_ref[b] * c2, l_row[b]);
       continue;
     }
-    const float inv = l_row[b] == 0.f ? 0.f : 1.0f / l_row[b];  // no key: zeros
+    if constexpr (RW > 1) continue;
+    const float inv = l_row[b] == 0.f ? 0.f : 1.0f / l_row[b];
     T* dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + tok[b]) * a.heads + head[b]) * hd;
 #pragma unroll
     for (int i = 0; i < DB; ++i)
