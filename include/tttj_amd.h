@@ -255,7 +255,8 @@ int tt_attention_fwd_prescaled(const void* q, const void* k, const void* vt, con
  * the end of the last; a token sees the keys of its own sequence, up to itself with `causal`.  Query
  * head h reads key / value head h / (heads / kv_heads).  Strides (`*_row`, `*_head`) are in elements;
  * features are adjacent, and pointers and strides aligned to 16 bytes.  head_dim is a multiple of 8 up
- * to 256, scale positive, dtype TT_FP16 or TT_BF16 for all four tensors.  Rows outside every sequence
+ * to 256, scale positive (below 2e38), dtype TT_FP16 or TT_BF16 for all four tensors.  out overlaps
+ * none of the others.  A row whose scores are all -infinity is +0.0.  Rows outside every sequence
  * are not written.  Values of `starts` outside [0, tokens] are taken as the nearest in it.  No
  * counterpart in the reference, whose attention takes padded batches with as many key heads as query
  * heads (kernels/case8_attention.py:48-206). */
@@ -277,7 +278,8 @@ int tt_packed_attention_fwd(const tt_packed_attention* args, void* stream);
  * lengths [batch] counts the keys of each sequence with the new ones, so that the n rows of sequence b
  * take positions lengths[b] - n ... lengths[b] - 1.  starts as above, or NULL: row b is the one new
  * token of sequence b (tokens == batch).  A token whose position is negative or past table_pages
- * pages, or whose page number is not in [0, pages), is not written.  No counterpart in the reference,
+ * pages, or whose page number is not in [0, pages), is not written.  Of two tokens with one place in
+ * the cache either may stay, in pieces of 16 bytes.  No counterpart in the reference,
  * which keeps no keys between calls. */
 typedef struct {
   int64_t size;

@@ -308,6 +308,46 @@ def test_one_head_for_all(h):
         _check(ops.cache_attention(q, kc, vc, table, _i32([500, 3]), starts), *_over_cache(q, k, v, counts, [500, 3]))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [8, 24, 40, 80, 200])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_padded_heads_in_shares(dtype, hd, n):
+    """Blocks that take several tiles one after the other, of heads that do not fill the tiles' width."""
+    counts = [n - b % n for b in range(120 if n < 40 else 12)]
+    lengths = [2000 if b == 3 else n + (b * 61) % 200 for b in range(len(counts))]
+    kc, vc, table, k, v = _store(lengths, 2, hd, 16, dtype)
+    q = _randn(8, sum(counts), 8, hd, dtype=dtype)
+    y = ops.cache_attention(q, kc, vc, table, _i32(lengths), None if n == 1 else _starts(counts))
+    _check(y, *_over_cache(q, k, v, counts, lengths))
+
+
+def test_shared_pages_and_views():
+    """Two sequences whose first pages are the same ones, described by strided tensors, and a cache of one page."""
+    kc, vc, table, k, v = _store([200, 90], 2, 64, 16)
+    both = table[:1].expand(2, -1)  # row stride 0
+    lengths = _i32([200, 7, 37, 7])[::2]
+    q = _randn(1, 2, 6, 64)
+    y = ops.cache_attention(q, kc, vc, both, lengths)
+    _check(y, *_over_cache(q, [k[0], k[0][:37]], [v[0], v[0][:37]], [1, 1], [200, 37]))
+    wide = torch.stack([table, table], 2)[..., 0]  # column stride 2
+    y = ops.cache_attention(q, kc, vc, wide, _i32([200, 90]), _i32([0, 9, 1, 9, 2])[::2])
+    _check(y, *_over_cache(q, k, v, [1, 1], [200, 90]))
+    one = _i32([[0]])
+    y = ops.cache_attention(q[:1], kc[int(table[1, 0]):][:1], vc[int(table[1, 0]):][:1], one, _i32([16]))
+    _check(y, *_over_cache(q[:1], [k[1][:16]], [v[1][:16]], [1], [16]))
+
+
+def test_falling_starts_write_what_they_can():
+    """Values of `starts` that fall or lie outside the rows (which no caller should pass) stay inside every tensor."""
+    kc, vc, table, k, v = _store([300, 40, 90], 2, 64, 16)
+    q, k1 = _randn(1, 100, 4, 64), _randn(2, 100, 2, 64)
+    for starts in ([0, 60, 30, 100], [-5, 50, 1 << 30, 100], [90, 40, 20, 0]):
+        around = torch.full((300, 256), 7.0, dtype=F16, device="cuda")
+        ops.packed_attention(q, k1, k1, _i32(starts), out=around[100:200])
+        ops.cache_attention(q, kc, vc, table, _i32([300, 40, 90]), _i32(starts), out=around[100:200])
+        assert bool((around[:100] == 7).all()) and bool((around[200:] == 7).all())
+
+
 def test_nothing_to_do():
     kc, vc, table, _, _ = _store([5], 2, 64, 16)
     none = torch.empty(0, 2, 64, dtype=F16, device="cuda")

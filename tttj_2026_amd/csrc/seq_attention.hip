@@ -241,7 +241,7 @@ extern "C" int tt_packed_attention_fwd(const tt_packed_attention* args, void* st
   using namespace tt;
   TT_ARGS(tt_packed_attention, "packed_attention");
   TT_CHECK(check_heads("packed_attention", c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, c.dtype));
-  TT_REQUIRE(c.scale > 0.f && c.scale < 3e38f, "packed_attention: scale %g is not positive and finite", c.scale);
+  TT_REQUIRE(c.scale > 0.f && c.scale < 2e38f, "packed_attention: scale %g is not positive and finite", c.scale);
   if (c.tokens == 0 || c.batch == 0) return TT_OK;
   TT_REQUIRE(c.q && c.k && c.v && c.starts && c.out, "packed_attention: null pointer");
   TT_CHECK(check_rows("packed_attention: q", c.q, c.q_row, c.q_head));
@@ -277,7 +277,7 @@ extern "C" int tt_cache_attention_fwd(const tt_cache_attention* args, void* stre
   TT_ARGS(tt_cache_attention, "cache_attention");
   TT_CHECK(check_heads("cache_attention", c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, c.dtype));
   TT_CHECK(check_pages("cache_attention", c.pages, c.page_size, c.table_pages));
-  TT_REQUIRE(c.scale > 0.f && c.scale < 3e38f, "cache_attention: scale %g is not positive and finite", c.scale);
+  TT_REQUIRE(c.scale > 0.f && c.scale < 2e38f, "cache_attention: scale %g is not positive and finite", c.scale);
   TT_REQUIRE(c.max_length >= 0, "cache_attention: max_length %d", c.max_length);
   if (c.tokens == 0 || c.batch == 0) return TT_OK;
   TT_REQUIRE(c.q && c.k_cache && c.v_cache && c.table && c.lengths && c.out, "cache_attention: null pointer");

@@ -372,12 +372,6 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   const T* const kh = static_cast<const T*>(a.k) + hkv * a.k_head;
   const T* const vh = static_cast<const T*>(a.v) + hkv * a.v_head;
 
-  if (hd < HD) {
-    for (int e = tid; e < 4 * KW * TILE / 8; e += 64 * RW * KW)
-      reinterpret_cast<u32x4*>(seq_lds)[e] = u32x4{0u, 0u, 0u, 0u};
-    __syncthreads();
-  }
-
   const float c2 = a.scale_log2, lazy = kSeqLazy / a.scale_log2;
   // LDS addresses of this lane's pieces of the first K and V block of a stage; the others lie at constant distances.
   // (The empty asm keeps each in one register: the compiler would spread the sums over many.)
@@ -397,6 +391,11 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   for (;;) {
   // (What follows from these is worked out again for each tile instead of being held in registers throughout.)
   asm volatile("" : "+v"(lane), "+v"(hf), "+v"(col));
+  if (hd < HD) {  // the tile before left its sums or rows there
+    for (int e = tid; e < 4 * KW * TILE / 8; e += 64 * RW * KW)
+      reinterpret_cast<u32x4*>(seq_lds)[e] = u32x4{0u, 0u, 0u, 0u};
+    __syncthreads();
+  }
   int keys, kbeg = 0, kend = INT32_MAX, part = -1;
   if (shares) {
     while (x >= base + su.tiles * su.units) {  // the next sequence that has rows

@@ -253,7 +253,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     sequence b owns rows starts[b] ... starts[b + 1] - 1 and sees its own only (with ``causal``, each token those
     up to itself).  Query head h reads key / value head h // (heads // kv_heads).  ``scale`` defaults to
     head_dim^-1/2.  float16 or bfloat16, head_dim a multiple of 8 up to 256; q, k, v may be column slices of one
-    projection's output.  Rows outside every sequence are left as they are in ``out`` (arbitrary in a new tensor)."""
+    projection's output.  Rows outside every sequence are left as they are in ``out`` (arbitrary in a new tensor),
+    which may not overlap the other tensors."""
     dtype, device = _typed(q, "q")
     q, k, v = _rows(q, "q", dtype, device), _rows(k, "k", dtype, device), _rows(v, "v", dtype, device)
     tokens, heads, hd = q.shape
@@ -311,7 +312,8 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Token i of the n new ones of sequence b sees the keys at positions 0 ... lengths[b] - n + i; one that sees none
     (a length of 0 in a padded batch) gets zeros.  Without ``starts`` every sequence has one new token.
     ``max_length`` (default: what the table can hold) is the longest length the caller expects; it only decides how
-    the work is split.  Keys in a page whose number is no page of the cache are not read and count as NaN."""
+    the work is split.  Keys in a page whose number is no page of the cache are not read and count as NaN.  ``out`` may
+    not overlap the other tensors."""
     dtype, device = _typed(q, "q")
     q = _rows(q, "q", dtype, device)
     tokens, heads, hd = q.shape
