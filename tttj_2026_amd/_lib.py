@@ -8,6 +8,7 @@ exports need a gfx950 device.
 from __future__ import annotations
 
 import ctypes
+import functools
 import pathlib
 import struct
 import threading
@@ -131,6 +132,7 @@ def workspace_bytes(batch: int, seq: int, d_model: int, heads: int, ffn_dim: int
     return out.value
 
 
+@functools.lru_cache(maxsize=1024)  # depends on these numbers alone; 0.2 us instead of 1.5
 def cache_attention_workspace_bytes(tokens: int, batch: int, heads: int, kv_heads: int,
                                     head_dim: int, page_size: int, table_pages: int,
                                     max_length: int, single: bool) -> int:

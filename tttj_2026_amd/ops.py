@@ -176,7 +176,7 @@ def _call(name: str, args: bytes, device: torch.device) -> None:
 def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     """``t`` [T, heads, head_dim] in a form the kernels read: adjacent features, rows and heads 16 bytes aligned
     (a column slice of a fused projection's output is; anything else is copied)."""
-    if t.dim() != 3 or t.dtype != dtype or t.device != device:
+    if t.dim() != 3 or t.dtype is not dtype or t.device != device:
         raise ValueError(f"{name} must be a [tokens, heads, head_dim] tensor of {dtype} on {device}")
     row, head, feature = t.stride()
     if feature != 1 or (row | head) & 7 or t.data_ptr() & 15 or row >= 1 << 26:
@@ -185,9 +185,9 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) 
 
 
 def _int32(t: torch.Tensor, name: str, size: int, device: torch.device) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != size:
+    if t.dtype is not torch.int32 or t.device != device or t.shape != (size,):
         raise ValueError(f"{name} must be an int32 tensor of {size} elements on {device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _heads(heads: int, kv_heads: int, hd: int) -> None:
@@ -199,10 +199,10 @@ def _heads(heads: int, kv_heads: int, hd: int) -> None:
 
 def _typed(t: torch.Tensor, name: str):
     """(dtype, device) of a tensor that the others of a call have to match."""
-    dtype, device = t.dtype, t.device
-    if dtype not in _SEQ_DTYPES or device.type != "cuda":
+    dtype = t.dtype
+    if dtype not in _SEQ_DTYPES or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor of float16 or bfloat16")
-    return dtype, device
+    return dtype, t.device
 
 
 def _context(out: Optional[torch.Tensor], tokens: int, width: int, dtype: torch.dtype,
@@ -217,7 +217,7 @@ def _context(out: Optional[torch.Tensor], tokens: int, width: int, dtype: torch.
 
 def _cache(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device: torch.device):
     """Strides of one half of a cache, [pages, page_size, kv_heads, head_dim] (used in place, so never copied)."""
-    if t.dim() != 4 or t.shape[1:] != shape[1:] or t.shape[0] != shape[0] or t.dtype != dtype or t.device != device:
+    if len(shape) != 4 or t.shape != shape or t.dtype is not dtype or t.device != device:
         raise ValueError(f"{name} must be a [pages, page_size, kv_heads, head_dim] tensor of shape {list(shape)} and "
                          f"{dtype} on {device}")
     page, row, head, feature = t.stride()
@@ -231,10 +231,10 @@ def _sequences(tokens: int, page_table: torch.Tensor, lengths: torch.Tensor, sta
     """Checks of the description of a batch over a cache; (page_table, lengths, starts)."""
     batch = lengths.shape[0] if lengths.dim() == 1 else -1
     lengths = _int32(lengths, "lengths", batch, device)
-    if (page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != device
+    if (page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.device != device
             or page_table.shape[0] != batch or page_table.shape[1] == 0):
         raise ValueError(f"page_table must be an int32 tensor [{batch}, pages per sequence] on {device}")
-    if page_table.stride(1) != 1:
+    if not page_table.is_contiguous() and page_table.stride(1) != 1:
         page_table = page_table.contiguous()
     if starts is not None:
         starts = _int32(starts, "starts", batch + 1, device)
