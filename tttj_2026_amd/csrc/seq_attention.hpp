@@ -325,7 +325,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   constexpr int TILE = KT * HD;
   static_assert(WROWS % 16 == 0 && RPC <= 16, "a wave copies whole 16-row groups");
 
-  extern __shared__ __align__(16) char seq_lds[];
+  extern __shared__ __align__(512) char seq_lds[];
 
   const int hkv = blockIdx.x % a.kv_heads;
   const int slot = blockIdx.x / a.kv_heads;
@@ -374,16 +374,19 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
 
   const float c2 = a.scale_log2, lazy = kSeqLazy / a.scale_log2;
   // LDS addresses of this lane's pieces of the first K and V block of a stage; the others lie at constant distances.
-  // (The empty asm keeps each in one register: the compiler would spread the sums over many.)
-  uint32_t kread[KSTEPS], vread[DB];
+  // (The empty asm keeps each in one register: the compiler would spread the sums over many.)  Rows of 512 bytes
+  // leave no registers for them: there the pieces of a row are told apart by an XOR of the first one's address.
+  constexpr bool FAR = PIPE && HD > 128;
+  constexpr int KA = FAR ? 1 : KSTEPS, VA = FAR ? 1 : DB;
+  uint32_t kread[KA], vread[VA];
 #pragma unroll
-  for (int kk = 0; kk < KSTEPS; ++kk) {
+  for (int kk = 0; kk < KA; ++kk) {
     kread[kk] = lds_address(sk + col * HD + kswz<HD>(col, 2 * kk + hf) * 8);
     asm volatile("" : "+v"(kread[kk]));
   }
   const int vrow = 4 * hf + ((lane >> 2) & 3);
 #pragma unroll
-  for (int i = 0; i < DB; ++i) {
+  for (int i = 0; i < VA; ++i) {
     const int c = vseg<HD>(vrow, 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1));
     vread[i] = lds_address(sv + vrow * HD + c * 8 + 4 * (lane & 1));
     asm volatile("" : "+v"(vread[i]));
@@ -562,15 +565,46 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   using Scores = floatx16[CB][SB];
   using Probs = v8[CB][SB][2];
   auto read_k = [&](int kk, int st, int kb) TT_INLINE -> v8 {  // 32 keys, features 16 kk + 8 hf + {0..7}
-    return *(const __attribute__((address_space(3))) v8*)(kread[kk] + 2 * (st * TILE + kb * 32 * HD));
+    const uint32_t stage = 2 * (st * TILE + kb * 32 * HD);
+    const uint32_t at = FAR ? (kread[0] + stage) ^ (32 * kk) : kread[kk] + stage;
+    return *(const __attribute__((address_space(3))) v8*)at;
   };
   auto read_v = [&](int i, int st, int kc) TT_INLINE -> v8 {
     // features 32 i + l % 32; keys 16 kc + 4 hf + {0..3} and 8 further: the order of the lane's probabilities
-    const uint32_t at = vread[i] + 2 * (st * TILE + kc * 16 * HD);
+    const uint32_t stage = 2 * st * TILE, key = 2 * kc * 16 * HD;
+    const uint32_t at = (FAR ? (vread[0] + stage) ^ (64 * i) : vread[i] + stage) + key;
     const shortx4 x0 = read_tr16((const lds_short*)at), x1 = read_tr16((const lds_short*)(at + 16 * HD));
     return __builtin_bit_cast(v8, shortx8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]});
   };
+  // FAR: one wave per SIMD, so nothing else runs while it waits for a fragment.  Fragments are read four products
+  // before theirs (read just before, as registers are too few for the compiler to do otherwise by itself, prompts of
+  // 4 x 4096 tokens on 16 heads of 256 took 1440 us; so 1120).
+  constexpr int AHEAD = 4;
+  auto ahead = [&](auto read, int reads, auto multiply, auto n) TT_INLINE {
+    v8 x[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) x[j] = read(j);
+    if (reads == 1) __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);  // LDS reads
+    else __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      multiply(j, x[j % AHEAD]);
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a product
+      if (j + AHEAD >= n) continue;
+      x[j % AHEAD] = read(j + AHEAD);
+      if (reads == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      else __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+  };
   auto scores = [&](Scores& s, int st, int kb0) TT_INLINE {
+    if constexpr (FAR) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[0][0][e] = 0.f;
+      ahead([&](int kk) TT_INLINE { return read_k(kk, st, kb0); }, 1,
+            [&](int kk, v8 x) TT_INLINE { s[0][0] = Num<T>::mfma(x, qf[0][kk], s[0][0]); },
+            std::integral_constant<int, KSTEPS>{});
+      return;
+    }
 #pragma unroll
     for (int kb = 0; kb < SB; ++kb)
 #pragma unroll
@@ -663,6 +697,12 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         for (int c = 0; c < 2; ++c) asm volatile("" : "+v"(p16[b][kb][c]));
   };
   auto add_values = [&](const Probs& p16, int st, int kb0) TT_INLINE {
+    if constexpr (FAR) {
+      ahead([&](int j) TT_INLINE { return read_v(j % DB, st, 2 * kb0 + j / DB); }, 2,
+            [&](int j, v8 x) TT_INLINE { o[0][j % DB] = Num<T>::mfma(x, p16[0][0][j / DB], o[0][j % DB]); },
+            std::integral_constant<int, 2 * DB>{});
+      return;
+    }
 #pragma unroll
     for (int kb = 0; kb < SB; ++kb)
 #pragma unroll
