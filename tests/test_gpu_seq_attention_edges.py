@@ -321,6 +321,20 @@ def test_padded_heads_in_shares(dtype, hd, n):
     _check(y, *_over_cache(q, k, v, counts, lengths))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [8, 72, 128, 200, 256])
+@pytest.mark.parametrize("counts,lengths,h", [([40], [5000], 4), ([1], [4000], 130), ([60, 3, 200], [2500, 3, 1700], 2)])
+def test_parts_of_wide_tiles(dtype, hd, counts, lengths, h):
+    """Tiles of 128 rows whose keys are split into many or few parts, infinities among the values of the last keys."""
+    kc, vc, table, k, v = _store(lengths, 1, hd, 32, dtype)
+    for b, n in enumerate(lengths):
+        v[b][-1, 0, 0], v[b][-2, 0, hd - 1], v[b][-(counts[b] // 2) - 1, 0, hd // 2] = float("inf"), float("-inf"), float("nan")
+        _write(kc, vc, table.cpu(), b, 0, k[b], v[b])
+    q = _randn(8, sum(counts), h, hd, dtype=dtype)
+    starts = None if counts == [1] else _starts(counts)
+    _check(ops.cache_attention(q, kc, vc, table, _i32(lengths), starts), *_over_cache(q, k, v, counts, lengths))
+
+
 def test_shared_pages_and_views():
     """Two sequences whose first pages are the same ones, described by strided tensors, and a cache of one page."""
     kc, vc, table, k, v = _store([200, 90], 2, 64, 16)

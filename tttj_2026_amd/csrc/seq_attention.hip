@@ -5,6 +5,22 @@
 
 namespace tt {
 
+// The parts that a tile's keys were split into: `parts` of them, part p written by block first + p to its second entry
+// where the tile's keys begin there, and to its first otherwise.
+struct SeqParts {
+  int first, parts;
+};
+
+__device__ __forceinline__ SeqParts seq_parts(const SeqShare& sh, int tile) {
+  const int begin = sh.base + tile * sh.units.units;
+  const int first = (begin + kSeqTileCost) / sh.share;
+  return SeqParts{first, (begin + sh.units.units - 1) / sh.share - first + 1};
+}
+
+__device__ __forceinline__ int64_t seq_entry(const SeqAttnArgs& a, const SeqParts& t, int p, int hkv) {
+  return (2 * (int64_t)(t.first + p) + (p == 0 ? 1 : 0)) * a.kv_heads + hkv;
+}
+
 // out = sum_s w_s O_s / sum_s w_s l_s over the shares s that a row's keys lie in, w_s = 2^(m_s - max m).  W waves per
 // (token, head): head_dim / 4 lanes (rounded up to a power of two) take a part, the parts are dealt to 64 W / that
 // many groups of lanes, four loads of each in flight, and the groups are added up at the end.  Rows of tiles that lie
@@ -27,12 +43,10 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int rows_
   const int hkv = head / a.group;
   const int r = (token - u.first) * a.group + head - hkv * a.group;
   const int tile = r / rows_per_tile;
-  const int share = sh.share, begin = sh.base + tile * u.units;
-  const int first = (begin + kSeqTileCost) / share, parts = (begin + u.units - 1) / share - first + 1;
+  const SeqParts t = seq_parts(sh, tile);
+  const int parts = t.parts;
   if (parts == 1) return;
-  // part p of the tile belongs to slot first + p: its second entry where the keys begin there, its first otherwise
-  const int64_t place = (int64_t)hkv * rows_per_tile + r - tile * rows_per_tile, step = 2 * (int64_t)a.kv_heads * rows_per_tile;
-  const auto at = [&](int p) -> int64_t { return (first + p) * step + (p == 0 ? step / 2 : 0) + place; };
+  const auto at = [&](int p) -> int64_t { return seq_entry(a, t, p, hkv) * rows_per_tile + r - tile * rows_per_tile; };
   float m = -INFINITY;
   for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.part_ml[at(p)].x);
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
@@ -83,6 +97,110 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int rows_
   if (live && lane < lanes)
     *reinterpret_cast<v4*>(static_cast<T*>(a.out) + (int64_t)row * a.head_dim + d) =
         v4{(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+}
+
+// The same for tiles of 128 rows, whose parts lie as wide_place says: W waves per 32 rows and 8 P features, each a
+// W-th of the parts with a maximum and a sum of its own; lanes hold a row and 4 features of each 8.
+template <typename T, int W, int P>
+__global__ __launch_bounds__(64 * W) void seq_merge_wide_kernel(SeqAttnArgs a, int units) {
+  __shared__ floatx4 s_o[W][P][64];
+  __shared__ float2 s_ml[W][64];
+  constexpr int R = 128;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit = (int)blockIdx.x % units, rest = (int)blockIdx.x / units;
+  const int rw = rest & 3, hkv = (rest >> 2) % a.kv_heads;
+  const SeqTile sq = seq_tile(a, (rest >> 2) / a.kv_heads, R);
+  const int r = 32 * rw + (lane & 31), rows = sq.count * a.group - sq.tile * R;  // row of the tile; rows from there on
+  if (sq.tile < 0 || 32 * rw >= rows) return;
+  const SeqParts t = seq_parts(seq_share(a, 0, sq.seq, R), sq.tile);
+  if (t.parts == 1) return;
+  const int d0 = 8 * P * unit, hd = a.head_dim;
+  const int place = wide_place(hd, r, d0 + 4 * (lane >> 5));
+  float m = -INFINITY, l = 0.f;
+  floatx4 o[P];
+#pragma unroll
+  for (int g = 0; g < P; ++g) o[g] = floatx4{0.f, 0.f, 0.f, 0.f};
+  // A part (or a wave) without a maximum saw no key (its sum, 0, is its weight) or only NaN (NaN is).
+  const auto weight = [&](float2 ml) -> float {
+    return ml.x == -INFINITY ? ml.y : __builtin_amdgcn_exp2f(ml.x - m);
+  };
+  const bool own = r < rows;  // entries of rows behind the last are not written
+  for (int p0 = wave; p0 < t.parts; p0 += 4 * W) {
+    float2 y[4];
+    floatx4 v[4][P];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t e = seq_entry(a, t, min(p0 + i * W, t.parts - 1), hkv) * R;
+      y[i] = make_float2(-INFINITY, 0.f);
+      if (own) y[i] = a.part_ml[e + r];
+#pragma unroll
+      for (int g = 0; g < P; ++g) {
+        v[i][g] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (own && d0 + 8 * g < hd) v[i][g] = *reinterpret_cast<const floatx4*>(a.part_o + e * hd + place + 256 * g);
+      }
+    }
+    float m_new = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (p0 + i * W < t.parts) m_new = fmaxf(m_new, y[i].x);
+    const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+    m = m_new;
+    l *= corr;
+#pragma unroll
+    for (int g = 0; g < P; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[g][e] *= corr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (p0 + i * W >= t.parts) break;
+      const float w = weight(y[i]);
+      l = fmaf(w, y[i].y, l);
+#pragma unroll
+      for (int g = 0; g < P; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[g][e] = fmaf(w, v[i][g][e], o[g][e]);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < P; ++g) s_o[wave][g][lane] = o[g];
+  s_ml[wave][lane] = make_float2(m, l);
+  __syncthreads();
+  if (wave >= P || !own || d0 + 8 * wave >= hd) return;
+  float2 y[W];
+  m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    y[w] = s_ml[w][lane];
+    m = fmaxf(m, y[w].x);
+  }
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const float f = weight(y[w]);
+    const floatx4 x = s_o[w][wave][lane];
+    l = fmaf(f, y[w].y, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, x[e], sum[e]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const int row = sq.tile * R + r, token = row / a.group;
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<v4*>(static_cast<T*>(a.out) +
+                         ((int64_t)(sq.first + token) * a.heads + hkv * a.group + row - token * a.group) * hd + d0 +
+                         8 * wave + 4 * (lane >> 5)) =
+      v4{(T)(sum[0] * inv), (T)(sum[1] * inv), (T)(sum[2] * inv), (T)(sum[3] * inv)};
+}
+
+template <typename T>
+static int launch_seq_merge_wide(const SeqAttnArgs& a, int tiles, bool many_parts, hipStream_t stream) {
+  const int pieces = a.head_dim / 8, units = many_parts ? pieces : (pieces + 3) / 4;
+  const int blocks = tiles * a.kv_heads * 4 * units;
+  if (many_parts)
+    hipLaunchKernelGGL((seq_merge_wide_kernel<T, 16, 1>), dim3(blocks), dim3(1024), 0, stream, a, units);
+  else
+    hipLaunchKernelGGL((seq_merge_wide_kernel<T, 4, 4>), dim3(blocks), dim3(256), 0, stream, a, units);
+  return launch_status("seq_merge_wide_kernel");
 }
 
 template <typename T>
@@ -154,6 +272,7 @@ static int seq_resident(bool wide, int head_dim) {
 struct SeqPlan {
   SeqShape shape;
   int rows;  // of a block
+  int tiles;  // per kv head, at most
   int slots, mode;
   int64_t part_rows;  // rows of the workspace
   bool many_parts;
@@ -171,7 +290,7 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   const int64_t tiles = single ? tokens * ((G + p.rows - 1) / p.rows) : tokens * G / p.rows + batch;
   const int64_t blocks = tiles * kv_heads, held_blocks = (int64_t)seq_resident(wide, head_dim) * cus;
   p.shape = wide ? SeqShape::kWide : blocks <= cus ? SeqShape::kDeep : SeqShape::kNarrow;
-  p.slots = (int)tiles;
+  p.tiles = p.slots = (int)tiles;
   p.mode = kSeqInOrder;
   // Keys up to which a block takes a tile alone, in rounds of the block's waves: dealing keys out costs a second launch,
   // and parts that are written and read.  Measured on MI355X per call, alone -> in shares: 16 blocks of 8 waves on
@@ -307,6 +426,9 @@ extern "C" int tt_cache_attention_fwd(const tt_cache_attention* args, void* stre
   a.part_ml = reinterpret_cast<float2*>(a.part_o + p.part_rows * c.head_dim);
   TT_CHECK(launch_seq_attention(a, true, p.shape, c.dtype, (hipStream_t)stream));
   if (p.mode != kSeqShares) return TT_OK;
+  if (p.shape == SeqShape::kWide)
+    return c.dtype == TT_FP16 ? launch_seq_merge_wide<half>(a, p.tiles, p.many_parts, (hipStream_t)stream)
+                              : launch_seq_merge_wide<bf16>(a, p.tiles, p.many_parts, (hipStream_t)stream);
   return c.dtype == TT_FP16 ? launch_seq_merge<half>(a, p.rows, p.many_parts, (hipStream_t)stream)
                           : launch_seq_merge<bf16>(a, p.rows, p.many_parts, (hipStream_t)stream);
 }

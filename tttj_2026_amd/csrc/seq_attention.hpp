@@ -93,9 +93,16 @@ struct SeqAttnArgs {
   float scale_log2;        // c log2(e)
   int slots;               // blocks of the launch per kv head
   int mode;                // kSeqInOrder, kSeqHeaviest or kSeqShares
-  float* part_o;           // kSeqShares: [2 slots][kv_heads][R][head_dim], the rows of tiles that lie in several shares
+  float* part_o;           // kSeqShares: [2 slots][kv_heads][R * head_dim], the rows of tiles that lie in several shares
   float2* part_ml;         // ... [2 slots][kv_heads][R], their maximum (log2 domain) and sum
 };
+
+// Where feature d of row r of a tile lies in a part of 128 rows: as the lanes hold them, 32 rows x 8 features in turn, so
+// that every store is one run of 1 KiB (in rows of features, where a store touches 32 rows, 16 chunks of 128 rows on heads
+// of 256 over 4096 keys took 33 us + 10 to join; so 29 + 8).
+__device__ __forceinline__ int wide_place(int head_dim, int r, int d) {
+  return (((r >> 5) * (head_dim >> 3) + (d >> 3)) * 64 + ((d >> 2) & 1) * 32 + (r & 31)) * 4 + (d & 3);
+}
 
 // How row tiles are given to blocks.
 constexpr int kSeqInOrder = 0;   // a tile each, the last sequence's last tile first
@@ -1017,13 +1024,14 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     const int r = wr0 + 32 * b + col;
     if (r >= rows) continue;
     if (part >= 0) {
-      float* dst = a.part_o + (part0 + r) * hd;
+      float* const dst = RW > 1 ? a.part_o + (part0 + r0) * hd + wide_place(hd, r - r0, 4 * hf)
+                                : a.part_o + (part0 + r) * hd + 4 * hf;
 #pragma unroll
       for (int i = 0; i < DB; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           if (32 * i + 8 * g < hd && (i * 4 + g) % KW == grp)
-            *reinterpret_cast<floatx4*>(dst + 32 * i + 8 * g + 4 * hf) =
+            *reinterpret_cast<floatx4*>(dst + (4 * i + g) * (RW > 1 ? 256 : 8)) =
                 floatx4{o[b][i][4 * g], o[b][i][4 * g + 1], o[b][i][4 * g + 2], o[b][i][4 * g + 3]};
       if (hf == 0 && grp == 0) a.part_ml[part0 + r] = make_float2(m_ref[b] * c2, l_row[b]);
       continue;
@@ -1063,7 +1071,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           const int token = r / G;
           if (key >= seq_limit(a, token, sq.count, keys)) continue;
           if (part >= 0) {
-            a.part_o[(part0 + r) * hd + d] += (float)y;
+            a.part_o[RW > 1 ? (part0 + r0) * hd + wide_place(hd, r - r0, d) : (part0 + r) * hd + d] += (float)y;
           } else {
             T* const dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + token) * a.heads + hkv * G + r - token * G) * hd + d;
             *dst = (T)((float)*dst + (float)y);
