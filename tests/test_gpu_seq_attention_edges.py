@@ -323,7 +323,7 @@ def test_padded_heads_in_shares(dtype, hd, n):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("hd", [8, 72, 128, 200, 256])
-@pytest.mark.parametrize("counts,lengths,h", [([40], [5000], 4), ([1], [4000], 130), ([60, 3, 200], [2500, 3, 1700], 2)])
+@pytest.mark.parametrize("counts,lengths,h", [([40], [5000], 4), ([16], [17000], 8), ([1], [4000], 130), ([60, 3, 200], [2500, 3, 1700], 2)])
 def test_parts_of_wide_tiles(dtype, hd, counts, lengths, h):
     """Tiles of 128 rows whose keys are split into many or few parts, infinities among the values of the last keys."""
     kc, vc, table, k, v = _store(lengths, 1, hd, 32, dtype)

@@ -24,7 +24,9 @@ __device__ __forceinline__ int64_t seq_entry(const SeqAttnArgs& a, const SeqPart
 // out = sum_s w_s O_s / sum_s w_s l_s over the shares s that a row's keys lie in, w_s = 2^(m_s - max m).  W waves per
 // (token, head): head_dim / 4 lanes (rounded up to a power of two) take a part, the parts are dealt to 64 W / that
 // many groups of lanes, four loads of each in flight, and the groups are added up at the end.  Rows of tiles that lie
-// in one share were written by its block.
+// in one share were written by its block.  Bound by latency, that of five loads which depend on one another (first rows,
+// lengths, sums, sums' weights): 5.9 us for 64 tokens on 32 heads of 128 (2 MiB read), 6.1 us for 4 tokens on
+// 64 heads with 17 parts each (3 MiB).
 template <typename T, int W>
 __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int rows_per_tile, int lanes) {
   __shared__ float s_sum[W > 1 ? W : 1][W > 1 ? 64 : 1][5];
@@ -100,7 +102,8 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int rows_
 }
 
 // The same for tiles of 128 rows, whose parts lie as wide_place says: W waves per 32 rows and 8 P features, each a
-// W-th of the parts with a maximum and a sum of its own; lanes hold a row and 4 features of each 8.
+// W-th of the parts with a maximum and a sum of its own; lanes hold a row and 4 features of each 8.  Bound by latency as
+// above where parts are few, then by reading them: 9.2 us for 3 chunks on heads of 256 (31 MiB, 3.2 TB/s).
 template <typename T, int W, int P>
 __global__ __launch_bounds__(64 * W) void seq_merge_wide_kernel(SeqAttnArgs a, int units) {
   __shared__ floatx4 s_o[W][P][64];
@@ -224,7 +227,9 @@ struct AppendArgs {
   int pages, table_pages, page_shift;
 };
 
-// One wave per token: its K and V rows go to their place in the cache.
+// One wave per token: its K and V rows go to their place in the cache, 16 bytes a lane.  No computation: bound by HBM
+// (36000 tokens on 8 heads of 128 45 us, 6.5 TB/s read and written, with part of it in the last level cache; 59 us a call
+// in a stream of such calls), and by the call for few (64 tokens: 3.3 us of 9.4).
 __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
   const int lane = threadIdx.x & 63;
   const int token = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -268,7 +273,7 @@ static int seq_resident(bool wide, int head_dim) {
   return head_dim <= 32 ? 6 : head_dim <= 64 ? 4 : 2;
 }
 
-// How a call is given to blocks.
+// How a call is given to blocks.  Figures: MI355X, us per call, heads of 128 unless another width is named.
 struct SeqPlan {
   SeqShape shape;
   int rows;  // of a block
@@ -285,10 +290,15 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   const int64_t G = heads / kv_heads;
   const int cus = device_cus();
   const bool paged = max_length >= 0;
+  // 128 rows share every tile of keys that they read, 32 rows waste fewer products on rows that are not there.  With
+  // 40 / 64 / 96 rows a sequence, 16 sequences of 2000 keys on 4 heads: 32-row tiles 27.8 / 28.3 / 28.4, 128-row tiles
+  // 27.9 / 29 / 32; but 64 rows over 4000 keys, 64 sequences on 8 heads: 377 and 191 (every key is read twice).
   const bool wide = !paged || (single ? G > 32 : tokens * G > 32 * (int64_t)batch);
   p.rows = wide ? 128 : 32;
   const int64_t tiles = single ? tokens * ((G + p.rows - 1) / p.rows) : tokens * G / p.rows + batch;
   const int64_t blocks = tiles * kv_heads, held_blocks = (int64_t)seq_resident(wide, head_dim) * cus;
+  // Up to a block per CU the waves of a block are as many as its LDS feeds, else two: 16 sequences of 4 tokens, 1000 keys
+  // on 4 heads of 64, 17.4 with two waves and 12.3 with eight; 16 drafts of 1 to 7 tokens, to 2100 keys, 28.3 and 14.8.
   p.shape = wide ? SeqShape::kWide : blocks <= cus ? SeqShape::kDeep : SeqShape::kNarrow;
   p.tiles = p.slots = (int)tiles;
   p.mode = kSeqInOrder;
@@ -300,6 +310,8 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   // from 1 to 4000 39 -> 32; 512 of two waves on heads of 128, 1000 keys (16) 43 -> 47, lengths to 4000 125 -> 107.
   const int keys_per_round = 32 * (p.shape == SeqShape::kDeep ? (head_dim <= 64 ? 8 : head_dim <= 128 ? 4 : 2) : 2);
   const int alone = (blocks <= cus / 4 ? 6 : 16) * keys_per_round;
+  // Beyond the blocks that the chip holds (four times as many of 32 rows), tiles spread by themselves: 1088 tiles of 128
+  // rows over 500 to 4600 keys, 195 alone and 272 in shares; 800 of 32 rows over 1 to 4000 keys, 193 and 162.
   if (paged && max_length > alone && batch <= 512 && blocks < (wide ? 1 : 4) * held_blocks &&
       tiles * (held / kSeqUnit + 1 + kSeqTileCost) < (1LL << 31)) {
     p.mode = kSeqShares;
@@ -309,8 +321,13 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
     if (slots > (units + kSeqMinShare - 1) / kSeqMinShare) slots = (units + kSeqMinShare - 1) / kSeqMinShare;
     p.slots = (int)(slots > 1 ? slots : 1);
     p.part_rows = 2 * (int64_t)p.slots * kv_heads * p.rows;
-    p.many_parts = p.slots > 8 * tiles && tokens * heads <= 2048;
+    // Many parts of few rows are joined by more waves each: one chunk of 16 tokens over 30000 keys on one head (8 query
+    // heads) 29.4 -> 23.5, but 4 of them over 8000 keys on 8 heads (16 parts a tile) 35 -> 48; 4 single tokens over
+    // 100000 keys 287 -> 284.5, but 64 over 1 to 4000 keys 106 -> 107.5.
+    p.many_parts = p.slots > (wide ? 32 : 8) * tiles && tokens * heads <= 2048;
   } else if (!single && batch <= 64 && blocks > held_blocks && tokens * G < (1LL << 30)) {
+    // More tiles than the chip holds: the last to start should be the shortest.  2 prompts of 4096 tokens on 16 heads of
+    // 64 in order 106, heaviest first 91; 12 prompts of very different lengths 123 and 123.
     p.mode = kSeqHeaviest;
   }
   return p;

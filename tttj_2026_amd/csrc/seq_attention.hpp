@@ -8,11 +8,24 @@
 // so one tile of K and V serves all heads of its group, and the rows of a tile span few tokens, which keeps the
 // part of a causal tile that is computed and masked small.
 //
-// A block owns 32 RW rows of one (sequence, kv head) and a range of keys.  Its waves form KW groups of RW: the waves
-// of a group share key tiles of KT keys, staged in LDS two deep, and each owns 32 rows; the groups take alternate
-// tiles and are merged through LDS at the end.  RW 4, KW 1 is the tile for many rows (bound by the matrix unit and
-// exp), RW 1 with KW 2 or 4 the one for single tokens (bound by HBM: every wave streams tiles of its own, without a
-// barrier).  Keys are also split over blocks where rows are few; seq_merge_kernel joins those parts.
+// A block takes tiles of 32 RW rows of one (sequence, kv head), and of each all keys or a range.  Its waves form KW groups
+// of RW: the waves of a group share key tiles of KT keys, staged in LDS two deep, and each owns 32 rows; the groups
+// take alternate tiles and are joined through LDS at the end.
+// * RW 4, KW 1, KT 64 (wide: prompts and chunks).  Bound by the matrix unit and the vector instructions of the softmax
+//   beside it: one 32x32x16 product leaves room for about four of them, and 5.6 to 8 are needed (heads of 128).  The exps
+//   of 32 keys run beside the products Q K^T of the next 32, so K is staged 32 keys ahead of V.
+// * RW 1, KT 32, KW 2 (narrow; 1 above heads of 128) and, where blocks are few, KW 8 / 4 / 2 (deep; heads to 64 / 128 /
+//   256): single tokens and drafts.  Bound by HBM: every wave streams tiles of its own without a barrier, close to two
+//   in flight.  KW 1 / 2 / 4 for 64 tokens over 1 to 4000 keys on 8 heads of 128: 130 / 108 / 117 us.
+// How tiles are given to blocks: kSeq... below.  Where a tile's keys are split over blocks, parts of O with a maximum and
+// a sum each go through a workspace, and the seq_merge kernels join them.
+//
+// Measured on MI355X: prompts of 8192 and 3130 tokens, causal, 32 heads of 128 on 8, bf16: 600 us, 1.05 PFLOP/s (matrix
+// unit 55% busy, vector units 46%, at the power limit: 1.83 to 1.94 GHz); 2 x 4096 tokens on 16 heads of 64 90 us, 0.77
+// PFLOP/s; 12 prompts of 85 to 1500 tokens 115 us, 0.69 (a block takes 7 us to start and end, 1.8 us a tile of keys); 4 x
+// 4096 on 16 heads of 256 625 us, 0.88 PFLOP/s; 512 new tokens each for 8 sequences of up to 4608 keys 191 us, 0.86
+// PFLOP/s (2.1 us a tile: pages are looked up beside it).  4 tokens over 100000 keys each, 8 heads of 128: 285 us, 5.8 TB/s; 64
+// over 1 to 4000: 105 us.
 //
 // Per wave and tile: S^T = K Q^T with v_mfma_f32_32x32x16 (lane l holds row l % 32; of its 32 keys per block those
 // with bit 2 equal to l / 32), softmax with a running maximum and sum in fp32, O^T += V^T P^T.  K and V stay in the
@@ -110,8 +123,9 @@ constexpr int kSeqHeaviest = 1;  // a tile each, those with most keys first, ove
 constexpr int kSeqShares = 2;    // all (tile, 64 keys) units of a kv head in equal shares, one per block
 constexpr int kSeqUnit = 64;
 constexpr int kSeqLevels = 32;
-constexpr int kSeqMinShare = 4;  // units: a smaller share does not pay for joining it
-constexpr int kSeqTileCost = 2;  // units that beginning and ending a tile takes the time of
+constexpr int kSeqMinShare = 4;  // units (4 / 6 / 8 / 12: chunks of 3 prompts on heads of 256 37.7 / 42 / 45.6 / 57 us)
+constexpr int kSeqTileCost = 2;  // units that a tile's beginning and end take the time of (0 / 2 / 4: the same chunks 45.8
+                                 // / 38.6 / 39.5 us, 64 tokens over 1 to 4000 keys 106.6 / 105 / 107)
 
 constexpr float kSeqLazy = 8.0f;   // log2 growth of a row's maximum that moves its reference
 constexpr float kSeqShift = 7.0f;  // log2 of the factor on the probabilities: 2^(8 + 7) < 65504
@@ -771,7 +785,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         pin(p16);
         __builtin_amdgcn_sched_barrier(0);
         mask_scores(sn, t0 + 32 * (h + 1), bad >> (2 * h + 2));
-        __builtin_amdgcn_s_setprio(1);
+        __builtin_amdgcn_s_setprio(1);  // (prompts take 1 to 3% longer without)
         add_sums(p16);
         add_values(p16, st, h);
         row_max(sn, mt);
