@@ -328,10 +328,11 @@ __device__ __forceinline__ SeqShare seq_share(const SeqAttnArgs& a, int slot, in
   }
 }
 
-template <typename T, int HD, int CB, int RW, int KW, int KT, bool PAGED, int WPE = (HD <= 64 ? 3 : HD <= 128 ? 2 : 1)>
+template <typename T, int HD, int RW, int KW, int KT, bool PAGED, int WPE = (HD <= 64 ? 3 : HD <= 128 ? 2 : 1)>
 __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void seq_attention_kernel(SeqAttnArgs a) {
   using v2 = typename Num<T>::v2;
   using v8 = typename Num<T>::v8;
+  constexpr int CB = 1;                     // 32-row blocks of a wave (2 leave registers for one wave per SIMD only)
   constexpr int WR = 32 * CB;               // rows of a wave
   constexpr int R = WR * RW;
   constexpr bool PIPE = RW > 1;              // softmax beside the next keys' products

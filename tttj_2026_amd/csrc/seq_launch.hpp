@@ -12,7 +12,7 @@ namespace tt {
 // or two waves; and of 32 rows with as many waves as the LDS holds tiles for, where blocks are few.
 enum class SeqShape { kWide, kNarrow, kDeep };
 
-template <typename T, int HD, int CB, int RW, int KW, int KT, bool PAGED>
+template <typename T, int HD, int RW, int KW, int KT, bool PAGED>
 int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
   constexpr int lds = 2 * 2 * KW * KT * HD * (int)sizeof(T);  // K and V, two tiles deep
   static_assert(KW == 1 || lds >= KW * (HD / 8 * 64 * 16 + 32 * 8), "the groups are joined in the tiles' LDS");
@@ -21,7 +21,7 @@ int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
   TT_HIP(hipGetDevice(&dev));
   const uint64_t bit = 1ull << (dev & 63);
   if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
-    TT_HIP(hipFuncSetAttribute((const void*)seq_attention_kernel<T, HD, CB, RW, KW, KT, PAGED>,
+    TT_HIP(hipFuncSetAttribute((const void*)seq_attention_kernel<T, HD, RW, KW, KT, PAGED>,
                                hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
@@ -29,17 +29,17 @@ int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
   constexpr int threads = 64 * RW * KW;
   TT_REQUIRE(blocks * threads < (1LL << 32), "attention: %lld blocks are more than one launch takes",
              (long long)blocks);
-  hipLaunchKernelGGL((seq_attention_kernel<T, HD, CB, RW, KW, KT, PAGED>), dim3((unsigned)blocks), dim3(threads), lds,
+  hipLaunchKernelGGL((seq_attention_kernel<T, HD, RW, KW, KT, PAGED>), dim3((unsigned)blocks), dim3(threads), lds,
                      stream, a);
   return launch_status("seq_attention_kernel");
 }
 
 template <int HD, typename T>
 int launch_seq_type(const SeqAttnArgs& a, bool paged, SeqShape shape, hipStream_t stream) {
-  if (!paged) return launch_seq<T, HD, 1, 4, 1, 64, false>(a, stream);
-  if (shape == SeqShape::kDeep) return launch_seq<T, HD, 1, 1, (HD <= 64 ? 8 : HD <= 128 ? 4 : 2), 32, true>(a, stream);
-  if (shape == SeqShape::kNarrow) return launch_seq<T, HD, 1, 1, (HD <= 128 ? 2 : 1), 32, true>(a, stream);
-  return launch_seq<T, HD, 1, 4, 1, 64, true>(a, stream);
+  if (!paged) return launch_seq<T, HD, 4, 1, 64, false>(a, stream);
+  if (shape == SeqShape::kDeep) return launch_seq<T, HD, 1, (HD <= 64 ? 8 : HD <= 128 ? 4 : 2), 32, true>(a, stream);
+  if (shape == SeqShape::kNarrow) return launch_seq<T, HD, 1, (HD <= 128 ? 2 : 1), 32, true>(a, stream);
+  return launch_seq<T, HD, 4, 1, 64, true>(a, stream);
 }
 
 template <int HD>
