@@ -241,6 +241,16 @@ def test_offsets_past_32_bits():
     _check(y[-100:], *_over_prompts(q[-100:], k[-100:], v[-100:], [100]))
 
 
+def test_output_offsets_past_32_bits():
+    """An output of more than 2^31 elements, of query rows that are one row (stride 0)."""
+    t, hd = 70000, 64
+    h, n = 512, 5
+    q = _randn(2, 1, h, hd).expand(t, -1, -1)  # row stride 0
+    k, v = _randn(3, t, 1, hd), _randn(4, t, 1, hd)
+    y = ops.packed_attention(q, k, v, _i32([t - n, t]))
+    _check(y[-n:], *_over_prompts(q[-n:], k[-n:], v[-n:], [n]))
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_rising_and_large_scores(dtype, hd):
