@@ -155,16 +155,17 @@ def attention(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, mask: Optional
 
 _SEQ_DTYPES = {torch.float16: _lib.FP16, torch.bfloat16: _lib.BF16}
 
-# The current stream of a device as an integer, without a Stream object (0.1 us instead of 2).
+# The current device, and a device's current stream as an integer, without the objects around them (0.1 us instead of
+# 0.3 and 2).
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call(name: str, args: bytes, device: torch.device) -> None:
-    """One library call with packed arguments, on the current stream of ``device``."""
-    index, before = device.index, torch.cuda.current_device()
+def _call(name: str, args: bytes, index: int) -> None:
+    """One library call with packed arguments, on the current stream of device ``index``."""
     fn = getattr(_lib.load(), name)
-    if index == before:
+    if index == _current_device():
         rc = fn(args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -173,20 +174,36 @@ def _call(name: str, args: bytes, device: torch.device) -> None:
         _lib.check(rc, name)
 
 
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """``t`` [T, heads, head_dim] in a form the kernels read: adjacent features, rows and heads 16 bytes aligned
-    (a column slice of a fused projection's output is; anything else is copied)."""
-    if t.dim() != 3 or t.dtype is not dtype or t.device != device:
-        raise ValueError(f"{name} must be a [tokens, heads, head_dim] tensor of {dtype} on {device}")
+# The small calls below take a third of their time on the host to look their tensors over, so each attribute is asked
+# for once and handed on.
+
+def _typed(t: torch.Tensor, name: str):
+    """(dtype, device index) of a tensor that the others of a call have to match."""
+    dtype = t.dtype
+    if dtype not in _SEQ_DTYPES or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor of float16 or bfloat16")
+    return dtype, t.get_device()
+
+
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, index: int):
+    """(tensor, shape, pointer, row stride, head stride) of ``t`` [T, heads, head_dim] in a form the kernels read:
+    adjacent features, rows and heads 16 bytes aligned (a column slice of a fused projection's output is; anything else
+    is copied)."""
+    shape = t.shape
+    if len(shape) != 3 or t.dtype is not dtype or t.get_device() != index:
+        raise ValueError(f"{name} must be a [tokens, heads, head_dim] tensor of {dtype} on cuda:{index}")
     row, head, feature = t.stride()
-    if feature != 1 or (row | head) & 7 or t.data_ptr() & 15 or row >= 1 << 26:
+    pointer = t.data_ptr()
+    if feature != 1 or (row | head) & 7 or pointer & 15 or row >= 1 << 26:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        row, head, _ = t.stride()
+        pointer = t.data_ptr()
+    return t, shape, pointer, row, head
 
 
-def _int32(t: torch.Tensor, name: str, size: int, device: torch.device) -> torch.Tensor:
-    if t.dtype is not torch.int32 or t.device != device or t.shape != (size,):
-        raise ValueError(f"{name} must be an int32 tensor of {size} elements on {device}")
+def _int32(t: torch.Tensor, name: str, size: int, index: int) -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.get_device() != index or t.shape != (size,):
+        raise ValueError(f"{name} must be an int32 tensor of {size} elements on cuda:{index}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -197,50 +214,49 @@ def _heads(heads: int, kv_heads: int, hd: int) -> None:
         raise ValueError(f"head_dim {hd} is not a multiple of 8 from 8 to 256")
 
 
-def _typed(t: torch.Tensor, name: str):
-    """(dtype, device) of a tensor that the others of a call have to match."""
-    dtype = t.dtype
-    if dtype not in _SEQ_DTYPES or not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor of float16 or bfloat16")
-    return dtype, t.device
-
-
-def _context(out: Optional[torch.Tensor], tokens: int, width: int, dtype: torch.dtype,
-             device: torch.device) -> torch.Tensor:
+def _context(out: Optional[torch.Tensor], q: torch.Tensor, tokens: int, width: int) -> torch.Tensor:
     if out is None:
-        return torch.empty((tokens, width), dtype=dtype, device=device)
-    if (out.shape != (tokens, width) or out.dtype != dtype or out.device != device or not out.is_contiguous()
+        return q.new_empty((tokens, width))
+    if (out.shape != (tokens, width) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous()
             or out.data_ptr() & 15):
-        raise ValueError(f"out must be a contiguous, 16-byte aligned [{tokens}, {width}] tensor of {dtype} on {device}")
+        raise ValueError(f"out must be a contiguous, 16-byte aligned [{tokens}, {width}] tensor of {q.dtype} on "
+                         f"{q.device}")
     return out
 
 
-def _cache(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device: torch.device):
-    """Strides of one half of a cache, [pages, page_size, kv_heads, head_dim] (used in place, so never copied)."""
-    if len(shape) != 4 or t.shape != shape or t.dtype is not dtype or t.device != device:
+def _cache(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int):
+    """(pointer, page, token and head strides) of one half of a cache, [pages, page_size, kv_heads, head_dim] (used in
+    place, so never copied)."""
+    if len(shape) != 4 or t.shape != shape or t.dtype is not dtype or t.get_device() != index:
         raise ValueError(f"{name} must be a [pages, page_size, kv_heads, head_dim] tensor of shape {list(shape)} and "
-                         f"{dtype} on {device}")
+                         f"{dtype} on cuda:{index}")
     page, row, head, feature = t.stride()
-    if feature != 1 or (page | row | head) & 7 or t.data_ptr() & 15:
+    pointer = t.data_ptr()
+    if feature != 1 or (page | row | head) & 7 or pointer & 15:
         raise ValueError(f"{name} needs adjacent features, and pages, tokens and heads 16 bytes aligned")
-    return page, row, head
+    return pointer, page, row, head
 
 
 def _sequences(tokens: int, page_table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor],
-               device: torch.device):
-    """Checks of the description of a batch over a cache; (page_table, lengths, starts)."""
-    batch = lengths.shape[0] if lengths.dim() == 1 else -1
-    lengths = _int32(lengths, "lengths", batch, device)
-    if (page_table.dim() != 2 or page_table.dtype is not torch.int32 or page_table.device != device
-            or page_table.shape[0] != batch or page_table.shape[1] == 0):
-        raise ValueError(f"page_table must be an int32 tensor [{batch}, pages per sequence] on {device}")
-    if not page_table.is_contiguous() and page_table.stride(1) != 1:
+               index: int):
+    """Checks of the description of a batch over a cache; (page_table, lengths, starts, batch, pages per sequence, the
+    table's row stride)."""
+    shape = lengths.shape
+    batch = shape[0] if len(shape) == 1 else -1
+    lengths = _int32(lengths, "lengths", batch, index)
+    shape = page_table.shape
+    if (len(shape) != 2 or shape[0] != batch or shape[1] == 0 or page_table.dtype is not torch.int32
+            or page_table.get_device() != index):
+        raise ValueError(f"page_table must be an int32 tensor [{batch}, pages per sequence] on cuda:{index}")
+    row, column = page_table.stride()
+    if column != 1 and shape[1] > 1:
         page_table = page_table.contiguous()
+        row = shape[1]
     if starts is not None:
-        starts = _int32(starts, "starts", batch + 1, device)
+        starts = _int32(starts, "starts", batch + 1, index)
     elif tokens != batch:
         raise ValueError(f"{tokens} tokens for {batch} sequences need starts")
-    return page_table, lengths, starts
+    return page_table, lengths, starts, batch, shape[1], row
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, *,
@@ -255,23 +271,24 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     head_dim^-1/2.  float16 or bfloat16, head_dim a multiple of 8 up to 256; q, k, v may be column slices of one
     projection's output.  Rows outside every sequence are left as they are in ``out`` (arbitrary in a new tensor),
     which may not overlap the other tensors."""
-    dtype, device = _typed(q, "q")
-    q, k, v = _rows(q, "q", dtype, device), _rows(k, "k", dtype, device), _rows(v, "v", dtype, device)
-    tokens, heads, hd = q.shape
-    kv_heads = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != hd:
+    dtype, index = _typed(q, "q")
+    q, (tokens, heads, hd), q_at, q_row, q_head = _rows(q, "q", dtype, index)
+    k, shape, k_at, k_row, k_head = _rows(k, "k", dtype, index)
+    v, v_shape, v_at, v_row, v_head = _rows(v, "v", dtype, index)
+    kv_heads = shape[1]
+    if shape != v_shape or shape[0] != tokens or shape[2] != hd:
         raise ValueError("k and v must have one shape, and q's number of tokens and head_dim")
     _heads(heads, kv_heads, hd)
-    batch = starts.shape[0] - 1 if starts.dim() == 1 else -1
+    shape = starts.shape
+    batch = shape[0] - 1 if len(shape) == 1 else -1
     if batch < 0:
         raise ValueError("starts must be an int32 tensor of B + 1 elements")
-    starts = _int32(starts, "starts", batch + 1, device)
-    out = _context(out, tokens, heads * hd, dtype, device)
+    starts = _int32(starts, "starts", batch + 1, index)
+    out = _context(out, q, tokens, heads * hd)
     args = _lib.PACKED_ATTENTION
     _call("tt_packed_attention_fwd", args.pack(
-        args.size, q.data_ptr(), k.data_ptr(), v.data_ptr(), starts.data_ptr(), out.data_ptr(), *q.stride()[:2],
-        *k.stride()[:2], *v.stride()[:2], tokens, batch, heads, kv_heads, hd, causal, _SEQ_DTYPES[dtype],
-        hd ** -0.5 if scale is None else scale), device)
+        args.size, q_at, k_at, v_at, starts.data_ptr(), out.data_ptr(), q_row, q_head, k_row, k_head, v_row, v_head,
+        tokens, batch, heads, kv_heads, hd, causal, _SEQ_DTYPES[dtype], hd ** -0.5 if scale is None else scale), index)
     return out
 
 
@@ -286,21 +303,21 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     the n tokens of sequence b, rows starts[b] ... starts[b + 1] - 1 (or row b alone without ``starts``), take
     positions lengths[b] - n ... lengths[b] - 1.  Tokens whose position is negative or beyond the table, or whose
     page is no page of the cache, are not written."""
-    dtype, device = _typed(k, "k")
-    k, v = _rows(k, "k", dtype, device), _rows(v, "v", dtype, device)
-    tokens, kv_heads, hd = k.shape
-    if k.shape != v.shape:
+    dtype, index = _typed(k, "k")
+    k, shape, k_at, k_row, k_head = _rows(k, "k", dtype, index)
+    v, v_shape, v_at, v_row, v_head = _rows(v, "v", dtype, index)
+    if shape != v_shape:
         raise ValueError("k and v must have one shape")
+    tokens, kv_heads, hd = shape
     _heads(kv_heads, kv_heads, hd)
-    shape = (k_cache.shape[0], k_cache.shape[1], kv_heads, hd) if k_cache.dim() == 4 else ()
-    kc = _cache(k_cache, "k_cache", shape, dtype, device)
-    vc = _cache(v_cache, "v_cache", shape, dtype, device)
-    table, lengths, starts = _sequences(tokens, page_table, lengths, starts, device)
+    shape = (*k_cache.shape[:2], kv_heads, hd)
+    k_half, v_half = _cache(k_cache, "k_cache", shape, dtype, index), _cache(v_cache, "v_cache", shape, dtype, index)
+    table, lengths, starts, batch, table_pages, table_row = _sequences(tokens, page_table, lengths, starts, index)
     args = _lib.CACHE_ROWS
     _call("tt_cache_append", args.pack(
-        args.size, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(),
-        lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), *k.stride()[:2], *v.stride()[:2], *kc, *vc,
-        table.stride(0), tokens, lengths.shape[0], kv_heads, hd, shape[0], shape[1], table.shape[1], 0), device)
+        args.size, k_at, v_at, k_half[0], v_half[0], table.data_ptr(), lengths.data_ptr(),
+        0 if starts is None else starts.data_ptr(), k_row, k_head, v_row, v_head, *k_half[1:], *v_half[1:], table_row,
+        tokens, batch, kv_heads, hd, shape[0], shape[1], table_pages, 0), index)
 
 
 def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -314,26 +331,23 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``max_length`` (default: what the table can hold) is the longest length the caller expects; it only decides how
     the work is split.  Keys in a page whose number is no page of the cache are not read and count as NaN.  ``out`` may
     not overlap the other tensors."""
-    dtype, device = _typed(q, "q")
-    q = _rows(q, "q", dtype, device)
-    tokens, heads, hd = q.shape
-    shape = (*k_cache.shape[:3], hd) if k_cache.dim() == 4 else ()
-    kc = _cache(k_cache, "k_cache", shape, dtype, device)
-    vc = _cache(v_cache, "v_cache", shape, dtype, device)
+    dtype, index = _typed(q, "q")
+    q, (tokens, heads, hd), q_at, q_row, q_head = _rows(q, "q", dtype, index)
+    shape = (*k_cache.shape[:3], hd)
+    k_half, v_half = _cache(k_cache, "k_cache", shape, dtype, index), _cache(v_cache, "v_cache", shape, dtype, index)
     pages, page, kv_heads, _ = shape
     _heads(heads, kv_heads, hd)
-    table, lengths, starts = _sequences(tokens, page_table, lengths, starts, device)
-    out = _context(out, tokens, heads * hd, dtype, device)
-    batch, table_pages = table.shape
+    table, lengths, starts, batch, table_pages, table_row = _sequences(tokens, page_table, lengths, starts, index)
+    out = _context(out, q, tokens, heads * hd)
     held = table_pages * page
     max_length = held if max_length is None else min(int(max_length), held)
     nbytes = _lib.cache_attention_workspace_bytes(tokens, batch, heads, kv_heads, hd, page, table_pages, max_length,
                                                   starts is None)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     args = _lib.CACHE_ATTENTION
     _call("tt_cache_attention_fwd", args.pack(
-        args.size, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+        args.size, q_at, k_half[0], v_half[0], table.data_ptr(), lengths.data_ptr(),
         0 if starts is None else starts.data_ptr(), out.data_ptr(), 0 if work is None else work.data_ptr(), nbytes,
-        *q.stride()[:2], *kc, *vc, table.stride(0), tokens, batch, heads, kv_heads, hd, pages, page, table_pages,
-        max_length, _SEQ_DTYPES[dtype], hd ** -0.5 if scale is None else scale, 0), device)
+        q_row, q_head, *k_half[1:], *v_half[1:], table_row, tokens, batch, heads, kv_heads, hd, pages, page, table_pages,
+        max_length, _SEQ_DTYPES[dtype], hd ** -0.5 if scale is None else scale, 0), index)
     return out
