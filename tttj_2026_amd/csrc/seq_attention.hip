@@ -229,7 +229,7 @@ struct AppendArgs {
 
 // One wave per token: its K and V rows go to their place in the cache, 16 bytes a lane.  No computation: bound by HBM
 // (36000 tokens on 8 heads of 128 45 us, 6.5 TB/s read and written, with part of it in the last level cache; 59 us a call
-// in a stream of such calls), and by the call for few (64 tokens: 3.3 us of 9.4).
+// in a stream of such calls), and by the call for few (64 tokens: 3.3 us of 8.2).
 __global__ __launch_bounds__(256) void cache_append_kernel(AppendArgs a) {
   const int lane = threadIdx.x & 63;
   const int token = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -348,6 +348,6 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _call("tt_cache_attention_fwd", args.pack(
         args.size, q_at, k_half[0], v_half[0], table.data_ptr(), lengths.data_ptr(),
         0 if starts is None else starts.data_ptr(), out.data_ptr(), 0 if work is None else work.data_ptr(), nbytes,
-        q_row, q_head, *k_half[1:], *v_half[1:], table_row, tokens, batch, heads, kv_heads, hd, pages, page, table_pages,
-        max_length, _SEQ_DTYPES[dtype], hd ** -0.5 if scale is None else scale, 0), index)
+        q_row, q_head, *k_half[1:], *v_half[1:], table_row, tokens, batch, heads, kv_heads, hd, pages, page,
+        table_pages, max_length, _SEQ_DTYPES[dtype], hd ** -0.5 if scale is None else scale, 0), index)
     return out
