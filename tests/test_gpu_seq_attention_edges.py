@@ -2,6 +2,8 @@
 sequences, strides, offsets past 32 bits, large and tiny scores, batches beyond the lanes of a wave, captured graphs,
 other streams, refusals, and a run of all three as a program makes it.  Bounds as in test_gpu_seq_attention.py."""
 
+import threading
+
 import pytest
 import torch
 
@@ -418,6 +420,33 @@ def test_graphs_and_streams():
             y = step()
         torch.cuda.current_stream().wait_stream(side)
         assert torch.equal(y, want) and torch.isnan(junk)
+
+
+def test_calls_at_once():
+    """Two threads with a stream each call over one cache, keys in shares, without waiting for one another."""
+    lengths = [3000, 1, 700]
+    kc, vc, table, k, v = _store(lengths, 2, 128, 32)
+    n = _i32(lengths)
+    cases = [(_randn(1, 3, 8, 128), None), (_randn(2, 120, 8, 128), _starts([100, 0, 20]))]
+    want = [ops.cache_attention(q, kc, vc, table, n, starts) for q, starts in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(ops.cache_attention(cases[i][0], kc, vc, table, n, cases[i][1]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i, (q, starts) in enumerate(cases):
+        counts = [1, 1, 1] if starts is None else [100, 0, 20]
+        _check(want[i], *_over_cache(q, k, v, counts, lengths))
+        assert len(got[i]) == 20 and all(torch.equal(y, want[i]) for y in got[i])
 
 
 def test_prompt_chunks_and_tokens():
