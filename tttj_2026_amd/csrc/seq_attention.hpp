@@ -530,16 +530,16 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   auto issue_v = [&](const Places& p, int st) TT_INLINE {
     issue_half(false, p, sv + st * TILE, 0);
   };
-  // After the copies of this wave's V rows have landed: rows of keys behind the last are cleared (0 times whatever lay
-  // there would not be 0), and where some rows of the block see keys that others do not, infinities and NaN are taken
-  // out of V: 0 times those would reach the rows that do not see them.  Such values are added to the rows that do see
-  // them at the end (restore_odd).
+  // After the copies of this wave's V rows have landed: rows of keys behind the last that any row of the block sees are
+  // cleared (0 times whatever lay there would not be 0), and where some rows of the block see keys that others do not,
+  // infinities and NaN are taken out of V: 0 times those would reach the rows that do not see them.  Such values are
+  // added to the rows that do see them at the end (restore_odd).
   const bool mixed = block_lo < block_end;
   bool odd = false;
   auto settle_v = [&](int t0, int st) TT_INLINE {
     const int g0 = rw * WROWS;
     u32x4* const tile = reinterpret_cast<u32x4*>(sv + st * TILE + g0 * HD);
-    const int n = min(max(keys - (t0 + g0), 0), WROWS);
+    const int n = min(max(kend - (t0 + g0), 0), WROWS);
     if (mixed && t0 + KT > block_lo) {
       constexpr uint32_t kCarry = (0x8000u - Num<T>::kExp) * 0x10001u;  // an exponent of ones carries into the sign
       for (int e = lane; e < n * CH; e += 64) {
