@@ -468,7 +468,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     const int key = min(t0 + 16 * (lane & 7), max(keys - 1, 0));
     return a.table[sq.seq * a.table_row + (key >> a.page_shift)];
   };
-  // Which of those lie outside the cache (a bit each); their keys are not read and count as NaN.
+  // Which of those lie outside the cache (a bit each); their keys are not read (place: no bytes there) and count as NaN.
+  // Rows that do not see them multiply whatever the tile then holds in V by 0 as they do other values (settle_v).
   auto bad_groups = [&](int pe, int t0) TT_INLINE -> uint32_t {
     return (uint32_t)__ballot((uint32_t)pe >= (uint32_t)a.pages && t0 + 16 * lane < keys) & 0xffu;
   };
@@ -479,10 +480,11 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     uint32_t k_bytes, v_bytes;
   };
   auto place = [&](int t, int pe) TT_INLINE -> Places {
-    const int n = min(max(keys - t, 0), 16);
+    int n = min(max(keys - t, 0), 16);
     Places p;
     if constexpr (PAGED) {
-      const uint32_t page = (uint32_t)pe < (uint32_t)a.pages ? pe : 0, in = t & ((1 << a.page_shift) - 1);
+      if ((uint32_t)pe >= (uint32_t)a.pages) n = pe = 0;
+      const uint32_t page = pe, in = t & ((1 << a.page_shift) - 1);
       p.k = 2 * (page * (uint64_t)a.k_page + in * (uint64_t)a.k_row);
       p.v = 2 * (page * (uint64_t)a.v_page + in * (uint64_t)a.v_row);
     } else {
