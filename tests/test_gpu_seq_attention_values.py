@@ -61,3 +61,61 @@ def test_bad_page_behind_a_row(number, hd, h, counts):
     assert torch.isnan(y[fine:]).all()
     ref, mag = _over_cache(q, k, v, counts, lengths)
     _check(y[:fine], ref[:fine], mag[:fine])
+
+
+def _far(n, hkv, hd, gap, rising, dtype, seed):
+    """K whose first feature alone counts (for the q below): scores fall or rise by `gap` (log2) along the keys; V with an
+    infinity in the 10th key, two that cancel and a NaN elsewhere."""
+    k = _randn(seed, n, hkv, hd, dtype=dtype)
+    at = torch.linspace(0, gap, n, device="cuda")[:, None]
+    k[..., 0] = at if rising else -at
+    v = _randn(seed + 1, n, hkv, hd, dtype=dtype)
+    v[9 if rising else -10, :, 1], v[n // 2, :, 2] = INF, -INF
+    v[9, :, 4], v[-10, :, 4], v[n // 3, 0, 5] = INF, -INF, NAN
+    q = torch.zeros(n, 2 * hkv, hd, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    return q, k, v, 0.6931471805599453
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [32, 128, 256])
+@pytest.mark.parametrize("gap", [60, 400])
+@pytest.mark.parametrize("rising", [False, True])
+def test_infinities_with_small_probabilities(dtype, hd, gap, rising):
+    """A row that sees an infinity in V has it in its result, however small the key's probability: no probability is 0 by
+    the definition."""
+    q, k, v, scale = _far(700, 2, hd, gap, rising, dtype, 11)
+    for causal in (True, False):
+        y = ops.packed_attention(q, k, v, _starts([700]), causal=causal, scale=scale)
+        _check(y, *_over_prompts(q, k, v, [700], causal, scale))
+    lengths = [3000, 700]
+    kc, vc, table, ks, vs = _store(lengths, 2, hd, 32, dtype)
+    for b, n in enumerate(lengths):
+        _, ks[b], vs[b], scale = _far(n, 2, hd, gap, rising, dtype, 21 + b)
+        _write(kc, vc, table.cpu(), b, 0, ks[b], vs[b])
+    for counts in ([1, 1], [5, 2], [300, 2]):
+        for most in (None, 10):  # keys in shares or not
+            y = ops.cache_attention(q[:sum(counts)], kc, vc, table, _i32(lengths), _starts(counts), scale=scale,
+                                    max_length=most)
+            _check(y, *_over_cache(q[:sum(counts)], ks, vs, counts, lengths, scale))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [32, 128, 256])
+def test_rows_whose_scores_are_all_infinitely_low(dtype, hd):
+    """... are +0.0, whatever V holds; the rows beside them see what they should."""
+    q, k, v = (_randn(s, 300, n, hd, dtype=dtype) for s, n in ((1, 4), (2, 2), (3, 2)))
+    k[..., 0] = -INF
+    q[..., 0] = 0.5
+    q[200:, :, 0] = -0.5  # scores of +infinity: NaN
+    v[0, 0, 1], v[100, 1, 2] = INF, NAN
+    starts, lengths = _starts([300]), _i32([300])
+    kc, vc = (torch.full((10, 32, 2, hd), NAN, dtype=dtype, device="cuda") for _ in range(2))
+    table = torch.arange(10, dtype=torch.int32, device="cuda")[None]
+    ops.cache_append(k, v, kc, vc, table, lengths, starts)
+    ys = [ops.packed_attention(q, k, v, starts), ops.cache_attention(q, kc, vc, table, lengths, starts),
+          ops.cache_attention(q, kc, vc, table, lengths, starts, max_length=1)]
+    for y in ys:
+        assert not y[:200].view(torch.int16).any() and torch.isnan(y[200:]).all()
+    one = ops.cache_attention(q[:1], kc, vc, table, lengths)
+    assert not one.view(torch.int16).any()

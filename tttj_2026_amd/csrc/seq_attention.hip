@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int rows_
     for (int i = 0; i < 4; ++i) {
       if (p0 + i * groups >= parts) break;
       // a part without a maximum saw no key (its sum, 0, is its weight) or only NaN (NaN is)
-      const float w = y[i].x == -INFINITY ? y[i].y : __builtin_amdgcn_exp2f(y[i].x - m);
+      const float w = y[i].x == -INFINITY ? y[i].y : seq_weight(y[i].x - m);
       l = fmaf(w, y[i].y, l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(w, v[i][e], o[e]);
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64 * W) void seq_merge_wide_kernel(SeqAttnArgs a, i
   for (int g = 0; g < P; ++g) o[g] = floatx4{0.f, 0.f, 0.f, 0.f};
   // A part (or a wave) without a maximum saw no key (its sum, 0, is its weight) or only NaN (NaN is).
   const auto weight = [&](float2 ml) -> float {
-    return ml.x == -INFINITY ? ml.y : __builtin_amdgcn_exp2f(ml.x - m);
+    return ml.x == -INFINITY ? ml.y : seq_weight(ml.x - m);
   };
   const bool own = r < rows;  // entries of rows behind the last are not written
   for (int p0 = wave; p0 < t.parts; p0 += 4 * W) {
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * W) void seq_merge_wide_kernel(SeqAttnArgs a, i
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (p0 + i * W < t.parts) m_new = fmaxf(m_new, y[i].x);
-    const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+    const float corr = m_new == -INFINITY ? 1.f : seq_weight(m - m_new);
     m = m_new;
     l *= corr;
 #pragma unroll

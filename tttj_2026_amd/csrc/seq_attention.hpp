@@ -130,6 +130,12 @@ constexpr int kSeqTileCost = 2;  // units that a tile's beginning and end take t
 constexpr float kSeqLazy = 8.0f;   // log2 growth of a row's maximum that moves its reference
 constexpr float kSeqShift = 7.0f;  // log2 of the factor on the probabilities: 2^(8 + 7) < 65504
 
+// exp2 of a difference of maxima, as the weight of sums that are joined: never 0, so that an infinity among them stays one
+// (2^-126 of any finite sum is far below half a step of the others).
+__device__ __forceinline__ float seq_weight(float log2) {
+  return fmaxf(__builtin_amdgcn_exp2f(log2), 0x1p-126f);
+}
+
 // V tiles are read by ds_read_b64_tr_b16: half a wave reads 64 bytes of each of 4 consecutive rows.  The 64-byte
 // segments of a row are exchanged by its number so that those 4 pieces lie in different quarters of the 64 banks.
 template <int HD>
@@ -535,21 +541,24 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   // After the copies of this wave's V rows have landed: rows of keys behind the last that any row of the block sees are
   // cleared (0 times whatever lay there would not be 0), and where some rows of the block see keys that others do not,
   // infinities and NaN are taken out of V: 0 times those would reach the rows that do not see them.  Such values are
-  // added to the rows that do see them at the end (restore_odd).
+  // added to the rows that do see them at the end (restore_odd); `odd`: this wave took some out.
   const bool mixed = block_lo < block_end;
   bool odd = false;
+  const auto odd_pair = [](uint32_t x) TT_INLINE -> uint32_t {  // of two values: bits 0 and 16
+    constexpr uint32_t kCarry = (0x8000u - Num<T>::kExp) * 0x10001u;  // an exponent of ones carries into the sign
+    return (((x & 0x7fff7fffu) + kCarry) >> 15) & 0x10001u;
+  };
   auto settle_v = [&](int t0, int st) TT_INLINE {
     const int g0 = rw * WROWS;
     u32x4* const tile = reinterpret_cast<u32x4*>(sv + st * TILE + g0 * HD);
     const int n = min(max(kend - (t0 + g0), 0), WROWS);
     if (mixed && t0 + KT > block_lo) {
-      constexpr uint32_t kCarry = (0x8000u - Num<T>::kExp) * 0x10001u;  // an exponent of ones carries into the sign
       for (int e = lane; e < n * CH; e += 64) {
         u32x4 x = tile[e];
         uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t m = (((x[i] & 0x7fff7fffu) + kCarry) >> 15) & 0x10001u;
+          const uint32_t m = odd_pair(x[i]);
           any |= m;
           x[i] &= ~(m * 0xffffu);
         }
@@ -573,16 +582,32 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   floatx16 o[CB][DB];
   float m_ref[CB], l_run[CB], mc[CB], thr[CB];
 
-  // Asked for after the first copies, which need addresses of their own first.
+  // Asked for after the first copies, which need addresses of their own first.  Branches are the wave's: where lanes went
+  // around loads past head_dim by themselves, the compiler saved registers that every lane needs for the next tile in that
+  // branch's last block, with half of the lanes off.
   v8 qf[CB][KSTEPS];
   auto load_q = [&]() TT_INLINE {
+    int width = hd;
+    asm volatile("" : "+s"(width));  // (the comparisons would be kept in registers)
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
       const T* qp = static_cast<const T*>(a.q) + (int64_t)(sq.first + tok[b]) * a.q_row + head[b] * a.q_head;
+      if (!FAR && width == HD) {
 #pragma unroll
-      for (int kk = 0; kk < KSTEPS; ++kk) {
-        if (16 * kk + 8 * hf < hd) qf[b][kk] = *reinterpret_cast<const v8*>(qp + 16 * kk + 8 * hf);
-        else qf[b][kk] = __builtin_bit_cast(v8, u32x4{0u, 0u, 0u, 0u});
+        for (int kk = 0; kk < KSTEPS; ++kk) qf[b][kk] = *reinterpret_cast<const v8*>(qp + 16 * kk + 8 * hf);
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) {
+          const u32x4 none = {0u, 0u, 0u, 0u};
+          u32x4 x = none;
+          if (16 * kk + 8 < width) {
+            x = *reinterpret_cast<const u32x4*>(qp + 16 * kk + 8 * hf);
+          } else if (16 * kk < width) {
+            x = *reinterpret_cast<const u32x4*>(qp + 16 * kk);
+            x = hf == 0 ? x : none;
+          }
+          qf[b][kk] = __builtin_bit_cast(v8, x);
+        }
       }
     }
   };
@@ -678,7 +703,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     for (int b = 0; b < CB; ++b) {
       const float m_new = fmaxf(m_ref[b], mt[b]);
       const bool none = m_new == -INFINITY;  // no key of this row so far: o and l are 0
-      const float corr = none ? 1.f : __builtin_amdgcn_exp2f((m_ref[b] - m_new) * c2);
+      const float corr = none ? 1.f : seq_weight((m_ref[b] - m_new) * c2);
       m_ref[b] = m_new;
       mc[b] = none ? 0.f : m_new * c2 - kSeqShift;
       thr[b] = none ? -INFINITY : m_new + lazy;
@@ -949,17 +974,32 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       }
     }
   }
-  if (RW * KW > 1 && mixed) odd = __syncthreads_or(odd) != 0;
-
-  // Sums of this wave's rows over both halves of the wave; then, over the groups, by all of them: group g joins the
-  // g-th, (g + KW)-th, ... of the 4-feature pieces that a lane holds, from [group][piece][lane] and (maximum, sum) in LDS.
+  // Sums of this wave's rows over both halves of the wave.
   float l_row[CB];
 #pragma unroll
   for (int b = 0; b < CB; ++b) l_row[b] = xhalf_sum(l_run[b]);
+
+  // A sum that is NaN though its row's scores are not holds infinities of V (restore_odd); the sum of the sums tells, or
+  // raises a false alarm.
+  static_assert(CB == 1, "one block of rows per wave");
+  float all = 0.f;
+#pragma unroll
+  for (int i = 0; i < DB; ++i) {
+    float sum = o[0][i][0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) sum += o[0][i][e];
+    all += sum;
+  }
+  bool lost = all != all && l_row[0] == l_row[0];
+  if (RW > 1 && mixed) odd = __syncthreads_or(odd) != 0;
+
+  // Over the groups, by all of them: group g joins the g-th, (g + KW)-th, ... of the 4-feature pieces that a lane holds,
+  // from [group][piece][lane] and (maximum, sum) in LDS.
   if constexpr (KW > 1) {
     static_assert(CB == 1 && RW == 1, "groups are waves with one block of rows");
     floatx4* const pieces = reinterpret_cast<floatx4*>(seq_lds);
     float2* const sums = reinterpret_cast<float2*>(pieces + KW * DB * 4 * 64);
+    int* const flags = reinterpret_cast<int*>(sums + KW * 32);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < DB; ++i)
@@ -968,7 +1008,13 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         pieces[(grp * DB * 4 + i * 4 + g) * 64 + lane] =
             floatx4{o[0][i][4 * g], o[0][i][4 * g + 1], o[0][i][4 * g + 2], o[0][i][4 * g + 3]};
     if (hf == 0) sums[grp * 32 + col] = make_float2(m_ref[0], l_row[0]);
+    const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0, any_lost = __builtin_amdgcn_ballot_w64(lost) != 0;
+    flags[grp] = (any_odd ? 1 : 0) | (any_lost ? 2 : 0);
     __syncthreads();
+    int flag = 0;
+#pragma unroll
+    for (int g = 0; g < KW; ++g) flag |= flags[g];
+    odd = (flag & 1) != 0, lost = (flag & 2) != 0;
     float2 ml[KW];
     float m = -INFINITY;
 #pragma unroll
@@ -980,7 +1026,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
 #pragma unroll
     for (int g = 0; g < KW; ++g) {
       // a group without a maximum saw no key (its sum, 0, is its weight) or only NaN (NaN is)
-      w[g] = ml[g].x == -INFINITY ? ml[g].y : __builtin_amdgcn_exp2f((ml[g].x - m) * c2);
+      w[g] = ml[g].x == -INFINITY ? ml[g].y : seq_weight((ml[g].x - m) * c2);
       l = fmaf(w[g], ml[g].y, l);
     }
     m_ref[0] = m;
@@ -1067,32 +1113,65 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
                  (T)(o[b][i][4 * g + 3] * inv)};
         }
   }
-  if (mixed && __builtin_amdgcn_ballot_w64(odd) != 0) {
-    // restore_odd: a wave adds the infinities and NaN of V that were taken out to those of its rows that see them.
+  // restore_odd: the infinities and NaN of V.  No probability of a key that a row sees is 0 by the definition, so such a
+  // value alone decides the sums that it enters.  Where settle_v took some out, or where a sum is NaN (an infinity times a
+  // probability that is 0 in T), a wave adds them to what its rows that see them have in memory; adding one twice changes
+  // nothing.  (A row with scores of -infinity only has no sum, and stays 0.)
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd || lost) != 0, 0)) {
+    __builtin_amdgcn_s_waitcnt(0);
     __threadfence_block();
     if constexpr (KW > 1) __syncthreads();
-    const int from = kbeg + max(block_lo - kbeg, 0) / KT * KT;
-    for (int key = from; grp == 0 && key < lim_hi; ++key) {
-      const T* vp = vh;
-      if constexpr (PAGED) {
-        const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
-        if ((uint32_t)page >= (uint32_t)a.pages) continue;
-        vp += page * a.v_page + (key & ((1 << a.page_shift) - 1)) * a.v_row;
-      } else {
-        vp += (int64_t)(sq.first + key) * a.v_row;
-      }
-      for (int d = lane; d < hd; d += 64) {
-        const T y = vp[d];
-        if ((__builtin_bit_cast(uint16_t, y) & Num<T>::kExp) != Num<T>::kExp) continue;
-        for (int r = wr0; r < min(wr0 + WR, rows); ++r) {
-          const int token = r / G;
-          if (key >= seq_limit(a, token, sq.count, keys)) continue;
-          if (part >= 0) {
-            a.part_o[RW > 1 ? (part0 + r0) * hd + wide_place(hd, r - r0, d) : (part0 + r) * hd + d] += (float)y;
-          } else {
-            T* const dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + token) * a.heads + hkv * G + r - token * G) * hd + d;
-            *dst = (T)((float)*dst + (float)y);
-          }
+    if (grp == 0 && wave_active) {
+      int l = lane;
+      asm volatile("" : "+v"(l));  // (what follows from it is worked out again instead of being held in registers)
+      const int h = l >> 5, row = wr0 + (l & 31), r = min(row, rows - 1), token = r / G;
+      const int seen = l_row[0] == 0.f ? 0 : seq_limit(a, token, sq.count, keys);
+      const bool any_lost = __builtin_amdgcn_ballot_w64(lost) != 0;
+      T* const out =
+          static_cast<T*>(a.out) + ((int64_t)(sq.first + token) * a.heads + hkv * G + r - token * G) * hd + 4 * h;
+      float* const sum = RW > 1 ? a.part_o + (part0 + r0) * hd + wide_place(hd, r - r0, 4 * h)
+                                : a.part_o + (part0 + r) * hd + 4 * h;
+      typedef T v4 __attribute__((ext_vector_type(4)));
+      const auto update = [&](int c, auto value) TT_INLINE {  // features 8 c + 4 h + {0..3} of this lane's row
+        if (part >= 0) {
+          floatx4* const dst = reinterpret_cast<floatx4*>(sum + c * (RW > 1 ? 256 : 8));
+          floatx4 y = *dst;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = value(y[e], e);
+          *dst = y;
+        } else {
+          v4* const dst = reinterpret_cast<v4*>(out + 8 * c);
+          v4 y = *dst;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = (T)value((float)y[e], e);
+          *dst = y;
+        }
+      };
+      const auto values = [&](int key) TT_INLINE -> const T* {  // nullptr: in no page
+        if constexpr (PAGED) {
+          const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
+          if ((uint32_t)page >= (uint32_t)a.pages) return nullptr;
+          return vh + page * a.v_page + (key & ((1 << a.page_shift) - 1)) * a.v_row;
+        } else {
+          return vh + (int64_t)(sq.first + key) * a.v_row;
+        }
+      };
+      if (any_lost && row < rows && l_row[0] == l_row[0])
+        for (int c = 0; 8 * c < hd; ++c) update(c, [](float y, int) TT_INLINE { return y != y ? 0.f : y; });
+      for (int k0 = any_lost ? kbeg : kbeg + max(block_lo - kbeg, 0) / KT * KT; k0 < lim_hi; k0 += RPC) {
+        const T* const vp = values(min(k0 + l / CH, lim_hi - 1));  // RPC keys, 16 bytes per lane
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (vp != nullptr && l % CH * 8 < hd) x = *reinterpret_cast<const u32x4*>(vp + l % CH * 8);
+        uint64_t found =
+            __builtin_amdgcn_ballot_w64((odd_pair(x[0]) | odd_pair(x[1]) | odd_pair(x[2]) | odd_pair(x[3])) != 0);
+        for (; found != 0; found &= found - 1) {
+          const int n = __ffsll((unsigned long long)found) - 1, c = n % CH, key = min(k0 + n / CH, lim_hi - 1);
+          const v4 z = *reinterpret_cast<const v4*>(values(key) + 8 * c + 4 * h);
+          if (row < rows && key < seen)
+            update(c, [&](float y, int e) TT_INLINE {
+              const T w = z[e];
+              return (__builtin_bit_cast(uint16_t, w) & Num<T>::kExp) == Num<T>::kExp ? y + (float)w : y;
+            });
         }
       }
     }

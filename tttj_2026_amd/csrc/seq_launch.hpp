@@ -15,7 +15,7 @@ enum class SeqShape { kWide, kNarrow, kDeep };
 template <typename T, int HD, int RW, int KW, int KT, bool PAGED>
 int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
   constexpr int lds = 2 * 2 * KW * KT * HD * (int)sizeof(T);  // K and V, two tiles deep
-  static_assert(KW == 1 || lds >= KW * (HD / 8 * 64 * 16 + 32 * 8), "the groups are joined in the tiles' LDS");
+  static_assert(KW == 1 || lds >= KW * (HD / 8 * 64 * 16 + 32 * 8 + 4), "the groups are joined in the tiles' LDS");
   static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic LDS is raised
   int dev = 0;
   TT_HIP(hipGetDevice(&dev));
