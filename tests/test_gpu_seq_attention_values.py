@@ -119,3 +119,39 @@ def test_rows_whose_scores_are_all_infinitely_low(dtype, hd):
         assert not y[:200].view(torch.int16).any() and torch.isnan(y[200:]).all()
     one = ops.cache_attention(q[:1], kc, vc, table, lengths)
     assert not one.view(torch.int16).any()
+
+
+def _all_forms(q, k, v, lengths, scale=None):
+    """Outputs of the last 300 tokens of a prompt and of its last token over the cache, with their references: as a
+    prompt, as a chunk and as a single token, keys in shares or not."""
+    n, hkv, hd = k.shape
+    limits = torch.arange(n - len(q) + 1, n + 1)
+    yield ops.packed_attention(torch.cat([q.new_zeros(n - len(q), *q.shape[1:]), q]), k, v, _starts([n]),
+                               scale=scale)[n - len(q):], *_attend(q, k, v, limits, scale)
+    pages = -(-n // 32)
+    kc, vc = (torch.zeros(pages, 32, hkv, hd, dtype=k.dtype, device="cuda") for _ in range(2))
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").flip(0)[None]
+    ops.cache_append(k, v, kc, vc, table, _i32([n]), _starts([n]))
+    for rows in (q, q[-1:]):
+        for most in (None, 10):
+            yield ops.cache_attention(rows, kc, vc, table, _i32([n]), _starts([len(rows)]), scale=scale,
+                                      max_length=most), *_attend(rows, k, v, limits[-len(rows):], scale)
+
+
+@pytest.mark.parametrize("hd", [32, 128, 256])
+def test_large_and_small_values_of_bfloat16(hd):
+    """V over bfloat16's range: its largest values do not overflow the sums, small ones are not lost, and large ones of keys
+    with probabilities that are 0 in fp32 do not show.  Relative to sum p |v| alone: products p v are made with p times
+    2^-24, so were those below fp32's 2^-126 lost, at 1e-24 = 2^-79.7 they would be 2500 of p below 2^-22 of the largest,
+    0.0006 of the sum and a third of u."""
+    q, k, v = (_randn(s, n, h, hd, dtype=BF16) for s, n, h in ((1, 300, 4), (2, 2500, 2), (3, 2500, 2)))
+    u = torch.finfo(BF16).eps / 2
+    for size in (8e37, 1e-24):
+        for y, ref, mag in _all_forms(q, k, v.clamp(-4, 4) * size, 2500):
+            assert bool(((y.double() - ref).abs() <= 4 * u * mag).all())
+    k[..., 0] = 0
+    q[..., 0] = 1
+    k[[5, 1200, 2100], :, 0] = -1000.0 * hd ** 0.5
+    v[[5, 1200, 2100]] = 3e38
+    for y, ref, mag in _all_forms(q, k, v, 2500):
+        _check(y, ref, mag)

@@ -33,8 +33,9 @@
 // the keys in the order in which a lane holds its probabilities, so neither needs a shuffle.
 // Scores are multiplied by c log2(e) in fp32 (rounding q c to 16 bits would cost as much precision as rounding the
 // probabilities does).  Probabilities are rounded to the type of V for the matrix unit, relative to a maximum that
-// is moved only when it grows by more than 2^8 (lazy rescaling), and times 2^7, so that fp16 holds what is down to
-// 2^-31 of the largest: 100000 keys of 2^-25 each still count.
+// is moved only when it grows by more than 2^8 (lazy rescaling), and times 2^7 in fp16, which so holds what is down to
+// 2^-31 of the largest: 100000 keys of 2^-25 each still count; times 2^-24 in bf16, whose values go up to 2^128 and would
+// overflow the sums (its probabilities go down to 2^-102 of the largest).
 #pragma once
 
 #include "attention_block.hpp"
@@ -58,6 +59,7 @@ struct Num<half> {
   using v2 = half2v;
   using v8 = half8;
   static constexpr uint16_t kExp = 0x7c00;  // the exponent's bits: all set in infinities and NaN
+  static constexpr float kShift = 7.f;      // log2 of the factor on the probabilities (kSeqLazy): 2^(8 + 7) < 65504
   static __device__ __forceinline__ floatx16 mfma(v8 a, v8 b, floatx16 c) { return mfma32x32x16(a, b, c); }
   static __device__ __forceinline__ float add2(v2 p, float c) {
     return __builtin_amdgcn_fdot2(p, v2{(half)1.f, (half)1.f}, c, false);
@@ -68,6 +70,7 @@ struct Num<bf16> {
   using v2 = bf16x2;
   using v8 = bf16x8;
   static constexpr uint16_t kExp = 0x7f80;
+  static constexpr float kShift = -24.f;  // 65536 keys of 2^(8 - 24) times the largest value do not overflow fp32
   static __device__ __forceinline__ floatx16 mfma(v8 a, v8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -128,12 +131,11 @@ constexpr int kSeqTileCost = 2;  // units that a tile's beginning and end take t
                                  // / 38.6 / 39.5 us, 64 tokens over 1 to 4000 keys 106.6 / 105 / 107)
 
 constexpr float kSeqLazy = 8.0f;   // log2 growth of a row's maximum that moves its reference
-constexpr float kSeqShift = 7.0f;  // log2 of the factor on the probabilities: 2^(8 + 7) < 65504
 
 // exp2 of a difference of maxima, as the weight of sums that are joined: never 0, so that an infinity among them stays one
-// (2^-126 of any finite sum is far below half a step of the others).
+// (2^-149, for less than 2^-126, of any finite sum is below half a step of the others).
 __device__ __forceinline__ float seq_weight(float log2) {
-  return fmaxf(__builtin_amdgcn_exp2f(log2), 0x1p-126f);
+  return fmaxf(__builtin_amdgcn_exp2f(log2), 0x1p-149f);
 }
 
 // V tiles are read by ds_read_b64_tr_b16: half a wave reads 64 bytes of each of 4 consecutive rows.  The 64-byte
@@ -705,7 +707,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       const bool none = m_new == -INFINITY;  // no key of this row so far: o and l are 0
       const float corr = none ? 1.f : seq_weight((m_ref[b] - m_new) * c2);
       m_ref[b] = m_new;
-      mc[b] = none ? 0.f : m_new * c2 - kSeqShift;
+      mc[b] = none ? 0.f : m_new * c2 - Num<T>::kShift;
       thr[b] = none ? -INFINITY : m_new + lazy;
       l_run[b] *= corr;
 #pragma unroll
@@ -772,7 +774,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         for (int e = 0; e < 16; ++e) o[b][i][e] = 0.f;
       m_ref[b] = -INFINITY;  // the maximum that the sums are relative to, in units of the raw scores
       l_run[b] = 0.f;        // this lane's half of the row's sum
-      mc[b] = 0.f;           // m_ref c log2(e) - 7
+      mc[b] = 0.f;           // m_ref c log2(e) - kShift
       thr[b] = -INFINITY;    // a tile maximum above this moves m_ref
     }
 
@@ -1080,7 +1082,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     }
   }
 
-  // Other output rows, or a part's sums: O in units of exp2(m - 7), the maximum in log2 units, the sum.
+  // Other output rows, or a part's sums: O and the sum in units of exp2(m - kShift), the maximum in log2 units.
   const int64_t part0 = ((int64_t)part * a.kv_heads + hkv) * R - r0;  // + row
 #pragma unroll
   for (int b = 0; b < CB; ++b) {
