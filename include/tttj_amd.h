@@ -257,9 +257,9 @@ int tt_attention_fwd_prescaled(const void* q, const void* k, const void* vt, con
  * features are adjacent, and pointers and strides aligned to 16 bytes.  head_dim is a multiple of 8 up
  * to 256, scale positive (below 2e38), dtype TT_FP16 or TT_BF16 for all four tensors.  out overlaps
  * none of the others.  A row whose scores are all -infinity is +0.0.  Rows outside every sequence
- * are not written.  Values of `starts` outside [0, tokens] are taken as the nearest in it.  No
- * counterpart in the reference, whose attention takes padded batches with as many key heads as query
- * heads (kernels/case8_attention.py:48-206). */
+ * are not written.  Values of `starts` outside [0, tokens] are taken as the nearest in it; where they
+ * fall, rows are arbitrary or left as they were.  No counterpart in the reference, whose attention
+ * takes padded batches with as many key heads as query heads (kernels/case8_attention.py:48-206). */
 typedef struct {
   int64_t size;
   const void *q, *k, *v;

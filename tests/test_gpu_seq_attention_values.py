@@ -155,3 +155,24 @@ def test_large_and_small_values_of_bfloat16(hd):
     v[[5, 1200, 2100]] = 3e38
     for y, ref, mag in _all_forms(q, k, v, 2500):
         _check(y, ref, mag)
+
+
+@pytest.mark.parametrize("length", [5000, 1 << 27])
+def test_falling_starts_with_keys_in_shares(length):
+    """Starts that go up and down between the same rows give every second sequence all of them; with the longest lengths
+    their units of keys pass 32 bits many times over.  Nothing outside the output is written, and rising starts in the
+    same call's place are right again."""
+    batch, tokens, page = 512, 512, 256
+    kc, vc = _randn(1, 4, page, 1, 64), _randn(2, 4, page, 1, 64)
+    table = torch.zeros(1, length // page + 1, dtype=torch.int32, device="cuda").expand(batch, -1)
+    q = _randn(3, tokens, 8, 64)
+    lengths = torch.full((batch,), length, dtype=torch.int32, device="cuda")
+    around = torch.full((3 * tokens, 512), 7.0, dtype=F16, device="cuda")
+    for starts in ([tokens * (b % 2) for b in range(batch + 1)], [tokens - b for b in range(batch + 1)]):
+        ops.cache_attention(q, kc, vc, table, lengths, _i32(starts), out=around[tokens:2 * tokens])
+        torch.cuda.synchronize()
+        assert bool((around[:tokens] == 7).all()) and bool((around[2 * tokens:] == 7).all())
+    lengths.fill_(page)
+    y = ops.cache_attention(q, kc, vc, table, lengths, _i32(list(range(batch + 1))))
+    limits = torch.full((tokens,), page)
+    _check(y, *_attend(q, kc[0], vc[0], limits))

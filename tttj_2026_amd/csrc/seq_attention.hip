@@ -41,6 +41,7 @@ __global__ __launch_bounds__(256) void seq_merge_kernel(SeqAttnArgs a, int rows_
     if (token < own.x || token >= own.x + own.y) return;  // a row of no sequence
   }
   const SeqShare sh = seq_share(a, 0, seq, rows_per_tile);
+  if (sh.total == 0) return;
   const SeqUnits u = sh.units;
   const int hkv = head / a.group;
   const int r = (token - u.first) * a.group + head - hkv * a.group;
@@ -115,7 +116,9 @@ __global__ __launch_bounds__(64 * W) void seq_merge_wide_kernel(SeqAttnArgs a, i
   const SeqTile sq = seq_tile(a, (rest >> 2) / a.kv_heads, R);
   const int r = 32 * rw + (lane & 31), rows = sq.count * a.group - sq.tile * R;  // row of the tile; rows from there on
   if (sq.tile < 0 || 32 * rw >= rows) return;
-  const SeqParts t = seq_parts(seq_share(a, 0, sq.seq, R), sq.tile);
+  const SeqShare sh = seq_share(a, 0, sq.seq, R);
+  if (sh.total == 0) return;
+  const SeqParts t = seq_parts(sh, sq.tile);
   if (t.parts == 1) return;
   const int d0 = 8 * P * unit, hd = a.head_dim;
   const int place = wide_place(hd, r, d0 + 4 * (lane >> 5));
@@ -313,7 +316,7 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   // Beyond the blocks that the chip holds (four times as many of 32 rows), tiles spread by themselves: 1088 tiles of 128
   // rows over 500 to 4600 keys, 195 alone and 272 in shares; 800 of 32 rows over 1 to 4000 keys, 193 and 162.
   if (paged && max_length > alone && batch <= 512 && blocks < (wide ? 1 : 4) * held_blocks &&
-      tiles * (held / kSeqUnit + 1 + kSeqTileCost) < (1LL << 31)) {
+      tiles * (held / kSeqUnit + 1 + kSeqTileCost) + held_blocks < (1LL << 31)) {
     p.mode = kSeqShares;
     if (!wide) p.shape = SeqShape::kNarrow;
     const int64_t units = tiles * ((max_length + kSeqUnit - 1) / kSeqUnit + kSeqTileCost);

@@ -297,11 +297,15 @@ struct SeqShare {
   SeqUnits units;
 };
 
-// The shares of a launch, and the sequence that holds the first unit of block `slot` (seq < 0), or sequence `seq`.
+// The shares of a launch, and the sequence that holds the first unit of block `slot` (seq < 0), or sequence `seq`.  Where
+// `starts` falls anywhere, rows belong to several sequences and the units have no bound: there are none (total 0).
 __device__ __forceinline__ SeqShare seq_share(const SeqAttnArgs& a, int slot, int seq, int rows_per_tile) {
   const int lane = threadIdx.x & 63;
+  bool falls = false;
   const auto units_of = [&](int b) -> SeqUnits {
-    return b < a.batch ? seq_units(a, b, rows_per_tile) : SeqUnits{0, 0, 0, 0, 1};
+    if (b >= a.batch) return SeqUnits{0, 0, 0, 0, 1};
+    falls |= a.starts != nullptr && seq_start(a.starts, b, a.tokens) > seq_start(a.starts, b + 1, a.tokens);
+    return seq_units(a, b, rows_per_tile);
   };
   SeqShare s;
   SeqUnits u = units_of(lane);
@@ -315,6 +319,7 @@ __device__ __forceinline__ SeqShare seq_share(const SeqAttnArgs& a, int slot, in
     }
     s.total += wave_sum_int(n);
   }
+  if (__builtin_amdgcn_ballot_w64(falls) != 0) s.total = 0;
   s.share = max((s.total + a.slots - 1) / a.slots, kSeqMinShare);
   const int64_t x = (int64_t)slot * s.share;
   s.base = 0;
