@@ -69,6 +69,7 @@ SIGNATURES = {
 PACKED_ATTENTION = struct.Struct("q3QQQ6q7if")
 CACHE_ROWS = struct.Struct("q2Q2Q3Q11q8i")
 CACHE_ATTENTION = struct.Struct("q3Q3Q2Qq9q10ifi")
+PACK_ERRORS = (struct.error, OverflowError)  # a number that its field cannot hold
 
 _lock = threading.Lock()
 _lib = None

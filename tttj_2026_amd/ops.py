@@ -286,9 +286,14 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     starts = _int32(starts, "starts", batch + 1, index)
     out = _context(out, q, tokens, heads * hd)
     args = _lib.PACKED_ATTENTION
-    _call("tt_packed_attention_fwd", args.pack(
-        args.size, q_at, k_at, v_at, starts.data_ptr(), out.data_ptr(), q_row, q_head, k_row, k_head, v_row, v_head,
-        tokens, batch, heads, kv_heads, hd, causal, _SEQ_DTYPES[dtype], hd ** -0.5 if scale is None else scale), index)
+    try:
+        packed = args.pack(
+            args.size, q_at, k_at, v_at, starts.data_ptr(), out.data_ptr(), q_row, q_head, k_row, k_head, v_row,
+            v_head, tokens, batch, heads, kv_heads, hd, causal, _SEQ_DTYPES[dtype],
+            hd ** -0.5 if scale is None else scale)
+    except _lib.PACK_ERRORS as e:
+        raise ValueError(f"packed_attention: {e}") from None
+    _call("tt_packed_attention_fwd", packed, index)
     return out
 
 
@@ -314,10 +319,14 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     k_half, v_half = _cache(k_cache, "k_cache", shape, dtype, index), _cache(v_cache, "v_cache", shape, dtype, index)
     table, lengths, starts, batch, table_pages, table_row = _sequences(tokens, page_table, lengths, starts, index)
     args = _lib.CACHE_ROWS
-    _call("tt_cache_append", args.pack(
-        args.size, k_at, v_at, k_half[0], v_half[0], table.data_ptr(), lengths.data_ptr(),
-        0 if starts is None else starts.data_ptr(), k_row, k_head, v_row, v_head, *k_half[1:], *v_half[1:], table_row,
-        tokens, batch, kv_heads, hd, shape[0], shape[1], table_pages, 0), index)
+    try:
+        packed = args.pack(
+            args.size, k_at, v_at, k_half[0], v_half[0], table.data_ptr(), lengths.data_ptr(),
+            0 if starts is None else starts.data_ptr(), k_row, k_head, v_row, v_head, *k_half[1:], *v_half[1:],
+            table_row, tokens, batch, kv_heads, hd, shape[0], shape[1], table_pages, 0)
+    except _lib.PACK_ERRORS as e:
+        raise ValueError(f"cache_append: {e}") from None
+    _call("tt_cache_append", packed, index)
 
 
 def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -345,9 +354,13 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                                   starts is None)
     work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     args = _lib.CACHE_ATTENTION
-    _call("tt_cache_attention_fwd", args.pack(
-        args.size, q_at, k_half[0], v_half[0], table.data_ptr(), lengths.data_ptr(),
-        0 if starts is None else starts.data_ptr(), out.data_ptr(), 0 if work is None else work.data_ptr(), nbytes,
-        q_row, q_head, *k_half[1:], *v_half[1:], table_row, tokens, batch, heads, kv_heads, hd, pages, page,
-        table_pages, max_length, _SEQ_DTYPES[dtype], hd ** -0.5 if scale is None else scale, 0), index)
+    try:
+        packed = args.pack(
+            args.size, q_at, k_half[0], v_half[0], table.data_ptr(), lengths.data_ptr(),
+            0 if starts is None else starts.data_ptr(), out.data_ptr(), 0 if work is None else work.data_ptr(), nbytes,
+            q_row, q_head, *k_half[1:], *v_half[1:], table_row, tokens, batch, heads, kv_heads, hd, pages, page,
+            table_pages, max_length, _SEQ_DTYPES[dtype], hd ** -0.5 if scale is None else scale, 0)
+    except _lib.PACK_ERRORS as e:
+        raise ValueError(f"cache_attention: {e}") from None
+    _call("tt_cache_attention_fwd", packed, index)
     return out
