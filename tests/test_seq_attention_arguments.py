@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tttj_2026_amd import ops
+from tttj_2026_amd import _lib, ops
 
 
 @pytest.fixture
@@ -40,3 +40,12 @@ def test_more_tokens_and_pages_than_an_int32(host):
         ops.cache_append(one, one, pages, pages, table, starts[:1], torch.tensor([0, 1], dtype=torch.int32))
     with pytest.raises(ValueError, match="cache_attention"):
         ops.cache_attention(one, pages, pages, table, starts[:1])
+
+
+@pytest.mark.parametrize("hd,waves", [(64, 2), (128, 2), (136, 1), (256, 1)])
+def test_keys_are_dealt_out_after_16_rounds_of_a_block(hd, waves):
+    """More blocks of 32 rows than CUs: a block of `waves` waves takes 16 rounds of 32 keys each alone."""
+    size = _lib.cache_attention_workspace_bytes
+    rows, longest = 300, 16 * 32 * waves
+    assert size(rows, rows, 8, 2, hd, 16, 128, longest, True) == 0
+    assert size(rows, rows, 8, 2, hd, 16, 128, longest + 1, True) > 0

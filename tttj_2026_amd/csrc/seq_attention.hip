@@ -310,8 +310,10 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   // heads of 64, 1000 keys (4 rounds) 9.3 -> 11.0 us, 2000 12.9 -> 11.5; 8 blocks of 4 on heads of 128, 500 keys 9.9 ->
   // 12.4, 1000 (8 rounds) 14.1 -> 12.7.  Blocks that fill a good part of the chip gain less: 256 on heads of 64, 4000
   // keys (16 rounds) 46 -> 50, 8000 99 -> 105; 128 on heads of 128, 2000 (16) 27 -> 30, 4000 49 -> 48, and with lengths
-  // from 1 to 4000 39 -> 32; 512 of two waves on heads of 128, 1000 keys (16) 43 -> 47, lengths to 4000 125 -> 107.
-  const int keys_per_round = 32 * (p.shape == SeqShape::kDeep ? (head_dim <= 64 ? 8 : head_dim <= 128 ? 4 : 2) : 2);
+  // from 1 to 4000 39 -> 32; 512 of two waves on heads of 128, 1000 keys (16) 43 -> 47, lengths to 4000 125 -> 107; 512 of
+  // one wave on heads of 256, 700 keys (22) 66 -> 69, lengths to 700 43.3 -> 42.5, to 1020 60 -> 54; 300 of one, 700 keys
+  // 42 -> 49, lengths to 700 40 -> 34.
+  const int keys_per_round = wide ? 64 : 32 * seq_waves(p.shape, head_dim);
   const int alone = (blocks <= cus / 4 ? 6 : 16) * keys_per_round;
   // Beyond the blocks that the chip holds (four times as many of 32 rows), tiles spread by themselves: 1088 tiles of 128
   // rows over 500 to 4600 keys, 195 alone and 272 in shares; 800 of 32 rows over 1 to 4000 keys, 193 and 162.

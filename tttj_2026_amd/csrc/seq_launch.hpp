@@ -12,6 +12,11 @@ namespace tt {
 // or two waves; and of 32 rows with as many waves as the LDS holds tiles for, where blocks are few.
 enum class SeqShape { kWide, kNarrow, kDeep };
 
+// Waves of a block of 32 rows on heads up to `hd`.
+constexpr int seq_waves(SeqShape shape, int hd) {
+  return shape == SeqShape::kDeep ? (hd <= 64 ? 8 : hd <= 128 ? 4 : 2) : (hd <= 128 ? 2 : 1);
+}
+
 template <typename T, int HD, int RW, int KW, int KT, bool PAGED>
 int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
   constexpr int lds = 2 * 2 * KW * KT * HD * (int)sizeof(T);  // K and V, two tiles deep
@@ -37,8 +42,8 @@ int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
 template <int HD, typename T>
 int launch_seq_type(const SeqAttnArgs& a, bool paged, SeqShape shape, hipStream_t stream) {
   if (!paged) return launch_seq<T, HD, 4, 1, 64, false>(a, stream);
-  if (shape == SeqShape::kDeep) return launch_seq<T, HD, 1, (HD <= 64 ? 8 : HD <= 128 ? 4 : 2), 32, true>(a, stream);
-  if (shape == SeqShape::kNarrow) return launch_seq<T, HD, 1, (HD <= 128 ? 2 : 1), 32, true>(a, stream);
+  if (shape == SeqShape::kDeep) return launch_seq<T, HD, 1, seq_waves(SeqShape::kDeep, HD), 32, true>(a, stream);
+  if (shape == SeqShape::kNarrow) return launch_seq<T, HD, 1, seq_waves(SeqShape::kNarrow, HD), 32, true>(a, stream);
   return launch_seq<T, HD, 4, 1, 64, true>(a, stream);
 }
 
