@@ -345,11 +345,8 @@ template <typename T, int HD, int RW, int KW, int KT, bool PAGED, int WPE = (HD 
 __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void seq_attention_kernel(SeqAttnArgs a) {
   using v2 = typename Num<T>::v2;
   using v8 = typename Num<T>::v8;
-  constexpr int CB = 1;                     // 32-row blocks of a wave (2 leave registers for one wave per SIMD only)
-  constexpr int WR = 32 * CB;               // rows of a wave
-  constexpr int R = WR * RW;
+  constexpr int R = 32 * RW;                // rows of a block (64 a wave leave registers for one wave per SIMD only)
   constexpr bool PIPE = RW > 1;              // softmax beside the next keys' products
-  constexpr int SB = PIPE ? 1 : KT / 32;    // 32-key blocks whose scores are taken at once
   constexpr int KSTEPS = HD / 16;           // k-steps of S^T
   constexpr int DB = HD / 32;               // 32-row blocks of O^T
   constexpr int CH = HD / 8;                // 16-byte chunks of a row
@@ -462,19 +459,13 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   const int ntiles = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
 
   // Rows of this wave; those behind the last repeat it and are not stored, so limits rise along the rows.
-  const int wr0 = r0 + rw * WR;
+  const int wr0 = r0 + rw * 32;
   const bool wave_active = wr0 < rows;
   const int block_lo = seq_limit(a, r0 / G, sq.count, keys);  // the first row's
   const int lim_lo = seq_limit(a, min(wr0, rows - 1) / G, sq.count, keys);
-  const int lim_hi = min(seq_limit(a, min(wr0 + WR - 1, rows - 1) / G, sq.count, keys), kend);
-  int tok[CB], head[CB], lim[CB];
-#pragma unroll
-  for (int b = 0; b < CB; ++b) {
-    const int r = min(wr0 + 32 * b + col, rows - 1);
-    tok[b] = r / G;
-    head[b] = hkv * G + r - tok[b] * G;
-    lim[b] = seq_limit(a, tok[b], sq.count, keys);
-  }
+  const int lim_hi = min(seq_limit(a, min(wr0 + 31, rows - 1) / G, sq.count, keys), kend);
+  const int own = min(wr0 + col, rows - 1);  // this lane's row
+  const int tok = own / G, head = hkv * G + own - tok * G, lim = seq_limit(a, tok, sq.count, keys);
 
   // Paged: lane l holds the page of the 16-key group l behind key t0 (of the first 8).
   auto tile_pages = [&](int t0) TT_INLINE -> int {
@@ -586,40 +577,37 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     if constexpr (RW > 1) raw_barrier();
   };
 
-  floatx16 o[CB][DB];
-  float m_ref[CB], l_run[CB], mc[CB], thr[CB];
+  floatx16 o[DB];
+  float m_ref, l_run, mc, thr;
 
   // Asked for after the first copies, which need addresses of their own first.  Branches are the wave's: where lanes went
   // around loads past head_dim by themselves, the compiler saved registers that every lane needs for the next tile in that
   // branch's last block, with half of the lanes off.
-  v8 qf[CB][KSTEPS];
+  v8 qf[KSTEPS];
   auto load_q = [&]() TT_INLINE {
     int width = hd;
     asm volatile("" : "+s"(width));  // (the comparisons would be kept in registers)
+    const T* qp = static_cast<const T*>(a.q) + (int64_t)(sq.first + tok) * a.q_row + head * a.q_head;
+    if (!FAR && width == HD) {
 #pragma unroll
-    for (int b = 0; b < CB; ++b) {
-      const T* qp = static_cast<const T*>(a.q) + (int64_t)(sq.first + tok[b]) * a.q_row + head[b] * a.q_head;
-      if (!FAR && width == HD) {
+      for (int kk = 0; kk < KSTEPS; ++kk) qf[kk] = *reinterpret_cast<const v8*>(qp + 16 * kk + 8 * hf);
+    } else {
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) qf[b][kk] = *reinterpret_cast<const v8*>(qp + 16 * kk + 8 * hf);
-      } else {
-#pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) {
-          const u32x4 none = {0u, 0u, 0u, 0u};
-          u32x4 x = none;
-          if (16 * kk + 8 < width) {
-            x = *reinterpret_cast<const u32x4*>(qp + 16 * kk + 8 * hf);
-          } else if (16 * kk < width) {
-            x = *reinterpret_cast<const u32x4*>(qp + 16 * kk);
-            x = hf == 0 ? x : none;
-          }
-          qf[b][kk] = __builtin_bit_cast(v8, x);
+      for (int kk = 0; kk < KSTEPS; ++kk) {
+        const u32x4 none = {0u, 0u, 0u, 0u};
+        u32x4 x = none;
+        if (16 * kk + 8 < width) {
+          x = *reinterpret_cast<const u32x4*>(qp + 16 * kk + 8 * hf);
+        } else if (16 * kk < width) {
+          x = *reinterpret_cast<const u32x4*>(qp + 16 * kk);
+          x = hf == 0 ? x : none;
         }
+        qf[kk] = __builtin_bit_cast(v8, x);
       }
     }
   };
-  using Scores = floatx16[CB][SB];
-  using Probs = v8[CB][SB][2];
+  using Scores = floatx16;  // of 32 keys
+  using Probs = v8[2];
   auto read_k = [&](int kk, int st, int kb) TT_INLINE -> v8 {  // 32 keys, features 16 kk + 8 hf + {0..7}
     const uint32_t stage = 2 * (st * TILE + kb * 32 * HD);
     const uint32_t at = FAR ? (kread[0] + stage) ^ (32 * kk) : kread[kk] + stage;
@@ -652,143 +640,92 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       else __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
   };
-  auto scores = [&](Scores& s, int st, int kb0) TT_INLINE {
+  auto scores = [&](Scores& s, int st, int kb) TT_INLINE {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
     if constexpr (FAR) {
+      ahead([&](int kk) TT_INLINE { return read_k(kk, st, kb); }, 1,
+            [&](int kk, v8 x) TT_INLINE { s = Num<T>::mfma(x, qf[kk], s); }, std::integral_constant<int, KSTEPS>{});
+    } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[0][0][e] = 0.f;
-      ahead([&](int kk) TT_INLINE { return read_k(kk, st, kb0); }, 1,
-            [&](int kk, v8 x) TT_INLINE { s[0][0] = Num<T>::mfma(x, qf[0][kk], s[0][0]); },
-            std::integral_constant<int, KSTEPS>{});
-      return;
+      for (int kk = 0; kk < KSTEPS; ++kk) s = Num<T>::mfma(read_k(kk, st, kb), qf[kk], s);
     }
-#pragma unroll
-    for (int kb = 0; kb < SB; ++kb)
-#pragma unroll
-      for (int kk = 0; kk < KSTEPS; ++kk) {
-        const v8 x = read_k(kk, st, kb0 + kb);
-#pragma unroll
-        for (int b = 0; b < CB; ++b) {
-          if (kk == 0) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[b][kb][e] = 0.f;
-          }
-          s[b][kb] = Num<T>::mfma(x, qf[b][kk], s[b][kb]);
-        }
-      }
   };
   auto mask_scores = [&](Scores& s, int t0, uint32_t bad) TT_INLINE {
-    if (t0 + 32 * SB <= lim_lo && bad == 0) return;
+    if (t0 + 32 <= lim_lo && bad == 0) return;
+    const int rem = lim - t0 - 4 * hf;
 #pragma unroll
-    for (int b = 0; b < CB; ++b) {
-      const int rem = lim[b] - t0 - 4 * hf;
-#pragma unroll
-      for (int kb = 0; kb < SB; ++kb)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if ((bad >> (2 * kb + (j >> 3))) & 1u) s[b][kb][j] = __builtin_nanf("");
-          s[b][kb][j] = 32 * kb + 8 * (j >> 2) + (j & 3) < rem ? s[b][kb][j] : -INFINITY;
-        }
+    for (int j = 0; j < 16; ++j) {
+      if ((bad >> (j >> 3)) & 1u) s[j] = __builtin_nanf("");
+      s[j] = 8 * (j >> 2) + (j & 3) < rem ? s[j] : -INFINITY;
     }
   };
-  auto row_max = [&](const Scores& s, float (&mt)[CB]) TT_INLINE {
+  auto row_max = [&](const Scores& s) TT_INLINE -> float {
+    float mx = s[0];
 #pragma unroll
-    for (int b = 0; b < CB; ++b) {
-      float mx = s[b][0][0];
-#pragma unroll
-      for (int kb = 0; kb < SB; ++kb)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[b][kb][j]);
-      mt[b] = xhalf_max(mx);
-    }
+    for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[j]);
+    return xhalf_max(mx);
   };
-  auto move_max = [&](const float (&mt)[CB]) TT_INLINE {
-    bool grows = mt[0] > thr[0];
+  auto move_max = [&](float mt) TT_INLINE {
+    if (__builtin_amdgcn_ballot_w64(mt > thr) == 0) return;
+    const float m_new = fmaxf(m_ref, mt);
+    const bool none = m_new == -INFINITY;  // no key of this row so far: o and l are 0
+    const float corr = none ? 1.f : seq_weight((m_ref - m_new) * c2);
+    m_ref = m_new;
+    mc = none ? 0.f : m_new * c2 - Num<T>::kShift;
+    thr = none ? -INFINITY : m_new + lazy;
+    l_run *= corr;
 #pragma unroll
-    for (int b = 1; b < CB; ++b) grows |= mt[b] > thr[b];
-    if (__builtin_amdgcn_ballot_w64(grows) == 0) return;
+    for (int i = 0; i < DB; ++i)
 #pragma unroll
-    for (int b = 0; b < CB; ++b) {
-      const float m_new = fmaxf(m_ref[b], mt[b]);
-      const bool none = m_new == -INFINITY;  // no key of this row so far: o and l are 0
-      const float corr = none ? 1.f : seq_weight((m_ref[b] - m_new) * c2);
-      m_ref[b] = m_new;
-      mc[b] = none ? 0.f : m_new * c2 - Num<T>::kShift;
-      thr[b] = none ? -INFINITY : m_new + lazy;
-      l_run[b] *= corr;
-#pragma unroll
-      for (int i = 0; i < DB; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[b][i][e] *= corr;
-    }
+      for (int e = 0; e < 16; ++e) o[i][e] *= corr;
   };
   auto probabilities = [&](const Scores& s, Probs& p16) TT_INLINE {
 #pragma unroll
-    for (int b = 0; b < CB; ++b)
-#pragma unroll
-      for (int kb = 0; kb < SB; ++kb)
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][kb][j], c2, -mc[b]));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b][kb][j + 1], c2, -mc[b]));
-          p16[b][kb][j >> 3][j & 7] = (T)p0;
-          p16[b][kb][j >> 3][(j & 7) + 1] = (T)p1;
-        }
+    for (int j = 0; j < 16; j += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[j], c2, -mc));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[j + 1], c2, -mc));
+      p16[j >> 3][j & 7] = (T)p0;
+      p16[j >> 3][(j & 7) + 1] = (T)p1;
+    }
   };
   auto add_sums = [&](const Probs& p16) TT_INLINE {
 #pragma unroll
-    for (int b = 0; b < CB; ++b)
-#pragma unroll
-      for (int kb = 0; kb < SB; ++kb)
-#pragma unroll
-        for (int j = 0; j < 16; j += 2)
-          l_run[b] = Num<T>::add2(v2{p16[b][kb][j >> 3][j & 7], p16[b][kb][j >> 3][(j & 7) + 1]}, l_run[b]);
+    for (int j = 0; j < 16; j += 2) l_run = Num<T>::add2(v2{p16[j >> 3][j & 7], p16[j >> 3][(j & 7) + 1]}, l_run);
   };
   // The probabilities are made by here.
   auto pin = [&](Probs& p16) TT_INLINE {
 #pragma unroll
-    for (int b = 0; b < CB; ++b)
-#pragma unroll
-      for (int kb = 0; kb < SB; ++kb)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) asm volatile("" : "+v"(p16[b][kb][c]));
+    for (int c = 0; c < 2; ++c) asm volatile("" : "+v"(p16[c]));
   };
-  auto add_values = [&](const Probs& p16, int st, int kb0) TT_INLINE {
+  auto add_values = [&](const Probs& p16, int st, int kb) TT_INLINE {
     if constexpr (FAR) {
-      ahead([&](int j) TT_INLINE { return read_v(j % DB, st, 2 * kb0 + j / DB); }, 2,
-            [&](int j, v8 x) TT_INLINE { o[0][j % DB] = Num<T>::mfma(x, p16[0][0][j / DB], o[0][j % DB]); },
+      ahead([&](int j) TT_INLINE { return read_v(j % DB, st, 2 * kb + j / DB); }, 2,
+            [&](int j, v8 x) TT_INLINE { o[j % DB] = Num<T>::mfma(x, p16[j / DB], o[j % DB]); },
             std::integral_constant<int, 2 * DB>{});
-      return;
-    }
-#pragma unroll
-    for (int kb = 0; kb < SB; ++kb)
+    } else {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < DB; ++i) {
-          const v8 x = read_v(i, st, 2 * (kb0 + kb) + c);
-#pragma unroll
-          for (int b = 0; b < CB; ++b) o[b][i] = Num<T>::mfma(x, p16[b][kb][c], o[b][i]);
-        }
+        for (int i = 0; i < DB; ++i) o[i] = Num<T>::mfma(read_v(i, st, 2 * kb + c), p16[c], o[i]);
+    }
   };
   {
 #pragma unroll
-    for (int b = 0; b < CB; ++b) {
+    for (int i = 0; i < DB; ++i)
 #pragma unroll
-      for (int i = 0; i < DB; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[b][i][e] = 0.f;
-      m_ref[b] = -INFINITY;  // the maximum that the sums are relative to, in units of the raw scores
-      l_run[b] = 0.f;        // this lane's half of the row's sum
-      mc[b] = 0.f;           // m_ref c log2(e) - kShift
-      thr[b] = -INFINITY;    // a tile maximum above this moves m_ref
-    }
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    m_ref = -INFINITY;  // the maximum that the sums are relative to, in units of the raw scores
+    l_run = 0.f;        // this lane's half of the row's sum
+    mc = 0.f;           // m_ref c log2(e) - kShift
+    thr = -INFINITY;    // a tile maximum above this moves m_ref
 
     if constexpr (PIPE) {
       static_assert(KW == 1 && KT == 64, "two steps of 32 keys per tile");
       const int steps = wave_active && lim_hi > kbeg ? (lim_hi - kbeg + 31) / 32 : 0;  // of this wave
       int pe = 0, pe_next = 0;  // pages from this tile's and the next tile's first key on
       Scores sa, sb;
-      float mt[CB];
+      float mt;
       if (ntiles > 0) {
         if constexpr (PAGED) {
           pe = tile_pages(kbeg);
@@ -805,7 +742,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       if (steps > 0) {
         scores(sa, 1, 1);
         mask_scores(sa, kbeg, PAGED ? bad_groups(pe, kbeg) : 0);
-        row_max(sa, mt);
+        mt = row_max(sa);
         move_max(mt);
       }
       lds_done();
@@ -823,7 +760,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         __builtin_amdgcn_s_setprio(1);  // (prompts take 1 to 3% longer without)
         add_sums(p16);
         add_values(p16, st, h);
-        row_max(sn, mt);
+        mt = row_max(sn);
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(0);
         move_max(mt);
@@ -911,7 +848,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     } else {
       // Tiles grp, grp + KW, ... by this wave alone.  The tile after the next is asked for as soon as this one's
       // fragments are in registers, so that close to two tiles are in flight all the time.
-      static_assert(RW == 1 && CB == 1 && SB == 1, "a wave's own tiles of 32 keys");
+      static_assert(RW == 1 && KT == 32, "a wave's own tiles of 32 keys");
       constexpr int COPIES = 2 * PG * CPG;  // of a tile
       const int rounds = (ntiles - grp + KW - 1) / KW;
       const int t_first = kbeg + grp * KT;
@@ -951,11 +888,11 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         __builtin_amdgcn_sched_barrier(0);
         Scores s;
         Probs p16;
-        float mt[CB];
+        float mt;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[0][0][e] = 0.f;
+        for (int e = 0; e < 16; ++e) s[e] = 0.f;
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) s[0][0] = Num<T>::mfma(kf[kk], qf[0][kk], s[0][0]);
+        for (int kk = 0; kk < KSTEPS; ++kk) s = Num<T>::mfma(kf[kk], qf[kk], s);
         const uint32_t bad = PAGED ? bad_groups(pe0, t0) : 0;
         const int pn = pe2;
         if constexpr (PAGED) {
@@ -970,40 +907,37 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           issue_v(at, st);
         }
         mask_scores(s, t0, bad);
-        row_max(s, mt);
+        mt = row_max(s);
         move_max(mt);
         probabilities(s, p16);
         add_sums(p16);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < DB; ++i) o[0][i] = Num<T>::mfma(vf[c][i], p16[0][0][c], o[0][i]);
+          for (int i = 0; i < DB; ++i) o[i] = Num<T>::mfma(vf[c][i], p16[c], o[i]);
       }
     }
   }
   // Sums of this wave's rows over both halves of the wave.
-  float l_row[CB];
-#pragma unroll
-  for (int b = 0; b < CB; ++b) l_row[b] = xhalf_sum(l_run[b]);
+  float l_row = xhalf_sum(l_run);
 
   // A sum that is NaN though its row's scores are not holds infinities of V (restore_odd); the sum of the sums tells, or
   // raises a false alarm.
-  static_assert(CB == 1, "one block of rows per wave");
   float all = 0.f;
 #pragma unroll
   for (int i = 0; i < DB; ++i) {
-    float sum = o[0][i][0];
+    float sum = o[i][0];
 #pragma unroll
-    for (int e = 1; e < 16; ++e) sum += o[0][i][e];
+    for (int e = 1; e < 16; ++e) sum += o[i][e];
     all += sum;
   }
-  bool lost = all != all && l_row[0] == l_row[0];
+  bool lost = all != all && l_row == l_row;
   if (RW > 1 && mixed) odd = __syncthreads_or(odd) != 0;
 
   // Over the groups, by all of them: group g joins the g-th, (g + KW)-th, ... of the 4-feature pieces that a lane holds,
   // from [group][piece][lane] and (maximum, sum) in LDS.
   if constexpr (KW > 1) {
-    static_assert(CB == 1 && RW == 1, "groups are waves with one block of rows");
+    static_assert(RW == 1, "groups are waves");
     floatx4* const pieces = reinterpret_cast<floatx4*>(seq_lds);
     float2* const sums = reinterpret_cast<float2*>(pieces + KW * DB * 4 * 64);
     int* const flags = reinterpret_cast<int*>(sums + KW * 32);
@@ -1013,8 +947,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         pieces[(grp * DB * 4 + i * 4 + g) * 64 + lane] =
-            floatx4{o[0][i][4 * g], o[0][i][4 * g + 1], o[0][i][4 * g + 2], o[0][i][4 * g + 3]};
-    if (hf == 0) sums[grp * 32 + col] = make_float2(m_ref[0], l_row[0]);
+            floatx4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+    if (hf == 0) sums[grp * 32 + col] = make_float2(m_ref, l_row);
     const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0, any_lost = __builtin_amdgcn_ballot_w64(lost) != 0;
     flags[grp] = (any_odd ? 1 : 0) | (any_lost ? 2 : 0);
     __syncthreads();
@@ -1036,8 +970,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       w[g] = ml[g].x == -INFINITY ? ml[g].y : seq_weight((ml[g].x - m) * c2);
       l = fmaf(w[g], ml[g].y, l);
     }
-    m_ref[0] = m;
-    l_row[0] = l;
+    m_ref = m;
+    l_row = l;
 #pragma unroll
     for (int i = 0; i < DB; ++i)
 #pragma unroll
@@ -1051,7 +985,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           for (int e = 0; e < 4; ++e) sum[e] = fmaf(w[k], y[e], sum[e]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[0][i][4 * g + e] = sum[e];
+        for (int e = 0; e < 4; ++e) o[i][4 * g + e] = sum[e];
       }
   }
 
@@ -1060,22 +994,21 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   // number, against bank conflicts.)
   if constexpr (RW > 1) {
     if (part < 0) {
-      static_assert(CB == 1, "one block of rows per wave");
       constexpr int SW = CH < 16 ? CH - 1 : 15;
       T* const tile = reinterpret_cast<T*>(seq_lds) + rw * 32 * HD;
       __syncthreads();
-      const float inv = l_row[0] == 0.f ? 0.f : 1.0f / l_row[0];  // no key: zeros
+      const float inv = l_row == 0.f ? 0.f : 1.0f / l_row;  // no key: zeros
 #pragma unroll
       for (int i = 0; i < DB; ++i)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           typedef T v4 __attribute__((ext_vector_type(4)));
           *reinterpret_cast<v4*>(tile + col * HD + (((4 * i + g) ^ (col & SW)) * 8 + 4 * hf)) =
-              v4{(T)(o[0][i][4 * g] * inv), (T)(o[0][i][4 * g + 1] * inv), (T)(o[0][i][4 * g + 2] * inv),
-                 (T)(o[0][i][4 * g + 3] * inv)};
+              v4{(T)(o[i][4 * g] * inv), (T)(o[i][4 * g + 1] * inv), (T)(o[i][4 * g + 2] * inv),
+                 (T)(o[i][4 * g + 3] * inv)};
         }
       lds_done();
-      const int place = tok[0] * a.heads + head[0];  // lane r holds row r's
+      const int place = tok * a.heads + head;  // lane r holds row r's
       T* const out = static_cast<T*>(a.out) + (int64_t)sq.first * a.heads * hd;
 #pragma unroll
       for (int e = 0; e < 32 * CH / 64; ++e) {
@@ -1089,10 +1022,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
 
   // Other output rows, or a part's sums: O and the sum in units of exp2(m - kShift), the maximum in log2 units.
   const int64_t part0 = ((int64_t)part * a.kv_heads + hkv) * R - r0;  // + row
-#pragma unroll
-  for (int b = 0; b < CB; ++b) {
-    const int r = wr0 + 32 * b + col;
-    if (r >= rows) continue;
+  const int r = wr0 + col;
+  if (r < rows) {
     if (part >= 0) {
       float* const dst = RW > 1 ? a.part_o + (part0 + r0) * hd + wide_place(hd, r - r0, 4 * hf)
                                 : a.part_o + (part0 + r) * hd + 4 * hf;
@@ -1102,24 +1033,24 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         for (int g = 0; g < 4; ++g)
           if (32 * i + 8 * g < hd && (i * 4 + g) % KW == grp)
             *reinterpret_cast<floatx4*>(dst + (4 * i + g) * (RW > 1 ? 256 : 8)) =
-                floatx4{o[b][i][4 * g], o[b][i][4 * g + 1], o[b][i][4 * g + 2], o[b][i][4 * g + 3]};
-      if (hf == 0 && grp == 0) a.part_ml[part0 + r] = make_float2(m_ref[b] * c2, l_row[b]);
-      continue;
+                floatx4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
+      if (hf == 0 && grp == 0) a.part_ml[part0 + r] = make_float2(m_ref * c2, l_row);
+    } else if constexpr (RW == 1) {
+      const float inv = l_row == 0.f ? 0.f : 1.0f / l_row;
+      T* dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + tok) * a.heads + head) * hd;
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (32 * i + 8 * g < hd && (i * 4 + g) % KW == grp) {
+            typedef T v4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<v4*>(dst + 32 * i + 8 * g + 4 * hf) =
+                v4{(T)(o[i][4 * g] * inv), (T)(o[i][4 * g + 1] * inv), (T)(o[i][4 * g + 2] * inv),
+                   (T)(o[i][4 * g + 3] * inv)};
+          }
     }
-    if constexpr (RW > 1) continue;
-    const float inv = l_row[b] == 0.f ? 0.f : 1.0f / l_row[b];
-    T* dst = static_cast<T*>(a.out) + ((int64_t)(sq.first + tok[b]) * a.heads + head[b]) * hd;
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (32 * i + 8 * g < hd && (i * 4 + g) % KW == grp) {
-          typedef T v4 __attribute__((ext_vector_type(4)));
-          *reinterpret_cast<v4*>(dst + 32 * i + 8 * g + 4 * hf) =
-              v4{(T)(o[b][i][4 * g] * inv), (T)(o[b][i][4 * g + 1] * inv), (T)(o[b][i][4 * g + 2] * inv),
-                 (T)(o[b][i][4 * g + 3] * inv)};
-        }
   }
+
   // restore_odd: the infinities and NaN of V.  No probability of a key that a row sees is 0 by the definition, so such a
   // value alone decides the sums that it enters.  Where settle_v took some out, or where a sum is NaN (an infinity times a
   // probability that is 0 in T), a wave adds them to what its rows that see them have in memory; adding one twice changes
@@ -1132,7 +1063,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       int l = lane;
       asm volatile("" : "+v"(l));  // (what follows from it is worked out again instead of being held in registers)
       const int h = l >> 5, row = wr0 + (l & 31), r = min(row, rows - 1), token = r / G;
-      const int seen = l_row[0] == 0.f ? 0 : seq_limit(a, token, sq.count, keys);
+      const int seen = l_row == 0.f ? 0 : seq_limit(a, token, sq.count, keys);
       const bool any_lost = __builtin_amdgcn_ballot_w64(lost) != 0;
       T* const out =
           static_cast<T*>(a.out) + ((int64_t)(sq.first + token) * a.heads + hkv * G + r - token * G) * hd + 4 * h;
@@ -1163,7 +1094,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           return vh + (int64_t)(sq.first + key) * a.v_row;
         }
       };
-      if (any_lost && row < rows && l_row[0] == l_row[0])
+      if (any_lost && row < rows && l_row == l_row)
         for (int c = 0; 8 * c < hd; ++c) update(c, [](float y, int) TT_INLINE { return y != y ? 0.f : y; });
       for (int k0 = any_lost ? kbeg : kbeg + max(block_lo - kbeg, 0) / KT * KT; k0 < lim_hi; k0 += RPC) {
         const T* const vp = values(min(k0 + l / CH, lim_hi - 1));  // RPC keys, 16 bytes per lane
