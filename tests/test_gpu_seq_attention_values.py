@@ -176,3 +176,20 @@ def test_falling_starts_with_keys_in_shares(length):
     y = ops.cache_attention(q, kc, vc, table, lengths, _i32(list(range(batch + 1))))
     limits = torch.full((tokens,), page)
     _check(y, *_attend(q, kc[0], vc[0], limits))
+
+
+@pytest.mark.parametrize("dtype,hd", [(F16, 64), (BF16, 128), (BF16, 256)])
+@pytest.mark.parametrize("counts,lengths", [
+    ([600, 1, 1, 0, 3], [700, 9000, 1, 30, 5000]),                      # tiles of 128 rows, keys dealt out
+    ([1, 2600, 1, 40], [7000, 2600, 90, 3000]),                         # ... more tiles than the chip holds
+    ([300] + [1] * 200, [800] + [1 + 37 * b % 1900 for b in range(200)]),  # tiles of 32 rows
+])
+def test_chunks_and_single_tokens_in_one_call(dtype, hd, counts, lengths):
+    """New tokens of prompts that are read in pieces beside single tokens over long contexts."""
+    kc, vc, table, k, v = _store(lengths, 2, hd, 16, dtype)
+    q = _randn(7, sum(counts), 8, hd, dtype=dtype)
+    ref = _over_cache(q, k, v, counts, lengths)
+    for most in (None, max(lengths), 1):
+        y = ops.cache_attention(q, kc, vc, table, _i32(lengths), _starts(counts), max_length=most)
+        _check(y, *ref)
+        assert torch.equal(y, ops.cache_attention(q, kc, vc, table, _i32(lengths), _starts(counts), max_length=most))
