@@ -256,8 +256,9 @@ int tt_attention_fwd_prescaled(const void* q, const void* k, const void* vt, con
  * head h reads key / value head h / (heads / kv_heads).  Strides (`*_row`, `*_head`) are in elements;
  * features are adjacent, and pointers and strides aligned to 16 bytes.  head_dim is a multiple of 8 up
  * to 256, scale positive (below 2e38), dtype TT_FP16 or TT_BF16 for all four tensors.  out overlaps
- * none of the others.  A row whose scores are all -infinity is +0.0.  Rows outside every sequence
- * are not written.  Values of `starts` outside [0, tokens] are taken as the nearest in it; where they
+ * none of the others.  A row whose scores are all -infinity is +0.0; infinities and NaN of v reach the
+ * rows that see them, and no other, whatever their probability.  Rows outside every sequence are not
+ * written.  Values of `starts` outside [0, tokens] are taken as the nearest in it; where they
  * fall, rows are arbitrary or left as they were.  No counterpart in the reference, whose attention
  * takes padded batches with as many key heads as query heads (kernels/case8_attention.py:48-206). */
 typedef struct {

@@ -20,12 +20,12 @@
 // How tiles are given to blocks: kSeq... below.  Where a tile's keys are split over blocks, parts of O with a maximum and
 // a sum each go through a workspace, and the seq_merge kernels join them.
 //
-// Measured on MI355X: prompts of 8192 and 3130 tokens, causal, 32 heads of 128 on 8, bf16: 600 us, 1.05 PFLOP/s (matrix
-// unit 55% busy, vector units 46%, at the power limit: 1.83 to 1.94 GHz); 2 x 4096 tokens on 16 heads of 64 90 us, 0.77
-// PFLOP/s; 12 prompts of 85 to 1500 tokens 115 us, 0.69 (a block takes 7 us to start and end, 1.8 us a tile of keys); 4 x
-// 4096 on 16 heads of 256 625 us, 0.88 PFLOP/s; 512 new tokens each for 8 sequences of up to 4608 keys 191 us, 0.86
-// PFLOP/s (2.1 us a tile: pages are looked up beside it).  4 tokens over 100000 keys each, 8 heads of 128: 285 us, 5.8 TB/s; 64
-// over 1 to 4000: 105 us.
+// Measured on MI355X: prompts of 8192 and 3130 tokens, causal, 32 heads of 128 on 8, bf16: 576 us, 1.09 PFLOP/s (matrix
+// unit 57% busy, vector units 47%, one of them 82%, at 1.80 GHz); 2 x 4096 tokens on 16 heads of 64 87 us, 0.79 PFLOP/s;
+// 12 prompts of 85 to 1500 tokens 113 us, 0.70 (a block takes 7 us to start and end, 1.8 us a tile of keys); 4 x 4096 on 16
+// heads of 256 631 to 650 us, 0.85 PFLOP/s; 512 new tokens each for 8 sequences of up to 4608 keys 184 us, 0.89 PFLOP/s (2.1
+// us a tile: pages are looked up beside it).  4 tokens over 100000 keys each, 8 heads of 128: 287 us, 5.7 TB/s; 64 over 1 to
+// 4000: 106 us.
 //
 // Per wave and tile: S^T = K Q^T with v_mfma_f32_32x32x16 (lane l holds row l % 32; of its 32 keys per block those
 // with bit 2 equal to l / 32), softmax with a running maximum and sum in fp32, O^T += V^T P^T.  K and V stay in the

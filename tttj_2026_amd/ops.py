@@ -301,8 +301,8 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
                  page_table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None) -> None:
     """Write the keys and values of new tokens, k and v [T, kv_heads, head_dim], into a paged cache, in place.
 
-    k_cache and v_cache are [pages, page_size, kv_heads, head_dim] (any strides that keep features adjacent and
-    16-byte alignment, e.g. both halves of one tensor, or a permuted [pages, kv_heads, page_size, head_dim]);
+    k_cache and v_cache are [pages, page_size, kv_heads, head_dim] (any strides that keep features adjacent, 16-byte
+    alignment and tokens less than 2^26 elements apart, e.g. both halves of one tensor, or a permuted [pages, kv_heads, page_size, head_dim]);
     page_size is a power of two from 16 on.  Position t of sequence b lies in page page_table[b, t // page_size]
     (int32 [B, n]) at t % page_size.  ``lengths`` (int32 [B]) counts the keys of each sequence with the new ones:
     the n tokens of sequence b, rows starts[b] ... starts[b + 1] - 1 (or row b alone without ``starts``), take
