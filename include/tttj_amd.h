@@ -316,6 +316,50 @@ int tt_cache_attention_workspace_bytes(int tokens, int batch, int heads, int kv_
                                        int64_t* bytes);
 int tt_cache_attention_fwd(const tt_cache_attention* args, void* stream);
 
+/* The same cache in 8 bits.  k_cache and v_cache hold e4m3 values (bytes; page, token and head strides
+ * `kc_*`, `vc_*` / `k_*`, `v_*` aligned to 16), and k_scales and v_scales a power of two 2^(s - 127) (a
+ * byte s; any strides) for each `block` tokens of a page and head: the value is the product.  block is
+ * a power of two from 16 to page_size, head_dim a multiple of 16.
+ *
+ * Append: a block's scale is the smallest that holds the largest finite magnitude of its tokens (at
+ * most 448 times the scale; 2^-127 where all are 0), and at least the scale that was there if older tokens of the
+ * sequence lie in the block, which are then rounded to the larger scale.  Values are rounded to the nearest
+ * e4m3 (ties to even) but not past 1.875 times the largest power of two of `dtype`; infinities and NaN
+ * become NaN.  Tokens behind the last of a sequence stay as they are.  Of two sequences that write to one block
+ * in one call the bytes of either may stay.  A scale of 255 is no number: it stays, and the keys of its block count
+ * as NaN in the attention, like those of a page outside the cache.
+ *
+ * Attention: K and V are widened to `dtype` (q's and out's): exact, but for products beyond its range.
+ * The workspace is that of tt_cache_attention8_workspace_bytes. */
+typedef struct {
+  int64_t size;
+  const void *k, *v;
+  void *k_cache, *v_cache;
+  uint8_t *k_scales, *v_scales;
+  const int32_t *table, *lengths, *starts;
+  int64_t k_row, k_head, v_row, v_head, kc_page, kc_row, kc_head, vc_page, vc_row, vc_head;
+  int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head, table_row;
+  int32_t tokens, batch, kv_heads, head_dim, pages, page_size, table_pages, block, dtype, reserved;
+} tt_cache_rows8;
+int tt_cache_append8(const tt_cache_rows8* args, void* stream);
+
+typedef struct {
+  int64_t size;
+  const void *q, *k_cache, *v_cache;
+  const uint8_t *k_scales, *v_scales;
+  const int32_t *table, *lengths, *starts;
+  void *out, *workspace;
+  int64_t workspace_bytes;
+  int64_t q_row, q_head, k_page, k_row, k_head, v_page, v_row, v_head;
+  int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head, table_row;
+  int32_t tokens, batch, heads, kv_heads, head_dim, pages, page_size, table_pages, max_length, block, dtype;
+  float scale;
+} tt_cache_attention8;
+int tt_cache_attention8_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int head_dim,
+                                        int page_size, int table_pages, int max_length, int single,
+                                        int64_t* bytes);
+int tt_cache_attention8_fwd(const tt_cache_attention8* args, void* stream);
+
 /* Where a forward's intermediates of its LAST layer are left in the workspace, for per-stage checks
  * of the fused plans (the megakernel's tasks and the fused-LN tiles never materialise LN1 / LN2 or
  * the other stages on their own): byte offsets of the Q / K / V^T planes (the TT_EPI_QKV layout;

@@ -57,6 +57,9 @@ SIGNATURES = {
     "tt_cache_append": (_I, [_P, _P]),
     "tt_cache_attention_workspace_bytes": (_I, [_I] * 9 + [ctypes.POINTER(_I64)]),
     "tt_cache_attention_fwd": (_I, [_P, _P]),
+    "tt_cache_append8": (_I, [_P, _P]),
+    "tt_cache_attention8_workspace_bytes": (_I, [_I] * 9 + [ctypes.POINTER(_I64)]),
+    "tt_cache_attention8_fwd": (_I, [_P, _P]),
     "tt_transformer_fwd": (_I, [_P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "tt_noalloc_scratch_bytes": (_I, [ctypes.POINTER(_I64)]),
     "tt_transformer_fwd_noalloc": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
@@ -69,6 +72,8 @@ SIGNATURES = {
 PACKED_ATTENTION = struct.Struct("q3QQQ6q7if")
 CACHE_ROWS = struct.Struct("q2Q2Q3Q11q8i")
 CACHE_ATTENTION = struct.Struct("q3Q3Q2Qq9q10ifi")
+CACHE_ROWS8 = struct.Struct("q2Q2Q2Q3Q17q10i")
+CACHE_ATTENTION8 = struct.Struct("q3Q2Q3Q2Qq15q11if")
 PACK_ERRORS = (struct.error, OverflowError)  # a number that its field cannot hold
 
 _lock = threading.Lock()
@@ -136,12 +141,11 @@ def workspace_bytes(batch: int, seq: int, d_model: int, heads: int, ffn_dim: int
 @functools.lru_cache(maxsize=1024)  # depends on these numbers alone; 0.2 us instead of 1.5
 def cache_attention_workspace_bytes(tokens: int, batch: int, heads: int, kv_heads: int,
                                     head_dim: int, page_size: int, table_pages: int,
-                                    max_length: int, single: bool) -> int:
+                                    max_length: int, single: bool, eight_bits: bool = False) -> int:
     out = _I64()
-    check(load().tt_cache_attention_workspace_bytes(tokens, batch, heads, kv_heads, head_dim,
-                                                    page_size, table_pages, max_length, int(single),
-                                                    ctypes.byref(out)),
-          "tt_cache_attention_workspace_bytes")
+    name = f"tt_cache_attention{'8' if eight_bits else ''}_workspace_bytes"
+    check(getattr(load(), name)(tokens, batch, heads, kv_heads, head_dim, page_size, table_pages, max_length,
+                                int(single), ctypes.byref(out)), name)
     return out.value
 
 

@@ -43,6 +43,8 @@ SOURCE_FLAGS = {
     "rowchain.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "seq_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "seq_attention_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "seq_attention8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "seq_attention8_wide.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "megakernel.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

@@ -1,0 +1,72 @@
+// Argument checks that the entry points over packed rows and the paged cache share.
+#pragma once
+
+#include "common.hpp"
+
+namespace tt {
+
+inline int check_heads(const char* what, int tokens, int batch, int heads, int kv_heads, int head_dim, int dtype) {
+  TT_REQUIRE(tokens >= 0 && batch >= 0, "%s: bad shape (tokens %d, batch %d)", what, tokens, batch);
+  TT_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: heads %d are no multiple of kv_heads %d", what,
+             heads, kv_heads);
+  TT_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "%s: head_dim %d is no multiple of 8 up to 256",
+             what, head_dim);
+  TT_REQUIRE((int64_t)tokens * heads < (1LL << 31), "%s: %d rows of %d heads", what, tokens, heads);
+  TT_REQUIRE(dtype == TT_FP16 || dtype == TT_BF16, "%s: bad dtype %d", what, dtype);
+  return TT_OK;
+}
+
+// Rows and heads are read 16 bytes at a time, and 16 rows at an offset of 32 bits.
+inline int check_rows(const char* what, const void* p, int64_t row, int64_t head) {
+  TT_REQUIRE(((uintptr_t)p & 15) == 0 && row % 8 == 0 && head % 8 == 0, "%s: not aligned to 16 bytes", what);
+  TT_REQUIRE(row >= 0 && head >= 0 && row < (1LL << 26), "%s: row stride of %lld elements", what, (long long)row);
+  return TT_OK;
+}
+
+inline int check_pages(const char* what, int pages, int page_size, int table_pages) {
+  TT_REQUIRE(pages > 0 && table_pages > 0, "%s: no pages (%d in the cache, %d per sequence)", what, pages, table_pages);
+  TT_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "%s: page_size %d is no power of two from 16 on",
+             what, page_size);
+  TT_REQUIRE((int64_t)page_size * table_pages <= (1LL << 30), "%s: %d pages of %d per sequence", what, table_pages,
+             page_size);
+  return TT_OK;
+}
+
+// A cache in 8 bits: rows and heads 16 bytes apart, a scale for each `block` tokens of a page and head.
+inline int check_head8(const char* what, int head_dim) {
+  TT_REQUIRE(head_dim % 16 == 0, "%s: head_dim %d is no multiple of 16, which a cache in 8 bits needs", what, head_dim);
+  return TT_OK;
+}
+
+inline int check_rows8(const char* what, const void* p, int64_t page, int64_t row, int64_t head) {
+  TT_REQUIRE(((uintptr_t)p & 15) == 0 && page % 16 == 0 && row % 16 == 0 && head % 16 == 0, "%s: not aligned to 16 bytes",
+             what);
+  TT_REQUIRE(page >= 0 && row >= 0 && head >= 0 && row < (1LL << 26), "%s: strides of %lld, %lld and %lld bytes", what,
+             (long long)page, (long long)row, (long long)head);
+  return TT_OK;
+}
+
+inline int check_block(const char* what, int block, int page_size) {
+  TT_REQUIRE(block >= 16 && block <= page_size && (block & (block - 1)) == 0,
+             "%s: a scale for each %d tokens of pages of %d (powers of two, from 16 on)", what, block, page_size);
+  return TT_OK;
+}
+
+inline int check_scales(const char* what, const void* p, int64_t page, int64_t block, int64_t head) {
+  TT_REQUIRE(p != nullptr && page >= 0 && block >= 0 && head >= 0, "%s: null pointer, or strides of %lld, %lld and %lld",
+             what, (long long)page, (long long)block, (long long)head);
+  return TT_OK;
+}
+
+}  // namespace tt
+
+#define TT_CHECK(call)            \
+  do {                            \
+    const int rc_ = (call);       \
+    if (rc_ != TT_OK) return rc_; \
+  } while (0)
+
+// The structure is the caller's: its size first.
+#define TT_ARGS(type, what)                                                                             \
+  TT_REQUIRE(args != nullptr && args->size == (int64_t)sizeof(type), what ": not a " #type " structure"); \
+  const type& c = *args

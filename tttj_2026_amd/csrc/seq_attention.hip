@@ -271,8 +271,9 @@ int launch_seq_attention(const SeqAttnArgs& a, bool paged, SeqShape shape, int d
 }
 
 // Blocks of a kernel that a CU holds (its registers, and its LDS: 16, 32, 64 or 128 KiB and a little more each).
-static int seq_resident(bool wide, int head_dim) {
+static int seq_resident(bool wide, int head_dim, bool bytes) {
   if (wide) return head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1;
+  if (bytes) return head_dim <= 64 ? 6 : 4;  // half the LDS: its registers
   return head_dim <= 32 ? 6 : head_dim <= 64 ? 4 : 2;
 }
 
@@ -288,7 +289,7 @@ struct SeqPlan {
 
 // max_length < 0: packed sequences (no keys but their own).
 static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int head_dim, int64_t held, int max_length,
-                        bool single) {
+                        bool single, bool bytes = false) {
   SeqPlan p{};
   const int64_t G = heads / kv_heads;
   const int cus = device_cus();
@@ -299,7 +300,7 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   const bool wide = !paged || (single ? G > 32 : tokens * G > 32 * (int64_t)batch);
   p.rows = wide ? 128 : 32;
   const int64_t tiles = single ? tokens * ((G + p.rows - 1) / p.rows) : tokens * G / p.rows + batch;
-  const int64_t blocks = tiles * kv_heads, held_blocks = (int64_t)seq_resident(wide, head_dim) * cus;
+  const int64_t blocks = tiles * kv_heads, held_blocks = (int64_t)seq_resident(wide, head_dim, bytes) * cus;
   // Up to a block per CU the waves of a block are as many as its LDS feeds, else two: 16 sequences of 4 tokens, 1000 keys
   // on 4 heads of 64, 17.4 with two waves and 12.3 with eight; 16 drafts of 1 to 7 tokens, to 2100 keys, 28.3 and 14.8.
   p.shape = wide ? SeqShape::kWide : blocks <= cus ? SeqShape::kDeep : SeqShape::kNarrow;
@@ -338,45 +339,7 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   return p;
 }
 
-static int check_heads(const char* what, int tokens, int batch, int heads, int kv_heads, int head_dim, int dtype) {
-  TT_REQUIRE(tokens >= 0 && batch >= 0, "%s: bad shape (tokens %d, batch %d)", what, tokens, batch);
-  TT_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: heads %d are no multiple of kv_heads %d", what,
-             heads, kv_heads);
-  TT_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "%s: head_dim %d is no multiple of 8 up to 256",
-             what, head_dim);
-  TT_REQUIRE((int64_t)tokens * heads < (1LL << 31), "%s: %d rows of %d heads", what, tokens, heads);
-  TT_REQUIRE(dtype == TT_FP16 || dtype == TT_BF16, "%s: bad dtype %d", what, dtype);
-  return TT_OK;
-}
-
-// Rows and heads are read 16 bytes at a time, and 16 rows at an offset of 32 bits.
-static int check_rows(const char* what, const void* p, int64_t row, int64_t head) {
-  TT_REQUIRE(((uintptr_t)p & 15) == 0 && row % 8 == 0 && head % 8 == 0, "%s: not aligned to 16 bytes", what);
-  TT_REQUIRE(row >= 0 && head >= 0 && row < (1LL << 26), "%s: row stride of %lld elements", what, (long long)row);
-  return TT_OK;
-}
-
-static int check_pages(const char* what, int pages, int page_size, int table_pages) {
-  TT_REQUIRE(pages > 0 && table_pages > 0, "%s: no pages (%d in the cache, %d per sequence)", what, pages, table_pages);
-  TT_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "%s: page_size %d is no power of two from 16 on",
-             what, page_size);
-  TT_REQUIRE((int64_t)page_size * table_pages <= (1LL << 30), "%s: %d pages of %d per sequence", what, table_pages,
-             page_size);
-  return TT_OK;
-}
-
 }  // namespace tt
-
-#define TT_CHECK(call)            \
-  do {                            \
-    const int rc_ = (call);       \
-    if (rc_ != TT_OK) return rc_; \
-  } while (0)
-
-// The structure is the caller's: its size first.
-#define TT_ARGS(type, what)                                                                             \
-  TT_REQUIRE(args != nullptr && args->size == (int64_t)sizeof(type), what ": not a " #type " structure"); \
-  const type& c = *args
 
 extern "C" int tt_packed_attention_fwd(const tt_packed_attention* args, void* stream) {
   using namespace tt;
@@ -399,44 +362,45 @@ extern "C" int tt_packed_attention_fwd(const tt_packed_attention* args, void* st
   return launch_seq_attention(a, false, SeqShape::kWide, c.dtype, (hipStream_t)stream);
 }
 
-extern "C" int tt_cache_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int head_dim,
-                                                  int page_size, int table_pages, int max_length, int single,
-                                                  int64_t* bytes) {
-  using namespace tt;
-  TT_CHECK(check_heads("cache_attention", tokens, batch, heads, kv_heads, head_dim, TT_FP16));
-  TT_CHECK(check_pages("cache_attention", 1, page_size, table_pages));
-  TT_REQUIRE(max_length >= 0 && bytes != nullptr, "cache_attention: max_length %d", max_length);
+namespace tt {
+
+static int workspace_bytes(const char* what, bool bytes_cache, int tokens, int batch, int heads, int kv_heads, int head_dim,
+                           int page_size, int table_pages, int max_length, int single, int64_t* bytes) {
+  TT_CHECK(check_heads(what, tokens, batch, heads, kv_heads, head_dim, TT_FP16));
+  if (bytes_cache) TT_CHECK(check_head8(what, head_dim));
+  TT_CHECK(check_pages(what, 1, page_size, table_pages));
+  TT_REQUIRE(max_length >= 0 && bytes != nullptr, "%s: max_length %d", what, max_length);
   *bytes = 0;
   if (tokens == 0 || batch == 0) return TT_OK;
   *bytes = 4 * (head_dim + 2) * seq_plan(tokens, batch, heads, kv_heads, head_dim, (int64_t)page_size * table_pages,
-                                         max_length, single != 0).part_rows;
+                                         max_length, single != 0, bytes_cache).part_rows;
   return TT_OK;
 }
 
-extern "C" int tt_cache_attention_fwd(const tt_cache_attention* args, void* stream) {
-  using namespace tt;
-  TT_ARGS(tt_cache_attention, "cache_attention");
-  TT_CHECK(check_heads("cache_attention", c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, c.dtype));
-  TT_CHECK(check_pages("cache_attention", c.pages, c.page_size, c.table_pages));
-  TT_REQUIRE(c.scale > 0.f && c.scale < 2e38f, "cache_attention: scale %g is not positive and finite", c.scale);
-  TT_REQUIRE(c.max_length >= 0, "cache_attention: max_length %d", c.max_length);
+// What both forms of the cache have in common: the checks of a call, and its launches.
+template <class C>
+static int check_cache_attention(const char* what, const C& c) {
+  TT_CHECK(check_heads(what, c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, c.dtype));
+  TT_CHECK(check_pages(what, c.pages, c.page_size, c.table_pages));
+  TT_REQUIRE(c.scale > 0.f && c.scale < 2e38f, "%s: scale %g is not positive and finite", what, c.scale);
+  TT_REQUIRE(c.max_length >= 0, "%s: max_length %d", what, c.max_length);
   if (c.tokens == 0 || c.batch == 0) return TT_OK;
-  TT_REQUIRE(c.q && c.k_cache && c.v_cache && c.table && c.lengths && c.out, "cache_attention: null pointer");
-  TT_REQUIRE(c.starts != nullptr || c.tokens == c.batch, "cache_attention: %d tokens for %d sequences without starts",
-             c.tokens, c.batch);
+  TT_REQUIRE(c.q && c.k_cache && c.v_cache && c.table && c.lengths && c.out, "%s: null pointer", what);
+  TT_REQUIRE(c.starts != nullptr || c.tokens == c.batch, "%s: %d tokens for %d sequences without starts", what, c.tokens,
+             c.batch);
   TT_CHECK(check_rows("cache_attention: q", c.q, c.q_row, c.q_head));
-  TT_CHECK(check_rows("cache_attention: k_cache", c.k_cache, c.k_row, c.k_head));
-  TT_CHECK(check_rows("cache_attention: v_cache", c.v_cache, c.v_row, c.v_head));
-  TT_REQUIRE(c.k_page % 8 == 0 && c.v_page % 8 == 0 && c.k_page >= 0 && c.v_page >= 0 && c.table_row >= 0,
-             "cache_attention: page strides %lld, %lld", (long long)c.k_page, (long long)c.v_page);
-  TT_CHECK(check_rows("cache_attention: out", c.out, 0, 0));
-  const SeqPlan p = seq_plan(c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, (int64_t)c.page_size * c.table_pages, c.max_length,
-                             c.starts == nullptr);
+  TT_REQUIRE(c.k_page >= 0 && c.v_page >= 0 && c.table_row >= 0, "%s: page strides %lld, %lld", what, (long long)c.k_page,
+             (long long)c.v_page);
+  return check_rows("cache_attention: out", c.out, 0, 0);
+}
+
+template <class C>
+static int run_cache_attention(const char* what, const C& c, SeqAttnArgs& a, bool bytes_cache, hipStream_t stream) {
+  const SeqPlan p = seq_plan(c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, (int64_t)c.page_size * c.table_pages,
+                             c.max_length, c.starts == nullptr, bytes_cache);
   const int64_t bytes = 4 * (c.head_dim + 2) * p.part_rows;
   TT_REQUIRE(bytes == 0 || (c.workspace != nullptr && c.workspace_bytes >= bytes && ((uintptr_t)c.workspace & 15) == 0),
-             "cache_attention: a workspace of %lld bytes is needed, %lld given", (long long)bytes,
-             (long long)c.workspace_bytes);
-  SeqAttnArgs a{};
+             "%s: a workspace of %lld bytes is needed, %lld given", what, (long long)bytes, (long long)c.workspace_bytes);
   a.q = c.q, a.k = c.k_cache, a.v = c.v_cache, a.out = c.out, a.starts = c.starts, a.lengths = c.lengths, a.table = c.table;
   a.q_row = c.q_row, a.q_head = c.q_head, a.k_row = c.k_row, a.k_head = c.k_head, a.v_row = c.v_row, a.v_head = c.v_head;
   a.k_page = c.k_page, a.v_page = c.v_page, a.table_row = c.table_row;
@@ -446,13 +410,61 @@ extern "C" int tt_cache_attention_fwd(const tt_cache_attention* args, void* stre
   a.slots = p.slots, a.mode = p.mode;
   a.part_o = static_cast<float*>(c.workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + p.part_rows * c.head_dim);
-  TT_CHECK(launch_seq_attention(a, true, p.shape, c.dtype, (hipStream_t)stream));
+  TT_CHECK(bytes_cache ? launch_seq8_attention(a, p.shape, c.dtype, stream)
+                       : launch_seq_attention(a, true, p.shape, c.dtype, stream));
   if (p.mode != kSeqShares) return TT_OK;
   if (p.shape == SeqShape::kWide)
-    return c.dtype == TT_FP16 ? launch_seq_merge_wide<half>(a, p.tiles, p.many_parts, (hipStream_t)stream)
-                              : launch_seq_merge_wide<bf16>(a, p.tiles, p.many_parts, (hipStream_t)stream);
-  return c.dtype == TT_FP16 ? launch_seq_merge<half>(a, p.rows, p.many_parts, (hipStream_t)stream)
-                          : launch_seq_merge<bf16>(a, p.rows, p.many_parts, (hipStream_t)stream);
+    return c.dtype == TT_FP16 ? launch_seq_merge_wide<half>(a, p.tiles, p.many_parts, stream)
+                              : launch_seq_merge_wide<bf16>(a, p.tiles, p.many_parts, stream);
+  return c.dtype == TT_FP16 ? launch_seq_merge<half>(a, p.rows, p.many_parts, stream)
+                          : launch_seq_merge<bf16>(a, p.rows, p.many_parts, stream);
+}
+
+}  // namespace tt
+
+extern "C" int tt_cache_attention_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int head_dim,
+                                                  int page_size, int table_pages, int max_length, int single,
+                                                  int64_t* bytes) {
+  return tt::workspace_bytes("cache_attention", false, tokens, batch, heads, kv_heads, head_dim, page_size, table_pages,
+                             max_length, single, bytes);
+}
+
+extern "C" int tt_cache_attention8_workspace_bytes(int tokens, int batch, int heads, int kv_heads, int head_dim,
+                                                   int page_size, int table_pages, int max_length, int single,
+                                                   int64_t* bytes) {
+  return tt::workspace_bytes("cache_attention", true, tokens, batch, heads, kv_heads, head_dim, page_size, table_pages,
+                             max_length, single, bytes);
+}
+
+extern "C" int tt_cache_attention_fwd(const tt_cache_attention* args, void* stream) {
+  using namespace tt;
+  TT_ARGS(tt_cache_attention, "cache_attention");
+  TT_CHECK(check_cache_attention("cache_attention", c));
+  if (c.tokens == 0 || c.batch == 0) return TT_OK;
+  TT_CHECK(check_rows("cache_attention: k_cache", c.k_cache, c.k_row, c.k_head));
+  TT_CHECK(check_rows("cache_attention: v_cache", c.v_cache, c.v_row, c.v_head));
+  TT_REQUIRE(c.k_page % 8 == 0 && c.v_page % 8 == 0, "cache_attention: page strides %lld, %lld", (long long)c.k_page,
+             (long long)c.v_page);
+  SeqAttnArgs a{};
+  return run_cache_attention("cache_attention", c, a, false, (hipStream_t)stream);
+}
+
+extern "C" int tt_cache_attention8_fwd(const tt_cache_attention8* args, void* stream) {
+  using namespace tt;
+  TT_ARGS(tt_cache_attention8, "cache_attention");
+  TT_CHECK(check_cache_attention("cache_attention", c));
+  TT_CHECK(check_head8("cache_attention", c.head_dim));
+  TT_CHECK(check_block("cache_attention", c.block, c.page_size));
+  if (c.tokens == 0 || c.batch == 0) return TT_OK;
+  TT_CHECK(check_rows8("cache_attention: k_cache", c.k_cache, c.k_page, c.k_row, c.k_head));
+  TT_CHECK(check_rows8("cache_attention: v_cache", c.v_cache, c.v_page, c.v_row, c.v_head));
+  TT_CHECK(check_scales("cache_attention: k_scales", c.k_scales, c.ks_page, c.ks_block, c.ks_head));
+  TT_CHECK(check_scales("cache_attention: v_scales", c.v_scales, c.vs_page, c.vs_block, c.vs_head));
+  SeqAttnArgs a{};
+  a.k_scale = c.k_scales, a.v_scale = c.v_scales, a.block_shift = __builtin_ctz(c.block);
+  a.ks_page = c.ks_page, a.ks_block = c.ks_block, a.ks_head = c.ks_head;
+  a.vs_page = c.vs_page, a.vs_block = c.vs_block, a.vs_head = c.vs_head;
+  return run_cache_attention("cache_attention", c, a, true, (hipStream_t)stream);
 }
 
 extern "C" int tt_cache_append(const tt_cache_rows* args, void* stream) {

@@ -64,6 +64,11 @@ struct Num<half> {
   static __device__ __forceinline__ float add2(v2 p, float c) {
     return __builtin_amdgcn_fdot2(p, v2{(half)1.f, (half)1.f}, c, false);
   }
+  static constexpr int kTop = 127 + 7;  // above this scale (as e8m0) the largest of e4m3, 448, lies past the type's
+  template <bool HI>
+  static __device__ __forceinline__ uint32_t widen(uint32_t x, float scale) {  // bytes 0, 1 (2, 3) of e4m3
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, HI));
+  }
 };
 template <>
 struct Num<bf16> {
@@ -77,13 +82,41 @@ struct Num<bf16> {
   static __device__ __forceinline__ float add2(v2 p, float c) {
     return __builtin_amdgcn_fdot2_f32_bf16(p, v2{(bf16)1.f, (bf16)1.f}, c, false);
   }
+  static constexpr int kTop = 127 + 119;
+  template <bool HI>
+  static __device__ __forceinline__ uint32_t widen(uint32_t x, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, HI));
+  }
 };
+
+// Eight values of an 8-bit cache in T: e4m3 times a power of two, the bits of an e8m0 as an exponent (exact wherever T
+// holds the product; past T's largest they are infinities).
+template <typename T>
+__device__ __forceinline__ u32x4 widen8(u32x2 x, float scale) {
+  return u32x4{Num<T>::template widen<false>(x[0], scale), Num<T>::template widen<true>(x[0], scale),
+               Num<T>::template widen<false>(x[1], scale), Num<T>::template widen<true>(x[1], scale)};
+}
+__device__ __forceinline__ float e8m0(uint32_t e) { return __builtin_bit_cast(float, e << 23); }
+
+// The smallest magnitude of e4m3 (7 bits) that is no number or, times 2^(e - 127), past T's largest.
+template <typename T>
+__device__ __forceinline__ uint32_t widen_limit(int e) {
+  const int over = e - Num<T>::kTop - 1;  // 2^(8 - over) and above lie past it
+  if (over < 0) return 0x7f;
+  return over <= 14 ? 0x78 - 8 * over : 1 << max(17 - over, 0);  // (below 2^-6 e4m3 counts in steps of 2^-9)
+}
 
 // ds_read_b64_tr_b16 (16 lanes transpose their 4 rows of 16).  The __restrict gives the read alias information;
 // without any, the compiler lets it wait for every global -> LDS copy in flight.
 using lds_short = __attribute__((address_space(3))) short;
 __device__ __forceinline__ shortx4 read_tr16(const lds_short* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4*)p);
+}
+
+// ds_read_b64_tr_b8: 16 lanes transpose their 8 rows of 16 bytes.
+__device__ __forceinline__ u32x2 read_tr8(const lds_short* __restrict__ p) {
+  typedef int intx2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) intx2*)p));
 }
 
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
@@ -111,6 +144,10 @@ struct SeqAttnArgs {
   int mode;                // kSeqInOrder, kSeqHeaviest or kSeqShares
   float* part_o;           // kSeqShares: [2 slots][kv_heads][R * head_dim], the rows of tiles that lie in several shares
   float2* part_ml;         // ... [2 slots][kv_heads][R], their maximum (log2 domain) and sum
+  // 8-bit cache: the exponents (e8m0) of k and v, one per 2^block_shift tokens of a page and head; strides in bytes.
+  const uint8_t *k_scale, *v_scale;
+  int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head;
+  int block_shift;
 };
 
 // Where feature d of row r of a tile lies in a part of 128 rows: as the lanes hold them, 32 rows x 8 features in turn, so
@@ -145,6 +182,21 @@ __device__ __forceinline__ int vseg(int row, int c) {
   if constexpr (HD >= 128) return c ^ ((row & 3) << 2);
   else if constexpr (HD == 64) return c ^ ((row & 2) << 1);
   else return c;
+}
+
+// The same for tiles of an 8-bit cache, whose LDS rows are HD bytes in chunks of 16.  K: 16 lanes read one chunk of 16
+// rows.  V: 16 lanes read one chunk of rows 4 h ... 4 h + 3 and 8 further, and 16 others the next chunk.
+template <int HD>
+__device__ __forceinline__ int kswz8(int row, int c) {
+  if constexpr (HD == 256) return c ^ (row & 15);
+  else if constexpr (HD == 128) return c ^ ((row >> 1) & 7);
+  else return c ^ ((row >> 2) & 3);
+}
+template <int HD>
+__device__ __forceinline__ int vseg8(int row, int c) {
+  if constexpr (HD == 256) return c ^ ((row & 3) << 1 | (row & 8));
+  else if constexpr (HD == 128) return c ^ ((row & 2) | ((row & 8) >> 1));
+  else return c ^ ((row & 8) >> 2);
 }
 
 // The sequence that owns row tile `slot`.  Sequence b's tiles start at slot floor(starts[b] G / R) + b, which
@@ -341,7 +393,8 @@ __device__ __forceinline__ SeqShare seq_share(const SeqAttnArgs& a, int slot, in
   }
 }
 
-template <typename T, int HD, int RW, int KW, int KT, bool PAGED, int WPE = (HD <= 64 ? 3 : HD <= 128 ? 2 : 1)>
+template <typename T, int HD, int RW, int KW, int KT, bool PAGED, bool C8 = false,
+          int WPE = (HD <= 64 ? 3 : HD <= 128 ? 2 : 1)>
 __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void seq_attention_kernel(SeqAttnArgs a) {
   using v2 = typename Num<T>::v2;
   using v8 = typename Num<T>::v8;
@@ -349,13 +402,21 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   constexpr bool PIPE = RW > 1;              // softmax beside the next keys' products
   constexpr int KSTEPS = HD / 16;           // k-steps of S^T
   constexpr int DB = HD / 32;               // 32-row blocks of O^T
-  constexpr int CH = HD / 8;                // 16-byte chunks of a row
-  constexpr int RPC = 64 / CH;              // rows per 1 KiB copy
+  constexpr int CH = HD / 8;                // 16-byte chunks of a row of T
+  constexpr int RPC = 64 / CH;              // rows of T in 1 KiB
+  // An 8-bit cache's tiles: wide blocks widen them to T on their way into LDS, each row once for all waves; narrow ones
+  // copy their bytes, and a wave widens the fragments that it reads.
+  constexpr bool RAW = C8 && !PIPE;
+  using E = std::conditional_t<RAW, uint8_t, T>;
+  constexpr int EB = C8 ? 1 : 2;            // bytes of a value in memory
+  constexpr int CB = HD * EB / 16;          // 16-byte chunks of a row in memory
+  constexpr int RPB = 64 / CB;              // rows per 1 KiB copy
   constexpr int WROWS = KT / RW;            // rows of a tile that one wave copies
   constexpr int PG = WROWS / 16;            // ... in groups of 16, each of which lies in one page
-  constexpr int CPG = 16 / RPC;             // copies per group
+  constexpr int CPG = 16 / RPB;             // copies per group
   constexpr int TILE = KT * HD;
-  static_assert(WROWS % 16 == 0 && RPC <= 16, "a wave copies whole 16-row groups");
+  static_assert(WROWS % 16 == 0 && RPB <= 16, "a wave copies whole 16-row groups");
+  static_assert(!C8 || (PAGED && HD >= 64), "8 bits: a cache");
 
   extern __shared__ __align__(512) char seq_lds[];
 
@@ -367,8 +428,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = RW == 1 ? 0 : wave % RW, grp = RW == 1 ? wave : wave / RW;
   int hf = lane >> 5, col = lane & 31;
-  T* const sk = reinterpret_cast<T*>(seq_lds) + (size_t)grp * 2 * TILE;
-  T* const sv = reinterpret_cast<T*>(seq_lds) + (size_t)KW * 2 * TILE + (size_t)grp * 2 * TILE;
+  E* const sk = reinterpret_cast<E*>(seq_lds) + (size_t)grp * 2 * TILE;
+  E* const sv = reinterpret_cast<E*>(seq_lds) + (size_t)KW * 2 * TILE + (size_t)grp * 2 * TILE;
 
   // What this block does: a row tile with all its keys, or (kSeqShares) units x ... share_end - 1, tile after tile.
   SeqTile sq;
@@ -389,45 +450,55 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     if (sq.tile < 0 || sq.tile * R >= sq.count * G) return;
   }
 
-  // Copy sources: lane l of copy c of a group fetches row c RPC + l / CH of the group into the next 16 bytes of
+  // Copy sources: lane l of copy c of a group fetches row c RPB + l / CB of the group into the next 16 bytes of
   // LDS, from the chunk that belongs there.  Chunks at or past head_dim lie outside the buffer: LDS keeps the zeros
   // that it is cleared to (or receives those that such a load returns).
   const int hd = a.head_dim;
   uint32_t koff[CPG], voff[CPG];
 #pragma unroll
   for (int c = 0; c < CPG; ++c) {
-    const int row = c * RPC + lane / CH;
-    const int kc = kswz<HD>(row, lane % CH) * 8, vc = vseg<HD>(row, lane % CH) * 8;
-    koff[c] = kc < hd ? (uint32_t)(row * (int)a.k_row + kc) * 2 : 0x80000000u;
-    voff[c] = vc < hd ? (uint32_t)(row * (int)a.v_row + vc) * 2 : 0x80000000u;
+    const int row = c * RPB + lane / CB;
+    int kc = lane % CB, vc = lane % CB;
+    if constexpr (RAW) kc = kswz8<HD>(row, kc) * 16, vc = vseg8<HD>(row, vc) * 16;
+    else if constexpr (C8) kc *= 16, vc *= 16;
+    else kc = kswz<HD>(row, kc) * 8, vc = vseg<HD>(row, vc) * 8;
+    koff[c] = kc < hd ? (uint32_t)(row * (int)a.k_row + kc) * EB : 0x80000000u;
+    voff[c] = vc < hd ? (uint32_t)(row * (int)a.v_row + vc) * EB : 0x80000000u;
   }
-  const T* const kh = static_cast<const T*>(a.k) + hkv * a.k_head;
-  const T* const vh = static_cast<const T*>(a.v) + hkv * a.v_head;
+  using Mem = std::conditional_t<C8, uint8_t, T>;
+  const Mem* const kh = static_cast<const Mem*>(a.k) + hkv * a.k_head;
+  const Mem* const vh = static_cast<const Mem*>(a.v) + hkv * a.v_head;
 
   const float c2 = a.scale_log2, lazy = kSeqLazy / a.scale_log2;
   // LDS addresses of this lane's pieces of the first K and V block of a stage; the others lie at constant distances.
   // (The empty asm keeps each in one register: the compiler would spread the sums over many.)  Rows of 512 bytes
   // leave no registers for them: there the pieces of a row are told apart by an XOR of the first one's address.
   constexpr bool FAR = PIPE && HD > 128;
-  constexpr int KA = FAR ? 1 : KSTEPS, VA = FAR ? 1 : DB;
+  constexpr int KA = FAR ? 1 : RAW ? KSTEPS / 2 : KSTEPS, VA = FAR ? 1 : DB;
   uint32_t kread[KA], vread[VA];
 #pragma unroll
   for (int kk = 0; kk < KA; ++kk) {
-    kread[kk] = lds_address(sk + col * HD + kswz<HD>(col, 2 * kk + hf) * 8);
+    if constexpr (RAW) kread[kk] = lds_address(sk + col * HD + kswz8<HD>(col, 2 * kk + hf) * 16);
+    else kread[kk] = lds_address(sk + col * HD + kswz<HD>(col, 2 * kk + hf) * 8);
     asm volatile("" : "+v"(kread[kk]));
   }
-  const int vrow = 4 * hf + ((lane >> 2) & 3);
+  // (RAW: 16 lanes read 8 rows, 4 hf ... 4 hf + 3 and 8 further, in the order of the lane's probabilities)
+  const int vrow = RAW ? 4 * hf + ((lane >> 1) & 3) + (lane & 8) : 4 * hf + ((lane >> 2) & 3);
 #pragma unroll
   for (int i = 0; i < VA; ++i) {
-    const int c = vseg<HD>(vrow, 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1));
-    vread[i] = lds_address(sv + vrow * HD + c * 8 + 4 * (lane & 1));
+    if constexpr (RAW) {
+      vread[i] = lds_address(sv + vrow * HD + vseg8<HD>(vrow, 2 * i + ((lane >> 4) & 1)) * 16 + 8 * (lane & 1));
+    } else {
+      const int c = vseg<HD>(vrow, 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1));
+      vread[i] = lds_address(sv + vrow * HD + c * 8 + 4 * (lane & 1));
+    }
     asm volatile("" : "+v"(vread[i]));
   }
   for (;;) {
   // (What follows from these is worked out again for each tile instead of being held in registers throughout.)
   asm volatile("" : "+v"(lane), "+v"(hf), "+v"(col));
   if (hd < HD) {  // the tile before left its sums or rows there
-    for (int e = tid; e < 4 * KW * TILE / 8; e += 64 * RW * KW)
+    for (int e = tid; e < 4 * KW * TILE * (int)sizeof(E) / 16; e += 64 * RW * KW)
       reinterpret_cast<u32x4*>(seq_lds)[e] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
@@ -477,6 +548,22 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   auto bad_groups = [&](int pe, int t0) TT_INLINE -> uint32_t {
     return (uint32_t)__ballot((uint32_t)pe >= (uint32_t)a.pages && t0 + 16 * lane < keys) & 0xffu;
   };
+  // 8 bits: the scales of those groups, K's in the low byte and V's above it (blocks of tokens hold whole groups).  A
+  // group one of whose scales is none (255) counts as one outside the cache; its V is multiplied by 2^-127.
+  auto tile_scales = [&](int pe, int t0) TT_INLINE -> int {
+    const uint32_t in = min(t0 + 16 * (lane & 7), max(keys - 1, 0)) & ((1 << a.page_shift) - 1);
+    const uint32_t page = (uint32_t)pe < (uint32_t)a.pages ? pe : 0, block = in >> a.block_shift;
+    const int k = a.k_scale[page * (uint64_t)a.ks_page + block * (uint64_t)a.ks_block + hkv * a.ks_head];
+    const int v = a.v_scale[page * (uint64_t)a.vs_page + block * (uint64_t)a.vs_block + hkv * a.vs_head];
+    return v << 8 | k;
+  };
+  auto bad_scales = [&](int se, int t0) TT_INLINE -> uint32_t {
+    return (uint32_t)__ballot(((se & 255) == 255 || se >> 8 == 255) && t0 + 16 * lane < keys) & 0xffu;
+  };
+  auto scale_of = [&](int se, int group, bool is_k) TT_INLINE -> float {
+    const uint32_t e = (__builtin_amdgcn_readlane(se, group) >> (is_k ? 0 : 8)) & 255;
+    return e8m0(e == 255 ? 0 : e);
+  };
   // Where those groups lie in K and V (bytes), and how many bytes there belong to keys; worked out by the lanes for
   // pages, whose numbers they hold, and by the scalar unit otherwise.
   struct Places {
@@ -489,23 +576,25 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     if constexpr (PAGED) {
       if ((uint32_t)pe >= (uint32_t)a.pages) n = pe = 0;
       const uint32_t page = pe, in = t & ((1 << a.page_shift) - 1);
-      p.k = 2 * (page * (uint64_t)a.k_page + in * (uint64_t)a.k_row);
-      p.v = 2 * (page * (uint64_t)a.v_page + in * (uint64_t)a.v_row);
+      p.k = EB * (page * (uint64_t)a.k_page + in * (uint64_t)a.k_row);
+      p.v = EB * (page * (uint64_t)a.v_page + in * (uint64_t)a.v_row);
     } else {
       const uint32_t row = sq.first + min(t, keys - 1);
       p.k = 2 * (row * (uint64_t)a.k_row);
       p.v = 2 * (row * (uint64_t)a.v_row);
     }
-    p.k_bytes = n == 0 ? 0 : 2 * ((n - 1) * (uint32_t)a.k_row + hd);
-    p.v_bytes = n == 0 ? 0 : 2 * ((n - 1) * (uint32_t)a.v_row + hd);
+    p.k_bytes = n == 0 ? 0 : EB * ((n - 1) * (uint32_t)a.k_row + hd);
+    p.v_bytes = n == 0 ? 0 : EB * ((n - 1) * (uint32_t)a.v_row + hd);
     return p;
   };
   auto places = [&](int pe, int t0) TT_INLINE -> Places {
     if constexpr (PAGED) return place(t0 + 16 * (lane & 7), pe);
     else return Places{(uint64_t)t0, 0, 0, 0};
   };
-  // Copies of this wave's rows of a K (V) tile whose first 16 keys are group `group` of `at`.
-  auto issue_half = [&](bool is_k, const Places& at, T* tile, int group) TT_INLINE {
+  // Copies of this wave's rows of a K (V) tile whose first 16 keys are group `group` of `at` (wide blocks, 8 bits: into
+  // registers, from where write_half takes them into LDS).
+  using Staged = u32x4[C8 && PIPE ? CPG : 1];
+  auto issue_half = [&](bool is_k, const Places& at, E* tile, int group, Staged& staged) TT_INLINE {
 #pragma unroll
     for (int p = 0; p < PG; ++p) {
       const int g = rw * PG + p;
@@ -523,18 +612,40 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         bytes = is_k ? q.k_bytes : q.v_bytes;
       }
       const __amdgpu_buffer_rsrc_t r = buffer_rsrc(reinterpret_cast<const char*>(is_k ? kh : vh) + where, bytes);
+      if constexpr (C8 && PIPE) {
 #pragma unroll
-      for (int c = 0; c < CPG; ++c)
-        lds_copy16_buf(r, is_k ? koff[c] : voff[c], reinterpret_cast<half*>(tile + (g * 16 + c * RPC) * HD));
+        for (int c = 0; c < CPG; ++c) staged[c] = load16<kLoadDefault>(r, is_k ? koff[c] : voff[c]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < CPG; ++c)
+          lds_copy16_buf(r, is_k ? koff[c] : voff[c], reinterpret_cast<half*>(tile + (g * 16 + c * RPB) * HD));
+      }
     }
   };
+  auto write_half = [&](bool is_k, int se, E* tile, int group, const Staged& staged) TT_INLINE {
+    if constexpr (C8 && PIPE) {
+      static_assert(PG == 1, "a group per wave");
+      if (group + rw < 0) return;
+      const float scale = scale_of(se, group + rw, is_k);
+#pragma unroll
+      for (int c = 0; c < CPG; ++c) {
+        const int row = rw * 16 + c * RPB + lane / CB, chunk = 2 * (lane % CB);
+        T* const to = tile + row * HD;
+        const int at = is_k ? kswz<HD>(row, chunk) : vseg<HD>(row, chunk);  // the next chunk lies beside it
+        const u32x4 x = staged[c];
+        *reinterpret_cast<u32x4*>(to + at * 8) = widen8<T>(u32x2{x[0], x[1]}, scale);
+        *reinterpret_cast<u32x4*>(to + (at ^ 1) * 8) = widen8<T>(u32x2{x[2], x[3]}, scale);
+      }
+    }
+  };
+  Staged k_staged, v_staged;
   // The K tile staged with a V tile begins KLEAD keys later: the scores run that far ahead.
   constexpr int KLEAD = PIPE ? 32 : 0;
   auto issue_k = [&](const Places& p, int st) TT_INLINE {
-    issue_half(true, p, sk + st * TILE, KLEAD / 16);
+    issue_half(true, p, sk + st * TILE, KLEAD / 16, k_staged);
   };
   auto issue_v = [&](const Places& p, int st) TT_INLINE {
-    issue_half(false, p, sv + st * TILE, 0);
+    issue_half(false, p, sv + st * TILE, 0, v_staged);
   };
   // After the copies of this wave's V rows have landed: rows of keys behind the last that any row of the block sees are
   // cleared (0 times whatever lay there would not be 0), and where some rows of the block see keys that others do not,
@@ -546,19 +657,31 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     constexpr uint32_t kCarry = (0x8000u - Num<T>::kExp) * 0x10001u;  // an exponent of ones carries into the sign
     return (((x & 0x7fff7fffu) + kCarry) >> 15) & 0x10001u;
   };
-  auto settle_v = [&](int t0, int st) TT_INLINE {
+  constexpr int CL = HD * (int)sizeof(E) / 16;  // chunks of a row in LDS
+  auto settle_v = [&](int t0, int st, int se) TT_INLINE {
     const int g0 = rw * WROWS;
     u32x4* const tile = reinterpret_cast<u32x4*>(sv + st * TILE + g0 * HD);
     const int n = min(max(kend - (t0 + g0), 0), WROWS);
     if (mixed && t0 + KT > block_lo) {
-      for (int e = lane; e < n * CH; e += 64) {
+      for (int e = lane; e < n * CL; e += 64) {
         u32x4 x = tile[e];
         uint32_t any = 0;
+        uint32_t carry = 0;  // RAW: takes a byte that is no number, or too large, to 128 and above
+        if constexpr (RAW) {
+          const int v0 = __builtin_amdgcn_readlane(se, 0) >> 8, v1 = __builtin_amdgcn_readlane(se, 1) >> 8;
+          carry = (0x80 - widen_limit<T>(e / CL < 16 ? v0 : v1)) * 0x01010101u;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t m = odd_pair(x[i]);
-          any |= m;
-          x[i] &= ~(m * 0xffffu);
+          if constexpr (RAW) {
+            const uint32_t m = (((x[i] & 0x7f7f7f7fu) + carry) >> 7) & 0x01010101u;
+            any |= m;
+            x[i] &= ~(m * 0xffu);
+          } else {
+            const uint32_t m = odd_pair(x[i]);
+            any |= m;
+            x[i] &= ~(m * 0xffffu);
+          }
         }
         if (any != 0) {
           tile[e] = x;
@@ -567,13 +690,19 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       }
     }
     if (n < WROWS)
-      for (int e = n * CH + lane; e < WROWS * CH; e += 64) tile[e] = u32x4{0u, 0u, 0u, 0u};
+      for (int e = n * CL + lane; e < WROWS * CL; e += 64) tile[e] = u32x4{0u, 0u, 0u, 0u};
     lds_done();
   };
-  auto land_v = [&](int t0, int st) TT_INLINE {
-    __builtin_amdgcn_s_waitcnt(0);
-    asm volatile("" ::: "memory");
-    settle_v(t0, st);
+  auto land_v = [&](int t0, int st, int se) TT_INLINE {
+    if constexpr (C8 && PIPE) {
+      write_half(true, se, sk + st * TILE, KLEAD / 16, k_staged);
+      write_half(false, se, sv + st * TILE, 0, v_staged);
+      lds_done();
+    } else {
+      __builtin_amdgcn_s_waitcnt(0);
+      asm volatile("" ::: "memory");
+    }
+    settle_v(t0, st, se);
     if constexpr (RW > 1) raw_barrier();
   };
 
@@ -588,7 +717,24 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     int width = hd;
     asm volatile("" : "+s"(width));  // (the comparisons would be kept in registers)
     const T* qp = static_cast<const T*>(a.q) + (int64_t)(sq.first + tok) * a.q_row + head * a.q_head;
-    if (!FAR && width == HD) {
+    if constexpr (RAW) {  // features 32 j + 16 hf + {0..7} and the next 8, as a lane reads those of its keys
+#pragma unroll
+      for (int j = 0; j < KSTEPS / 2; ++j) {
+        const u32x4 none = {0u, 0u, 0u, 0u};
+        u32x4 x = none, y = none;
+        if (32 * j + 16 < width) {
+          x = *reinterpret_cast<const u32x4*>(qp + 32 * j + 16 * hf);
+          y = *reinterpret_cast<const u32x4*>(qp + 32 * j + 16 * hf + 8);
+        } else if (32 * j < width) {
+          x = *reinterpret_cast<const u32x4*>(qp + 32 * j);
+          y = *reinterpret_cast<const u32x4*>(qp + 32 * j + 8);
+          x = hf == 0 ? x : none;
+          y = hf == 0 ? y : none;
+        }
+        qf[2 * j] = __builtin_bit_cast(v8, x);
+        qf[2 * j + 1] = __builtin_bit_cast(v8, y);
+      }
+    } else if (!FAR && width == HD) {
 #pragma unroll
       for (int kk = 0; kk < KSTEPS; ++kk) qf[kk] = *reinterpret_cast<const v8*>(qp + 16 * kk + 8 * hf);
     } else {
@@ -619,6 +765,13 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     const uint32_t at = (FAR ? (vread[0] + stage) ^ (64 * i) : vread[i] + stage) + key;
     const shortx4 x0 = read_tr16((const lds_short*)at), x1 = read_tr16((const lds_short*)(at + 16 * HD));
     return __builtin_bit_cast(v8, shortx8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]});
+  };
+  // RAW: features 32 j + 16 hf + {0..15} of key l % 32; and features 32 i + l % 32 of the keys as above.
+  auto read_kb = [&](int j, int st) TT_INLINE -> u32x4 {
+    return *(const __attribute__((address_space(3))) u32x4*)(kread[j] + st * TILE);
+  };
+  auto read_vb = [&](int i, int st, int kc) TT_INLINE -> u32x2 {
+    return read_tr8((const lds_short*)(vread[i] + st * TILE + kc * 16 * HD));
   };
   // FAR: one wave per SIMD, so nothing else runs while it waits for a fragment.  Fragments are read four products
   // before theirs (read just before, as registers are too few for the compiler to do otherwise by itself, prompts of
@@ -724,6 +877,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       static_assert(KW == 1 && KT == 64, "two steps of 32 keys per tile");
       const int steps = wave_active && lim_hi > kbeg ? (lim_hi - kbeg + 31) / 32 : 0;  // of this wave
       int pe = 0, pe_next = 0;  // pages from this tile's and the next tile's first key on
+      int se = 0;               // 8 bits: the scales there
+      Staged k_first;
       Scores sa, sb;
       float mt;
       if (ntiles > 0) {
@@ -732,16 +887,22 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           pe_next = tile_pages(kbeg + KT);
         }
         const Places at = places(pe, kbeg);
+        if constexpr (C8) se = tile_scales(pe, kbeg);
         // the first 32 keys go where the second half of a K tile before the first would lie
-        issue_half(true, at, sk + TILE, -2);
+        issue_half(true, at, sk + TILE, -2, k_first);
         issue_k(at, 0);
         issue_v(at, 0);
       }
       load_q();
-      land_v(kbeg, 0);
+      if (!C8 || ntiles > 0) {
+        write_half(true, se, sk + TILE, -2, k_first);
+        land_v(kbeg, 0, se);
+      }
       if (steps > 0) {
         scores(sa, 1, 1);
-        mask_scores(sa, kbeg, PAGED ? bad_groups(pe, kbeg) : 0);
+        uint32_t bad = PAGED ? bad_groups(pe, kbeg) : 0;
+        if constexpr (C8) bad |= bad_scales(se, kbeg);
+        mask_scores(sa, kbeg, bad);
         mt = row_max(sa);
         move_max(mt);
       }
@@ -787,11 +948,13 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       auto fetch = [&](int r, int st) TT_INLINE {
         const int t0 = kbeg + r * KT;
         if constexpr (PAGED) bad = bad_groups(pe, t0);
+        if constexpr (C8) bad |= bad_scales(se, t0);
         if (r + 1 >= ntiles) return;
         if constexpr (PAGED) {
           pe = pe_next;
           pe_next = tile_pages(t0 + 2 * KT);
           const Places at = places(pe, t0 + KT);
+          if constexpr (C8) se = tile_scales(pe, t0 + KT);
           issue_k(at, st ^ 1);
           issue_v(at, st ^ 1);
         } else {
@@ -799,12 +962,12 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           const int left = keys - (t0 + KT + rw * WROWS);
           const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(k_next, bytes_of(left - KLEAD, (int)a.k_row));
           const __amdgpu_buffer_rsrc_t vr = buffer_rsrc(v_next, bytes_of(left, (int)a.v_row));
-          T* const kt = sk + (st ^ 1) * TILE + rw * WROWS * HD;
-          T* const vt = sv + (st ^ 1) * TILE + rw * WROWS * HD;
+          E* const kt = sk + (st ^ 1) * TILE + rw * WROWS * HD;
+          E* const vt = sv + (st ^ 1) * TILE + rw * WROWS * HD;
 #pragma unroll
-          for (int c = 0; c < CPG; ++c) lds_copy16_buf(kr, koff[c], reinterpret_cast<half*>(kt + c * RPC * HD));
+          for (int c = 0; c < CPG; ++c) lds_copy16_buf(kr, koff[c], reinterpret_cast<half*>(kt + c * RPB * HD));
 #pragma unroll
-          for (int c = 0; c < CPG; ++c) lds_copy16_buf(vr, voff[c], reinterpret_cast<half*>(vt + c * RPC * HD));
+          for (int c = 0; c < CPG; ++c) lds_copy16_buf(vr, voff[c], reinterpret_cast<half*>(vt + c * RPB * HD));
           k_next += 2 * KT * a.k_row;
           v_next += 2 * KT * a.v_row;
         }
@@ -814,7 +977,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         fetch(r, st);
         step(t0, st, 0, bad, sa, sb);
         step(t0, st, 1, bad, sb, sa);
-        land_v(t0 + KT, st ^ 1);
+        land_v(t0 + KT, st ^ 1, se);
       };
       // Tiles both of whose steps have a next one, up to head_dim 128 two per pass so that their stages are constants
       // (beyond, the code would not fit the instruction cache); then this wave's last tile; then those that only
@@ -841,7 +1004,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           last_step(st, 0, sa);
         }
         for (++r; r < ntiles; ++r) {
-          land_v(kbeg + r * KT, r & 1);
+          land_v(kbeg + r * KT, r & 1, se);
           fetch(r, r & 1);
         }
       }
@@ -853,6 +1016,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       const int rounds = (ntiles - grp + KW - 1) / KW;
       const int t_first = kbeg + grp * KT;
       int pe0 = 0, pe1 = 0, pe2 = 0;  // pages of this tile, the next and the one after it
+      int se0 = 0, se1 = 0;           // 8 bits: the scales of this tile and the next
       if (rounds > 0) {
         if constexpr (PAGED) {
           pe0 = tile_pages(t_first);
@@ -860,6 +1024,10 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           pe2 = tile_pages(t_first + 2 * KW * KT);
         }
         const Places at = places(pe0, t_first);
+        if constexpr (C8) {
+          se0 = tile_scales(pe0, t_first);
+          se1 = tile_scales(pe1, t_first + KW * KT);
+        }
         issue_k(at, 0);
         issue_v(at, 0);
         if (rounds > 1) {
@@ -876,31 +1044,57 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         if (r + 1 < rounds) wait_vmcnt<COPIES>();
         else wait_vmcnt<0>();
         asm volatile("" ::: "memory");
-        settle_v(t0, st);
+        settle_v(t0, st, se0);
         // A wave has its SIMD to itself: all fragments are read before the first product, and only the first waits.
-        v8 kf[KSTEPS], vf[2][DB];
+        v8 kf[RAW ? 1 : KSTEPS], vf[RAW ? 1 : 2][RAW ? 1 : DB];
+        u32x4 kb[RAW ? KSTEPS / 2 : 1];  // 8 bits
+        u32x2 vb[RAW ? 2 : 1][RAW ? DB : 1];
+        if constexpr (RAW) {
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) kf[kk] = read_k(kk, st, 0);
+          for (int j = 0; j < KSTEPS / 2; ++j) kb[j] = read_kb(j, st);
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < DB; ++i) vf[c][i] = read_v(i, st, c);
+            for (int i = 0; i < DB; ++i) vb[c][i] = read_vb(i, st, c);
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < KSTEPS; ++kk) kf[kk] = read_k(kk, st, 0);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < DB; ++i) vf[c][i] = read_v(i, st, c);
+        }
         __builtin_amdgcn_sched_barrier(0);
         Scores s;
         Probs p16;
         float mt;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = 0.f;
+        float scale_v[2];
+        if constexpr (RAW) {
+          const float k0 = scale_of(se0, 0, true), k1 = scale_of(se0, 1, true), scale_k = col < 16 ? k0 : k1;
+          scale_v[0] = scale_of(se0, 0, false);
+          scale_v[1] = scale_of(se0, 1, false);
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; ++kk) s = Num<T>::mfma(kf[kk], qf[kk], s);
-        const uint32_t bad = PAGED ? bad_groups(pe0, t0) : 0;
+          for (int kk = 0; kk < KSTEPS; ++kk) {
+            const u32x2 x = {kb[kk / 2][2 * (kk & 1)], kb[kk / 2][2 * (kk & 1) + 1]};
+            s = Num<T>::mfma(__builtin_bit_cast(v8, widen8<T>(x, scale_k)), qf[kk], s);
+          }
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < KSTEPS; ++kk) s = Num<T>::mfma(kf[kk], qf[kk], s);
+        }
+        uint32_t bad = PAGED ? bad_groups(pe0, t0) : 0;
+        if constexpr (C8) bad |= bad_scales(se0, t0);
         const int pn = pe2;
         if constexpr (PAGED) {
           pe0 = pe1;
           pe1 = pe2;
           pe2 = tile_pages(t0 + 3 * KW * KT);
         }
+        se0 = se1;
         if (r + 2 < rounds) {
+          if constexpr (C8) se1 = tile_scales(pn, t0 + 2 * KW * KT);  // (before the copies: they are waited for first)
           lds_done();
           const Places at = places(pn, t0 + 2 * KW * KT);
           issue_k(at, st);
@@ -914,7 +1108,11 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < DB; ++i) o[i] = Num<T>::mfma(vf[c][i], p16[c], o[i]);
+          for (int i = 0; i < DB; ++i) {
+            if constexpr (RAW)
+              o[i] = Num<T>::mfma(__builtin_bit_cast(v8, widen8<T>(vb[c][i], scale_v[c])), p16[c], o[i]);
+            else o[i] = Num<T>::mfma(vf[c][i], p16[c], o[i]);
+          }
       }
     }
   }
@@ -1085,7 +1283,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           *dst = y;
         }
       };
-      const auto values = [&](int key) TT_INLINE -> const T* {  // nullptr: in no page
+      const auto values = [&](int key) TT_INLINE -> const Mem* {  // nullptr: in no page
         if constexpr (PAGED) {
           const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
           if ((uint32_t)page >= (uint32_t)a.pages) return nullptr;
@@ -1096,15 +1294,32 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       };
       if (any_lost && row < rows && l_row == l_row)
         for (int c = 0; 8 * c < hd; ++c) update(c, [](float y, int) TT_INLINE { return y != y ? 0.f : y; });
+      // 8 bits: the scale of a key's V (a key without one is NaN in all rows that see it, as its scores are)
+      const auto scale_at = [&](int key) TT_INLINE -> float {
+        const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
+        const int block = (key & ((1 << a.page_shift) - 1)) >> a.block_shift;
+        const uint32_t e = a.v_scale[page * a.vs_page + block * a.vs_block + hkv * a.vs_head];
+        return e8m0(e == 255 ? 0 : e);
+      };
       for (int k0 = any_lost ? kbeg : kbeg + max(block_lo - kbeg, 0) / KT * KT; k0 < lim_hi; k0 += RPC) {
-        const T* const vp = values(min(k0 + l / CH, lim_hi - 1));  // RPC keys, 16 bytes per lane
+        const int key = min(k0 + l / CH, lim_hi - 1);
+        const Mem* const vp = values(key);  // RPC keys, 8 values per lane
         u32x4 x = {0u, 0u, 0u, 0u};
-        if (vp != nullptr && l % CH * 8 < hd) x = *reinterpret_cast<const u32x4*>(vp + l % CH * 8);
+        if (vp != nullptr && l % CH * 8 < hd) {
+          if constexpr (C8) x = widen8<T>(*reinterpret_cast<const u32x2*>(vp + l % CH * 8), scale_at(key));
+          else x = *reinterpret_cast<const u32x4*>(vp + l % CH * 8);
+        }
         uint64_t found =
             __builtin_amdgcn_ballot_w64((odd_pair(x[0]) | odd_pair(x[1]) | odd_pair(x[2]) | odd_pair(x[3])) != 0);
         for (; found != 0; found &= found - 1) {
           const int n = __ffsll((unsigned long long)found) - 1, c = n % CH, key = min(k0 + n / CH, lim_hi - 1);
-          const v4 z = *reinterpret_cast<const v4*>(values(key) + 8 * c + 4 * h);
+          v4 z;
+          if constexpr (C8) {
+            const u32x4 y = widen8<T>(*reinterpret_cast<const u32x2*>(values(key) + 8 * c), scale_at(key));
+            z = __builtin_bit_cast(v4, h == 0 ? u32x2{y[0], y[1]} : u32x2{y[2], y[3]});
+          } else {
+            z = *reinterpret_cast<const v4*>(values(key) + 8 * c + 4 * h);
+          }
           if (row < rows && key < seen)
             update(c, [&](float y, int e) TT_INLINE {
               const T w = z[e];

@@ -2,6 +2,7 @@
 // 128) and seq_attention_wide.hip (up to 256).
 #pragma once
 
+#include "cache_checks.hpp"
 #include "seq_attention.hpp"
 
 #include <atomic>
@@ -17,16 +18,18 @@ constexpr int seq_waves(SeqShape shape, int hd) {
   return shape == SeqShape::kDeep ? (hd <= 64 ? 8 : hd <= 128 ? 4 : 2) : (hd <= 128 ? 2 : 1);
 }
 
-template <typename T, int HD, int RW, int KW, int KT, bool PAGED>
+template <typename T, int HD, int RW, int KW, int KT, bool PAGED, bool C8 = false>
 int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
-  constexpr int lds = 2 * 2 * KW * KT * HD * (int)sizeof(T);  // K and V, two tiles deep
-  static_assert(KW == 1 || lds >= KW * (HD / 8 * 64 * 16 + 32 * 8 + 4), "the groups are joined in the tiles' LDS");
+  // K and V, two tiles deep (narrow blocks over an 8-bit cache hold its bytes); the groups are joined there.
+  constexpr int tiles = 2 * 2 * KW * KT * HD * (C8 && RW == 1 ? 1 : (int)sizeof(T));
+  constexpr int joined = KW == 1 ? 0 : KW * (HD / 8 * 64 * 16 + 32 * 8 + 4);
+  constexpr int lds = tiles > joined ? tiles : joined;
   static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic LDS is raised
   int dev = 0;
   TT_HIP(hipGetDevice(&dev));
   const uint64_t bit = 1ull << (dev & 63);
   if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
-    TT_HIP(hipFuncSetAttribute((const void*)seq_attention_kernel<T, HD, RW, KW, KT, PAGED>,
+    TT_HIP(hipFuncSetAttribute((const void*)seq_attention_kernel<T, HD, RW, KW, KT, PAGED, C8>,
                                hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
@@ -34,7 +37,7 @@ int launch_seq(const SeqAttnArgs& a, hipStream_t stream) {
   constexpr int threads = 64 * RW * KW;
   TT_REQUIRE(blocks * threads < (1LL << 32), "attention: %lld blocks are more than one launch takes",
              (long long)blocks);
-  hipLaunchKernelGGL((seq_attention_kernel<T, HD, RW, KW, KT, PAGED>), dim3((unsigned)blocks), dim3(threads), lds,
+  hipLaunchKernelGGL((seq_attention_kernel<T, HD, RW, KW, KT, PAGED, C8>), dim3((unsigned)blocks), dim3(threads), lds,
                      stream, a);
   return launch_status("seq_attention_kernel");
 }
@@ -47,6 +50,20 @@ int launch_seq_type(const SeqAttnArgs& a, bool paged, SeqShape shape, hipStream_
   return launch_seq<T, HD, 4, 1, 64, true>(a, stream);
 }
 
+// Over an 8-bit cache.
+template <int HD, typename T>
+int launch_seq8_type(const SeqAttnArgs& a, SeqShape shape, hipStream_t stream) {
+  if (shape == SeqShape::kDeep) return launch_seq<T, HD, 1, seq_waves(SeqShape::kDeep, HD), 32, true, true>(a, stream);
+  if (shape == SeqShape::kNarrow)
+    return launch_seq<T, HD, 1, seq_waves(SeqShape::kNarrow, HD), 32, true, true>(a, stream);
+  return launch_seq<T, HD, 4, 1, 64, true, true>(a, stream);
+}
+
+template <int HD>
+int launch_seq8_hd(const SeqAttnArgs& a, SeqShape shape, int dtype, hipStream_t stream) {
+  return dtype == TT_FP16 ? launch_seq8_type<HD, half>(a, shape, stream) : launch_seq8_type<HD, bf16>(a, shape, stream);
+}
+
 template <int HD>
 int launch_seq_hd(const SeqAttnArgs& a, bool paged, SeqShape shape, int dtype, hipStream_t stream) {
   return dtype == TT_FP16 ? launch_seq_type<HD, half>(a, paged, shape, stream)
@@ -54,5 +71,7 @@ int launch_seq_hd(const SeqAttnArgs& a, bool paged, SeqShape shape, int dtype, h
 }
 
 int launch_seq_attention_wide(const SeqAttnArgs& a, bool paged, SeqShape shape, int dtype, hipStream_t stream);
+int launch_seq8_attention(const SeqAttnArgs& a, SeqShape shape, int dtype, hipStream_t stream);       // 8-bit cache
+int launch_seq8_attention_wide(const SeqAttnArgs& a, SeqShape shape, int dtype, hipStream_t stream);  // heads above 128
 
 }  // namespace tt

@@ -297,8 +297,35 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     return out
 
 
+def _cache8(t: torch.Tensor, name: str, shape, index: int):
+    """``_cache`` of one half of a cache in 8 bits."""
+    if len(shape) != 4 or t.shape != shape or t.dtype is not torch.float8_e4m3fn or t.get_device() != index:
+        raise ValueError(f"{name} must be a [pages, page_size, kv_heads, head_dim] tensor of shape {list(shape)} and "
+                         f"{torch.float8_e4m3fn} on cuda:{index}")
+    page, row, head, feature = t.stride()
+    pointer = t.data_ptr()
+    if feature != 1 or (page | row | head) & 15 or pointer & 15:
+        raise ValueError(f"{name} needs adjacent features, and pages, tokens and heads 16 bytes aligned")
+    return pointer, page, row, head
+
+
+def _scales(k: Optional[torch.Tensor], v: Optional[torch.Tensor], pages: int, page: int, kv_heads: int, index: int):
+    """(k's pointer, v's pointer, tokens per scale, k's strides, v's strides) of the scales of a cache in 8 bits."""
+    if k is None or v is None:
+        raise ValueError("a cache in 8 bits needs both k_scales and v_scales")
+    shape = k.shape
+    blocks = shape[1] if len(shape) == 3 else 0
+    if (blocks <= 0 or page % blocks or shape != (pages, blocks, kv_heads) or v.shape != shape
+            or k.dtype is not torch.float8_e8m0fnu or v.dtype is not torch.float8_e8m0fnu
+            or k.get_device() != index or v.get_device() != index):
+        raise ValueError(f"k_scales and v_scales must be [{pages}, {page} / tokens per scale, {kv_heads}] tensors of "
+                         f"{torch.float8_e8m0fnu} on cuda:{index}")
+    return k.data_ptr(), v.data_ptr(), page // blocks, k.stride(), v.stride()
+
+
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-                 page_table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None) -> None:
+                 page_table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *,
+                 k_scales: Optional[torch.Tensor] = None, v_scales: Optional[torch.Tensor] = None) -> None:
     """Write the keys and values of new tokens, k and v [T, kv_heads, head_dim], into a paged cache, in place.
 
     k_cache and v_cache are [pages, page_size, kv_heads, head_dim] (any strides that keep features adjacent, 16-byte
@@ -307,7 +334,15 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     (int32 [B, n]) at t % page_size.  ``lengths`` (int32 [B]) counts the keys of each sequence with the new ones:
     the n tokens of sequence b, rows starts[b] ... starts[b + 1] - 1 (or row b alone without ``starts``), take
     positions lengths[b] - n ... lengths[b] - 1.  Tokens whose position is negative or beyond the table, or whose
-    page is no page of the cache, are not written."""
+    page is no page of the cache, are not written.
+
+    With ``k_scales`` and ``v_scales`` (float8_e8m0fnu [pages, page_size / block, kv_heads], block a power of two from
+    16 on) the cache is in 8 bits: k_cache and v_cache are float8_e4m3fn, and a value is the product of both.  A block's
+    scale is the smallest power of two that holds its tokens' largest finite magnitude.  Where a new token is too large
+    for the block that older ones of its sequence lie in, the scale grows and those are rounded to it.  Infinities and
+    NaN become NaN, head_dim is a multiple of 16, and two sequences may not write to one block in one call."""
+    if k_scales is not None or v_scales is not None:
+        return _append8(k, v, k_cache, v_cache, page_table, lengths, starts, k_scales, v_scales)
     dtype, index = _typed(k, "k")
     k, shape, k_at, k_row, k_head = _rows(k, "k", dtype, index)
     v, v_shape, v_at, v_row, v_head = _rows(v, "v", dtype, index)
@@ -329,9 +364,34 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     _call("tt_cache_append", packed, index)
 
 
+def _append8(k, v, k_cache, v_cache, page_table, lengths, starts, k_scales, v_scales) -> None:
+    dtype, index = _typed(k, "k")
+    k, shape, k_at, k_row, k_head = _rows(k, "k", dtype, index)
+    v, v_shape, v_at, v_row, v_head = _rows(v, "v", dtype, index)
+    if shape != v_shape:
+        raise ValueError("k and v must have one shape")
+    tokens, kv_heads, hd = shape
+    _heads(kv_heads, kv_heads, hd)
+    shape = (*k_cache.shape[:2], kv_heads, hd)
+    k_half, v_half = _cache8(k_cache, "k_cache", shape, index), _cache8(v_cache, "v_cache", shape, index)
+    ks_at, vs_at, block, ks, vs = _scales(k_scales, v_scales, shape[0], shape[1], kv_heads, index)
+    table, lengths, starts, batch, table_pages, table_row = _sequences(tokens, page_table, lengths, starts, index)
+    args = _lib.CACHE_ROWS8
+    try:
+        packed = args.pack(
+            args.size, k_at, v_at, k_half[0], v_half[0], ks_at, vs_at, table.data_ptr(), lengths.data_ptr(),
+            0 if starts is None else starts.data_ptr(), k_row, k_head, v_row, v_head, *k_half[1:], *v_half[1:], *ks,
+            *vs, table_row, tokens, batch, kv_heads, hd, shape[0], shape[1], table_pages, block, _SEQ_DTYPES[dtype], 0)
+    except _lib.PACK_ERRORS as e:
+        raise ValueError(f"cache_append: {e}") from None
+    _call("tt_cache_append8", packed, index)
+
+
 def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                     lengths: torch.Tensor, starts: Optional[torch.Tensor] = None, *, scale: Optional[float] = None,
-                    max_length: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    max_length: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                    k_scales: Optional[torch.Tensor] = None,
+                    v_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of new tokens q [T, heads, head_dim] over a paged cache that holds their keys and values already
     (``cache_append``, whose arguments these are) -> [T, heads * head_dim].
 
@@ -339,11 +399,18 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (a length of 0 in a padded batch) gets zeros.  Without ``starts`` every sequence has one new token.
     ``max_length`` (default: what the table can hold) is the longest length the caller expects; it only decides how
     the work is split.  Keys in a page whose number is no page of the cache are not read and count as NaN.  ``out`` may
-    not overlap the other tensors."""
+    not overlap the other tensors.
+
+    ``k_scales`` and ``v_scales`` as in ``cache_append``: the cache is in 8 bits, read as values of q's type."""
     dtype, index = _typed(q, "q")
     q, (tokens, heads, hd), q_at, q_row, q_head = _rows(q, "q", dtype, index)
     shape = (*k_cache.shape[:3], hd)
-    k_half, v_half = _cache(k_cache, "k_cache", shape, dtype, index), _cache(v_cache, "v_cache", shape, dtype, index)
+    eight = k_scales is not None or v_scales is not None
+    if eight:
+        k_half, v_half = _cache8(k_cache, "k_cache", shape, index), _cache8(v_cache, "v_cache", shape, index)
+    else:
+        k_half = _cache(k_cache, "k_cache", shape, dtype, index)
+        v_half = _cache(v_cache, "v_cache", shape, dtype, index)
     pages, page, kv_heads, _ = shape
     _heads(heads, kv_heads, hd)
     table, lengths, starts, batch, table_pages, table_row = _sequences(tokens, page_table, lengths, starts, index)
@@ -351,8 +418,22 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     held = table_pages * page
     max_length = held if max_length is None else min(int(max_length), held)
     nbytes = _lib.cache_attention_workspace_bytes(tokens, batch, heads, kv_heads, hd, page, table_pages, max_length,
-                                                  starts is None)
+                                                  starts is None, eight)
     work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    if eight:
+        ks_at, vs_at, block, ks, vs = _scales(k_scales, v_scales, pages, page, kv_heads, index)
+        args = _lib.CACHE_ATTENTION8
+        try:
+            packed = args.pack(
+                args.size, q_at, k_half[0], v_half[0], ks_at, vs_at, table.data_ptr(), lengths.data_ptr(),
+                0 if starts is None else starts.data_ptr(), out.data_ptr(), 0 if work is None else work.data_ptr(),
+                nbytes, q_row, q_head, *k_half[1:], *v_half[1:], *ks, *vs, table_row, tokens, batch, heads, kv_heads,
+                hd, pages, page, table_pages, max_length, block, _SEQ_DTYPES[dtype],
+                hd ** -0.5 if scale is None else scale)
+        except _lib.PACK_ERRORS as e:
+            raise ValueError(f"cache_attention: {e}") from None
+        _call("tt_cache_attention8_fwd", packed, index)
+        return out
     args = _lib.CACHE_ATTENTION
     try:
         packed = args.pack(
