@@ -360,6 +360,27 @@ int tt_cache_attention8_workspace_bytes(int tokens, int batch, int heads, int kv
                                         int64_t* bytes);
 int tt_cache_attention8_fwd(const tt_cache_attention8* args, void* stream);
 
+/* Rotary positions: in rows x [tokens, heads, head_dim] of `dtype` the first 2 `pairs` features of every
+ * head are turned in pairs, (i, i + pairs) or with `interleaved` (2 i, 2 i + 1), by position times
+ * frequencies[i] (doubles, radians per position) and multiplied by `magnitude`; with `transpose` they are
+ * turned back, which is the gradient.  The other features are copied.  The position of row t is
+ * positions[t], or with `lengths` (and `starts`) instead that of tt_cache_append's tokens; then rows outside
+ * every sequence stay as they are in out.  Strides are in elements, features adjacent, head_dim at most
+ * 256.  out is x itself, with its strides, or overlaps nothing.  No counterpart in the reference, which
+ * adds no positions. */
+typedef struct {
+  int64_t size;
+  const void* x;
+  void* out;
+  const double* frequencies;
+  const int32_t *positions, *lengths, *starts;
+  int64_t x_row, x_head, out_row, out_head;
+  int32_t tokens, batch, heads, head_dim, pairs, interleaved, transpose, dtype;
+  float magnitude;
+  int32_t reserved;
+} tt_rotary_rows;
+int tt_rotary(const tt_rotary_rows* args, void* stream);
+
 /* Where a forward's intermediates of its LAST layer are left in the workspace, for per-stage checks
  * of the fused plans (the megakernel's tasks and the fused-LN tiles never materialise LN1 / LN2 or
  * the other stages on their own): byte offsets of the Q / K / V^T planes (the TT_EPI_QKV layout;

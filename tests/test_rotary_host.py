@@ -1,0 +1,85 @@
+"""CPU tests of the rotary positions' host side: the argument structure and refusals before any launch."""
+
+import ctypes
+
+import pytest
+import torch
+
+from test_cache8_host import P, _fields
+from tttj_2026_amd import _lib, ops
+
+GOOD = dict(x=P, out=P + (1 << 16), frequencies=P, positions=P, x_row=640, x_head=64, out_row=512, out_head=64, tokens=4,
+            batch=0, heads=8, head_dim=64, pairs=32, interleaved=0, transpose=0, dtype=0, magnitude=1.0)
+
+
+def test_structure_is_the_header_s():
+    kind = type("rotary", (ctypes.Structure,), {"_fields_": _fields("tt_rotary_rows")})
+    assert ctypes.sizeof(kind) == _lib.ROTARY_ROWS.size
+    values = {n: i + 1 for i, (n, _) in enumerate(_fields("tt_rotary_rows"))}
+    s = kind(**values)
+    assert bytes(s) == _lib.ROTARY_ROWS.pack(*values.values())
+
+
+def _call(**change):
+    kind = type("rotary", (ctypes.Structure,), {"_fields_": _fields("tt_rotary_rows")})
+    values = {"size": ctypes.sizeof(kind), **GOOD, **change}
+    return _lib.load().tt_rotary(ctypes.byref(kind(**values)), None)
+
+
+def test_refusals():
+    assert _lib.load().tt_rotary(None, None) == _lib.TT_ERR_INVALID
+    in_place = dict(out=P)
+    for change in (dict(size=8), dict(tokens=-1), dict(batch=-1), dict(heads=0), dict(heads=-1), dict(pairs=0),
+                   dict(pairs=33), dict(pairs=-1), dict(head_dim=258), dict(dtype=2), dict(tokens=1 << 28),
+                   dict(tokens=1 << 26, heads=1), dict(magnitude=float("nan")), dict(magnitude=float("inf")),
+                   dict(positions=None), dict(lengths=P), dict(starts=P), dict(positions=None, lengths=P, batch=3),
+                   dict(x=None), dict(out=None), dict(frequencies=None), dict(frequencies=P + 4), dict(x=P + 1),
+                   dict(out=P + 1), dict(x_row=-1), dict(x_head=-1), dict(out_row=-1), dict(out_head=-1), dict(out_row=0),
+                   dict(out_head=0), in_place, dict(out=P, out_row=640, out_head=128)):
+        assert _call(**change) == _lib.TT_ERR_INVALID, change
+    for change in (dict(tokens=0), dict(positions=None, lengths=P, starts=P, batch=0)):
+        assert _call(**change) == _lib.TT_OK
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """Host tensors pass for the device's, up to the library call, which is counted."""
+    calls = []
+    monkeypatch.setattr(ops, "_typed", lambda t, name: (t.dtype, t.get_device()))
+    monkeypatch.setattr(ops, "_call", lambda name, args, index: calls.append(name))
+    return calls
+
+
+def test_tensors(host):
+    x, f = torch.zeros(4, 8, 64, dtype=torch.float16), ops.rotary_frequencies(64)
+    at, n = torch.zeros(4, dtype=torch.int32), torch.tensor([9, 9], dtype=torch.int32)
+    starts = torch.tensor([0, 3, 4], dtype=torch.int32)
+    ops.rotary(x, f, at), ops.rotary(x, f, lengths=n, starts=starts), ops.rotary(x, f, at, out=x)
+    ops.rotary(x, f, lengths=at), ops.rotary(x.transpose(1, 2), f[:4], at), ops.rotary(x, f[::2], at)
+    assert host == ["tt_rotary"] * 6
+    for args, how in (((x, f), {}), ((x, f, at.long()), {}), ((x, f, at[:3]), {}), ((x, f, at), dict(lengths=n)),
+                      ((x, f, at), dict(starts=starts)), ((x, f), dict(lengths=n)), ((x, f), dict(starts=starts)),
+                      ((x, f), dict(lengths=n, starts=n)), ((x, f.float(), at), {}), ((x, f.view(1, -1), at), {}),
+                      ((x, f[:0], at), {}), ((x[0], f, at), {}), ((x[:, :0], f, at), {}), ((x, f, at), dict(out=x[:3])),
+                      ((x, f, at), dict(out=x.float())), ((x, f, at), dict(out=torch.zeros(4, 64, 8).half().transpose(1, 2))),
+                      ((x.transpose(1, 2), f[:4], at), dict(out=x)), ((x, f, at), dict(magnitude=10 ** 400))):
+        with pytest.raises(ValueError):
+            ops.rotary(*args, **how)
+    y = x.transpose(1, 2)
+    with pytest.raises(ValueError):
+        ops.rotary(y, f[:4], at, out=y)
+    assert len(host) == 6
+
+
+def test_frequencies_are_refused():
+    for args, how in (((7,), {}), ((0,), {}), ((-2,), {}), ((8, 0.0), {}), ((8,), dict(factor=0.5)),
+                      ((8,), dict(scaling="cubic")), ((8,), dict(scaling="ramp")),
+                      ((8,), dict(scaling="ramp", original_length=100, low=4.0, high=4.0)),
+                      ((8, float("nan")), {}), ((8,), dict(factor=float("nan")))):
+        with pytest.raises(ValueError):
+            ops.rotary_frequencies(*args, **how)
+
+
+def test_host_tensors_are_refused():
+    with pytest.raises(ValueError):
+        ops.rotary(torch.zeros(4, 8, 64, dtype=torch.float16), ops.rotary_frequencies(64), torch.zeros(4, dtype=torch.int32))

@@ -60,6 +60,7 @@ SIGNATURES = {
     "tt_cache_append8": (_I, [_P, _P]),
     "tt_cache_attention8_workspace_bytes": (_I, [_I] * 9 + [ctypes.POINTER(_I64)]),
     "tt_cache_attention8_fwd": (_I, [_P, _P]),
+    "tt_rotary": (_I, [_P, _P]),
     "tt_transformer_fwd": (_I, [_P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "tt_noalloc_scratch_bytes": (_I, [ctypes.POINTER(_I64)]),
     "tt_transformer_fwd_noalloc": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
@@ -74,6 +75,7 @@ CACHE_ROWS = struct.Struct("q2Q2Q3Q11q8i")
 CACHE_ATTENTION = struct.Struct("q3Q3Q2Qq9q10ifi")
 CACHE_ROWS8 = struct.Struct("q2Q2Q2Q3Q17q10i")
 CACHE_ATTENTION8 = struct.Struct("q3Q2Q3Q2Qq15q11if")
+ROTARY_ROWS = struct.Struct("qQQQ3Q4q8ifi")
 PACK_ERRORS = (struct.error, OverflowError)  # a number that its field cannot hold
 
 _lock = threading.Lock()

@@ -7,6 +7,7 @@ Every function launches on the current stream of the input's device and raises o
 
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -444,4 +445,98 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     except _lib.PACK_ERRORS as e:
         raise ValueError(f"cache_attention: {e}") from None
     _call("tt_cache_attention_fwd", packed, index)
+    return out
+
+
+# ---- rotary positions ----
+
+def rotary_frequencies(dims: int, base: float = 10000.0, *, factor: float = 1.0, scaling: str = "linear",
+                       original_length: Optional[int] = None, low: float = 1.0, high: float = 4.0,
+                       device=None) -> torch.Tensor:
+    """Frequencies of ``rotary`` for ``dims`` turned features (an even number), in radians per position: base^(-2 i / dims)
+    for pair i, float64 [dims / 2], made for contexts ``factor`` times as long as those a model was trained on:
+
+    * ``"linear"``: all divided by ``factor`` (positions are squeezed);
+    * ``"base"``: a larger base, so that the slowest pair is divided by ``factor`` and the fastest stays;
+    * ``"ramp"``: pairs that turn at least ``high`` times in ``original_length`` positions stay, those that turn at most
+      ``low`` times are divided by ``factor``, and those between are mixed in proportion to their turns."""
+    if dims <= 0 or dims % 2 or not base > 0 or not factor >= 1:
+        raise ValueError(f"rotary frequencies of {dims} features with base {base} and factor {factor}")
+    pair = torch.arange(dims // 2, dtype=torch.float64)
+    if scaling == "base":
+        if dims > 2:
+            base = base * factor ** (dims / (dims - 2))
+        return (base ** (-2 * pair / dims)).to(device)
+    frequencies = base ** (-2 * pair / dims)
+    if scaling == "ramp":
+        if not original_length or original_length <= 0 or not high > low:
+            raise ValueError(f"a ramp needs the original length ({original_length}) and low < high ({low}, {high})")
+        turns = original_length * frequencies / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        return (keep * frequencies + (1 - keep) * frequencies / factor).to(device)
+    if scaling != "linear":
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return (frequencies / factor).to(device)
+
+
+def rotary(x: torch.Tensor, frequencies: torch.Tensor, positions: Optional[torch.Tensor] = None, *,
+           lengths: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None, interleaved: bool = False,
+           magnitude: float = 1.0, transpose: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Turn the heads of x [T, heads, head_dim] (float16 or bfloat16) by their tokens' positions.
+
+    ``frequencies`` (float64 [n], on the device; ``rotary_frequencies``) turns the first 2 n features of each head, in pairs
+    (i, i + n) or with ``interleaved`` (2 i, 2 i + 1), by position * frequencies[i] radians, times ``magnitude``; the
+    others stay.  Positions are ``positions`` (int32 [T]), or those that ``cache_append`` gives new tokens for
+    ``lengths`` and ``starts`` (there rows outside every sequence are left as they are in ``out``, arbitrary in a new
+    tensor).  With ``transpose`` they are turned back: the gradient of a loss for x is ``rotary`` of its gradient for the
+    result with ``transpose=True``.
+
+    Queries and keys that lie side by side in a projection's output are turned in one call, as heads of one tensor.
+    ``out`` is x itself (in place) or a tensor that overlaps nothing; features are adjacent in both, head_dim at most 256."""
+    dtype, index = _typed(x, "x")
+    shape = x.shape
+    if len(shape) != 3 or shape[1] == 0:
+        raise ValueError("x must be a [tokens, heads, head_dim] tensor")
+    tokens, heads, hd = shape
+    if out is None:
+        out = x.new_empty(shape)
+    elif out.shape != shape or out.dtype is not dtype or out.get_device() != index:
+        raise ValueError(f"out must be a {list(shape)} tensor of {dtype} on cuda:{index}")
+    row, head, feature = x.stride()
+    out_row, out_head, out_feature = out.stride()
+    if feature != 1 and hd > 1:
+        if out is x:
+            raise ValueError("in place, the features of x must be adjacent")
+        x = x.contiguous()
+        row, head, _ = x.stride()
+    if out_feature != 1 and hd > 1:
+        raise ValueError("the features of out must be adjacent")
+    pairs = frequencies.shape[0] if frequencies.dim() == 1 else 0
+    if pairs == 0 or frequencies.dtype is not torch.float64 or frequencies.get_device() != index:
+        raise ValueError(f"frequencies must be a float64 tensor of one dimension on cuda:{index}")
+    frequencies = frequencies.contiguous()
+    batch = 0
+    if positions is not None:
+        if lengths is not None or starts is not None:
+            raise ValueError("either positions or lengths and starts are given")
+        positions = _int32(positions, "positions", tokens, index)
+    else:
+        if lengths is None:
+            raise ValueError("positions or lengths are needed")
+        batch = lengths.shape[0] if lengths.dim() == 1 else -1
+        lengths = _int32(lengths, "lengths", batch, index)
+        if starts is not None:
+            starts = _int32(starts, "starts", batch + 1, index)
+        elif tokens != batch:
+            raise ValueError(f"{tokens} tokens for {batch} sequences need starts")
+    args = _lib.ROTARY_ROWS
+    try:
+        packed = args.pack(
+            args.size, x.data_ptr(), out.data_ptr(), frequencies.data_ptr(),
+            0 if positions is None else positions.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+            0 if starts is None else starts.data_ptr(), row, head, out_row, out_head, tokens, batch, heads, hd, pairs,
+            interleaved, transpose, _SEQ_DTYPES[dtype], magnitude, 0)
+    except _lib.PACK_ERRORS as e:
+        raise ValueError(f"rotary: {e}") from None
+    _call("tt_rotary", packed, index)
     return out
