@@ -381,6 +381,61 @@ typedef struct {
 } tt_rotary_rows;
 int tt_rotary(const tt_rotary_rows* args, void* stream);
 
+/* Pages of a cache.  The state is on the device: a page table [batch, columns] (rows table_row apart) and
+ * lengths [batch] as above (row b holds ceil(lengths[b] / page_size) pages, its first ones; the rest of a row counts
+ * for nothing), and uses [pages]: how many rows hold a page, and once more for each hold that the program has on it
+ * otherwise (a prompt kept for later).  A page with 0 is free.  The calls write the new state into tensors of
+ * its own (new_table [batch, columns] contiguous; -1 behind a row's pages) and copy pages in `part_count` tensors: halves
+ * of layers' caches, scales, or anything that has a dense piece of memory for each page, `page` bytes apart: `rows`
+ * rows of `row` bytes, each of which belongs to page_size / rows tokens (1: no order by tokens).  Tensors of one call
+ * overlap nowhere.  `parts` is read during the call.  Numbers outside [0, pages) are kept as they are, and nothing is read or
+ * written there.  The workspace (4-byte aligned, any contents, this call's alone until it is done) has the bytes that
+ * tt_cache_pages_workspace_bytes gives.  No counterpart in the reference, which keeps no keys between calls. */
+typedef struct {
+  void* data;
+  int64_t page, row;
+  int32_t rows, reserved;
+} tt_cache_part;
+int tt_cache_pages_workspace_bytes(int batch, int columns, int pages, int64_t* bytes);
+
+/* Row b becomes what row parents[b] was (NULL: itself; outside [0, batch): empty, which frees its pages), with
+ * counts[b] (NULL: 0) more tokens, or fewer, from 0 to what the table holds.  Whole pages are shared.  A page that is
+ * taken over in part, and so is about to be written, is kept by the first row that takes it so, unless a row
+ * holds it whole or the program holds it; the others get copies of the rows of it that hold their tokens.  New pages are the
+ * free ones of lowest number, row by row; where they run out, the table has -1. */
+typedef struct {
+  int64_t size;
+  const tt_cache_part* parts;
+  const int32_t *table, *lengths, *uses, *parents, *counts;
+  int32_t *new_table, *new_lengths, *new_uses;
+  void* workspace;
+  int64_t workspace_bytes, table_row;
+  int32_t part_count, batch, columns, pages, page_size, reserved;
+} tt_cache_fork_pages;
+int tt_cache_fork(const tt_cache_fork_pages* args, void* stream);
+
+/* Used pages whose numbers are at or past the number of used pages move to the free ones below it, both in rising
+ * order; the table and the uses follow. */
+typedef struct {
+  int64_t size;
+  const tt_cache_part* parts;
+  const int32_t *table, *lengths, *uses;
+  int32_t *new_table, *new_uses;
+  void* workspace;
+  int64_t workspace_bytes, table_row;
+  int32_t part_count, batch, columns, pages, page_size, reserved;
+} tt_cache_compact_pages;
+int tt_cache_compact(const tt_cache_compact_pages* args, void* stream);
+
+/* Whole pages source[i] -> target[i] (device, int32); no target is also a source, nor given twice. */
+typedef struct {
+  int64_t size;
+  const tt_cache_part* parts;
+  const int32_t *source, *target;
+  int32_t part_count, count, pages, reserved;
+} tt_cache_copy_pages;
+int tt_cache_copy(const tt_cache_copy_pages* args, void* stream);
+
 /* Where a forward's intermediates of its LAST layer are left in the workspace, for per-stage checks
  * of the fused plans (the megakernel's tasks and the fused-LN tiles never materialise LN1 / LN2 or
  * the other stages on their own): byte offsets of the Q / K / V^T planes (the TT_EPI_QKV layout;

@@ -61,6 +61,10 @@ SIGNATURES = {
     "tt_cache_attention8_workspace_bytes": (_I, [_I] * 9 + [ctypes.POINTER(_I64)]),
     "tt_cache_attention8_fwd": (_I, [_P, _P]),
     "tt_rotary": (_I, [_P, _P]),
+    "tt_cache_pages_workspace_bytes": (_I, [_I] * 3 + [ctypes.POINTER(_I64)]),
+    "tt_cache_fork": (_I, [_P, _P]),
+    "tt_cache_compact": (_I, [_P, _P]),
+    "tt_cache_copy": (_I, [_P, _P]),
     "tt_transformer_fwd": (_I, [_P, _P, _P, _P, _P, _I64, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "tt_noalloc_scratch_bytes": (_I, [ctypes.POINTER(_I64)]),
     "tt_transformer_fwd_noalloc": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
@@ -76,6 +80,10 @@ CACHE_ATTENTION = struct.Struct("q3Q3Q2Qq9q10ifi")
 CACHE_ROWS8 = struct.Struct("q2Q2Q2Q3Q17q10i")
 CACHE_ATTENTION8 = struct.Struct("q3Q2Q3Q2Qq15q11if")
 ROTARY_ROWS = struct.Struct("qQQQ3Q4q8ifi")
+CACHE_PART = struct.Struct("Q2q2i")
+CACHE_FORK = struct.Struct("qQ5Q3QQ2q6i")
+CACHE_COMPACT = struct.Struct("qQ3Q2QQ2q6i")
+CACHE_COPY = struct.Struct("qQ2Q4i")
 PACK_ERRORS = (struct.error, OverflowError)  # a number that its field cannot hold
 
 _lock = threading.Lock()
@@ -148,6 +156,14 @@ def cache_attention_workspace_bytes(tokens: int, batch: int, heads: int, kv_head
     name = f"tt_cache_attention{'8' if eight_bits else ''}_workspace_bytes"
     check(getattr(load(), name)(tokens, batch, heads, kv_heads, head_dim, page_size, table_pages, max_length,
                                 int(single), ctypes.byref(out)), name)
+    return out.value
+
+
+@functools.lru_cache(maxsize=256)
+def cache_pages_workspace_bytes(batch: int, columns: int, pages: int) -> int:
+    out = _I64()
+    check(load().tt_cache_pages_workspace_bytes(batch, columns, pages, ctypes.byref(out)),
+          "tt_cache_pages_workspace_bytes")
     return out.value
 
 

@@ -7,8 +7,9 @@ Every function launches on the current stream of the input's device and raises o
 
 from __future__ import annotations
 
+import ctypes
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -540,3 +541,125 @@ def rotary(x: torch.Tensor, frequencies: torch.Tensor, positions: Optional[torch
         raise ValueError(f"rotary: {e}") from None
     _call("tt_rotary", packed, index)
     return out
+
+
+# ---- pages of a cache ----
+
+def _parts(caches: Sequence[torch.Tensor]):
+    """(their description for the library, number of tensors, pages, page size, device index) of tensors [pages, ...] each
+    of whose pages is a dense piece of memory."""
+    described, pages, page_size, index = [], 0, 0, -1
+    for t in caches:
+        shape, stride = t.shape, t.stride()
+        if len(shape) < 2 or not t.is_cuda or 0 in shape:
+            raise ValueError("caches must be CUDA tensors [pages, page_size or blocks of it, ...] that hold something")
+        if not described:
+            pages, page_size, index = shape[0], shape[1], t.get_device()
+        elif shape[0] != pages or t.get_device() != index:
+            raise ValueError(f"caches must have {pages} pages each, all on cuda:{index}")
+        if page_size % shape[1]:
+            raise ValueError(f"{shape[1]} rows of a page cannot share {page_size} tokens evenly")
+        size = t.element_size()
+        row = 1
+        for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
+            if n != 1 and s != row:
+                row = 0
+                break
+            row *= n
+        if row:
+            rows = shape[1]
+            row = row // rows * size
+        else:  # in another order: dense all the same?
+            rows, row = 1, 1
+            for s, n in sorted((s, n) for n, s in zip(shape[1:], stride[1:]) if n != 1):
+                if s != row:
+                    raise ValueError("a page of a cache must be a dense piece of memory")
+                row *= n
+            row *= size
+        step = stride[0] * size
+        if pages > 1 and step < rows * row:
+            raise ValueError("the pages of a cache must not overlap")
+        described.append(_lib.CACHE_PART.pack(t.data_ptr(), step, row, rows, 0))
+    if not described:
+        raise ValueError("caches holds no tensor")
+    return ctypes.create_string_buffer(b"".join(described)), len(described), pages, page_size, index
+
+
+def _state(page_table: torch.Tensor, lengths: torch.Tensor, uses: torch.Tensor, pages: int, index: int):
+    """Checks of a cache's state; (page_table, lengths, uses, batch, columns, the table's row stride)."""
+    batch = lengths.shape[0] if lengths.dim() == 1 else -1
+    lengths = _int32(lengths, "lengths", batch, index)
+    uses = _int32(uses, "uses", pages, index)
+    shape = page_table.shape
+    if (len(shape) != 2 or shape[0] != batch or shape[1] == 0 or page_table.dtype is not torch.int32
+            or page_table.get_device() != index):
+        raise ValueError(f"page_table must be an int32 tensor [{batch}, pages per sequence] on cuda:{index}")
+    if page_table.stride(1) != 1 or page_table.stride(0) < 0:
+        page_table = page_table.contiguous()
+    return page_table, lengths, uses, batch, shape[1], page_table.stride(0)
+
+
+def cache_fork(caches: Sequence[torch.Tensor], page_table: torch.Tensor, lengths: torch.Tensor, uses: torch.Tensor,
+               parents: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None
+               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Continue, fork, reorder, free, extend or shorten the sequences of a paged cache -> (page_table, lengths, uses).
+
+    Row b of the new ``page_table`` (int32 [B, n]) and ``lengths`` (int32 [B]) is what row parents[b] was (without
+    ``parents``, int32 [B]: row b itself; a number outside 0 ... B - 1: an empty sequence, whose pages are given up), with
+    counts[b] tokens more or fewer (``counts``, int32 [B]; none without it), so that ``cache_append`` finds room for them.
+    ``uses`` (int32 [pages]) counts the rows that hold each page, and holds that the program has on one besides (a prompt
+    that is kept); pages with 0 are free.  Rows hold the pages of their lengths; what the table has behind those counts
+    for nothing and is -1 in the new one.
+
+    Whole pages are shared.  A page that is taken over in part is about to be written: the first row that takes it over so
+    keeps it, unless a row holds it whole or the program does, and the others get copies of their tokens in all ``caches``
+    (tensors [pages, page_size, ...], or [pages, blocks of a page, ...] as scales are, each of whose pages is a dense piece
+    of memory: K and V of every layer; the first one's second size is the page size).  New pages are the free ones of
+    lowest number, row by row; where they run out the table has -1, whose tokens ``cache_append`` does not write.
+    Nothing is read back: a step is a call whatever it comes to, and may be captured into a graph."""
+    parts, count, pages, page_size, index = _parts(caches)
+    page_table, lengths, uses, batch, columns, row = _state(page_table, lengths, uses, pages, index)
+    if parents is not None:
+        parents = _int32(parents, "parents", batch, index)
+    if counts is not None:
+        counts = _int32(counts, "counts", batch, index)
+    work = uses.new_empty(_lib.cache_pages_workspace_bytes(batch, columns, pages), dtype=torch.uint8)
+    table, after, held = uses.new_empty((batch, columns)), uses.new_empty(batch), uses.new_empty(pages)
+    args = _lib.CACHE_FORK
+    packed = args.pack(
+        args.size, ctypes.addressof(parts), page_table.data_ptr(), lengths.data_ptr(), uses.data_ptr(),
+        0 if parents is None else parents.data_ptr(), 0 if counts is None else counts.data_ptr(), table.data_ptr(),
+        after.data_ptr(), held.data_ptr(), work.data_ptr(), work.numel(), row, count, batch, columns, pages, page_size, 0)
+    _call("tt_cache_fork", packed, index)
+    return table, after, held
+
+
+def cache_compact(caches: Sequence[torch.Tensor], page_table: torch.Tensor, lengths: torch.Tensor, uses: torch.Tensor
+                  ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Move the used pages of a cache to its low end -> (page_table, uses); arguments as in ``cache_fork``.
+
+    Of U used pages those numbered U and above go to the free numbers below U, both in rising order, in all ``caches``;
+    what lies at and above U is free afterwards.  Other tables and lists of page numbers are the caller's to renumber:
+    page p is used if ``uses`` is not 0, and a page that moves keeps its count."""
+    parts, count, pages, page_size, index = _parts(caches)
+    page_table, lengths, uses, batch, columns, row = _state(page_table, lengths, uses, pages, index)
+    work = uses.new_empty(_lib.cache_pages_workspace_bytes(batch, columns, pages), dtype=torch.uint8)
+    table, held = uses.new_empty((batch, columns)), uses.new_empty(pages)
+    args = _lib.CACHE_COMPACT
+    packed = args.pack(
+        args.size, ctypes.addressof(parts), page_table.data_ptr(), lengths.data_ptr(), uses.data_ptr(), table.data_ptr(),
+        held.data_ptr(), work.data_ptr(), work.numel(), row, count, batch, columns, pages, page_size, 0)
+    _call("tt_cache_compact", packed, index)
+    return table, held
+
+
+def cache_copy(caches: Sequence[torch.Tensor], source: torch.Tensor, target: torch.Tensor) -> None:
+    """Copy pages source[i] to target[i] (int32 [N], on the device) in all ``caches`` (as in ``cache_fork``), in place.
+
+    Pairs with a number that is no page of the cache are skipped.  No target may be given twice or be a source."""
+    parts, count, pages, _, index = _parts(caches)
+    n = source.shape[0] if source.dim() == 1 else -1
+    source, target = _int32(source, "source", n, index), _int32(target, "target", n, index)
+    args = _lib.CACHE_COPY
+    packed = args.pack(args.size, ctypes.addressof(parts), source.data_ptr(), target.data_ptr(), count, n, pages, 0)
+    _call("tt_cache_copy", packed, index)
