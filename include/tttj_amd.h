@@ -389,7 +389,7 @@ int tt_rotary(const tt_rotary_rows* args, void* stream);
  * of layers' caches, scales, or anything that has a dense piece of memory for each page, `page` bytes apart: `rows`
  * rows of `row` bytes, each of which belongs to page_size / rows tokens (1: no order by tokens).  Tensors of one call
  * overlap nowhere.  `parts` is read during the call.  Numbers outside [0, pages) are kept as they are, and nothing is read or
- * written there.  The workspace (4-byte aligned, any contents, this call's alone until it is done) has the bytes that
+ * written there.  The workspace (16-byte aligned, any contents, this call's alone until it is done) has the bytes that
  * tt_cache_pages_workspace_bytes gives.  No counterpart in the reference, which keeps no keys between calls. */
 typedef struct {
   void* data;

@@ -40,7 +40,7 @@ def test_refusals(name):
     assert getattr(_lib.load(), CALLS[name][1])(None, None) == _lib.TT_ERR_INVALID
     for change in (dict(size=8), dict(batch=-1), dict(columns=0), dict(pages=0), dict(pages=-1), dict(page_size=8),
                    dict(page_size=48), dict(page_size=1 << 20, columns=1 << 11), dict(batch=1 << 27), dict(table_row=-1),
-                   dict(part_count=-1), dict(parts=None), dict(count=-1), dict(workspace=P + 2), dict(workspace_bytes=64)):
+                   dict(part_count=-1), dict(parts=None), dict(count=-1), dict(workspace=P + 8), dict(workspace_bytes=64)):
         change = {k: v for k, v in change.items() if k in fields}
         if change:
             assert _call(name, **change) == _lib.TT_ERR_INVALID, change
@@ -54,7 +54,7 @@ def test_refusals(name):
 
 def test_workspace():
     size = _lib.cache_pages_workspace_bytes
-    assert size(2, 8, 9) == 4 * (2 * 9 + 9 + 2 * 2 + 3 * 4 + 1)
+    assert size(2, 8, 9) == 4 * (4 * 2 + 2 * 9 + 9 + 3 * 4 + 1)
     assert _call("tt_cache_copy_pages", count=0) == _lib.TT_OK
     for bad in ((-1, 8, 9), (2, 0, 9), (2, 8, 0), (1 << 27, 8, 9)):
         with pytest.raises(ValueError):

@@ -7,16 +7,37 @@
 #include "kernels.hpp"
 #include "seq_attention.hpp"
 
+#include <atomic>
+
 namespace tt {
 
 constexpr int kPageThreads = 1024;
+constexpr int kPageWaves = kPageThreads / 64;
+constexpr int kEach = 4;              // pages that a thread looks at in turn
+constexpr int kSmallPages = 16384;    // up to this many, counters lie in LDS (8 bytes a page) ...
+constexpr int kSmallRows = 1024;      // ... and so do up to this many rows (16 bytes a row)
 
-// Counters that atomics of this launch change are read past the L1 (which may hold them as they were).
-__device__ __forceinline__ int fresh(const int* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void put(int* p, int v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Counters of the pages: in LDS, or for large caches in the workspace, where atomics change them and they are read past
+// the L1 (which may hold them as they were).
+template <bool SMALL>
+struct Counters {
+  int* at;
+  __device__ __forceinline__ int get(int i) const {
+    if constexpr (SMALL) return at[i];
+    else return __hip_atomic_load(at + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __device__ __forceinline__ void put(int i, int v) const {
+    if constexpr (SMALL) at[i] = v;
+    else __hip_atomic_store(at + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __device__ __forceinline__ void add(int i, int v) const { atomicAdd(at + i, v); }
+  __device__ __forceinline__ void least(int i, int v) const { atomicMin(at + i, v); }
+};
+
+template <bool SMALL>
+__device__ __forceinline__ void phase() {  // what was written is read by others from here on
+  if constexpr (!SMALL) __threadfence();
+  __syncthreads();
 }
 
 // Sum over the block's threads before this one; `total` over all.  (s_sums: an int per wave; free again at return.)
@@ -25,8 +46,8 @@ __device__ __forceinline__ int block_scan(int v, int* s_sums, int& total) {
   const int upto = wave_scan_int(v);
   if (lane == 63) s_sums[wave] = upto;
   __syncthreads();
-  const int sums = wave_scan_int(lane < kPageThreads / 64 ? s_sums[lane] : 0);
-  total = __builtin_amdgcn_readlane(sums, kPageThreads / 64 - 1);
+  const int sums = wave_scan_int(lane < kPageWaves ? s_sums[lane] : 0);
+  total = __builtin_amdgcn_readlane(sums, kPageWaves - 1);
   const int before = wave > 0 ? __builtin_amdgcn_readlane(sums, max(wave - 1, 0)) : 0;
   __syncthreads();
   return before + upto - v;
@@ -37,182 +58,254 @@ struct PagesArgs {
   int32_t *new_table, *new_lengths, *new_uses;
   int64_t table_row;
   int batch, columns, pages, page_shift, list;  // list: free pages that can be needed
-  int *hold, *first, *free_pages;               // [pages], [pages], [list]
-  int *begin, *whole;                           // [batch]
+  int *hold, *first, *free_pages;               // large: [pages], [pages], [list]
+  int4* rows;                                   // large: [batch]
   int *source, *target, *tokens, *copies;       // copies to make, and their number
-};
-
-// What becomes of row b: the row that it continues (or -1), its length, and the tokens that it takes over.
-struct ForkRow {
-  int parent, after, kept;
 };
 
 __device__ __forceinline__ int held_pages(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
 
-__device__ __forceinline__ ForkRow fork_row(const PagesArgs& a, int b) {
-  ForkRow r{-1, 0, 0};
+__device__ __forceinline__ int row_length(const PagesArgs& a, int b) {
+  return min(max(a.lengths[b], 0), a.columns << a.page_shift);
+}
+
+// What becomes of row b: the row that it continues (or -1), its length, the tokens that it takes over, and the pages that
+// row b held.
+__device__ __forceinline__ int4 fork_row(const PagesArgs& a, int b) {
   const int p = a.parents == nullptr ? b : a.parents[b];
-  if ((uint32_t)p >= (uint32_t)a.batch) return r;
-  const int most = a.columns << a.page_shift, before = min(max(a.lengths[p], 0), most);
-  r.parent = p;
-  r.after = (int)min(max((int64_t)before + (a.counts == nullptr ? 0 : a.counts[b]), (int64_t)0), (int64_t)most);
-  r.kept = min(before, r.after);
-  return r;
+  const int own = row_length(a, b);
+  const int64_t count = a.counts == nullptr ? 0 : a.counts[b];
+  if ((uint32_t)p >= (uint32_t)a.batch) return make_int4(-1, 0, 0, held_pages(own, a.page_shift));
+  const int before = row_length(a, p);
+  const int after = (int)min(max(before + count, (int64_t)0), (int64_t)(a.columns << a.page_shift));
+  return make_int4(p, after, min(before, after), held_pages(own, a.page_shift));
 }
 
 // Whole pages that a row takes over are shared.  One that it takes over in part is going to be written: of the rows that
 // do so the first keeps it, if no row holds it whole and the program has no hold on it; the others get copies.  New pages
 // are the lowest free ones, in the order of the rows.
+//
+// One block: each phase needs all that the one before it counted, and a barrier costs less than a launch.  A wave takes a
+// row at a time, a lane a column.  Bound by latency.
+template <bool SMALL>
 __global__ __launch_bounds__(kPageThreads) void cache_fork_kernel(PagesArgs a) {
-  __shared__ int s_sums[kPageThreads / 64];
-  const int tid = threadIdx.x, entries = a.batch * a.columns, page = 1 << a.page_shift;
+  extern __shared__ __align__(16) int pages_lds[];
+  __shared__ int s_sums[kPageWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int shift = a.page_shift, page = 1 << shift;
+  int4* const rows = SMALL ? reinterpret_cast<int4*>(pages_lds) : a.rows;
+  int* const lds_pages = pages_lds + 4 * a.batch;
+  const Counters<SMALL> hold{SMALL ? lds_pages : a.hold}, first{SMALL ? lds_pages + a.pages : a.first};
+  // (the first rows of the pages are done with before the free ones are listed)
+  const Counters<SMALL> free_pages{SMALL ? lds_pages + a.pages : a.free_pages};
+  for (int b = tid; b < a.batch; b += kPageThreads) rows[b] = fork_row(a, b);
   for (int p = tid; p < a.pages; p += kPageThreads) {
-    put(a.hold + p, a.uses[p]);
-    put(a.first + p, a.batch);
+    hold.put(p, a.uses[p]);
+    first.put(p, a.batch);
   }
-  __threadfence();
-  __syncthreads();
+  phase<SMALL>();
   // Holds after the call: without the rows as they were, with the pages that rows keep whole.
-  for (int e = tid; e < entries; e += kPageThreads) {
-    const int b = e / a.columns, i = e - b * a.columns;
-    const int length = min(max(a.lengths[b], 0), a.columns << a.page_shift);
-    if (i < held_pages(length, a.page_shift)) {
-      const int p = a.table[b * a.table_row + i];
-      if ((uint32_t)p < (uint32_t)a.pages) atomicAdd(a.hold + p, -1);
-    }
-    const ForkRow r = fork_row(a, b);
-    const int from = i << a.page_shift;
-    if (from < r.kept) {
-      const int p = a.table[r.parent * a.table_row + i];
-      if ((uint32_t)p < (uint32_t)a.pages) {
-        if (from + page <= r.kept) atomicAdd(a.hold + p, 1);
-        else atomicMin(a.first + p, b);
+  constexpr int AHEAD = 4;  // rows whose entries are asked for at once
+  for (int b0 = wave; b0 < a.batch; b0 += AHEAD * kPageWaves)
+    for (int i = lane; i < a.columns; i += 64) {
+      int had[AHEAD], has[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        had[j] = has[j] = -1;
+        const int b = b0 + j * kPageWaves;
+        if (b >= a.batch) continue;
+        const int4 r = rows[b];
+        if (i < r.w) had[j] = a.table[b * a.table_row + i];
+        if (i << shift < r.z) has[j] = a.table[r.x * a.table_row + i];
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if ((uint32_t)had[j] < (uint32_t)a.pages) hold.add(had[j], -1);
+        if ((uint32_t)has[j] < (uint32_t)a.pages) {
+          const int b = b0 + j * kPageWaves;
+          if ((i << shift) + page <= rows[b].z) hold.add(has[j], 1);
+          else first.least(has[j], b);
+        }
       }
     }
-  }
-  __threadfence();
-  __syncthreads();
+  phase<SMALL>();
   int needed = 0, copies = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kPageThreads) {
     const int b = b0 + tid;
     int need = 0, whole = 0, p = -1;
-    ForkRow r{-1, 0, 0};
+    int4 r = make_int4(-1, 0, 0, 0);
     bool copy = false;
     if (b < a.batch) {
-      r = fork_row(a, b);
-      whole = held_pages(r.kept, a.page_shift);
-      if (r.kept & (page - 1)) {
-        p = a.table[r.parent * a.table_row + whole - 1];
+      r = rows[b];
+      whole = held_pages(r.z, shift);
+      if (r.z & (page - 1)) {
+        p = a.table[r.x * a.table_row + whole - 1];
         if ((uint32_t)p < (uint32_t)a.pages) {
           // (only the first row of a page may find it unheld, and it alone changes that)
-          if (fresh(a.first + p) == b && fresh(a.hold + p) == 0) put(a.hold + p, 1);
+          if (first.get(p) == b && hold.get(p) == 0) hold.put(p, 1);
           else copy = true;
         }
       }
       whole -= copy ? 1 : 0;
-      need = held_pages(r.after, a.page_shift) - whole;
+      need = held_pages(r.y, shift) - whole;
     }
-    int total;
-    const int before = block_scan(need, s_sums, total);
-    int copied;
+    int total, copied;
+    const int begin = needed + block_scan(need, s_sums, total);
     const int at = copies + block_scan(copy ? 1 : 0, s_sums, copied);
     if (b < a.batch) {
-      put(a.begin + b, needed + before);
-      put(a.whole + b, whole);
-      a.new_lengths[b] = r.after;
+      rows[b] = make_int4(r.x, r.y, whole, begin);
+      a.new_lengths[b] = r.y;
       if (copy) {
-        put(a.source + at, p);
-        put(a.target + at, needed + before);  // its rank among the new pages so far
-        put(a.tokens + at, r.kept & (page - 1));
+        a.source[at] = p;
+        a.tokens[at] = r.z & (page - 1);
+        a.target[at] = -1 - b;  // its first new page, once there is one
       }
     }
     needed += total;
     copies += copied;
   }
-  __threadfence();
-  __syncthreads();
+  phase<SMALL>();
   int found = 0;
-  for (int p0 = 0; p0 < a.pages; p0 += kPageThreads) {
-    const int p = p0 + tid;
-    const int hold = p < a.pages ? fresh(a.hold + p) : 1;
-    if (p < a.pages) put(a.new_uses + p, hold);
-    int total;
-    const int rank = found + block_scan(hold == 0 ? 1 : 0, s_sums, total);
-    if (hold == 0 && rank < min(needed, a.list)) put(a.free_pages + rank, p);
+  for (int p0 = 0; p0 < a.pages; p0 += kEach * kPageThreads) {
+    int held[kEach], open = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int p = p0 + kEach * tid + j;
+      held[j] = p < a.pages ? hold.get(p) : 1;
+      open += held[j] == 0 ? 1 : 0;
+    }
+    int total, rank = block_scan(open, s_sums, total) + found;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int p = p0 + kEach * tid + j;
+      if (p >= a.pages) continue;
+      int uses = held[j];
+      if (uses == 0) {
+        if (rank < min(needed, a.list)) {
+          free_pages.put(rank, p);
+          uses = 1;
+        }
+        ++rank;
+      }
+      a.new_uses[p] = uses;
+    }
     found += total;
   }
-  found = min(found, a.list);
-  __threadfence();
-  __syncthreads();
-  for (int e = tid; e < entries; e += kPageThreads) {
-    const int b = e / a.columns, i = e - b * a.columns;
-    const ForkRow r = fork_row(a, b);
-    const int whole = fresh(a.whole + b);
-    int p = -1;
-    if (i < whole) {
-      p = a.table[r.parent * a.table_row + i];
-    } else if (i < held_pages(r.after, a.page_shift)) {
-      const int rank = fresh(a.begin + b) + i - whole;
-      if (rank < found) {
-        p = fresh(a.free_pages + rank);
-        put(a.new_uses + p, 1);
+  found = min(found, min(needed, a.list));
+  phase<SMALL>();
+  for (int b0 = wave; b0 < a.batch; b0 += AHEAD * kPageWaves)
+    for (int i = lane; i < a.columns; i += 64) {
+      int p[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        p[j] = -1;
+        const int b = b0 + j * kPageWaves;
+        if (b >= a.batch) continue;
+        const int4 r = rows[b];
+        if (i < r.z) {
+          p[j] = a.table[r.x * a.table_row + i];
+        } else if (i < held_pages(r.y, shift)) {
+          const int rank = r.w + i - r.z;
+          if (rank < found) p[j] = free_pages.get(rank);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int b = b0 + j * kPageWaves;
+        if (b < a.batch) a.new_table[(int64_t)b * a.columns + i] = p[j];
       }
     }
-    a.new_table[e] = p;
-  }
-  for (int c = tid; c < copies; c += kPageThreads) {
-    const int rank = fresh(a.target + c);
-    put(a.target + c, rank < found ? fresh(a.free_pages + rank) : -1);
+  for (int c = tid; c < copies; c += kPageThreads) {  // (a barrier and more since they were written)
+    const int rank = rows[-1 - __hip_atomic_load(a.target + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)].w;
+    a.target[c] = rank < found ? free_pages.get(rank) : -1;
   }
   if (tid == 0) *a.copies = copies;
 }
 
 // The used pages numbered from their count on move to the free ones below it, both in order: the fewest moves, none of
 // which reads what another writes.
+template <bool SMALL>
 __global__ __launch_bounds__(kPageThreads) void cache_compact_kernel(PagesArgs a) {
-  __shared__ int s_sums[kPageThreads / 64];
-  const int tid = threadIdx.x, entries = a.batch * a.columns;
+  extern __shared__ __align__(16) int pages_lds[];
+  __shared__ int s_sums[kPageWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // The number that a page gets; and the pages that move, then where to.
+  const Counters<SMALL> number{SMALL ? pages_lds : a.first}, movers{SMALL ? pages_lds + a.pages : a.source};
+  const Counters<SMALL> holes{SMALL ? pages_lds + a.pages + a.pages / 2 : a.target};
   int used = 0;
   for (int p = tid; p < a.pages; p += kPageThreads) used += a.uses[p] > 0 ? 1 : 0;
   int total;
   block_scan(used, s_sums, total);
   used = total;
-  int from = 0, to = 0;
-  for (int p0 = 0; p0 < a.pages; p0 += kPageThreads) {
-    const int p = p0 + tid;
-    const bool is_used = p < a.pages && a.uses[p] > 0;
-    const bool moves = is_used && p >= used, fills = p < used && !is_used;
-    const int r = from + block_scan(moves ? 1 : 0, s_sums, total);
-    from += total;
-    const int s = to + block_scan(fills ? 1 : 0, s_sums, total);
-    to += total;
-    if (moves) put(a.source + r, p);
-    if (fills) put(a.target + s, p);
-    if (p < a.pages) {
-      put(a.new_uses + p, is_used && !moves ? a.uses[p] : 0);
-      put(a.first + p, p);
+  int moving = 0, filling = 0;
+  for (int p0 = 0; p0 < a.pages; p0 += kEach * kPageThreads) {
+    int uses[kEach], both = 0;  // moves in the upper half, holes in the lower
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int p = p0 + kEach * tid + j;
+      uses[j] = p < a.pages ? max(a.uses[p], 0) : 0;
+      both += (uses[j] > 0 && p >= used ? 1 << 16 : 0) + (p < used && uses[j] == 0 ? 1 : 0);
+    }
+    static_assert(kEach * kPageThreads < 1 << 15, "both counts fit");
+    const int before = block_scan(both, s_sums, total);
+    int r = moving + (before >> 16), s = filling + (before & 0xffff);
+    moving += total >> 16;
+    filling += total & 0xffff;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int p = p0 + kEach * tid + j;
+      if (p >= a.pages) continue;
+      const bool moves = uses[j] > 0 && p >= used;
+      if (moves) movers.put(r++, p);
+      else if (p < used && uses[j] == 0) holes.put(s++, p);
+      number.put(p, p);
+      if (moves || p >= used) a.new_uses[p] = 0;
+      else if (uses[j] > 0) a.new_uses[p] = uses[j];
     }
   }
-  __threadfence();
-  __syncthreads();
-  for (int r = tid; r < from; r += kPageThreads) {
-    const int p = fresh(a.source + r), q = fresh(a.target + r);
-    put(a.first + p, q);
-    put(a.new_uses + q, a.uses[p]);
-  }
-  __threadfence();
-  __syncthreads();
-  for (int e = tid; e < entries; e += kPageThreads) {
-    const int b = e / a.columns, i = e - b * a.columns;
-    const int length = min(max(a.lengths[b], 0), a.columns << a.page_shift);
-    int p = -1;
-    if (i < held_pages(length, a.page_shift)) {
-      p = a.table[b * a.table_row + i];
-      if ((uint32_t)p < (uint32_t)a.pages) p = fresh(a.first + p);
+  phase<SMALL>();
+  for (int r = tid; r < moving; r += kPageThreads) {
+    const int p = movers.get(r), q = holes.get(r);
+    number.put(p, q);
+    a.new_uses[q] = a.uses[p];
+    if constexpr (SMALL) {
+      a.source[r] = p;
+      a.target[r] = q;
     }
-    a.new_table[e] = p;
   }
-  if (tid == 0) *a.copies = from;
+  phase<SMALL>();
+  for (int b = wave; b < a.batch; b += kPageWaves) {
+    const int held = held_pages(row_length(a, b), a.page_shift);
+    for (int i = lane; i < a.columns; i += 64) {
+      int p = -1;
+      if (i < held) {
+        p = a.table[b * a.table_row + i];
+        if ((uint32_t)p < (uint32_t)a.pages) p = number.get(p);
+      }
+      a.new_table[(int64_t)b * a.columns + i] = p;
+    }
+  }
+  if (tid == 0) *a.copies = moving;
+}
+
+// One block, with `lds` bytes where that is enough for the counters.
+template <class K>
+static int launch_pages(const char* what, K small, K large, bool fits, int lds, const PagesArgs& a, std::atomic<uint64_t>& ready,
+                        hipStream_t stream) {
+  if (fits) {
+    int dev = 0;
+    TT_HIP(hipGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
+      TT_HIP(hipFuncSetAttribute((const void*)small, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                 16 * kSmallRows + 8 * kSmallPages));
+      ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(small, dim3(1), dim3(kPageThreads), lds, stream, a);
+  } else {
+    hipLaunchKernelGGL(large, dim3(1), dim3(kPageThreads), 0, stream, a);
+  }
+  return launch_status(what);
 }
 
 constexpr int kParts = 32;        // tensors of one launch
@@ -317,7 +410,7 @@ static int64_t pages_list(int64_t batch, int64_t columns, int64_t pages) {
 
 static int64_t pages_workspace(int64_t batch, int64_t columns, int64_t pages) {
   const int64_t copies = batch > pages / 2 ? batch : pages / 2;  // of a fork, and of a compaction
-  return 4 * (2 * pages + pages_list(batch, columns, pages) + 2 * batch + 3 * copies + 1);
+  return 4 * (4 * batch + 2 * pages + pages_list(batch, columns, pages) + 3 * copies + 1);
 }
 
 static int check_state(const char* what, int batch, int columns, int pages, int page_size) {
@@ -342,8 +435,8 @@ static PagesArgs pages_args(const C& c) {
     at += n;
     return p;
   };
+  a.rows = reinterpret_cast<int4*>(take(4 * (int64_t)c.batch));
   a.hold = take(c.pages), a.first = take(c.pages), a.free_pages = take(a.list);
-  a.begin = take(c.batch), a.whole = take(c.batch);
   a.source = take(copies), a.target = take(copies), a.tokens = take(copies), a.copies = take(1);
   return a;
 }
@@ -363,15 +456,17 @@ extern "C" int tt_cache_fork(const tt_cache_fork_pages* args, void* stream) {
   TT_ARGS(tt_cache_fork_pages, "cache_fork");
   TT_CHECK(check_state("cache_fork", c.batch, c.columns, c.pages, c.page_size));
   TT_CHECK(check_parts("cache_fork", c.parts, c.part_count, c.pages));
-  TT_REQUIRE(c.uses && c.new_uses && c.workspace && ((uintptr_t)c.workspace & 3) == 0 &&
+  TT_REQUIRE(c.uses && c.new_uses && c.workspace && ((uintptr_t)c.workspace & 15) == 0 &&
                  c.workspace_bytes >= pages_workspace(c.batch, c.columns, c.pages),
              "cache_fork: null pointer, or a workspace of %lld bytes", (long long)c.workspace_bytes);
   TT_REQUIRE(c.batch == 0 || (c.table && c.lengths && c.new_table && c.new_lengths && c.table_row >= 0),
              "cache_fork: null pointer, or table_row %lld", (long long)c.table_row);
   PagesArgs a = pages_args(c);
   a.parents = c.parents, a.counts = c.counts, a.new_lengths = c.new_lengths;
-  hipLaunchKernelGGL(cache_fork_kernel, dim3(1), dim3(kPageThreads), 0, (hipStream_t)stream, a);
-  TT_CHECK(launch_status("cache_fork_kernel"));
+  static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic LDS is raised
+  TT_CHECK(launch_pages("cache_fork_kernel", cache_fork_kernel<true>, cache_fork_kernel<false>,
+                        c.pages <= kSmallPages && c.batch <= kSmallRows, 16 * c.batch + 8 * c.pages, a, ready,
+                        (hipStream_t)stream));
   if (c.batch == 0) return TT_OK;
   return launch_copies(c.parts, c.part_count, a.source, a.target, a.tokens, a.copies, c.batch, c.pages, c.page_size,
                        (hipStream_t)stream);
@@ -382,14 +477,15 @@ extern "C" int tt_cache_compact(const tt_cache_compact_pages* args, void* stream
   TT_ARGS(tt_cache_compact_pages, "cache_compact");
   TT_CHECK(check_state("cache_compact", c.batch, c.columns, c.pages, c.page_size));
   TT_CHECK(check_parts("cache_compact", c.parts, c.part_count, c.pages));
-  TT_REQUIRE(c.uses && c.new_uses && c.workspace && ((uintptr_t)c.workspace & 3) == 0 &&
+  TT_REQUIRE(c.uses && c.new_uses && c.workspace && ((uintptr_t)c.workspace & 15) == 0 &&
                  c.workspace_bytes >= pages_workspace(c.batch, c.columns, c.pages),
              "cache_compact: null pointer, or a workspace of %lld bytes", (long long)c.workspace_bytes);
   TT_REQUIRE(c.batch == 0 || (c.table && c.lengths && c.new_table && c.table_row >= 0),
              "cache_compact: null pointer, or table_row %lld", (long long)c.table_row);
   const PagesArgs a = pages_args(c);
-  hipLaunchKernelGGL(cache_compact_kernel, dim3(1), dim3(kPageThreads), 0, (hipStream_t)stream, a);
-  TT_CHECK(launch_status("cache_compact_kernel"));
+  static std::atomic<uint64_t> ready{0};
+  TT_CHECK(launch_pages("cache_compact_kernel", cache_compact_kernel<true>, cache_compact_kernel<false>,
+                        c.pages <= kSmallPages, 8 * c.pages, a, ready, (hipStream_t)stream));
   if (c.pages < 2) return TT_OK;
   return launch_copies(c.parts, c.part_count, a.source, a.target, nullptr, a.copies, c.pages / 2, c.pages, c.page_size,
                        (hipStream_t)stream);
