@@ -271,9 +271,10 @@ int launch_seq_attention(const SeqAttnArgs& a, bool paged, SeqShape shape, int d
 }
 
 // Blocks of a kernel that a CU holds (its registers, and its LDS: 16, 32, 64 or 128 KiB and a little more each).
-static int seq_resident(bool wide, int head_dim, bool bytes) {
+static int seq_resident(bool wide, int head_dim, int bytes) {
   if (wide) return head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1;
-  if (bytes) return head_dim <= 64 ? 6 : 4;  // half the LDS: its registers
+  if (bytes > 1) return head_dim <= 64 && bytes == 2 ? 4 : 2;
+  if (bytes) return head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 4;
   return head_dim <= 32 ? 6 : head_dim <= 64 ? 4 : 2;
 }
 
@@ -287,9 +288,9 @@ struct SeqPlan {
   bool many_parts;
 };
 
-// max_length < 0: packed sequences (no keys but their own).
+// max_length < 0: packed sequences (no keys but their own).  bytes: over an 8-bit cache, the heads that share a narrow block.
 static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int head_dim, int64_t held, int max_length,
-                        bool single, bool bytes = false) {
+                        bool single, int bytes = 0) {
   SeqPlan p{};
   const int64_t G = heads / kv_heads;
   const int cus = device_cus();
@@ -314,7 +315,11 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   // from 1 to 4000 39 -> 32; 512 of two waves on heads of 128, 1000 keys (16) 43 -> 47, lengths to 4000 125 -> 107; 512 of
   // one wave on heads of 256, 700 keys (22) 66 -> 69, lengths to 700 43.3 -> 42.5, to 1020 60 -> 54; 300 of one, 700 keys
   // 42 -> 49, lengths to 700 40 -> 34.
-  const int keys_per_round = wide ? 64 : 32 * seq_waves(p.shape, head_dim);
+  const int keys_per_round = wide    ? 64
+                             : bytes ? seq8_keys(head_dim) * (p.shape == SeqShape::kNarrow && bytes > 1
+                                                                  ? 1
+                                                                  : seq8_waves(p.shape, head_dim))
+                                     : 32 * seq_waves(p.shape, head_dim);
   const int alone = (blocks <= cus / 4 ? 6 : 16) * keys_per_round;
   // Beyond the blocks that the chip holds (four times as many of 32 rows), tiles spread by themselves: 1088 tiles of 128
   // rows over 500 to 4600 keys, 195 alone and 272 in shares; 800 of 32 rows over 1 to 4000 keys, 193 and 162.
@@ -323,7 +328,7 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
     p.mode = kSeqShares;
     if (!wide) p.shape = SeqShape::kNarrow;
     const int64_t units = tiles * ((max_length + kSeqUnit - 1) / kSeqUnit + kSeqTileCost);
-    int64_t slots = held_blocks / kv_heads;
+    int64_t slots = held_blocks / (!wide && bytes > 1 ? kv_heads / bytes : kv_heads);
     if (slots > (units + kSeqMinShare - 1) / kSeqMinShare) slots = (units + kSeqMinShare - 1) / kSeqMinShare;
     p.slots = (int)(slots > 1 ? slots : 1);
     p.part_rows = 2 * (int64_t)p.slots * kv_heads * p.rows;
@@ -372,8 +377,14 @@ static int workspace_bytes(const char* what, bool bytes_cache, int tokens, int b
   TT_REQUIRE(max_length >= 0 && bytes != nullptr, "%s: max_length %d", what, max_length);
   *bytes = 0;
   if (tokens == 0 || batch == 0) return TT_OK;
-  *bytes = 4 * (head_dim + 2) * seq_plan(tokens, batch, heads, kv_heads, head_dim, (int64_t)page_size * table_pages,
-                                         max_length, single != 0, bytes_cache).part_rows;
+  // (which heads lie side by side is not known here: the most that either needs)
+  for (int side_by_side = 0; side_by_side < (bytes_cache ? 2 : 1); ++side_by_side) {
+    const int shared = !bytes_cache ? 0 : side_by_side ? seq8_heads(head_dim, kv_heads, head_dim, head_dim) : 1;
+    const int64_t need = 4 * (head_dim + 2) * seq_plan(tokens, batch, heads, kv_heads, head_dim,
+                                                       (int64_t)page_size * table_pages, max_length, single != 0,
+                                                       shared).part_rows;
+    if (need > *bytes) *bytes = need;
+  }
   return TT_OK;
 }
 
@@ -397,7 +408,8 @@ static int check_cache_attention(const char* what, const C& c) {
 template <class C>
 static int run_cache_attention(const char* what, const C& c, SeqAttnArgs& a, bool bytes_cache, hipStream_t stream) {
   const SeqPlan p = seq_plan(c.tokens, c.batch, c.heads, c.kv_heads, c.head_dim, (int64_t)c.page_size * c.table_pages,
-                             c.max_length, c.starts == nullptr, bytes_cache);
+                             c.max_length, c.starts == nullptr,
+                             bytes_cache ? seq8_heads(c.head_dim, c.kv_heads, c.k_head, c.v_head) : 0);
   const int64_t bytes = 4 * (c.head_dim + 2) * p.part_rows;
   TT_REQUIRE(bytes == 0 || (c.workspace != nullptr && c.workspace_bytes >= bytes && ((uintptr_t)c.workspace & 15) == 0),
              "%s: a workspace of %lld bytes is needed, %lld given", what, (long long)bytes, (long long)c.workspace_bytes);

@@ -393,9 +393,9 @@ __device__ __forceinline__ SeqShare seq_share(const SeqAttnArgs& a, int slot, in
   }
 }
 
-template <typename T, int HD, int RW, int KW, int KT, bool PAGED, bool C8 = false,
-          int WPE = (HD <= 64 ? 3 : HD <= 128 ? 2 : 1)>
-__global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void seq_attention_kernel(SeqAttnArgs a) {
+template <typename T, int HD, int RW, int KW, int KT, bool PAGED, bool C8 = false, int NH = 1,
+          int WPE = C8 && RW == 1 ? (HD <= 64 ? 2 : 1) : (HD <= 64 ? 3 : HD <= 128 ? 2 : 1)>
+__global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void seq_attention_kernel(SeqAttnArgs a) {
   using v2 = typename Num<T>::v2;
   using v8 = typename Num<T>::v8;
   constexpr int R = 32 * RW;                // rows of a block (64 a wave leave registers for one wave per SIMD only)
@@ -404,29 +404,36 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   constexpr int DB = HD / 32;               // 32-row blocks of O^T
   constexpr int CH = HD / 8;                // 16-byte chunks of a row of T
   constexpr int RPC = 64 / CH;              // rows of T in 1 KiB
-  // An 8-bit cache's tiles: wide blocks widen them to T on their way into LDS, each row once for all waves; narrow ones
-  // copy their bytes, and a wave widens the fragments that it reads.
+  // An 8-bit cache's tiles: narrow blocks copy their bytes, and a wave widens the fragments that it reads.  In wide ones each
+  // row is widened once for all waves: its bytes are copied to a place of the wave's own behind the tiles, and from there
+  // they go through registers into the tile as T, once its copies have landed.  (Loaded into registers they would be in
+  // flight there while the tile before is worked on, 16 registers more than there are: 208 us for 8 chunks of 512.)
   constexpr bool RAW = C8 && !PIPE;
   using E = std::conditional_t<RAW, uint8_t, T>;
   constexpr int EB = C8 ? 1 : 2;            // bytes of a value in memory
-  constexpr int CB = HD * EB / 16;          // 16-byte chunks of a row in memory
+  // NH waves of a block over an 8-bit cache share its tiles, each for a head of its own: HD bytes are less than memory is
+  // best read in.
+  static_assert(NH == 1 || (RAW && KW == 1), "heads side by side");
+  constexpr int ROW = NH * HD;              // values of a row of a tile
+  constexpr int CB = ROW * EB / 16;         // 16-byte chunks of a row in memory
   constexpr int RPB = 64 / CB;              // rows per 1 KiB copy
-  constexpr int WROWS = KT / RW;            // rows of a tile that one wave copies
+  constexpr int WROWS = KT / (RW * NH);     // rows of a tile that one wave copies
   constexpr int PG = WROWS / 16;            // ... in groups of 16, each of which lies in one page
   constexpr int CPG = 16 / RPB;             // copies per group
-  constexpr int TILE = KT * HD;
+  constexpr int TILE = KT * ROW;
   static_assert(WROWS % 16 == 0 && RPB <= 16, "a wave copies whole 16-row groups");
   static_assert(!C8 || (PAGED && HD >= 64), "8 bits: a cache");
 
   extern __shared__ __align__(512) char seq_lds[];
 
-  const int hkv = blockIdx.x % a.kv_heads;
-  const int slot = blockIdx.x / a.kv_heads;
+  const int slot = blockIdx.x / (a.kv_heads / NH);
   const int G = a.group;
   const int tid = threadIdx.x;
   int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rw = RW == 1 ? 0 : wave % RW, grp = RW == 1 ? wave : wave / RW;
+  const int rw = RW == 1 ? 0 : wave % RW, grp = NH > 1 ? 0 : RW == 1 ? wave : wave / RW;
+  const int hw = NH > 1 ? wave : 0, cw = NH > 1 ? hw : rw;  // this wave's head of the block's; its rows of a copied tile
+  const int hkv0 = blockIdx.x % (a.kv_heads / NH) * NH, hkv = hkv0 + hw;
   int hf = lane >> 5, col = lane & 31;
   E* const sk = reinterpret_cast<E*>(seq_lds) + (size_t)grp * 2 * TILE;
   E* const sv = reinterpret_cast<E*>(seq_lds) + (size_t)KW * 2 * TILE + (size_t)grp * 2 * TILE;
@@ -459,15 +466,21 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   for (int c = 0; c < CPG; ++c) {
     const int row = c * RPB + lane / CB;
     int kc = lane % CB, vc = lane % CB;
-    if constexpr (RAW) kc = kswz8<HD>(row, kc) * 16, vc = vseg8<HD>(row, vc) * 16;
+    if constexpr (RAW) kc = kswz8<ROW>(row, kc) * 16, vc = vseg8<ROW>(row, vc) * 16;
     else if constexpr (C8) kc *= 16, vc *= 16;
     else kc = kswz<HD>(row, kc) * 8, vc = vseg<HD>(row, vc) * 8;
+    if constexpr (NH > 1) {  // head_dim values of each head
+      const int k_at = kc / HD * (int)a.k_head + kc % HD, v_at = vc / HD * (int)a.v_head + vc % HD;
+      koff[c] = kc % HD < hd ? (uint32_t)(row * (int)a.k_row + k_at) : 0x80000000u;
+      voff[c] = vc % HD < hd ? (uint32_t)(row * (int)a.v_row + v_at) : 0x80000000u;
+      continue;
+    }
     koff[c] = kc < hd ? (uint32_t)(row * (int)a.k_row + kc) * EB : 0x80000000u;
     voff[c] = vc < hd ? (uint32_t)(row * (int)a.v_row + vc) * EB : 0x80000000u;
   }
   using Mem = std::conditional_t<C8, uint8_t, T>;
-  const Mem* const kh = static_cast<const Mem*>(a.k) + hkv * a.k_head;
-  const Mem* const vh = static_cast<const Mem*>(a.v) + hkv * a.v_head;
+  const Mem* const kh = static_cast<const Mem*>(a.k) + hkv0 * a.k_head;
+  const Mem* const vh = static_cast<const Mem*>(a.v) + hkv0 * a.v_head;
 
   const float c2 = a.scale_log2, lazy = kSeqLazy / a.scale_log2;
   // LDS addresses of this lane's pieces of the first K and V block of a stage; the others lie at constant distances.
@@ -478,7 +491,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   uint32_t kread[KA], vread[VA];
 #pragma unroll
   for (int kk = 0; kk < KA; ++kk) {
-    if constexpr (RAW) kread[kk] = lds_address(sk + col * HD + kswz8<HD>(col, 2 * kk + hf) * 16);
+    if constexpr (RAW) kread[kk] = lds_address(sk + col * ROW + kswz8<ROW>(col, hw * HD / 16 + 2 * kk + hf) * 16);
     else kread[kk] = lds_address(sk + col * HD + kswz<HD>(col, 2 * kk + hf) * 8);
     asm volatile("" : "+v"(kread[kk]));
   }
@@ -487,7 +500,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
 #pragma unroll
   for (int i = 0; i < VA; ++i) {
     if constexpr (RAW) {
-      vread[i] = lds_address(sv + vrow * HD + vseg8<HD>(vrow, 2 * i + ((lane >> 4) & 1)) * 16 + 8 * (lane & 1));
+      const int c = hw * HD / 16 + 2 * i + ((lane >> 4) & 1);
+      vread[i] = lds_address(sv + vrow * ROW + vseg8<ROW>(vrow, c) * 16 + 8 * (lane & 1));
     } else {
       const int c = vseg<HD>(vrow, 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1));
       vread[i] = lds_address(sv + vrow * HD + c * 8 + 4 * (lane & 1));
@@ -498,7 +512,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   // (What follows from these is worked out again for each tile instead of being held in registers throughout.)
   asm volatile("" : "+v"(lane), "+v"(hf), "+v"(col));
   if (hd < HD) {  // the tile before left its sums or rows there
-    for (int e = tid; e < 4 * KW * TILE * (int)sizeof(E) / 16; e += 64 * RW * KW)
+    constexpr int BEHIND = C8 && PIPE ? RW * 2 * CPG * 1024 : 0;  // bytes on their way into the tiles
+    for (int e = tid; e < (4 * KW * TILE * (int)sizeof(E) + BEHIND) / 16; e += 64 * RW * KW * NH)
       reinterpret_cast<u32x4*>(seq_lds)[e] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
@@ -548,20 +563,23 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
   auto bad_groups = [&](int pe, int t0) TT_INLINE -> uint32_t {
     return (uint32_t)__ballot((uint32_t)pe >= (uint32_t)a.pages && t0 + 16 * lane < keys) & 0xffu;
   };
-  // 8 bits: the scales of those groups, K's in the low byte and V's above it (blocks of tokens hold whole groups).  A
-  // group one of whose scales is none (255) counts as one outside the cache; its V is multiplied by 2^-127.
-  auto tile_scales = [&](int pe, int t0) TT_INLINE -> int {
+  // 8 bits: the scales of those groups (blocks of tokens hold whole groups), as they are loaded: whatever is done with them
+  // waits for them.  A group one of whose scales is none (255) counts as one outside the cache; its V is multiplied by
+  // 2^-127.
+  struct Scales {
+    uint32_t k, v;
+  };
+  auto tile_scales = [&](int pe, int t0) TT_INLINE -> Scales {
     const uint32_t in = min(t0 + 16 * (lane & 7), max(keys - 1, 0)) & ((1 << a.page_shift) - 1);
     const uint32_t page = (uint32_t)pe < (uint32_t)a.pages ? pe : 0, block = in >> a.block_shift;
-    const int k = a.k_scale[page * (uint64_t)a.ks_page + block * (uint64_t)a.ks_block + hkv * a.ks_head];
-    const int v = a.v_scale[page * (uint64_t)a.vs_page + block * (uint64_t)a.vs_block + hkv * a.vs_head];
-    return v << 8 | k;
+    return Scales{a.k_scale[page * (uint64_t)a.ks_page + block * (uint64_t)a.ks_block + hkv * a.ks_head],
+                  a.v_scale[page * (uint64_t)a.vs_page + block * (uint64_t)a.vs_block + hkv * a.vs_head]};
   };
-  auto bad_scales = [&](int se, int t0) TT_INLINE -> uint32_t {
-    return (uint32_t)__ballot(((se & 255) == 255 || se >> 8 == 255) && t0 + 16 * lane < keys) & 0xffu;
+  auto bad_scales = [&](const Scales& se, int t0) TT_INLINE -> uint32_t {
+    return (uint32_t)__ballot((se.k == 255 || se.v == 255) && t0 + 16 * lane < keys) & 0xffu;
   };
-  auto scale_of = [&](int se, int group, bool is_k) TT_INLINE -> float {
-    const uint32_t e = (__builtin_amdgcn_readlane(se, group) >> (is_k ? 0 : 8)) & 255;
+  auto scale_of = [&](const Scales& se, int group, bool is_k) TT_INLINE -> float {
+    const uint32_t e = __builtin_amdgcn_readlane(is_k ? se.k : se.v, group);
     return e8m0(e == 255 ? 0 : e);
   };
   // Where those groups lie in K and V (bytes), and how many bytes there belong to keys; worked out by the lanes for
@@ -583,69 +601,72 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       p.k = 2 * (row * (uint64_t)a.k_row);
       p.v = 2 * (row * (uint64_t)a.v_row);
     }
-    p.k_bytes = n == 0 ? 0 : EB * ((n - 1) * (uint32_t)a.k_row + hd);
-    p.v_bytes = n == 0 ? 0 : EB * ((n - 1) * (uint32_t)a.v_row + hd);
+    p.k_bytes = n == 0 ? 0 : EB * ((n - 1) * (uint32_t)a.k_row + (NH - 1) * (uint32_t)a.k_head + hd);
+    p.v_bytes = n == 0 ? 0 : EB * ((n - 1) * (uint32_t)a.v_row + (NH - 1) * (uint32_t)a.v_head + hd);
     return p;
   };
   auto places = [&](int pe, int t0) TT_INLINE -> Places {
     if constexpr (PAGED) return place(t0 + 16 * (lane & 7), pe);
     else return Places{(uint64_t)t0, 0, 0, 0};
   };
-  // Copies of this wave's rows of a K (V) tile whose first 16 keys are group `group` of `at` (wide blocks, 8 bits: into
-  // registers, from where write_half takes them into LDS).
-  using Staged = u32x4[C8 && PIPE ? CPG : 1];
-  auto issue_half = [&](bool is_k, const Places& at, E* tile, int group, Staged& staged) TT_INLINE {
+  // Copies of this wave's rows of a K (V) tile whose first 16 keys are group `group` of `at`, to `tile` (wide blocks, 8
+  // bits: their bytes to `bytes`, from where write_half takes them into the tile).
+  auto issue_half = [&](bool is_k, const Places& at, E* tile, int group, char* bytes = nullptr) TT_INLINE {
 #pragma unroll
     for (int p = 0; p < PG; ++p) {
-      const int g = rw * PG + p;
+      const int g = cw * PG + p;
       if (group + g < 0) continue;
       uint64_t where;
-      uint32_t bytes;
+      uint32_t size;
       if constexpr (PAGED) {
         const uint64_t w = is_k ? at.k : at.v;
         where = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), group + g) << 32 |
                 (uint32_t)__builtin_amdgcn_readlane((int)w, group + g);
-        bytes = __builtin_amdgcn_readlane((int)(is_k ? at.k_bytes : at.v_bytes), group + g);
+        size = __builtin_amdgcn_readlane((int)(is_k ? at.k_bytes : at.v_bytes), group + g);
       } else {
         const Places q = place((int)at.k + 16 * (group + g), 0);
         where = is_k ? q.k : q.v;
-        bytes = is_k ? q.k_bytes : q.v_bytes;
+        size = is_k ? q.k_bytes : q.v_bytes;
       }
-      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(reinterpret_cast<const char*>(is_k ? kh : vh) + where, bytes);
-      if constexpr (C8 && PIPE) {
+      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(reinterpret_cast<const char*>(is_k ? kh : vh) + where, size);
 #pragma unroll
-        for (int c = 0; c < CPG; ++c) staged[c] = load16<kLoadDefault>(r, is_k ? koff[c] : voff[c]);
-      } else {
-#pragma unroll
-        for (int c = 0; c < CPG; ++c)
-          lds_copy16_buf(r, is_k ? koff[c] : voff[c], reinterpret_cast<half*>(tile + (g * 16 + c * RPB) * HD));
+      for (int c = 0; c < CPG; ++c) {
+        half* const to = reinterpret_cast<half*>(tile + (g * 16 + c * RPB) * ROW);
+        lds_copy16_buf(r, is_k ? koff[c] : voff[c], C8 && PIPE ? reinterpret_cast<half*>(bytes + c * 1024) : to);
       }
     }
   };
-  auto write_half = [&](bool is_k, int se, E* tile, int group, const Staged& staged) TT_INLINE {
+  char* const k_bytes = seq_lds + 4 * TILE * sizeof(T) + (size_t)rw * 2 * CPG * 1024;  // wide, 8 bits
+  char* const v_bytes = k_bytes + CPG * 1024;
+  using Bytes = u32x4[CPG];
+  auto read_bytes = [&](Bytes& x, const char* bytes) TT_INLINE {
+#pragma unroll
+    for (int c = 0; c < CPG; ++c) x[c] = *reinterpret_cast<const u32x4*>(bytes + c * 1024 + lane * 16);
+  };
+  auto write_half = [&](bool is_k, const Scales& se, E* tile, int group, const Bytes& x) TT_INLINE {
     if constexpr (C8 && PIPE) {
       static_assert(PG == 1, "a group per wave");
-      if (group + rw < 0) return;
+      if (group < 0 && group + rw < 0) return;
       const float scale = scale_of(se, group + rw, is_k);
 #pragma unroll
       for (int c = 0; c < CPG; ++c) {
         const int row = rw * 16 + c * RPB + lane / CB, chunk = 2 * (lane % CB);
         T* const to = tile + row * HD;
         const int at = is_k ? kswz<HD>(row, chunk) : vseg<HD>(row, chunk);  // the next chunk lies beside it
-        const u32x4 x = staged[c];
-        *reinterpret_cast<u32x4*>(to + at * 8) = widen8<T>(u32x2{x[0], x[1]}, scale);
-        *reinterpret_cast<u32x4*>(to + (at ^ 1) * 8) = widen8<T>(u32x2{x[2], x[3]}, scale);
+        *reinterpret_cast<u32x4*>(to + at * 8) = widen8<T>(u32x2{x[c][0], x[c][1]}, scale);
+        *reinterpret_cast<u32x4*>(to + (at ^ 1) * 8) = widen8<T>(u32x2{x[c][2], x[c][3]}, scale);
       }
     }
   };
-  Staged k_staged, v_staged;
+  // Whether a tile's bytes are widened beside the products of the last step before it (heads above 128: after it).
+  constexpr bool BESIDE = C8 && PIPE && !FAR;
   // The K tile staged with a V tile begins KLEAD keys later: the scores run that far ahead.
   constexpr int KLEAD = PIPE ? 32 : 0;
   auto issue_k = [&](const Places& p, int st) TT_INLINE {
-    issue_half(true, p, sk + st * TILE, KLEAD / 16, k_staged);
+    issue_half(true, p, sk + st * TILE, KLEAD / 16, k_bytes);
   };
   auto issue_v = [&](const Places& p, int st) TT_INLINE {
-    issue_half(false, p, sv + st * TILE, 0, v_staged);
+    issue_half(false, p, sv + st * TILE, 0, v_bytes);
   };
   // After the copies of this wave's V rows have landed: rows of keys behind the last that any row of the block sees are
   // cleared (0 times whatever lay there would not be 0), and where some rows of the block see keys that others do not,
@@ -657,31 +678,19 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     constexpr uint32_t kCarry = (0x8000u - Num<T>::kExp) * 0x10001u;  // an exponent of ones carries into the sign
     return (((x & 0x7fff7fffu) + kCarry) >> 15) & 0x10001u;
   };
-  constexpr int CL = HD * (int)sizeof(E) / 16;  // chunks of a row in LDS
-  auto settle_v = [&](int t0, int st, int se) TT_INLINE {
+  auto settle_v = [&](int t0, int st) TT_INLINE {
     const int g0 = rw * WROWS;
     u32x4* const tile = reinterpret_cast<u32x4*>(sv + st * TILE + g0 * HD);
     const int n = min(max(kend - (t0 + g0), 0), WROWS);
     if (mixed && t0 + KT > block_lo) {
-      for (int e = lane; e < n * CL; e += 64) {
+      for (int e = lane; e < n * CH; e += 64) {
         u32x4 x = tile[e];
         uint32_t any = 0;
-        uint32_t carry = 0;  // RAW: takes a byte that is no number, or too large, to 128 and above
-        if constexpr (RAW) {
-          const int v0 = __builtin_amdgcn_readlane(se, 0) >> 8, v1 = __builtin_amdgcn_readlane(se, 1) >> 8;
-          carry = (0x80 - widen_limit<T>(e / CL < 16 ? v0 : v1)) * 0x01010101u;
-        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if constexpr (RAW) {
-            const uint32_t m = (((x[i] & 0x7f7f7f7fu) + carry) >> 7) & 0x01010101u;
-            any |= m;
-            x[i] &= ~(m * 0xffu);
-          } else {
-            const uint32_t m = odd_pair(x[i]);
-            any |= m;
-            x[i] &= ~(m * 0xffffu);
-          }
+          const uint32_t m = odd_pair(x[i]);
+          any |= m;
+          x[i] &= ~(m * 0xffffu);
         }
         if (any != 0) {
           tile[e] = x;
@@ -690,19 +699,35 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       }
     }
     if (n < WROWS)
-      for (int e = n * CL + lane; e < WROWS * CL; e += 64) tile[e] = u32x4{0u, 0u, 0u, 0u};
+      for (int e = n * CH + lane; e < WROWS * CH; e += 64) tile[e] = u32x4{0u, 0u, 0u, 0u};
     lds_done();
   };
-  auto land_v = [&](int t0, int st, int se) TT_INLINE {
-    if constexpr (C8 && PIPE) {
-      write_half(true, se, sk + st * TILE, KLEAD / 16, k_staged);
-      write_half(false, se, sv + st * TILE, 0, v_staged);
-      lds_done();
-    } else {
-      __builtin_amdgcn_s_waitcnt(0);
-      asm volatile("" ::: "memory");
+  // The same for the bytes of 16 keys of V from t0 on that a lane holds, with their scale: those that are no number in T.
+  auto settle_bytes = [&](u32x2& x, int t0, uint32_t scale) TT_INLINE {
+    const uint32_t carry = (0x80 - widen_limit<T>(scale)) * 0x01010101u;  // takes a byte that is none to 128 and above
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (mixed && t0 + 16 > block_lo) {
+        const uint32_t m = (((x[i] & 0x7f7f7f7fu) + carry) >> 7) & 0x01010101u;
+        odd |= m != 0;
+        x[i] &= ~(m * 0xffu);
+      }
+      const int n = min(max(kend - (t0 + 8 * i + 4 * hf), 0), 4);  // keys before the end
+      x[i] &= n == 4 ? ~0u : (1u << (8 * n)) - 1;
     }
-    settle_v(t0, st, se);
+  };
+  auto land_v = [&](int t0, int st, const Scales& se, bool written = false) TT_INLINE {
+    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("" ::: "memory");
+    if (C8 && PIPE && !written) {
+      Bytes x;
+      read_bytes(x, k_bytes);
+      write_half(true, se, sk + st * TILE, KLEAD / 16, x);
+      read_bytes(x, v_bytes);
+      write_half(false, se, sv + st * TILE, 0, x);
+      lds_done();
+    }
+    settle_v(t0, st);
     if constexpr (RW > 1) raw_barrier();
   };
 
@@ -767,11 +792,11 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     return __builtin_bit_cast(v8, shortx8{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]});
   };
   // RAW: features 32 j + 16 hf + {0..15} of key l % 32; and features 32 i + l % 32 of the keys as above.
-  auto read_kb = [&](int j, int st) TT_INLINE -> u32x4 {
-    return *(const __attribute__((address_space(3))) u32x4*)(kread[j] + st * TILE);
+  auto read_kb = [&](int j, int st, int kb) TT_INLINE -> u32x4 {
+    return *(const __attribute__((address_space(3))) u32x4*)(kread[j] + st * TILE + kb * 32 * ROW);
   };
   auto read_vb = [&](int i, int st, int kc) TT_INLINE -> u32x2 {
-    return read_tr8((const lds_short*)(vread[i] + st * TILE + kc * 16 * HD));
+    return read_tr8((const lds_short*)(vread[i] + st * TILE + kc * 16 * ROW));
   };
   // FAR: one wave per SIMD, so nothing else runs while it waits for a fragment.  Fragments are read four products
   // before theirs (read just before, as registers are too few for the compiler to do otherwise by itself, prompts of
@@ -877,10 +902,10 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       static_assert(KW == 1 && KT == 64, "two steps of 32 keys per tile");
       const int steps = wave_active && lim_hi > kbeg ? (lim_hi - kbeg + 31) / 32 : 0;  // of this wave
       int pe = 0, pe_next = 0;  // pages from this tile's and the next tile's first key on
-      int se = 0;               // 8 bits: the scales there
-      Staged k_first;
+      Scales se{0, 0};          // 8 bits: the scales there
       Scores sa, sb;
       float mt;
+      char* const k_first = reinterpret_cast<char*>(sv + TILE) + rw * CPG * 1024;
       if (ntiles > 0) {
         if constexpr (PAGED) {
           pe = tile_pages(kbeg);
@@ -889,15 +914,22 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         const Places at = places(pe, kbeg);
         if constexpr (C8) se = tile_scales(pe, kbeg);
         // the first 32 keys go where the second half of a K tile before the first would lie
+        // (8 bits: by way of the second V tile's place)
         issue_half(true, at, sk + TILE, -2, k_first);
         issue_k(at, 0);
         issue_v(at, 0);
       }
       load_q();
-      if (!C8 || ntiles > 0) {
-        write_half(true, se, sk + TILE, -2, k_first);
-        land_v(kbeg, 0, se);
+      if constexpr (C8) {
+        __builtin_amdgcn_s_waitcnt(0);
+        asm volatile("" ::: "memory");
+        if (ntiles > 0) {
+          Bytes x;
+          read_bytes(x, k_first);
+          write_half(true, se, sk + TILE, -2, x);
+        }
       }
+      land_v(kbeg, 0, se);
       if (steps > 0) {
         scores(sa, 1, 1);
         uint32_t bad = PAGED ? bad_groups(pe, kbeg) : 0;
@@ -910,7 +942,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       raw_barrier();  // the second tile's copies go where those first 32 keys lie
       // A step of 32 keys: the exps of its scores s run beside the products of the next 32 keys, and its P V beside
       // their maximum.
-      auto step = [&](int t0, int st, int h, uint32_t bad, Scores& s, Scores& sn) TT_INLINE {
+      auto step = [&](int t0, int st, int h, uint32_t bad, Scores& s, Scores& sn, bool widen = false) TT_INLINE {
         Probs p16;
         __builtin_amdgcn_sched_barrier(0);
         scores(sn, st, h);
@@ -919,8 +951,18 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         __builtin_amdgcn_sched_barrier(0);
         mask_scores(sn, t0 + 32 * (h + 1), bad >> (2 * h + 2));
         __builtin_amdgcn_s_setprio(1);  // (prompts take 1 to 3% longer without)
+        Bytes kx, vx;  // of the next tile; what held the scores has room for them
+        if (widen) {
+          wait_vmcnt<0>();
+          read_bytes(kx, k_bytes);
+          read_bytes(vx, v_bytes);
+        }
         add_sums(p16);
         add_values(p16, st, h);
+        if (widen) {
+          write_half(true, se, sk + (st ^ 1) * TILE, KLEAD / 16, kx);
+          write_half(false, se, sv + (st ^ 1) * TILE, 0, vx);
+        }
         mt = row_max(sn);
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(0);
@@ -976,8 +1018,8 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         const int t0 = kbeg + r * KT;
         fetch(r, st);
         step(t0, st, 0, bad, sa, sb);
-        step(t0, st, 1, bad, sb, sa);
-        land_v(t0 + KT, st ^ 1, se);
+        step(t0, st, 1, bad, sb, sa, BESIDE);
+        land_v(t0 + KT, st ^ 1, se, BESIDE);
       };
       // Tiles both of whose steps have a next one, up to head_dim 128 two per pass so that their stages are constants
       // (beyond, the code would not fit the instruction cache); then this wave's last tile; then those that only
@@ -1008,6 +1050,111 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           fetch(r, r & 1);
         }
       }
+    } else if constexpr (RAW) {
+      // The same over an 8-bit cache, in tiles of KT keys: what a tile asks for besides its keys (pages, scales, masks,
+      // waits) would take as long as 32 keys of half the bytes.  The scales of the tile after the next are asked for before
+      // its copies, so that what waits for the copies has them too.
+      static_assert(RW == 1, "a wave's own tiles");
+      constexpr int COPIES = 2 * PG * CPG, KB = KT / 32;
+      const int rounds = (ntiles - grp + KW - 1) / KW;
+      const int t_first = kbeg + grp * KT;
+      int pe0 = 0, pe1 = 0, pe2 = 0;
+      Scales se0{0, 0}, se1{0, 0};
+      if (rounds > 0) {
+        pe0 = tile_pages(t_first);
+        pe1 = tile_pages(t_first + KW * KT);
+        pe2 = tile_pages(t_first + 2 * KW * KT);
+        const Places at = places(pe0, t_first);
+        se0 = tile_scales(pe0, t_first);
+        se1 = tile_scales(pe1, t_first + KW * KT);
+        load_q();
+        issue_k(at, 0);
+        issue_v(at, 0);
+        if (rounds > 1) {
+          const Places next = places(pe1, t_first + KW * KT);
+          issue_k(next, 1);
+          issue_v(next, 1);
+          wait_vmcnt<(2 * COPIES < 63 ? 2 * COPIES : 63)>();
+        } else {
+          wait_vmcnt<COPIES>();
+        }
+        // (Q has come.  Left to itself, the compiler waits for it where it is used, in the loop, and there in every round for
+        // all copies but the last two: 4 to 5% of 64 tokens over 8000 keys.)
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) asm volatile("" : "+v"(qf[kk]));
+      }
+      for (int r = 0; r < rounds; ++r) {
+        const int t0 = t_first + r * KW * KT;
+        const int st = r & 1;
+        if (r + 1 < rounds) wait_vmcnt<COPIES>();
+        else wait_vmcnt<0>();
+        asm volatile("" ::: "memory");
+        if constexpr (NH > 1) raw_barrier();  // every wave's copies have landed
+        u32x4 kx[KB][KSTEPS / 2];
+        u32x2 vx[2 * KB][DB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int j = 0; j < KSTEPS / 2; ++j) kx[kb][j] = read_kb(j, st, kb);
+#pragma unroll
+        for (int c = 0; c < 2 * KB; ++c)
+#pragma unroll
+          for (int i = 0; i < DB; ++i) vx[c][i] = read_vb(i, st, c);
+        const uint32_t bad = bad_groups(pe0, t0) | bad_scales(se0, t0);
+        const int pn = pe2;
+        const Scales se = se0;
+        pe0 = pe1;
+        pe1 = pe2;
+        pe2 = tile_pages(t0 + 3 * KW * KT);
+        se0 = se1;
+        lds_done();
+        if (r + 2 < rounds) {
+          se1 = tile_scales(pn, t0 + 2 * KW * KT);
+          if constexpr (NH > 1) raw_barrier();  // every wave has read this stage
+          const Places at = places(pn, t0 + 2 * KW * KT);
+          issue_k(at, st);
+          issue_v(at, st);
+        }
+        if (t0 + KT > (mixed ? min(block_lo, kend) : kend)) {
+#pragma unroll
+          for (int c = 0; c < 2 * KB; ++c)
+#pragma unroll
+            for (int i = 0; i < DB; ++i) settle_bytes(vx[c][i], t0 + 16 * c, __builtin_amdgcn_readlane(se.v, c));
+        }
+        Scores s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const float k0 = scale_of(se, 2 * kb, true), k1 = scale_of(se, 2 * kb + 1, true), scale = col < 16 ? k0 : k1;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < KSTEPS; ++kk) {
+            const u32x2 x = {kx[kb][kk / 2][2 * (kk & 1)], kx[kb][kk / 2][2 * (kk & 1) + 1]};
+            s[kb] = Num<T>::mfma(__builtin_bit_cast(v8, widen8<T>(x, scale)), qf[kk], s[kb]);
+          }
+        }
+        float scale_v[2 * KB];
+#pragma unroll
+        for (int c = 0; c < 2 * KB; ++c) scale_v[c] = scale_of(se, c, false);
+        float mt = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          mask_scores(s[kb], t0 + 32 * kb, bad >> (2 * kb));
+          mt = fmaxf(mt, row_max(s[kb]));
+        }
+        move_max(mt);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          Probs p16;
+          probabilities(s[kb], p16);
+          add_sums(p16);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+              o[i] = Num<T>::mfma(__builtin_bit_cast(v8, widen8<T>(vx[2 * kb + c][i], scale_v[2 * kb + c])), p16[c], o[i]);
+        }
+      }
     } else {
       // Tiles grp, grp + KW, ... by this wave alone.  The tile after the next is asked for as soon as this one's
       // fragments are in registers, so that close to two tiles are in flight all the time.
@@ -1016,7 +1163,6 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
       const int rounds = (ntiles - grp + KW - 1) / KW;
       const int t_first = kbeg + grp * KT;
       int pe0 = 0, pe1 = 0, pe2 = 0;  // pages of this tile, the next and the one after it
-      int se0 = 0, se1 = 0;           // 8 bits: the scales of this tile and the next
       if (rounds > 0) {
         if constexpr (PAGED) {
           pe0 = tile_pages(t_first);
@@ -1024,10 +1170,6 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
           pe2 = tile_pages(t_first + 2 * KW * KT);
         }
         const Places at = places(pe0, t_first);
-        if constexpr (C8) {
-          se0 = tile_scales(pe0, t_first);
-          se1 = tile_scales(pe1, t_first + KW * KT);
-        }
         issue_k(at, 0);
         issue_v(at, 0);
         if (rounds > 1) {
@@ -1044,57 +1186,31 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         if (r + 1 < rounds) wait_vmcnt<COPIES>();
         else wait_vmcnt<0>();
         asm volatile("" ::: "memory");
-        settle_v(t0, st, se0);
+        settle_v(t0, st);
         // A wave has its SIMD to itself: all fragments are read before the first product, and only the first waits.
-        v8 kf[RAW ? 1 : KSTEPS], vf[RAW ? 1 : 2][RAW ? 1 : DB];
-        u32x4 kb[RAW ? KSTEPS / 2 : 1];  // 8 bits
-        u32x2 vb[RAW ? 2 : 1][RAW ? DB : 1];
-        if constexpr (RAW) {
+        v8 kf[KSTEPS], vf[2][DB];
 #pragma unroll
-          for (int j = 0; j < KSTEPS / 2; ++j) kb[j] = read_kb(j, st);
+        for (int kk = 0; kk < KSTEPS; ++kk) kf[kk] = read_k(kk, st, 0);
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < DB; ++i) vb[c][i] = read_vb(i, st, c);
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < KSTEPS; ++kk) kf[kk] = read_k(kk, st, 0);
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < DB; ++i) vf[c][i] = read_v(i, st, c);
-        }
+          for (int i = 0; i < DB; ++i) vf[c][i] = read_v(i, st, c);
         __builtin_amdgcn_sched_barrier(0);
         Scores s;
         Probs p16;
         float mt;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = 0.f;
-        float scale_v[2];
-        if constexpr (RAW) {
-          const float k0 = scale_of(se0, 0, true), k1 = scale_of(se0, 1, true), scale_k = col < 16 ? k0 : k1;
-          scale_v[0] = scale_of(se0, 0, false);
-          scale_v[1] = scale_of(se0, 1, false);
 #pragma unroll
-          for (int kk = 0; kk < KSTEPS; ++kk) {
-            const u32x2 x = {kb[kk / 2][2 * (kk & 1)], kb[kk / 2][2 * (kk & 1) + 1]};
-            s = Num<T>::mfma(__builtin_bit_cast(v8, widen8<T>(x, scale_k)), qf[kk], s);
-          }
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < KSTEPS; ++kk) s = Num<T>::mfma(kf[kk], qf[kk], s);
-        }
-        uint32_t bad = PAGED ? bad_groups(pe0, t0) : 0;
-        if constexpr (C8) bad |= bad_scales(se0, t0);
+        for (int kk = 0; kk < KSTEPS; ++kk) s = Num<T>::mfma(kf[kk], qf[kk], s);
+        const uint32_t bad = PAGED ? bad_groups(pe0, t0) : 0;
         const int pn = pe2;
         if constexpr (PAGED) {
           pe0 = pe1;
           pe1 = pe2;
           pe2 = tile_pages(t0 + 3 * KW * KT);
         }
-        se0 = se1;
         if (r + 2 < rounds) {
-          if constexpr (C8) se1 = tile_scales(pn, t0 + 2 * KW * KT);  // (before the copies: they are waited for first)
           lds_done();
           const Places at = places(pn, t0 + 2 * KW * KT);
           issue_k(at, st);
@@ -1108,11 +1224,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < DB; ++i) {
-            if constexpr (RAW)
-              o[i] = Num<T>::mfma(__builtin_bit_cast(v8, widen8<T>(vb[c][i], scale_v[c])), p16[c], o[i]);
-            else o[i] = Num<T>::mfma(vf[c][i], p16[c], o[i]);
-          }
+          for (int i = 0; i < DB; ++i) o[i] = Num<T>::mfma(vf[c][i], p16[c], o[i]);
       }
     }
   }
@@ -1130,7 +1242,19 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
     all += sum;
   }
   bool lost = all != all && l_row == l_row;
-  if (RW > 1 && mixed) odd = __syncthreads_or(odd) != 0;
+  if constexpr (C8 && RW > 1) {  // (the library's own would take LDS of its own, and the tiles and bytes fill it)
+    if (mixed) {
+      int* const flags = reinterpret_cast<int*>(seq_lds);
+      __syncthreads();
+      if (lane == 0) flags[wave] = 0;
+      if (odd) flags[wave] = 1;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < RW; ++w) odd |= flags[w] != 0;
+    }
+  } else if (RW > 1 && mixed) {
+    odd = __syncthreads_or(odd) != 0;
+  }
 
   // Over the groups, by all of them: group g joins the g-th, (g + KW)-th, ... of the 4-feature pieces that a lane holds,
   // from [group][piece][lane] and (maximum, sum) in LDS.
@@ -1287,7 +1411,7 @@ __global__ __launch_bounds__(64 * RW * KW) __attribute__((amdgpu_waves_per_eu(WP
         if constexpr (PAGED) {
           const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
           if ((uint32_t)page >= (uint32_t)a.pages) return nullptr;
-          return vh + page * a.v_page + (key & ((1 << a.page_shift) - 1)) * a.v_row;
+          return vh + hw * a.v_head + page * a.v_page + (key & ((1 << a.page_shift) - 1)) * a.v_row;
         } else {
           return vh + (int64_t)(sq.first + key) * a.v_row;
         }
