@@ -545,41 +545,50 @@ def rotary(x: torch.Tensor, frequencies: torch.Tensor, positions: Optional[torch
 
 # ---- pages of a cache ----
 
+def _layout(shape, stride, size: int):
+    """(bytes from a page to the next, rows of a page, bytes of a row) of a tensor [pages, ...]; rows is 1 where the tokens
+    of a page are not its outermost order."""
+    if len(shape) < 2 or 0 in shape:
+        raise ValueError("caches must be tensors [pages, page_size or blocks of it, ...] that hold something")
+    rows, row = shape[1], 1
+    for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
+        if n != 1 and s != row:
+            row = 0
+            break
+        row *= n
+    if not row:  # in another order: dense all the same?
+        rows, row = 1, 1
+        for s, n in sorted((s, n) for n, s in zip(shape[1:], stride[1:]) if n != 1):
+            if s != row:
+                raise ValueError("a page of a cache must be a dense piece of memory")
+            row *= n
+    row = row // rows * size
+    step = stride[0] * size
+    if shape[0] > 1 and step < rows * row:
+        raise ValueError("the pages of a cache must not overlap")
+    return step, rows, row
+
+
 def _parts(caches: Sequence[torch.Tensor]):
     """(their description for the library, number of tensors, pages, page size, device index) of tensors [pages, ...] each
     of whose pages is a dense piece of memory."""
     described, pages, page_size, index = [], 0, 0, -1
+    pack, last = _lib.CACHE_PART.pack, None
     for t in caches:
-        shape, stride = t.shape, t.stride()
-        if len(shape) < 2 or not t.is_cuda or 0 in shape:
-            raise ValueError("caches must be CUDA tensors [pages, page_size or blocks of it, ...] that hold something")
+        if not t.is_cuda:
+            raise ValueError("caches must be CUDA tensors")
+        shape = t.shape
+        what = shape, t.stride(), t.dtype
+        if what != last:  # (the halves of all layers are alike)
+            step, rows, row = _layout(shape, what[1], t.element_size())
+            last = what
         if not described:
             pages, page_size, index = shape[0], shape[1], t.get_device()
         elif shape[0] != pages or t.get_device() != index:
             raise ValueError(f"caches must have {pages} pages each, all on cuda:{index}")
         if page_size % shape[1]:
             raise ValueError(f"{shape[1]} rows of a page cannot share {page_size} tokens evenly")
-        size = t.element_size()
-        row = 1
-        for n, s in zip(reversed(shape[1:]), reversed(stride[1:])):
-            if n != 1 and s != row:
-                row = 0
-                break
-            row *= n
-        if row:
-            rows = shape[1]
-            row = row // rows * size
-        else:  # in another order: dense all the same?
-            rows, row = 1, 1
-            for s, n in sorted((s, n) for n, s in zip(shape[1:], stride[1:]) if n != 1):
-                if s != row:
-                    raise ValueError("a page of a cache must be a dense piece of memory")
-                row *= n
-            row *= size
-        step = stride[0] * size
-        if pages > 1 and step < rows * row:
-            raise ValueError("the pages of a cache must not overlap")
-        described.append(_lib.CACHE_PART.pack(t.data_ptr(), step, row, rows, 0))
+        described.append(pack(t.data_ptr(), step, row, rows, 0))
     if not described:
         raise ValueError("caches holds no tensor")
     return ctypes.create_string_buffer(b"".join(described)), len(described), pages, page_size, index
