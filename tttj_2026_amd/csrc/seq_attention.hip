@@ -320,10 +320,24 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
                                                                   ? 1
                                                                   : seq8_waves(p.shape, head_dim))
                                      : 32 * seq_waves(p.shape, head_dim);
-  const int alone = (blocks <= cus / 4 ? 6 : 16) * keys_per_round;
+  int rounds = blocks <= cus / 4 ? 6 : 16;
+  // Over an 8-bit cache rounds are longer (64 keys a wave on heads to 128) and bytes fewer.  Alone -> in shares, uniform
+  // lengths | from 1 on: 256 blocks on heads of 64, 1000 keys (2 rounds) 17.6 -> 18.8 | 13.5 -> 14.8, 2000 28.8 -> 23.8 | 22 ->
+  // 20; 32 on heads of 128, 1000 keys (4) 14.3 -> 17.4, 2000 21 -> 17.5; 128, 2000 (8) 24.5 -> 24.7 | 23 -> 21, 4000 38 -> 33;
+  // 16 on heads of 256, 1000 (8) 22.6 -> 23.6, 2000 35 -> 22; 256, 2000 (16) 49 -> 52 | 38 -> 34; 512 narrow ones on heads of
+  // 64, 500 (8) 16.6 -> 18.2 | 16 -> 15, 1000 28 -> 23; on heads of 128, 500 21 -> 25 | 20 -> 20, 1000 34 -> 35 | 34 -> 26;
+  // 1024 on heads of 64, 1000 (16) 30 -> 34 | 28 -> 25, 2000 53 -> 54 | 49 -> 34.
+  if (bytes && !wide) {
+    if (p.shape == SeqShape::kNarrow) rounds = head_dim <= 128 && blocks <= 2 * cus ? 10 : 16;
+    else rounds = head_dim <= 64 ? 3 : (head_dim <= 128 ? 5 : 8) * (blocks <= cus / 4 ? 1 : 2);
+  }
+  const int alone = rounds * keys_per_round;
   // Beyond the blocks that the chip holds (four times as many of 32 rows), tiles spread by themselves: 1088 tiles of 128
   // rows over 500 to 4600 keys, 195 alone and 272 in shares; 800 of 32 rows over 1 to 4000 keys, 193 and 162.
-  if (paged && max_length > alone && batch <= 512 && blocks < (wide ? 1 : 4) * held_blocks &&
+  // Heads that share a block count as one, for as many sequences as that pays: lengths from 1 to 2000 on 16 heads of 64, 128
+  // sequences 61 -> 53; 256 to 1500 112 -> 94; but 512 of 1100 keys on 4 heads 52 -> 63.
+  const int64_t most = (wide ? 1 : 4) * held_blocks, placed = !wide && bytes > 1 && batch <= 256 ? blocks / bytes : blocks;
+  if (paged && max_length > alone && batch <= 512 && placed < most &&
       tiles * (held / kSeqUnit + 1 + kSeqTileCost) + held_blocks < (1LL << 31)) {
     p.mode = kSeqShares;
     if (!wide) p.shape = SeqShape::kNarrow;
