@@ -318,8 +318,8 @@ int tt_cache_attention_fwd(const tt_cache_attention* args, void* stream);
 
 /* The same cache in 8 bits.  k_cache and v_cache hold e4m3 values (bytes; page, token and head strides
  * `kc_*`, `vc_*` / `k_*`, `v_*` aligned to 16), and k_scales and v_scales a power of two 2^(s - 127) (a
- * byte s; any strides) for each `block` tokens of a page and head: the value is the product.  block is
- * a power of two from 16 to page_size, head_dim a multiple of 16.
+ * byte s; strides `s_*` of both, which lie within 2 GiB each) for each `block` tokens of a page and head: the value is the
+ * product.  block is a power of two from 16 to page_size, head_dim a multiple of 16.
  *
  * Append: a block's scale is the smallest that holds the largest finite magnitude of its tokens (at
  * most 448 times the scale; 2^-127 where all are 0), and at least the scale that was there if older tokens of the
@@ -338,7 +338,7 @@ typedef struct {
   uint8_t *k_scales, *v_scales;
   const int32_t *table, *lengths, *starts;
   int64_t k_row, k_head, v_row, v_head, kc_page, kc_row, kc_head, vc_page, vc_row, vc_head;
-  int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head, table_row;
+  int64_t s_page, s_block, s_head, table_row;
   int32_t tokens, batch, kv_heads, head_dim, pages, page_size, table_pages, block, dtype, reserved;
 } tt_cache_rows8;
 int tt_cache_append8(const tt_cache_rows8* args, void* stream);
@@ -351,7 +351,7 @@ typedef struct {
   void *out, *workspace;
   int64_t workspace_bytes;
   int64_t q_row, q_head, k_page, k_row, k_head, v_page, v_row, v_head;
-  int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head, table_row;
+  int64_t s_page, s_block, s_head, table_row;
   int32_t tokens, batch, heads, kv_heads, head_dim, pages, page_size, table_pages, max_length, block, dtype;
   float scale;
 } tt_cache_attention8;

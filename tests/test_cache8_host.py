@@ -29,7 +29,7 @@ def _fields(name):
 
 STRUCTS = {"tt_cache_rows8": (_lib.CACHE_ROWS8, "tt_cache_append8"),
            "tt_cache_attention8": (_lib.CACHE_ATTENTION8, "tt_cache_attention8_fwd")}
-STRIDES = dict(ks_page=2, ks_block=2, ks_head=1, vs_page=2, vs_block=2, vs_head=1, table_row=8)
+STRIDES = dict(s_page=2, s_block=2, s_head=1, table_row=8)
 GOOD = {
     "tt_cache_rows8": dict(k=P, v=P, k_cache=P, v_cache=P, k_scales=P + 1, v_scales=P + 3, table=P, lengths=P, starts=P,
                            k_row=128, k_head=64, v_row=128, v_head=64, kc_page=2048, kc_row=128, kc_head=64,
@@ -77,6 +77,8 @@ def test_refusals(name):
                    dict(head_dim=24), dict(head_dim=272), dict(tokens=1 << 30, heads=8, kv_heads=8), dict(pages=0),
                    dict(table_pages=0), dict(page_size=8), dict(page_size=48), dict(page_size=1 << 20, table_pages=1 << 11),
                    dict(block=8), dict(block=0), dict(block=32), dict(block=48, page_size=64), dict(block=-16),
+                   dict(s_page=1 << 31), dict(s_block=1 << 31, page_size=32), dict(s_head=1 << 31), dict(s_page=1 << 28),
+                   dict(s_page=(1 << 28) - 1, s_head=8), dict(s_page=1 << 62, s_head=1 << 62),
                    dict(table_row=-1), dict(starts=None)):
         _refused(name, **{k: v for k, v in change.items() if k in fields})
     for field, kind in _fields(name):
@@ -86,7 +88,7 @@ def test_refusals(name):
             _refused(name, **{field: P + 8})
         if field.endswith(("_row", "_head", "_page", "_block")):
             _refused(name, **{field: -64})
-        if field.endswith(("_row", "_head", "_page")) and field[1] != "s" and field != "table_row":
+        if field.endswith(("_row", "_head", "_page")) and field[0] != "s" and field != "table_row":
             _refused(name, **{field: 68})
             if field not in ("q_row", "q_head") and (name == "tt_cache_attention8" or field[1] == "c"):
                 _refused(name, **{field: 72})  # 8 bytes: rows of a cache in 8 bits are read 16 at a time
@@ -141,7 +143,7 @@ def test_tensors(host):
 
     both(**good)
     halves = torch.zeros(9, 2, 32, 2, 64).to(E4M3).unbind(1)
-    both(*halves, k_scales=scales, v_scales=torch.zeros(2, 9, 2, dtype=torch.uint8).view(E8M0).permute(1, 2, 0))
+    both(*halves, **{n: torch.zeros(2, 9, 2, dtype=torch.uint8).view(E8M0).permute(1, 2, 0) for n in good})
     both(**{n: torch.zeros(9, 1, 2, dtype=torch.uint8).view(E8M0) for n in good})
     assert host == ["tt_cache_append8", "tt_cache_attention8_fwd"] * 3
     sixteen = cache.to(torch.float16)
@@ -153,7 +155,8 @@ def test_tensors(host):
            dict(good, k_cache=cache[..., :32], v_cache=cache[..., :32]),
            dict(good, k_cache=cache.transpose(2, 3), v_cache=cache.transpose(2, 3)),
            dict(good, v_cache=torch.zeros(cache.numel() + 8).to(E4M3)[8:].view(cache.shape)),
-           {n: torch.zeros(9, 3, 2, dtype=torch.uint8).view(E8M0) for n in good}]
+           {n: torch.zeros(9, 3, 2, dtype=torch.uint8).view(E8M0) for n in good},
+           dict(k_scales=scales, v_scales=torch.zeros(2, 9, 2, dtype=torch.uint8).view(E8M0).permute(1, 2, 0))]
     for change in bad:
         change = {"k_cache": cache, "v_cache": cache, **change}
         caches = change.pop("k_cache"), change.pop("v_cache")

@@ -77,8 +77,8 @@ SIGNATURES = {
 PACKED_ATTENTION = struct.Struct("q3QQQ6q7if")
 CACHE_ROWS = struct.Struct("q2Q2Q3Q11q8i")
 CACHE_ATTENTION = struct.Struct("q3Q3Q2Qq9q10ifi")
-CACHE_ROWS8 = struct.Struct("q2Q2Q2Q3Q17q10i")
-CACHE_ATTENTION8 = struct.Struct("q3Q2Q3Q2Qq15q11if")
+CACHE_ROWS8 = struct.Struct("q2Q2Q2Q3Q14q10i")
+CACHE_ATTENTION8 = struct.Struct("q3Q2Q3Q2Qq12q11if")
 ROTARY_ROWS = struct.Struct("qQQQ3Q4q8ifi")
 CACHE_PART = struct.Struct("Q2q2i")
 CACHE_FORK = struct.Struct("qQ5Q3QQ2q6i")

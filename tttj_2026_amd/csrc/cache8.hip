@@ -14,7 +14,7 @@ struct Append8Args {
   uint8_t *k_cache, *v_cache, *k_scales, *v_scales;
   const int32_t *starts, *lengths, *table;
   int64_t k_row, k_head, v_row, v_head, kc_page, kc_row, kc_head, vc_page, vc_row, vc_head;
-  int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head, table_row;
+  int64_t s_page, s_block, s_head, table_row;
   int tokens, batch, heads, chunks;  // a row: `chunks` times 8 values
   uint32_t by_chunks;                // 2^32 / chunks, rounded up
   int pages, table_pages, page_shift, block_shift, units;
@@ -123,8 +123,7 @@ __global__ __launch_bounds__(256, 4) void cache_append8_kernel(Append8Args a) {
   const uint16_t* const x = (is_v ? a.v + head * a.v_head : a.k + head * a.k_head) + (first + (lo - begin)) * row;
   uint8_t* const block = is_v ? a.v_cache + page * a.vc_page + in * a.vc_row + head * a.vc_head
                               : a.k_cache + page * a.kc_page + in * a.kc_row + head * a.kc_head;
-  uint8_t* const scale = is_v ? a.v_scales + page * a.vs_page + (in >> shift) * a.vs_block + head * a.vs_head
-                              : a.k_scales + page * a.ks_page + (in >> shift) * a.ks_block + head * a.ks_head;
+  uint8_t* const scale = (is_v ? a.v_scales : a.k_scales) + page * a.s_page + (in >> shift) * a.s_block + head * a.s_head;
   const int older = (int)(lo - base), pieces = (int)(hi - lo) * a.chunks;
   const uint32_t old = older > 0 ? *scale : 0;
   const auto place = [&](int piece) -> int2 {  // its token of the block's new ones, and its first value
@@ -209,8 +208,7 @@ extern "C" int tt_cache_append8(const tt_cache_rows8* args, void* stream) {
   TT_CHECK(check_rows("cache_append: v", c.v, c.v_row, c.v_head));
   TT_CHECK(check_rows8("cache_append: k_cache", c.k_cache, c.kc_page, c.kc_row, c.kc_head));
   TT_CHECK(check_rows8("cache_append: v_cache", c.v_cache, c.vc_page, c.vc_row, c.vc_head));
-  TT_CHECK(check_scales("cache_append: k_scales", c.k_scales, c.ks_page, c.ks_block, c.ks_head));
-  TT_CHECK(check_scales("cache_append: v_scales", c.v_scales, c.vs_page, c.vs_block, c.vs_head));
+  TT_CHECK(check_scales("cache_append", c));
   TT_REQUIRE(c.table_row >= 0, "cache_append: table_row %lld", (long long)c.table_row);
   Append8Args a{};
   a.k = static_cast<const uint16_t*>(c.k), a.v = static_cast<const uint16_t*>(c.v);
@@ -220,8 +218,7 @@ extern "C" int tt_cache_append8(const tt_cache_rows8* args, void* stream) {
   a.k_row = c.k_row, a.k_head = c.k_head, a.v_row = c.v_row, a.v_head = c.v_head;
   a.kc_page = c.kc_page, a.kc_row = c.kc_row, a.kc_head = c.kc_head;
   a.vc_page = c.vc_page, a.vc_row = c.vc_row, a.vc_head = c.vc_head;
-  a.ks_page = c.ks_page, a.ks_block = c.ks_block, a.ks_head = c.ks_head;
-  a.vs_page = c.vs_page, a.vs_block = c.vs_block, a.vs_head = c.vs_head, a.table_row = c.table_row;
+  a.s_page = c.s_page, a.s_block = c.s_block, a.s_head = c.s_head, a.table_row = c.table_row;
   a.tokens = c.tokens, a.batch = c.batch, a.heads = c.kv_heads, a.chunks = c.head_dim / 8;
   a.by_chunks = (uint32_t)(((1ull << 32) + a.chunks - 1) / a.chunks);
   a.pages = c.pages, a.table_pages = c.table_pages, a.page_shift = __builtin_ctz(c.page_size);

@@ -52,9 +52,16 @@ inline int check_block(const char* what, int block, int page_size) {
   return TT_OK;
 }
 
-inline int check_scales(const char* what, const void* p, int64_t page, int64_t block, int64_t head) {
-  TT_REQUIRE(p != nullptr && page >= 0 && block >= 0 && head >= 0, "%s: null pointer, or strides of %lld, %lld and %lld",
-             what, (long long)page, (long long)block, (long long)head);
+// (After check_block: an offset into the scales has 32 bits.)
+template <class C>
+int check_scales(const char* what, const C& c) {
+  TT_REQUIRE(c.k_scales != nullptr && c.v_scales != nullptr, "%s: null pointer", what);
+  const int64_t most = 1LL << 31, blocks = c.page_size / c.block;
+  TT_REQUIRE(c.s_page >= 0 && c.s_block >= 0 && c.s_head >= 0 && c.s_page < most && c.s_block < most && c.s_head < most &&
+                 (c.pages - 1) * c.s_page < most && (blocks - 1) * c.s_block < most && (c.kv_heads - 1) * c.s_head < most &&
+                 (c.pages - 1) * c.s_page + (blocks - 1) * c.s_block + (c.kv_heads - 1) * c.s_head < most,
+             "%s: scales %lld, %lld and %lld bytes apart do not lie within 2 GiB", what, (long long)c.s_page,
+             (long long)c.s_block, (long long)c.s_head);
   return TT_OK;
 }
 

@@ -323,13 +323,14 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   int rounds = blocks <= cus / 4 ? 6 : 16;
   // Over an 8-bit cache rounds are longer (64 keys a wave on heads to 128) and bytes fewer.  Alone -> in shares, uniform
   // lengths | from 1 on: 256 blocks on heads of 64, 1000 keys (2 rounds) 17.6 -> 18.8 | 13.5 -> 14.8, 2000 28.8 -> 23.8 | 22 ->
-  // 20; 32 on heads of 128, 1000 keys (4) 14.3 -> 17.4, 2000 21 -> 17.5; 128, 2000 (8) 24.5 -> 24.7 | 23 -> 21, 4000 38 -> 33;
+  // 20; 128, 2000 (4) 19.3 -> 19.2 | 16 -> 15, 16 drafts of 1 to 7 tokens to 2100 16.5 -> 18; 32 on heads of 128, 1000 keys (4) 14.3 -> 17.4, 2000 21 -> 17.5; 128, 2000 (8) 24.5 -> 24.7 | 23 -> 21, 4000 38 -> 33;
   // 16 on heads of 256, 1000 (8) 22.6 -> 23.6, 2000 35 -> 22; 256, 2000 (16) 49 -> 52 | 38 -> 34; 512 narrow ones on heads of
   // 64, 500 (8) 16.6 -> 18.2 | 16 -> 15, 1000 28 -> 23; on heads of 128, 500 21 -> 25 | 20 -> 20, 1000 34 -> 35 | 34 -> 26;
   // 1024 on heads of 64, 1000 (16) 30 -> 34 | 28 -> 25, 2000 53 -> 54 | 49 -> 34.
   if (bytes && !wide) {
     if (p.shape == SeqShape::kNarrow) rounds = head_dim <= 128 && blocks <= 2 * cus ? 10 : 16;
-    else rounds = head_dim <= 64 ? 3 : (head_dim <= 128 ? 5 : 8) * (blocks <= cus / 4 ? 1 : 2);
+    else if (head_dim <= 64) rounds = blocks <= cus / 2 ? 5 : 3;
+    else rounds = (head_dim <= 128 ? 5 : 8) * (blocks <= cus / 4 ? 1 : 2);
   }
   const int alone = rounds * keys_per_round;
   // Beyond the blocks that the chip holds (four times as many of 32 rows), tiles spread by themselves: 1088 tiles of 128
@@ -484,12 +485,10 @@ extern "C" int tt_cache_attention8_fwd(const tt_cache_attention8* args, void* st
   if (c.tokens == 0 || c.batch == 0) return TT_OK;
   TT_CHECK(check_rows8("cache_attention: k_cache", c.k_cache, c.k_page, c.k_row, c.k_head));
   TT_CHECK(check_rows8("cache_attention: v_cache", c.v_cache, c.v_page, c.v_row, c.v_head));
-  TT_CHECK(check_scales("cache_attention: k_scales", c.k_scales, c.ks_page, c.ks_block, c.ks_head));
-  TT_CHECK(check_scales("cache_attention: v_scales", c.v_scales, c.vs_page, c.vs_block, c.vs_head));
+  TT_CHECK(check_scales("cache_attention", c));
   SeqAttnArgs a{};
   a.k_scale = c.k_scales, a.v_scale = c.v_scales, a.block_shift = __builtin_ctz(c.block);
-  a.ks_page = c.ks_page, a.ks_block = c.ks_block, a.ks_head = c.ks_head;
-  a.vs_page = c.vs_page, a.vs_block = c.vs_block, a.vs_head = c.vs_head;
+  a.s_page = (int)c.s_page, a.s_block = (int)c.s_block, a.s_head = (int)c.s_head;
   return run_cache_attention("cache_attention", c, a, true, (hipStream_t)stream);
 }
 

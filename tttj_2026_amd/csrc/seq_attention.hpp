@@ -144,9 +144,10 @@ struct SeqAttnArgs {
   int mode;                // kSeqInOrder, kSeqHeaviest or kSeqShares
   float* part_o;           // kSeqShares: [2 slots][kv_heads][R * head_dim], the rows of tiles that lie in several shares
   float2* part_ml;         // ... [2 slots][kv_heads][R], their maximum (log2 domain) and sum
-  // 8-bit cache: the exponents (e8m0) of k and v, one per 2^block_shift tokens of a page and head; strides in bytes.
+  // 8-bit cache: the exponents (e8m0) of k and v, one per 2^block_shift tokens of a page and head; strides in bytes, of both
+  // (an offset has 32 bits).
   const uint8_t *k_scale, *v_scale;
-  int64_t ks_page, ks_block, ks_head, vs_page, vs_block, vs_head;
+  int s_page, s_block, s_head;
   int block_shift;
 };
 
@@ -567,19 +568,19 @@ __global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_
   // waits for them.  A group one of whose scales is none (255) counts as one outside the cache; its V is multiplied by
   // 2^-127.
   struct Scales {
-    uint32_t k, v;
+    uint8_t k, v;
   };
   auto tile_scales = [&](int pe, int t0) TT_INLINE -> Scales {
     const uint32_t in = min(t0 + 16 * (lane & 7), max(keys - 1, 0)) & ((1 << a.page_shift) - 1);
     const uint32_t page = (uint32_t)pe < (uint32_t)a.pages ? pe : 0, block = in >> a.block_shift;
-    return Scales{a.k_scale[page * (uint64_t)a.ks_page + block * (uint64_t)a.ks_block + hkv * a.ks_head],
-                  a.v_scale[page * (uint64_t)a.vs_page + block * (uint64_t)a.vs_block + hkv * a.vs_head]};
+    const uint32_t at = page * (uint32_t)a.s_page + block * (uint32_t)a.s_block + (uint32_t)(hkv * a.s_head);
+    return Scales{a.k_scale[at], a.v_scale[at]};
   };
   auto bad_scales = [&](const Scales& se, int t0) TT_INLINE -> uint32_t {
     return (uint32_t)__ballot((se.k == 255 || se.v == 255) && t0 + 16 * lane < keys) & 0xffu;
   };
   auto scale_of = [&](const Scales& se, int group, bool is_k) TT_INLINE -> float {
-    const uint32_t e = __builtin_amdgcn_readlane(is_k ? se.k : se.v, group);
+    const uint32_t e = __builtin_amdgcn_readlane(is_k ? se.k : se.v, group) & 255;
     return e8m0(e == 255 ? 0 : e);
   };
   // Where those groups lie in K and V (bytes), and how many bytes there belong to keys; worked out by the lanes for
@@ -595,7 +596,8 @@ __global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_
       if ((uint32_t)pe >= (uint32_t)a.pages) n = pe = 0;
       const uint32_t page = pe, in = t & ((1 << a.page_shift) - 1);
       p.k = EB * (page * (uint64_t)a.k_page + in * (uint64_t)a.k_row);
-      p.v = EB * (page * (uint64_t)a.v_page + in * (uint64_t)a.v_row);
+      if (C8 && a.k_page == a.v_page && a.k_row == a.v_row) p.v = p.k;  // (half of eight long multiplications)
+      else p.v = EB * (page * (uint64_t)a.v_page + in * (uint64_t)a.v_row);
     } else {
       const uint32_t row = sq.first + min(t, keys - 1);
       p.k = 2 * (row * (uint64_t)a.k_row);
@@ -1106,7 +1108,12 @@ __global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_
         pe0 = pe1;
         pe1 = pe2;
         pe2 = tile_pages(t0 + 3 * KW * KT);
-        se0 = se1;
+        // (The empty asm moves the scales on here, and they are held as the bytes that they are loaded as: the compiler would
+        // otherwise move or widen them at the end of the round, when the next ones are on their way, and wait for those, and
+        // so for the copies behind them: 64 tokens over 8000 keys 196 -> 207 us.)
+        uint32_t k1 = se1.k, v1 = se1.v;
+        asm volatile("" : "+v"(k1), "+v"(v1));
+        se0 = Scales{(uint8_t)k1, (uint8_t)v1};
         lds_done();
         if (r + 2 < rounds) {
           se1 = tile_scales(pn, t0 + 2 * KW * KT);
@@ -1422,7 +1429,7 @@ __global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_
       const auto scale_at = [&](int key) TT_INLINE -> float {
         const int page = a.table[sq.seq * a.table_row + (key >> a.page_shift)];
         const int block = (key & ((1 << a.page_shift) - 1)) >> a.block_shift;
-        const uint32_t e = a.v_scale[page * a.vs_page + block * a.vs_block + hkv * a.vs_head];
+        const uint32_t e = a.v_scale[page * a.s_page + block * a.s_block + hkv * a.s_head];
         return e8m0(e == 255 ? 0 : e);
       };
       for (int k0 = any_lost ? kbeg : kbeg + max(block_lo - kbeg, 0) / KT * KT; k0 < lim_hi; k0 += RPC) {

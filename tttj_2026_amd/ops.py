@@ -312,7 +312,7 @@ def _cache8(t: torch.Tensor, name: str, shape, index: int):
 
 
 def _scales(k: Optional[torch.Tensor], v: Optional[torch.Tensor], pages: int, page: int, kv_heads: int, index: int):
-    """(k's pointer, v's pointer, tokens per scale, k's strides, v's strides) of the scales of a cache in 8 bits."""
+    """(k's pointer, v's pointer, tokens per scale, strides) of the scales of a cache in 8 bits."""
     if k is None or v is None:
         raise ValueError("a cache in 8 bits needs both k_scales and v_scales")
     shape = k.shape
@@ -322,7 +322,10 @@ def _scales(k: Optional[torch.Tensor], v: Optional[torch.Tensor], pages: int, pa
             or k.get_device() != index or v.get_device() != index):
         raise ValueError(f"k_scales and v_scales must be [{pages}, {page} / tokens per scale, {kv_heads}] tensors of "
                          f"{torch.float8_e8m0fnu} on cuda:{index}")
-    return k.data_ptr(), v.data_ptr(), page // blocks, k.stride(), v.stride()
+    strides = k.stride()
+    if v.stride() != strides:
+        raise ValueError("k_scales and v_scales must have the same strides")
+    return k.data_ptr(), v.data_ptr(), page // blocks, strides
 
 
 def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -339,7 +342,7 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     page is no page of the cache, are not written.
 
     With ``k_scales`` and ``v_scales`` (float8_e8m0fnu [pages, page_size / block, kv_heads], block a power of two from
-    16 on) the cache is in 8 bits: k_cache and v_cache are float8_e4m3fn, and a value is the product of both.  A block's
+    16 on, both with the same strides) the cache is in 8 bits: k_cache and v_cache are float8_e4m3fn, and a value is the product of both.  A block's
     scale is the smallest power of two that holds its tokens' largest finite magnitude.  Where a new token is too large
     for the block that older ones of its sequence lie in, the scale grows and those are rounded to it.  Infinities and
     NaN become NaN, head_dim is a multiple of 16, and two sequences may not write to one block in one call."""
@@ -376,14 +379,14 @@ def _append8(k, v, k_cache, v_cache, page_table, lengths, starts, k_scales, v_sc
     _heads(kv_heads, kv_heads, hd)
     shape = (*k_cache.shape[:2], kv_heads, hd)
     k_half, v_half = _cache8(k_cache, "k_cache", shape, index), _cache8(v_cache, "v_cache", shape, index)
-    ks_at, vs_at, block, ks, vs = _scales(k_scales, v_scales, shape[0], shape[1], kv_heads, index)
+    ks_at, vs_at, block, strides = _scales(k_scales, v_scales, shape[0], shape[1], kv_heads, index)
     table, lengths, starts, batch, table_pages, table_row = _sequences(tokens, page_table, lengths, starts, index)
     args = _lib.CACHE_ROWS8
     try:
         packed = args.pack(
             args.size, k_at, v_at, k_half[0], v_half[0], ks_at, vs_at, table.data_ptr(), lengths.data_ptr(),
-            0 if starts is None else starts.data_ptr(), k_row, k_head, v_row, v_head, *k_half[1:], *v_half[1:], *ks,
-            *vs, table_row, tokens, batch, kv_heads, hd, shape[0], shape[1], table_pages, block, _SEQ_DTYPES[dtype], 0)
+            0 if starts is None else starts.data_ptr(), k_row, k_head, v_row, v_head, *k_half[1:], *v_half[1:],
+            *strides, table_row, tokens, batch, kv_heads, hd, shape[0], shape[1], table_pages, block, _SEQ_DTYPES[dtype], 0)
     except _lib.PACK_ERRORS as e:
         raise ValueError(f"cache_append: {e}") from None
     _call("tt_cache_append8", packed, index)
@@ -423,13 +426,13 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                                   starts is None, eight)
     work = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     if eight:
-        ks_at, vs_at, block, ks, vs = _scales(k_scales, v_scales, pages, page, kv_heads, index)
+        ks_at, vs_at, block, strides = _scales(k_scales, v_scales, pages, page, kv_heads, index)
         args = _lib.CACHE_ATTENTION8
         try:
             packed = args.pack(
                 args.size, q_at, k_half[0], v_half[0], ks_at, vs_at, table.data_ptr(), lengths.data_ptr(),
                 0 if starts is None else starts.data_ptr(), out.data_ptr(), 0 if work is None else work.data_ptr(),
-                nbytes, q_row, q_head, *k_half[1:], *v_half[1:], *ks, *vs, table_row, tokens, batch, heads, kv_heads,
+                nbytes, q_row, q_head, *k_half[1:], *v_half[1:], *strides, table_row, tokens, batch, heads, kv_heads,
                 hd, pages, page, table_pages, max_length, block, _SEQ_DTYPES[dtype],
                 hd ** -0.5 if scale is None else scale)
         except _lib.PACK_ERRORS as e:
