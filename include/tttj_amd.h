@@ -319,7 +319,7 @@ int tt_cache_attention_fwd(const tt_cache_attention* args, void* stream);
 /* The same cache in 8 bits.  k_cache and v_cache hold e4m3 values (bytes; page, token and head strides
  * `kc_*`, `vc_*` / `k_*`, `v_*` aligned to 16), and k_scales and v_scales a power of two 2^(s - 127) (a
  * byte s; strides `s_*` of both, which lie within 2 GiB each) for each `block` tokens of a page and head: the value is the
- * product.  block is a power of two from 16 to page_size, head_dim a multiple of 16.
+ * product.  block is a power of two from 16 to page_size (65536 at most), head_dim a multiple of 16.
  *
  * Append: a block's scale is the smallest that holds the largest finite magnitude of its tokens (at
  * most 448 times the scale; 2^-127 where all are 0), and at least the scale that was there if older tokens of the

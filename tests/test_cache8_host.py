@@ -76,7 +76,7 @@ def test_refusals(name):
     for change in (dict(tokens=-1), dict(batch=-1), dict(kv_heads=0), dict(kv_heads=-2), dict(head_dim=0), dict(dtype=2),
                    dict(head_dim=24), dict(head_dim=272), dict(tokens=1 << 30, heads=8, kv_heads=8), dict(pages=0),
                    dict(table_pages=0), dict(page_size=8), dict(page_size=48), dict(page_size=1 << 20, table_pages=1 << 11),
-                   dict(block=8), dict(block=0), dict(block=32), dict(block=48, page_size=64), dict(block=-16),
+                   dict(block=1 << 17, page_size=1 << 17), dict(block=8), dict(block=0), dict(block=32), dict(block=48, page_size=64), dict(block=-16),
                    dict(s_page=1 << 31), dict(s_block=1 << 31, page_size=32), dict(s_head=1 << 31), dict(s_page=1 << 28),
                    dict(s_page=(1 << 28) - 1, s_head=8), dict(s_page=1 << 62, s_head=1 << 62),
                    dict(table_row=-1), dict(starts=None)):

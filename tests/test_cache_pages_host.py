@@ -74,7 +74,7 @@ def host(monkeypatch):
         def __getattr__(self, name):
             return True if name == "is_cuda" else getattr(self.t, name)
 
-    monkeypatch.setattr(ops, "_parts", lambda caches: real([Device(t) for t in caches]))
+    monkeypatch.setattr(ops, "_parts", lambda caches, *how: real([Device(t) for t in caches], *how))
     monkeypatch.setattr(ops, "_call", lambda name, args, index: calls.append(name))
     return calls
 
@@ -83,12 +83,20 @@ def test_tensors(host):
     caches = list(torch.zeros(3, 9, 32, 2, 8).half())
     i32 = dict(dtype=torch.int32)
     table, n, uses = torch.zeros(4, 6, **i32), torch.zeros(4, **i32), torch.zeros(9, **i32)
-    good = [caches, [caches[0], torch.zeros(9, 2, 2)], [torch.zeros(9, 2, 32, 2, 8)[:, 0]],
+    good = [caches, [caches[0], torch.zeros(9, 2, 2, dtype=torch.uint8).view(torch.float8_e8m0fnu)], [torch.zeros(9, 2, 32, 2, 8)[:, 0]],
             [torch.zeros(9, 2, 32, 8).transpose(1, 2)], [torch.zeros(9, 32, 1, 8)], [torch.zeros(9, 32, 2, 8)[::1]]]
     for c in good:
         ops.cache_fork(c, table, n, uses, n, n), ops.cache_compact(c, table, n, uses), ops.cache_copy(c, n, n)
     assert len(host) == 3 * len(good)
-    for c in ([], [torch.zeros(9)], [caches[0], torch.zeros(8, 32, 2)], [caches[0], torch.zeros(9, 5, 2)],
+    halves = torch.zeros(9, 2, 32, 2, 8)
+    for c in ([caches[0], halves], [caches[0], torch.zeros(9, 2, 2)], [caches[0], torch.zeros(9, 5, 2)]):
+        with pytest.raises(ValueError):
+            ops.cache_fork(c, table, n, uses)
+        with pytest.raises(ValueError):
+            ops.cache_compact(c, table, n, uses)
+        ops.cache_copy(c, n, n)
+    del host[-3:]
+    for c in ([], [torch.zeros(9)], [caches[0], torch.zeros(8, 32, 2)],
               [torch.zeros(9, 32, 2, 8)[..., :4]], [torch.zeros(9, 32, 2, 8)[:, ::2]], [torch.zeros(9, 0, 2)],
               [torch.zeros(0, 32, 2)], [torch.zeros(1, 32, 2).expand(9, 32, 2)],
               [torch.zeros(9, 32, 1).expand(9, 32, 4)], [torch.zeros(9, 32, 2, 8).transpose(0, 1)]):

@@ -34,6 +34,17 @@ def test_heads_side_by_side(dtype, hd, h, hkv):
     _check(_run(q, cache, lengths, _starts(counts)), *_reference(q, cache, counts))
 
 
+@pytest.mark.parametrize("hd", [32, 64, 112, 128, 256])
+@pytest.mark.parametrize("h,hkv", [(40, 1), (66, 2), (100, 1)])
+def test_many_query_heads(hd, h, hkv):
+    """More rows a token than a narrow block has, alone, in a batch and with keys dealt out."""
+    for counts, lengths in (([1], [700]), ([1] * 5, [1, 64, 90, 2500, 17]), ([2, 9, 0], [300, 60, 5])):
+        cache = Cache(lengths, hkv, hd, 32, 32)
+        q = _randn(9, sum(counts), h, hd, dtype=BF16)
+        starts = None if set(counts) == {1} else _starts(counts)
+        _check(_run(q, cache, lengths, starts), *_reference(q, cache, counts))
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("hkv", [1, 2, 4])
 @pytest.mark.parametrize("counts,lengths", [([4, 2, 3], [700, 3000, 33]), ([90, 2], [200, 1500])])
@@ -196,6 +207,22 @@ def test_append_at_the_ends_of_the_types(dtype):
                          k_scales=dev["k_scales"], v_scales=dev["v_scales"])
         cache.append(0, 0, y, t, dtype), cache.append(1, 0, -y, t, dtype)
         _same(cache, dev)
+
+
+@pytest.mark.parametrize("hd", [16, 256])
+def test_append_large_blocks(hd):
+    """One scale for 4096 tokens: far more pieces than a block's lanes keep, older ones among them."""
+    cache = Cache([1000], 2, hd, 4096, 4096, room=[6000])
+    dev = cache.device()
+    x = (_randn(3, 2, 4500, 2, hd, dtype=torch.float32) * 6).to(BF16)
+    ops.cache_append(x[0].cuda(), x[1].cuda(), dev["k_cache"], dev["v_cache"], cache.table.cuda(), _i32([5500]),
+                     _i32([0, 4500]), k_scales=dev["k_scales"], v_scales=dev["v_scales"])
+    for half in range(2):
+        cache.append(half, 0, x[half], 1000, BF16)
+    cache.lengths = [5500]
+    _same(cache, dev)
+    q = _randn(4, 3, 4, hd, dtype=BF16)
+    _check(_run(q, cache, [5500], _starts([3])), *_reference(q, cache, [3]))
 
 
 def test_append_to_a_block_without_a_scale():

@@ -181,9 +181,10 @@ def test_fork(seed):
     assert len(lasts) == len(set(lasts)) and all(uses2[p] == 1 for p in lasts)
 
 
-@pytest.mark.parametrize("batch,columns,pages", [(3, 5, 4000), (1100, 2, 2500), (1, 5000, 6000), (2049, 3, 6000)])
+@pytest.mark.parametrize("batch,columns,pages", [(3, 5, 4000), (1100, 2, 2500), (1, 5000, 6000), (2049, 3, 6000),
+                                                 (70, 6, 16384), (70, 6, 16385), (40, 900, 50001)])
 def test_fork_of_many(batch, columns, pages):
-    """More rows, columns or pages than the block has threads."""
+    """More rows, columns or pages than the block has threads, or LDS room for counters."""
     rng = random.Random(batch)
     table, lengths, uses = _world(rng, batch, columns, 16, pages)
     parents = [rng.choice([b, b, rng.randrange(batch), -1]) for b in range(batch)]
@@ -193,6 +194,13 @@ def test_fork_of_many(batch, columns, pages):
     want = _copied(caches, new[3], 16)
     got = ops.cache_fork(caches, _i32(table), _i32(lengths), _i32(uses), _i32(parents), _i32(counts))
     for a, b in zip(got, new):
+        assert a.tolist() == b
+    _equal(caches, want)
+    table, lengths, uses = (x.tolist() for x in got)
+    new = _compact(table, lengths, uses, 16)
+    want = _copied(caches, new[2], 16)
+    moved = ops.cache_compact(caches, *got)
+    for a, b in zip(moved, new):
         assert a.tolist() == b
     _equal(caches, want)
 

@@ -31,7 +31,7 @@ def test_refusals():
     in_place = dict(out=P)
     for change in (dict(size=8), dict(tokens=-1), dict(batch=-1), dict(heads=0), dict(heads=-1), dict(pairs=0),
                    dict(pairs=33), dict(pairs=-1), dict(head_dim=258), dict(dtype=2), dict(tokens=1 << 28),
-                   dict(tokens=1 << 26, heads=1), dict(magnitude=float("nan")), dict(magnitude=float("inf")),
+                   dict(tokens=1 << 26, heads=1), dict(tokens=1, heads=(1 << 24) + 1), dict(magnitude=float("nan")), dict(magnitude=float("inf")),
                    dict(positions=None), dict(lengths=P), dict(starts=P), dict(positions=None, lengths=P, batch=3),
                    dict(x=None), dict(out=None), dict(frequencies=None), dict(frequencies=P + 4), dict(x=P + 1),
                    dict(out=P + 1), dict(x_row=-1), dict(x_head=-1), dict(out_row=-1), dict(out_head=-1), dict(out_row=0),

@@ -47,8 +47,8 @@ inline int check_rows8(const char* what, const void* p, int64_t page, int64_t ro
 }
 
 inline int check_block(const char* what, int block, int page_size) {
-  TT_REQUIRE(block >= 16 && block <= page_size && (block & (block - 1)) == 0,
-             "%s: a scale for each %d tokens of pages of %d (powers of two, from 16 on)", what, block, page_size);
+  TT_REQUIRE(block >= 16 && block <= page_size && block <= 65536 && (block & (block - 1)) == 0,
+             "%s: a scale for each %d tokens of pages of %d (powers of two, from 16 to 65536)", what, block, page_size);
   return TT_OK;
 }
 

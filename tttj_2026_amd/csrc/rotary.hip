@@ -155,8 +155,9 @@ extern "C" int tt_rotary(const tt_rotary_rows* args, void* stream) {
              c.batch, c.heads);
   TT_REQUIRE(c.pairs > 0 && c.head_dim <= 256 && 2 * (int64_t)c.pairs <= c.head_dim,
              "rotary: %d pairs of features in heads of %d (256 at most)", c.pairs, c.head_dim);
-  TT_REQUIRE((int64_t)c.tokens * c.heads < (1LL << 31) && c.tokens < (1 << 26), "rotary: %d tokens of %d heads", c.tokens,
-             c.heads);
+  TT_REQUIRE((int64_t)c.tokens * c.heads < (1LL << 31) && c.tokens < (1 << 26) &&
+                 (int64_t)c.heads * c.head_dim <= (1LL << 30),
+             "rotary: %d tokens of %d heads of %d", c.tokens, c.heads, c.head_dim);
   TT_REQUIRE(c.dtype == TT_FP16 || c.dtype == TT_BF16, "rotary: bad dtype %d", c.dtype);
   TT_REQUIRE(c.magnitude == c.magnitude && fabsf(c.magnitude) < INFINITY, "rotary: magnitude %g is not finite", c.magnitude);
   TT_REQUIRE((c.positions != nullptr) != (c.lengths != nullptr), "rotary: either positions or lengths are needed");

@@ -572,9 +572,9 @@ def _layout(shape, stride, size: int):
     return step, rows, row
 
 
-def _parts(caches: Sequence[torch.Tensor]):
+def _parts(caches: Sequence[torch.Tensor], by_tokens: bool = True):
     """(their description for the library, number of tensors, pages, page size, device index) of tensors [pages, ...] each
-    of whose pages is a dense piece of memory."""
+    of whose pages is a dense piece of memory; ``by_tokens``: parts of pages will be copied."""
     described, pages, page_size, index = [], 0, 0, -1
     pack, last = _lib.CACHE_PART.pack, None
     for t in caches:
@@ -589,8 +589,10 @@ def _parts(caches: Sequence[torch.Tensor]):
             pages, page_size, index = shape[0], shape[1], t.get_device()
         elif shape[0] != pages or t.get_device() != index:
             raise ValueError(f"caches must have {pages} pages each, all on cuda:{index}")
-        if page_size % shape[1]:
-            raise ValueError(f"{shape[1]} rows of a page cannot share {page_size} tokens evenly")
+        # (a [pages, 2, page_size, ...] tensor would pass for one of two blocks a page)
+        if by_tokens and shape[1] != page_size and (page_size % shape[1] or what[2] is not torch.float8_e8m0fnu):
+            raise ValueError(f"caches must be [pages, {page_size}, ...], or scales [pages, {page_size} / tokens per scale, "
+                             f"...]: got {list(shape)} of {what[2]}")
         described.append(pack(t.data_ptr(), step, row, rows, 0))
     if not described:
         raise ValueError("caches holds no tensor")
@@ -625,8 +627,8 @@ def cache_fork(caches: Sequence[torch.Tensor], page_table: torch.Tensor, lengths
 
     Whole pages are shared.  A page that is taken over in part is about to be written: the first row that takes it over so
     keeps it, unless a row holds it whole or the program does, and the others get copies of their tokens in all ``caches``
-    (tensors [pages, page_size, ...], or [pages, blocks of a page, ...] as scales are, each of whose pages is a dense piece
-    of memory: K and V of every layer; the first one's second size is the page size).  New pages are the free ones of
+    (tensors [pages, page_size, ...], and of an 8-bit cache the scales [pages, page_size / tokens per scale, ...], each of
+    whose pages is a dense piece of memory: K and V of every layer, one of them first).  New pages are the free ones of
     lowest number, row by row; where they run out the table has -1, whose tokens ``cache_append`` does not write.
     Nothing is read back: a step is a call whatever it comes to, and may be captured into a graph."""
     parts, count, pages, page_size, index = _parts(caches)
@@ -666,10 +668,11 @@ def cache_compact(caches: Sequence[torch.Tensor], page_table: torch.Tensor, leng
 
 
 def cache_copy(caches: Sequence[torch.Tensor], source: torch.Tensor, target: torch.Tensor) -> None:
-    """Copy pages source[i] to target[i] (int32 [N], on the device) in all ``caches`` (as in ``cache_fork``), in place.
+    """Copy pages source[i] to target[i] (int32 [N], on the device) in all ``caches`` (as in ``cache_fork``, or any others
+    [pages, ...] whose pages are dense), in place.
 
     Pairs with a number that is no page of the cache are skipped.  No target may be given twice or be a source."""
-    parts, count, pages, _, index = _parts(caches)
+    parts, count, pages, _, index = _parts(caches, False)
     n = source.shape[0] if source.dim() == 1 else -1
     source, target = _int32(source, "source", n, index), _int32(target, "target", n, index)
     args = _lib.CACHE_COPY
