@@ -27,6 +27,14 @@
 // us a tile: pages are looked up beside it).  4 tokens over 100000 keys each, 8 heads of 128: 287 us, 5.7 TB/s; 64 over 1 to
 // 4000: 106 us.
 //
+// The cache may be in 8 bits (C8): e4m3 and a power of two for each block of tokens and head, widened to T by one instruction
+// per two values.  Narrow blocks copy the bytes into LDS, in tiles of 64 keys on heads to 128, and 2 or 4 of their waves share
+// a tile, each for a head of its own, where heads lie side by side: pieces of 64, 128, 256 and 512 bytes a row are read at
+// 3.0, 5.5, 6.0 and 6.2 TB/s.  64 tokens over 8000 keys, 32 heads of 128 on 8, bf16: 195 us, 5.4 TB/s; over lengths from 126 on
+// 107 us, 4.9; 64 over 4000 keys on 16 heads of 64 105 us, 5.0; 4 over 100000 on 64 heads of 128 on 8 154 us, 5.3.  8 chunks of
+// 512 over up to 4608 keys 196 us, 0.84 PFLOP/s (16 bits: 183; 32 of 300 vector instructions a tile widen, and 10 more find
+// the scales).
+//
 // Per wave and tile: S^T = K Q^T with v_mfma_f32_32x32x16 (lane l holds row l % 32; of its 32 keys per block those
 // with bit 2 equal to l / 32), softmax with a running maximum and sum in fp32, O^T += V^T P^T.  K and V stay in the
 // row-major form of the projections and of the cache: ds_read_b64_tr_b16 transposes V on its way from LDS, and reads
@@ -198,6 +206,20 @@ __device__ __forceinline__ int vseg8(int row, int c) {
   if constexpr (HD == 256) return c ^ ((row & 3) << 1 | (row & 8));
   else if constexpr (HD == 128) return c ^ ((row & 2) | ((row & 8) >> 1));
   else return c ^ ((row & 8) >> 2);
+}
+
+// Tiles of T that are widened on their way into LDS: a lane writes two chunks, 2 c and 2 c + 1, and 8 lanes at a time 128
+// bytes without conflict if the even chunks of a row come first and the odd ones behind them (and with rows of 128 bytes,
+// halves of odd rows change places).  Reads as of the other tiles.  (8 chunks of 512: 197.6 -> 195.6 us.)
+template <int HD>
+__device__ __forceinline__ int kswz_widened(int row, int c) {
+  const int p = c >> 1 | (c & 1) << (HD == 128 ? 3 : 2);
+  return HD == 128 ? p ^ (row & 15) : p ^ ((row >> 1) & 7) ^ ((row & 1) << 2);
+}
+template <int HD>
+__device__ __forceinline__ int vseg_widened(int row, int c) {
+  const int p = c >> 1 | (c & 1) << (HD == 128 ? 3 : 2);
+  return HD == 128 ? p ^ ((row & 3) << 1) : p ^ ((row & 2) | (row & 1) << 2);
 }
 
 // The sequence that owns row tile `slot`.  Sequence b's tiles start at slot floor(starts[b] G / R) + b, which
@@ -407,8 +429,9 @@ __global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_
   constexpr int RPC = 64 / CH;              // rows of T in 1 KiB
   // An 8-bit cache's tiles: narrow blocks copy their bytes, and a wave widens the fragments that it reads.  In wide ones each
   // row is widened once for all waves: its bytes are copied to a place of the wave's own behind the tiles, and from there
-  // they go through registers into the tile as T, once its copies have landed.  (Loaded into registers they would be in
-  // flight there while the tile before is worked on, 16 registers more than there are: 208 us for 8 chunks of 512.)
+  // they go through registers into the tile as T, beside the products of the last step before it (8 chunks of 512 tokens:
+  // 212 us behind that step, 201 beside it; 200 with the bytes on their way in registers, 16 more than there are, some
+  // of which then lie in scratch memory).
   constexpr bool RAW = C8 && !PIPE;
   using E = std::conditional_t<RAW, uint8_t, T>;
   constexpr int EB = C8 ? 1 : 2;            // bytes of a value in memory
@@ -488,12 +511,14 @@ __global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_
   // (The empty asm keeps each in one register: the compiler would spread the sums over many.)  Rows of 512 bytes
   // leave no registers for them: there the pieces of a row are told apart by an XOR of the first one's address.
   constexpr bool FAR = PIPE && HD > 128;
+  // Whether a tile's bytes are widened beside the products of the last step before it (heads above 128: after it).
+  constexpr bool BESIDE = C8 && PIPE && !FAR;
   constexpr int KA = FAR ? 1 : RAW ? KSTEPS / 2 : KSTEPS, VA = FAR ? 1 : DB;
   uint32_t kread[KA], vread[VA];
 #pragma unroll
   for (int kk = 0; kk < KA; ++kk) {
     if constexpr (RAW) kread[kk] = lds_address(sk + col * ROW + kswz8<ROW>(col, hw * HD / 16 + 2 * kk + hf) * 16);
-    else kread[kk] = lds_address(sk + col * HD + kswz<HD>(col, 2 * kk + hf) * 8);
+    else kread[kk] = lds_address(sk + col * HD + (BESIDE ? kswz_widened<HD>(col, 2 * kk + hf) : kswz<HD>(col, 2 * kk + hf)) * 8);
     asm volatile("" : "+v"(kread[kk]));
   }
   // (RAW: 16 lanes read 8 rows, 4 hf ... 4 hf + 3 and 8 further, in the order of the lane's probabilities)
@@ -504,7 +529,8 @@ __global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_
       const int c = hw * HD / 16 + 2 * i + ((lane >> 4) & 1);
       vread[i] = lds_address(sv + vrow * ROW + vseg8<ROW>(vrow, c) * 16 + 8 * (lane & 1));
     } else {
-      const int c = vseg<HD>(vrow, 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1));
+      int c = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+      c = BESIDE ? vseg_widened<HD>(vrow, c) : vseg<HD>(vrow, c);
       vread[i] = lds_address(sv + vrow * HD + c * 8 + 4 * (lane & 1));
     }
     asm volatile("" : "+v"(vread[i]));
@@ -654,14 +680,18 @@ __global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_
       for (int c = 0; c < CPG; ++c) {
         const int row = rw * 16 + c * RPB + lane / CB, chunk = 2 * (lane % CB);
         T* const to = tile + row * HD;
-        const int at = is_k ? kswz<HD>(row, chunk) : vseg<HD>(row, chunk);  // the next chunk lies beside it
+        int at, next = 1;  // where the chunk lies, and what its place and the next chunk's differ by
+        if constexpr (BESIDE) {
+          at = is_k ? kswz_widened<HD>(row, chunk) : vseg_widened<HD>(row, chunk);
+          next = CH / 2;
+        } else {
+          at = is_k ? kswz<HD>(row, chunk) : vseg<HD>(row, chunk);
+        }
         *reinterpret_cast<u32x4*>(to + at * 8) = widen8<T>(u32x2{x[c][0], x[c][1]}, scale);
-        *reinterpret_cast<u32x4*>(to + (at ^ 1) * 8) = widen8<T>(u32x2{x[c][2], x[c][3]}, scale);
+        *reinterpret_cast<u32x4*>(to + (at ^ next) * 8) = widen8<T>(u32x2{x[c][2], x[c][3]}, scale);
       }
     }
   };
-  // Whether a tile's bytes are widened beside the products of the last step before it (heads above 128: after it).
-  constexpr bool BESIDE = C8 && PIPE && !FAR;
   // The K tile staged with a V tile begins KLEAD keys later: the scores run that far ahead.
   constexpr int KLEAD = PIPE ? 32 : 0;
   auto issue_k = [&](const Places& p, int st) TT_INLINE {
