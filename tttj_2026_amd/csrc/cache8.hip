@@ -86,7 +86,7 @@ __device__ __forceinline__ u32x2 rescale8(u32x2 x, float factor) {
 // W waves per (block of tokens, half, head).  Sequence b's blocks begin at unit floor(starts[b] / block) + 2 b, which
 // leaves it at least as many as its n new tokens touch (n / block + 2), so no table of them is needed.  Up to 8 pieces of
 // 16 bytes a lane stay in registers between the maximum and the rounding; what is beyond is read again.  Bound by HBM:
-// 36208 tokens on 8 heads of 128 47.6 us, 4.7 TB/s read and written.  (The launch bound is what makes the compiler widen
+// 36207 tokens on 8 heads of 128 47.6 us, 4.7 TB/s read and written.  (The launch bound is what makes the compiler widen
 // pieces one by one: it took 228 registers for 55 without it, and 97 us.)
 template <typename T, int W>
 __global__ __launch_bounds__(256, 4) void cache_append8_kernel(Append8Args a) {

@@ -35,7 +35,7 @@ __device__ __forceinline__ float2 cos_sin_turns(double t) {
 }
 
 // `waves` waves per token, each of which works out the token's cosines and sines for itself (a pair per lane, through LDS)
-// and turns every waves-th group of heads; a lane has the same V pairs in all of them.  Bound by HBM: 36208 tokens on 40 heads
+// and turns every waves-th group of heads; a lane has the same V pairs in all of them.  Bound by HBM: 36207 tokens on 40 heads
 // of 128 137 us, 5.4 TB/s read and written; 8192 tokens on 32 heads of 64, half of each turned, 14.5 us (16.3 with no load
 // before the position, 18 with the pieces that stay read at the end).
 template <typename T, int V, bool INTERLEAVED>

@@ -334,18 +334,19 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     """Write the keys and values of new tokens, k and v [T, kv_heads, head_dim], into a paged cache, in place.
 
     k_cache and v_cache are [pages, page_size, kv_heads, head_dim] (any strides that keep features adjacent, 16-byte
-    alignment and tokens less than 2^26 elements apart, e.g. both halves of one tensor, or a permuted [pages, kv_heads, page_size, head_dim]);
-    page_size is a power of two from 16 on.  Position t of sequence b lies in page page_table[b, t // page_size]
-    (int32 [B, n]) at t % page_size.  ``lengths`` (int32 [B]) counts the keys of each sequence with the new ones:
-    the n tokens of sequence b, rows starts[b] ... starts[b + 1] - 1 (or row b alone without ``starts``), take
+    alignment and tokens less than 2^26 elements apart, e.g. both halves of one tensor, or a permuted
+    [pages, kv_heads, page_size, head_dim]); page_size is a power of two from 16 on.  Position t of sequence b
+    lies in page page_table[b, t // page_size] (int32 [B, n]) at t % page_size.  ``lengths`` (int32 [B]) counts the keys
+    of each sequence with the new ones: the n tokens of sequence b, rows starts[b] ... starts[b + 1] - 1 (or row b alone without ``starts``), take
     positions lengths[b] - n ... lengths[b] - 1.  Tokens whose position is negative or beyond the table, or whose
     page is no page of the cache, are not written.
 
     With ``k_scales`` and ``v_scales`` (float8_e8m0fnu [pages, page_size / block, kv_heads], block a power of two from
-    16 on, both with the same strides) the cache is in 8 bits: k_cache and v_cache are float8_e4m3fn, and a value is the product of both.  A block's
-    scale is the smallest power of two that holds its tokens' largest finite magnitude.  Where a new token is too large
-    for the block that older ones of its sequence lie in, the scale grows and those are rounded to it.  Infinities and
-    NaN become NaN, head_dim is a multiple of 16, and two sequences may not write to one block in one call."""
+    16 on, both with the same strides) the cache is in 8 bits: k_cache and v_cache are float8_e4m3fn, and a value is the
+    product of both.  A block's scale is the smallest power of two that holds its tokens' largest finite magnitude.  Where
+    a new token is too large for the block that older ones of its sequence lie in, the scale grows and those are rounded
+    to it.  Infinities and NaN become NaN, head_dim is a multiple of 16, and two sequences may not write to one
+    block in one call."""
     if k_scales is not None or v_scales is not None:
         return _append8(k, v, k_cache, v_cache, page_table, lengths, starts, k_scales, v_scales)
     dtype, index = _typed(k, "k")
