@@ -323,10 +323,11 @@ static SeqPlan seq_plan(int64_t tokens, int batch, int heads, int kv_heads, int 
   int rounds = blocks <= cus / 4 ? 6 : 16;
   // Over an 8-bit cache rounds are longer (64 keys a wave on heads to 128) and bytes fewer.  Alone -> in shares, uniform
   // lengths | from 1 on: 256 blocks on heads of 64, 1000 keys (2 rounds) 17.6 -> 18.8 | 13.5 -> 14.8, 2000 28.8 -> 23.8 | 22 ->
-  // 20; 128, 2000 (4) 19.3 -> 19.2 | 16 -> 15, 16 drafts of 1 to 7 tokens to 2100 16.5 -> 18; 32 on heads of 128, 1000 keys (4) 14.3 -> 17.4, 2000 21 -> 17.5; 128, 2000 (8) 24.5 -> 24.7 | 23 -> 21, 4000 38 -> 33;
-  // 16 on heads of 256, 1000 (8) 22.6 -> 23.6, 2000 35 -> 22; 256, 2000 (16) 49 -> 52 | 38 -> 34; 512 narrow ones on heads of
-  // 64, 500 (8) 16.6 -> 18.2 | 16 -> 15, 1000 28 -> 23; on heads of 128, 500 21 -> 25 | 20 -> 20, 1000 34 -> 35 | 34 -> 26;
-  // 1024 on heads of 64, 1000 (16) 30 -> 34 | 28 -> 25, 2000 53 -> 54 | 49 -> 34.
+  // 20; 128, 2000 (4) 19.3 -> 19.2 | 16 -> 15, 16 drafts of 1 to 7 tokens to 2100 16.5 -> 18; 32 on heads of 128, 1000 keys
+  // (4) 14.3 -> 17.4, 2000 21 -> 17.5; 128, 2000 (8) 24.5 -> 24.7 | 23 -> 21, 4000 38 -> 33; 16 on heads of 256, 1000 (8)
+  // 22.6 -> 23.6, 2000 35 -> 22; 256, 2000 (16) 49 -> 52 | 38 -> 34; 512 narrow ones on heads of 64, 500 (8) 16.6 -> 18.2 |
+  // 16 -> 15, 1000 28 -> 23; on heads of 128, 500 21 -> 25 | 20 -> 20, 1000 34 -> 35 | 34 -> 26; 1024 on heads of 64, 1000
+  // (16) 30 -> 34 | 28 -> 25, 2000 53 -> 54 | 49 -> 34.
   if (bytes && !wide) {
     if (p.shape == SeqShape::kNarrow) rounds = head_dim <= 128 && blocks <= 2 * cus ? 10 : 16;
     else if (head_dim <= 64) rounds = blocks <= cus / 2 ? 5 : 3;
