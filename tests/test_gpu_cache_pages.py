@@ -217,6 +217,72 @@ def _compact(table, lengths, uses, page):
     return new, uses[0], [(p, q, page) for p, q in moves.items()]
 
 
+@pytest.mark.parametrize("seed", range(36))
+def test_large_states(seed):
+    """Either side of what one block does: 512 rows of 64 columns, 16384 pages."""
+    rng = random.Random(seed)
+    batch, columns, pages = [(512, 3, 900), (513, 3, 900), (8, 4096, 16384), (8, 4097, 16384), (257, 65, 9000), (513, 1, 2),
+                             (513, 64, 16384), (5, 2, 16384), (5, 2, 16385), (1, 1, 20001), (0, 4, 16385), (2, 70, 40960),
+                             ][seed % 12]
+    table, lengths, uses = _world(rng, batch, columns, 16, pages)
+    if seed // 12 == 1:  # the program holds most other pages, so that free ones run out
+        uses = [u or (rng.random() < 0.97) * rng.randint(1, 3) for u in uses]
+    elif seed // 12 == 2:  # or all
+        uses = [u or 1 for u in uses]
+    parents = [rng.choice([b, b, rng.randrange(batch), -1, batch, 0]) for b in range(batch)]
+    counts = [rng.choice([0, 1, 20, -7, -1000, 16 * columns, 2 ** 31 - 1, -2 ** 31]) for _ in range(batch)]
+    caches = _caches(pages, 16, heads=1)[-4::2]
+    state = (_i32(table).view(batch, columns), _i32(lengths), _i32(uses))
+    new = _fork(table, lengths, uses, parents, counts, 16) if batch else (table, lengths, uses, [])
+    want = _copied(caches, new[3], 16)
+    got = ops.cache_fork(caches, *state, _i32(parents), _i32(counts))
+    for a, b in zip(got, new):
+        assert a.tolist() == b
+    _equal(caches, want)
+    for state in (state, got):
+        table, lengths, uses = (x.tolist() for x in state)
+        new = _compact(table, lengths, uses, 16) if batch else _compact([[0]], [0], uses, 16)
+        want = _copied(caches, new[2], 16)
+        moved = ops.cache_compact(caches, *state)
+        assert moved[0].tolist() == (new[0] if batch else [])
+        assert moved[1].tolist() == new[1]
+        _equal(caches, want)
+
+
+def test_large_states_in_a_graph():
+    """A fork and a compaction whose phases are launches, replayed over states that change."""
+    batch, columns, pages = 40, 12, 17000
+    caches, worlds = _caches(pages, 16, heads=1)[-5:-1:2], []
+    rng = random.Random(1)
+    for _ in range(3):
+        state = _world(rng, batch, columns, 16, pages)
+        worlds.append((*state, [rng.randrange(-1, batch) for _ in range(batch)], [rng.randint(-40, 40) for _ in range(batch)]))
+    inputs = [_i32(x) for x in worlds[0]]
+
+    def steps():
+        table, lengths, uses = ops.cache_fork(caches, *inputs)
+        return (lengths, *ops.cache_compact(caches, table, lengths, uses))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        steps()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = steps()
+    for table, lengths, uses, parents, counts in worlds + worlds[:1]:
+        for x, y in zip(inputs, (table, lengths, uses, parents, counts)):
+            x.copy_(_i32(y))
+        forked = _fork(table, lengths, uses, parents, counts, 16)
+        new = _compact(*forked[:3], 16)
+        want = _copied(_copied(caches, forked[3], 16), new[2], 16)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert [x.tolist() for x in out] == [forked[1], new[0], new[1]]
+        _equal(caches, want)
+        torch.zeros(1000, device="cuda").sum().item()  # the program's own work between
+
+
 @pytest.mark.parametrize("seed", range(24))
 def test_compact(seed):
     rng = random.Random(seed)

@@ -2,7 +2,8 @@
 // the copies of pages that both ask for.
 //
 // The state is a page table [batch, columns], lengths [batch] and uses [pages] (how many rows hold a page, and what holds
-// the program has on it otherwise; 0: free).  One block works the new state out, phase by phase; a second launch copies.
+// the program has on it otherwise; 0: free).  One block works the new state out, phase by phase, with counters in LDS, and a
+// second launch copies; of a large state, each phase is a launch.
 #include "cache_checks.hpp"
 #include "kernels.hpp"
 #include "seq_attention.hpp"
@@ -14,31 +15,9 @@ namespace tt {
 constexpr int kPageThreads = 1024;
 constexpr int kPageWaves = kPageThreads / 64;
 constexpr int kEach = 4;              // pages that a thread looks at in turn
-constexpr int kSmallPages = 16384;    // up to this many, counters lie in LDS (8 bytes a page) ...
-constexpr int kSmallRows = 1024;      // ... and so do up to this many rows (16 bytes a row)
-
-// Counters of the pages: in LDS, or for large caches in the workspace, where atomics change them and they are read past
-// the L1 (which may hold them as they were).
-template <bool SMALL>
-struct Counters {
-  int* at;
-  __device__ __forceinline__ int get(int i) const {
-    if constexpr (SMALL) return at[i];
-    else return __hip_atomic_load(at + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __device__ __forceinline__ void put(int i, int v) const {
-    if constexpr (SMALL) at[i] = v;
-    else __hip_atomic_store(at + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __device__ __forceinline__ void add(int i, int v) const { atomicAdd(at + i, v); }
-  __device__ __forceinline__ void least(int i, int v) const { atomicMin(at + i, v); }
-};
-
-template <bool SMALL>
-__device__ __forceinline__ void phase() {  // what was written is read by others from here on
-  if constexpr (!SMALL) __threadfence();
-  __syncthreads();
-}
+constexpr int kSmallPages = 16384;    // one block: up to this many pages (8 bytes of LDS each) ...
+constexpr int kSmallRows = 512;       // ... and rows (16 bytes each), times their spans of 64 columns
+constexpr int kScanBlocks = 256;      // blocks of a launch that counts pages
 
 // Sum over the block's threads before this one; `total` over all.  (s_sums: an int per wave; free again at return.)
 __device__ __forceinline__ int block_scan(int v, int* s_sums, int& total) {
@@ -60,6 +39,7 @@ struct PagesArgs {
   int batch, columns, pages, page_shift, list;  // list: free pages that can be needed
   int *hold, *first, *free_pages;               // large: [pages], [pages], [list]
   int4* rows;                                   // large: [batch]
+  int *sums, *needed, *open;                    // large: [kScanBlocks], pages that are needed, and that are free
   int *source, *target, *tokens, *copies;       // copies to make, and their number
 };
 
@@ -84,53 +64,39 @@ __device__ __forceinline__ int4 fork_row(const PagesArgs& a, int b) {
 // Whole pages that a row takes over are shared.  One that it takes over in part is going to be written: of the rows that
 // do so the first keeps it, if no row holds it whole and the program has no hold on it; the others get copies.  New pages
 // are the lowest free ones, in the order of the rows.
-//
-// One block: each phase needs all that the one before it counted, and a barrier costs less than a launch.  A wave takes a
-// row at a time, a lane a column.  Bound by latency: 4.7 us for 4 rows of 35 columns and 90 pages, 9.4 for 128 of 35 and 1493
-// (33 with the counters in memory and a thread per entry).
-template <bool SMALL>
-__global__ __launch_bounds__(kPageThreads) void cache_fork_kernel(PagesArgs a) {
-  extern __shared__ __align__(16) int pages_lds[];
-  __shared__ int s_sums[kPageWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int shift = a.page_shift, page = 1 << shift;
-  int4* const rows = SMALL ? reinterpret_cast<int4*>(pages_lds) : a.rows;
-  int* const lds_pages = pages_lds + 4 * a.batch;
-  const Counters<SMALL> hold{SMALL ? lds_pages : a.hold}, first{SMALL ? lds_pages + a.pages : a.first};
-  // (the first rows of the pages are done with before the free ones are listed)
-  const Counters<SMALL> free_pages{SMALL ? lds_pages + a.pages : a.free_pages};
-  for (int b = tid; b < a.batch; b += kPageThreads) rows[b] = fork_row(a, b);
-  for (int p = tid; p < a.pages; p += kPageThreads) {
-    hold.put(p, a.uses[p]);
-    first.put(p, a.batch);
+constexpr int kAhead = 4;  // rows whose entries are asked for at once
+
+// Column i of rows b0, b0 + step, ...: `hold` comes to the holds after the call, without the rows as they were and with the
+// pages that rows keep whole; `first` to the first row that takes a page over in part.
+__device__ __forceinline__ void fork_count(const PagesArgs& a, const int4* rows, int* hold, int* first, int b0, int step,
+                                           int i) {
+  int had[kAhead], has[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    had[j] = has[j] = -1;
+    const int b = b0 + j * step;
+    if (b >= a.batch) continue;
+    const int4 r = rows[b];
+    if (i < r.w) had[j] = a.table[b * a.table_row + i];
+    if (i << a.page_shift < r.z) has[j] = a.table[r.x * a.table_row + i];
   }
-  phase<SMALL>();
-  // Holds after the call: without the rows as they were, with the pages that rows keep whole.
-  constexpr int AHEAD = 4;  // rows whose entries are asked for at once
-  for (int b0 = wave; b0 < a.batch; b0 += AHEAD * kPageWaves)
-    for (int i = lane; i < a.columns; i += 64) {
-      int had[AHEAD], has[AHEAD];
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        had[j] = has[j] = -1;
-        const int b = b0 + j * kPageWaves;
-        if (b >= a.batch) continue;
-        const int4 r = rows[b];
-        if (i < r.w) had[j] = a.table[b * a.table_row + i];
-        if (i << shift < r.z) has[j] = a.table[r.x * a.table_row + i];
-      }
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        if ((uint32_t)had[j] < (uint32_t)a.pages) hold.add(had[j], -1);
-        if ((uint32_t)has[j] < (uint32_t)a.pages) {
-          const int b = b0 + j * kPageWaves;
-          if ((i << shift) + page <= rows[b].z) hold.add(has[j], 1);
-          else first.least(has[j], b);
-        }
-      }
+  for (int j = 0; j < kAhead; ++j) {
+    if ((uint32_t)had[j] < (uint32_t)a.pages) atomicAdd(hold + had[j], -1);
+    if ((uint32_t)has[j] < (uint32_t)a.pages) {
+      const int b = b0 + j * step;
+      if ((i + 1) << a.page_shift <= rows[b].z) atomicAdd(hold + has[j], 1);
+      else atomicMin(first + has[j], b);
     }
-  phase<SMALL>();
-  int needed = 0, copies = 0;
+  }
+}
+
+// What each row needs and copies, by the whole block: rows become (row that it continues, length, pages taken over, the
+// first of its new pages in the list of free ones).
+__device__ __forceinline__ void fork_rows(const PagesArgs& a, int4* rows, int* hold, const int* first, int* s_sums,
+                                          int& needed, int& copies) {
+  const int tid = threadIdx.x, shift = a.page_shift, page = 1 << shift;
+  needed = copies = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kPageThreads) {
     const int b = b0 + tid;
     int need = 0, whole = 0, p = -1;
@@ -143,7 +109,7 @@ __global__ __launch_bounds__(kPageThreads) void cache_fork_kernel(PagesArgs a) {
         p = a.table[r.x * a.table_row + whole - 1];
         if ((uint32_t)p < (uint32_t)a.pages) {
           // (only the first row of a page may find it unheld, and it alone changes that)
-          if (first.get(p) == b && hold.get(p) == 0) hold.put(p, 1);
+          if (first[p] == b && hold[p] == 0) hold[p] = 1;
           else copy = true;
         }
       }
@@ -165,74 +131,199 @@ __global__ __launch_bounds__(kPageThreads) void cache_fork_kernel(PagesArgs a) {
     needed += total;
     copies += copied;
   }
-  phase<SMALL>();
+}
+
+// Free pages among kEach from p0 on of this thread get a rank from `found` on, and the first `take` a hold and a place in
+// the list; by the whole block.
+__device__ __forceinline__ void fork_list(const PagesArgs& a, const int* hold, int* free_pages, int p0, int end, int take,
+                                          int* s_sums, int& found) {
+  int held[kEach], open = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int p = p0 + kEach * (int)threadIdx.x + j;
+    held[j] = p < end ? hold[p] : 1;
+    open += held[j] == 0 ? 1 : 0;
+  }
+  int total, rank = block_scan(open, s_sums, total) + found;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int p = p0 + kEach * (int)threadIdx.x + j;
+    if (p >= end) continue;
+    int uses = held[j];
+    if (uses == 0) {
+      if (rank < take) {
+        free_pages[rank] = p;
+        uses = 1;
+      }
+      ++rank;
+    }
+    a.new_uses[p] = uses;
+  }
+  found += total;
+}
+
+// Column i of rows b0, b0 + step, ... of the new table; `found` free pages are listed.
+__device__ __forceinline__ void fork_table(const PagesArgs& a, const int4* rows, const int* free_pages, int found, int b0,
+                                           int step, int i) {
+  int p[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    p[j] = -1;
+    const int b = b0 + j * step;
+    if (b >= a.batch) continue;
+    const int4 r = rows[b];
+    if (i < r.z) {
+      p[j] = a.table[r.x * a.table_row + i];
+    } else if (i < held_pages(r.y, a.page_shift)) {
+      const int rank = r.w + i - r.z;
+      if (rank < found) p[j] = free_pages[rank];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    const int b = b0 + j * step;
+    if (b < a.batch) a.new_table[(int64_t)b * a.columns + i] = p[j];
+  }
+}
+
+__device__ __forceinline__ int copy_target(const int4* rows, const int* free_pages, int found, int row) {
+  const int rank = rows[row].w;
+  return rank < found ? free_pages[rank] : -1;
+}
+
+// One block: each phase needs all that the one before it counted, and a barrier costs less than a launch.  A wave takes a
+// row at a time, a lane a column.  Bound by latency: 4.7 us for 4 rows of 35 columns and 90 pages, 9.4 for 128 of 35 and 1493
+// (33 with the counters in memory and a thread per entry).
+__global__ __launch_bounds__(kPageThreads) void cache_fork_kernel(PagesArgs a) {
+  extern __shared__ __align__(16) int pages_lds[];
+  __shared__ int s_sums[kPageWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int4* const rows = reinterpret_cast<int4*>(pages_lds);
+  int* const hold = pages_lds + 4 * a.batch;
+  int* const first = hold + a.pages;
+  int* const free_pages = first;  // (which is done with before these are listed)
+  for (int b = tid; b < a.batch; b += kPageThreads) rows[b] = fork_row(a, b);
+  for (int p = tid; p < a.pages; p += kPageThreads) {
+    hold[p] = a.uses[p];
+    first[p] = a.batch;
+  }
+  __syncthreads();
+  for (int b0 = wave; b0 < a.batch; b0 += kAhead * kPageWaves)
+    for (int i = lane; i < a.columns; i += 64) fork_count(a, rows, hold, first, b0, kPageWaves, i);
+  __syncthreads();
+  int needed, copies;
+  fork_rows(a, rows, hold, first, s_sums, needed, copies);
+  __syncthreads();
+  const int take = min(needed, a.list);
   int found = 0;
-  for (int p0 = 0; p0 < a.pages; p0 += kEach * kPageThreads) {
-    int held[kEach], open = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int p = p0 + kEach * tid + j;
-      held[j] = p < a.pages ? hold.get(p) : 1;
-      open += held[j] == 0 ? 1 : 0;
-    }
-    int total, rank = block_scan(open, s_sums, total) + found;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int p = p0 + kEach * tid + j;
-      if (p >= a.pages) continue;
-      int uses = held[j];
-      if (uses == 0) {
-        if (rank < min(needed, a.list)) {
-          free_pages.put(rank, p);
-          uses = 1;
-        }
-        ++rank;
-      }
-      a.new_uses[p] = uses;
-    }
-    found += total;
-  }
-  found = min(found, min(needed, a.list));
-  phase<SMALL>();
-  for (int b0 = wave; b0 < a.batch; b0 += AHEAD * kPageWaves)
-    for (int i = lane; i < a.columns; i += 64) {
-      int p[AHEAD];
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        p[j] = -1;
-        const int b = b0 + j * kPageWaves;
-        if (b >= a.batch) continue;
-        const int4 r = rows[b];
-        if (i < r.z) {
-          p[j] = a.table[r.x * a.table_row + i];
-        } else if (i < held_pages(r.y, shift)) {
-          const int rank = r.w + i - r.z;
-          if (rank < found) p[j] = free_pages.get(rank);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        const int b = b0 + j * kPageWaves;
-        if (b < a.batch) a.new_table[(int64_t)b * a.columns + i] = p[j];
-      }
-    }
-  for (int c = tid; c < copies; c += kPageThreads) {  // (a barrier and more since they were written)
-    const int rank = rows[-1 - __hip_atomic_load(a.target + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)].w;
-    a.target[c] = rank < found ? free_pages.get(rank) : -1;
-  }
+  for (int p0 = 0; p0 < a.pages; p0 += kEach * kPageThreads)
+    fork_list(a, hold, free_pages, p0, a.pages, take, s_sums, found);
+  found = min(found, take);
+  __syncthreads();
+  for (int b0 = wave; b0 < a.batch; b0 += kAhead * kPageWaves)
+    for (int i = lane; i < a.columns; i += 64) fork_table(a, rows, free_pages, found, b0, kPageWaves, i);
+  for (int c = tid; c < copies; c += kPageThreads)  // (barriers lie between)
+    a.target[c] = copy_target(rows, free_pages, found,
+                              -1 - __hip_atomic_load(a.target + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
   if (tid == 0) *a.copies = copies;
+}
+
+// The same for large states, a launch per phase: 64 rows of 100 columns 28 us a call at 16385 pages, 28 at 10^6, most of it
+// the launches.
+__global__ __launch_bounds__(256) void cache_fork_begin_kernel(PagesArgs a) {
+  const int step = (int)gridDim.x * 256;
+  for (int b = (int)blockIdx.x * 256 + (int)threadIdx.x; b < a.batch; b += step) a.rows[b] = fork_row(a, b);
+  for (int p = (int)blockIdx.x * 256 + (int)threadIdx.x; p < a.pages; p += step) {
+    a.hold[p] = a.uses[p];
+    a.first[p] = a.batch;
+  }
+}
+
+// Waves take kAhead rows and 64 columns at a time.
+template <class F>
+__device__ __forceinline__ void each_entry(const PagesArgs& a, F&& f) {
+  const int spans = (a.columns + 63) / 64, tasks = (a.batch + kAhead - 1) / kAhead * spans;
+  for (int t = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); t < tasks; t += (int)gridDim.x * 4) {
+    const int i = t % spans * 64 + (int)(threadIdx.x & 63);
+    if (i < a.columns) f(t / spans * kAhead, i);
+  }
+}
+
+__global__ __launch_bounds__(256) void cache_fork_count_kernel(PagesArgs a) {
+  each_entry(a, [&](int b0, int i) { fork_count(a, a.rows, a.hold, a.first, b0, 1, i); });
+}
+
+__global__ __launch_bounds__(kPageThreads) void cache_fork_rows_kernel(PagesArgs a) {
+  __shared__ int s_sums[kPageWaves];
+  int needed, copies;
+  fork_rows(a, a.rows, a.hold, a.first, s_sums, needed, copies);
+  if (threadIdx.x == 0) *a.needed = needed, *a.copies = copies;
+}
+
+// Pages that a block of a launch over all of them looks at.
+struct Share {
+  int begin, end;
+};
+__device__ __forceinline__ Share share_of(const PagesArgs& a) {
+  const int most = kEach * kPageThreads, turns = (a.pages + most - 1) / most;
+  const int each = (turns + (int)gridDim.x - 1) / (int)gridDim.x * most;
+  const int begin = (int)min((int64_t)blockIdx.x * each, (int64_t)a.pages);
+  return {begin, (int)min((int64_t)begin + each, (int64_t)a.pages)};
+}
+
+// sums: how many of each block's pages are free, or for a compaction used.
+__global__ __launch_bounds__(kPageThreads) void cache_count_kernel(PagesArgs a, const int* pages, bool used) {
+  __shared__ int s_sums[kPageWaves];
+  const Share s = share_of(a);
+  int n = 0, total;
+  for (int p = s.begin + (int)threadIdx.x; p < s.end; p += kPageThreads) n += (used ? pages[p] > 0 : pages[p] == 0) ? 1 : 0;
+  block_scan(n, s_sums, total);
+  if (threadIdx.x == 0) a.sums[blockIdx.x] = total;
+}
+
+// The sum before this block's; `total` of all.
+__device__ __forceinline__ int sums_before(const PagesArgs& a, int* s_sums, int& total) {
+  static_assert(kScanBlocks <= kPageThreads, "a thread per block");
+  const int tid = threadIdx.x, n = tid < (int)gridDim.x ? a.sums[tid] : 0;
+  int before;
+  block_scan(tid < (int)blockIdx.x ? n : 0, s_sums, before);
+  block_scan(n, s_sums, total);
+  return before;
+}
+
+__global__ __launch_bounds__(kPageThreads) void cache_fork_list_kernel(PagesArgs a) {
+  __shared__ int s_sums[kPageWaves];
+  const Share s = share_of(a);
+  const int take = min(*a.needed, a.list);
+  int total, found = sums_before(a, s_sums, total);
+  for (int p0 = s.begin; p0 < s.end; p0 += kEach * kPageThreads)
+    fork_list(a, a.hold, a.free_pages, p0, s.end, take, s_sums, found);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.open = min(total, take);
+}
+
+__global__ __launch_bounds__(256) void cache_fork_table_kernel(PagesArgs a) {
+  const int found = *a.open, copies = *a.copies;
+  each_entry(a, [&](int b0, int i) { fork_table(a, a.rows, a.free_pages, found, b0, 1, i); });
+  for (int c = (int)blockIdx.x * 256 + (int)threadIdx.x; c < copies; c += (int)gridDim.x * 256)
+    a.target[c] = copy_target(a.rows, a.free_pages, found, -1 - a.target[c]);
 }
 
 // The used pages numbered from their count on move to the free ones below it, both in order: the fewest moves, none of
 // which reads what another writes.
-template <bool SMALL>
+__device__ __forceinline__ int compacted(const PagesArgs& a, const int* number, int b, int i, int held) {
+  if (i >= held) return -1;
+  const int p = a.table[b * a.table_row + i];
+  return (uint32_t)p < (uint32_t)a.pages ? number[p] : p;
+}
+
 __global__ __launch_bounds__(kPageThreads) void cache_compact_kernel(PagesArgs a) {
   extern __shared__ __align__(16) int pages_lds[];
   __shared__ int s_sums[kPageWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // The number that a page gets; and the pages that move, then where to.
-  const Counters<SMALL> number{SMALL ? pages_lds : a.first}, movers{SMALL ? pages_lds + a.pages : a.source};
-  const Counters<SMALL> holes{SMALL ? pages_lds + a.pages + a.pages / 2 : a.target};
+  int* const number = pages_lds;
+  int* const movers = pages_lds + a.pages;
+  int* const holes = movers + a.pages / 2;
   int used = 0;
   for (int p = tid; p < a.pages; p += kPageThreads) used += a.uses[p] > 0 ? 1 : 0;
   int total;
@@ -257,56 +348,147 @@ __global__ __launch_bounds__(kPageThreads) void cache_compact_kernel(PagesArgs a
       const int p = p0 + kEach * tid + j;
       if (p >= a.pages) continue;
       const bool moves = uses[j] > 0 && p >= used;
-      if (moves) movers.put(r++, p);
-      else if (p < used && uses[j] == 0) holes.put(s++, p);
-      number.put(p, p);
+      if (moves) movers[r++] = p;
+      else if (p < used && uses[j] == 0) holes[s++] = p;
+      number[p] = p;
       if (moves || p >= used) a.new_uses[p] = 0;
       else if (uses[j] > 0) a.new_uses[p] = uses[j];
     }
   }
-  phase<SMALL>();
+  __syncthreads();
   for (int r = tid; r < moving; r += kPageThreads) {
-    const int p = movers.get(r), q = holes.get(r);
-    number.put(p, q);
+    const int p = movers[r], q = holes[r];
+    number[p] = q;
     a.new_uses[q] = a.uses[p];
-    if constexpr (SMALL) {
-      a.source[r] = p;
-      a.target[r] = q;
-    }
+    a.source[r] = p;
+    a.target[r] = q;
   }
-  phase<SMALL>();
+  __syncthreads();
   for (int b = wave; b < a.batch; b += kPageWaves) {
     const int held = held_pages(row_length(a, b), a.page_shift);
-    for (int i = lane; i < a.columns; i += 64) {
-      int p = -1;
-      if (i < held) {
-        p = a.table[b * a.table_row + i];
-        if ((uint32_t)p < (uint32_t)a.pages) p = number.get(p);
-      }
-      a.new_table[(int64_t)b * a.columns + i] = p;
-    }
+    for (int i = lane; i < a.columns; i += 64) a.new_table[(int64_t)b * a.columns + i] = compacted(a, number, b, i, held);
   }
   if (tid == 0) *a.copies = moving;
 }
 
-// One block, with `lds` bytes where that is enough for the counters.
-template <class K>
-static int launch_pages(const char* what, K small, K large, bool fits, int lds, const PagesArgs& a, std::atomic<uint64_t>& ready,
-                        hipStream_t stream) {
-  if (fits) {
-    int dev = 0;
-    TT_HIP(hipGetDevice(&dev));
-    const uint64_t bit = 1ull << (dev & 63);
-    if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
-      TT_HIP(hipFuncSetAttribute((const void*)small, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                 16 * kSmallRows + 8 * kSmallPages));
-      ready.fetch_or(bit, std::memory_order_relaxed);
+// Large: with u of the U used pages below page p, p is hole number p - u, or of the pages that move the one with U - 1 - u
+// behind it; so the sums of used pages are all that blocks need of one another.  (hold: pages that move, the last first,
+// and in its upper half the holes.  first: the numbers that pages get.)
+__global__ __launch_bounds__(kPageThreads) void cache_compact_list_kernel(PagesArgs a) {
+  __shared__ int s_sums[kPageWaves];
+  const Share s = share_of(a);
+  int used, below = sums_before(a, s_sums, used);
+  for (int p0 = s.begin; p0 < s.end; p0 += kEach * kPageThreads) {
+    int uses[kEach], n = 0, total;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int p = p0 + kEach * (int)threadIdx.x + j;
+      uses[j] = p < s.end ? max(a.uses[p], 0) : 0;
+      n += uses[j] > 0 ? 1 : 0;
     }
-    hipLaunchKernelGGL(small, dim3(1), dim3(kPageThreads), lds, stream, a);
-  } else {
-    hipLaunchKernelGGL(large, dim3(1), dim3(kPageThreads), 0, stream, a);
+    int u = below + block_scan(n, s_sums, total);
+    below += total;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int p = p0 + kEach * (int)threadIdx.x + j;
+      if (p >= s.end) continue;
+      if (p == used) *a.copies = used - u;
+      a.first[p] = p;
+      if (p >= used) {
+        if (uses[j] > 0) a.hold[used - 1 - u] = p;
+        a.new_uses[p] = 0;
+      } else if (uses[j] == 0) {
+        a.hold[a.pages / 2 + p - u] = p;
+      } else {
+        a.new_uses[p] = uses[j];
+      }
+      u += uses[j] > 0 ? 1 : 0;
+    }
   }
+  if (blockIdx.x == 0 && threadIdx.x == 0 && used == a.pages) *a.copies = 0;
+}
+
+__global__ __launch_bounds__(256) void cache_compact_moves_kernel(PagesArgs a) {
+  const int moving = *a.copies;
+  for (int r = (int)blockIdx.x * 256 + (int)threadIdx.x; r < moving; r += (int)gridDim.x * 256) {
+    const int p = a.hold[moving - 1 - r], q = a.hold[a.pages / 2 + r];
+    a.first[p] = q;
+    a.new_uses[q] = a.uses[p];
+    a.source[r] = p;
+    a.target[r] = q;
+  }
+}
+
+__global__ __launch_bounds__(256) void cache_compact_table_kernel(PagesArgs a) {
+  each_entry(a, [&](int b0, int i) {
+    for (int b = b0; b < min(b0 + kAhead, a.batch); ++b)
+      a.new_table[(int64_t)b * a.columns + i] = compacted(a, a.first, b, i, held_pages(row_length(a, b), a.page_shift));
+  });
+}
+
+// One block, with `lds` bytes for the counters.
+template <class K>
+static int launch_pages(const char* what, K kernel, int lds, const PagesArgs& a, std::atomic<uint64_t>& ready,
+                        hipStream_t stream) {
+  int dev = 0;
+  TT_HIP(hipGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
+    TT_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                               16 * kSmallRows + 8 * kSmallPages));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  hipLaunchKernelGGL(kernel, dim3(1), dim3(kPageThreads), lds, stream, a);
   return launch_status(what);
+}
+
+// One block's phases against a launch for each, us a call of a fork (in a graph) and of a compaction: 64 rows of 64 columns 16
+// to 30 (18 to 24) and 14 to 23 at 500 pages, 16 to 28 (18 to 30) and 19 to 25 at 16384; 512 of 64 20 to 30 (24 to 24) and 15 to
+// 24 at 500 pages, 27 to 29 (31 to 30) and 26 to 21 at 16384; 1000 of 16 33 to 30 (38 to 26) and 21 to 24, 45 to 29 (49 to 30)
+// and 39 to 24; 256 of 256 27 to 29 (31 to 23) and 14 to 24, 35 to 29 (39 to 31) and 25 to 23.  Past the LDS, with counters
+// in memory and one block all the same: 300000 pages 302 to 27 and 319 to 23, 10^6 903 to 28 and 1115 to 27.
+static bool one_block(const PagesArgs& a) {
+  return a.pages <= kSmallPages && (int64_t)a.batch * ((a.columns + 63) / 64) <= kSmallRows;
+}
+
+static int blocks_for(int64_t n, int each, int most) {
+  const int64_t blocks = (n + each - 1) / each;
+  return (int)(blocks < 1 ? 1 : blocks < most ? blocks : most);
+}
+
+static int entry_blocks(const PagesArgs& a) {
+  return blocks_for((int64_t)((a.batch + kAhead - 1) / kAhead) * ((a.columns + 63) / 64), 4, 1024);
+}
+
+static int scan_blocks(const PagesArgs& a) { return blocks_for(a.pages, kEach * kPageThreads, kScanBlocks); }
+
+static int launch_large_fork(const PagesArgs& a, hipStream_t stream) {
+  const dim3 entries(entry_blocks(a)), scan(scan_blocks(a)), few(256), many(kPageThreads);
+  hipLaunchKernelGGL(cache_fork_begin_kernel, dim3(blocks_for(a.pages > a.batch ? a.pages : a.batch, 256, 1024)), few, 0,
+                     stream, a);
+  TT_CHECK(launch_status("cache_fork_begin_kernel"));
+  hipLaunchKernelGGL(cache_fork_count_kernel, entries, few, 0, stream, a);
+  TT_CHECK(launch_status("cache_fork_count_kernel"));
+  hipLaunchKernelGGL(cache_fork_rows_kernel, dim3(1), many, 0, stream, a);
+  TT_CHECK(launch_status("cache_fork_rows_kernel"));
+  hipLaunchKernelGGL(cache_count_kernel, scan, many, 0, stream, a, (const int*)a.hold, false);
+  TT_CHECK(launch_status("cache_count_kernel"));
+  hipLaunchKernelGGL(cache_fork_list_kernel, scan, many, 0, stream, a);
+  TT_CHECK(launch_status("cache_fork_list_kernel"));
+  hipLaunchKernelGGL(cache_fork_table_kernel, entries, few, 0, stream, a);
+  return launch_status("cache_fork_table_kernel");
+}
+
+static int launch_large_compact(const PagesArgs& a, hipStream_t stream) {
+  const dim3 scan(scan_blocks(a)), few(256), many(kPageThreads);
+  hipLaunchKernelGGL(cache_count_kernel, scan, many, 0, stream, a, a.uses, true);
+  TT_CHECK(launch_status("cache_count_kernel"));
+  hipLaunchKernelGGL(cache_compact_list_kernel, scan, many, 0, stream, a);
+  TT_CHECK(launch_status("cache_compact_list_kernel"));
+  hipLaunchKernelGGL(cache_compact_moves_kernel, dim3(blocks_for(a.pages / 2, 256, 1024)), few, 0, stream, a);
+  TT_CHECK(launch_status("cache_compact_moves_kernel"));
+  hipLaunchKernelGGL(cache_compact_table_kernel, dim3(entry_blocks(a)), few, 0, stream, a);
+  return launch_status("cache_compact_table_kernel");
 }
 
 constexpr int kParts = 32;        // tensors of one launch
@@ -415,7 +597,7 @@ static int64_t pages_list(int64_t batch, int64_t columns, int64_t pages) {
 
 static int64_t pages_workspace(int64_t batch, int64_t columns, int64_t pages) {
   const int64_t copies = batch > pages / 2 ? batch : pages / 2;  // of a fork, and of a compaction
-  return 4 * (4 * batch + 2 * pages + pages_list(batch, columns, pages) + 3 * copies + 1);
+  return 4 * (4 * batch + 2 * pages + pages_list(batch, columns, pages) + 3 * copies + 3 + kScanBlocks);
 }
 
 static int check_state(const char* what, int batch, int columns, int pages, int page_size) {
@@ -443,6 +625,7 @@ static PagesArgs pages_args(const C& c) {
   a.rows = reinterpret_cast<int4*>(take(4 * (int64_t)c.batch));
   a.hold = take(c.pages), a.first = take(c.pages), a.free_pages = take(a.list);
   a.source = take(copies), a.target = take(copies), a.tokens = take(copies), a.copies = take(1);
+  a.needed = take(1), a.open = take(1), a.sums = take(kScanBlocks);
   return a;
 }
 
@@ -469,9 +652,10 @@ extern "C" int tt_cache_fork(const tt_cache_fork_pages* args, void* stream) {
   PagesArgs a = pages_args(c);
   a.parents = c.parents, a.counts = c.counts, a.new_lengths = c.new_lengths;
   static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic LDS is raised
-  TT_CHECK(launch_pages("cache_fork_kernel", cache_fork_kernel<true>, cache_fork_kernel<false>,
-                        c.pages <= kSmallPages && c.batch <= kSmallRows, 16 * c.batch + 8 * c.pages, a, ready,
-                        (hipStream_t)stream));
+  if (one_block(a))
+    TT_CHECK(launch_pages("cache_fork_kernel", cache_fork_kernel, 16 * c.batch + 8 * c.pages, a, ready, (hipStream_t)stream));
+  else
+    TT_CHECK(launch_large_fork(a, (hipStream_t)stream));
   if (c.batch == 0) return TT_OK;
   return launch_copies(c.parts, c.part_count, a.source, a.target, a.tokens, a.copies, c.batch, c.pages, c.page_size,
                        (hipStream_t)stream);
@@ -489,8 +673,10 @@ extern "C" int tt_cache_compact(const tt_cache_compact_pages* args, void* stream
              "cache_compact: null pointer, or table_row %lld", (long long)c.table_row);
   const PagesArgs a = pages_args(c);
   static std::atomic<uint64_t> ready{0};
-  TT_CHECK(launch_pages("cache_compact_kernel", cache_compact_kernel<true>, cache_compact_kernel<false>,
-                        c.pages <= kSmallPages, 8 * c.pages, a, ready, (hipStream_t)stream));
+  if (one_block(a))
+    TT_CHECK(launch_pages("cache_compact_kernel", cache_compact_kernel, 8 * c.pages, a, ready, (hipStream_t)stream));
+  else
+    TT_CHECK(launch_large_compact(a, (hipStream_t)stream));
   if (c.pages < 2) return TT_OK;
   return launch_copies(c.parts, c.part_count, a.source, a.target, nullptr, a.copies, c.pages / 2, c.pages, c.page_size,
                        (hipStream_t)stream);
