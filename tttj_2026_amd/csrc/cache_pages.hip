@@ -447,8 +447,8 @@ static int launch_pages(const char* what, K kernel, int lds, const PagesArgs& a,
 // 24 at 500 pages, 27 to 29 (31 to 30) and 26 to 21 at 16384; 1000 of 16 33 to 30 (38 to 26) and 21 to 24, 45 to 29 (49 to 30)
 // and 39 to 24; 256 of 256 27 to 29 (31 to 23) and 14 to 24, 35 to 29 (39 to 31) and 25 to 23.  Past the LDS, with counters
 // in memory and one block all the same: 300000 pages 302 to 27 and 319 to 23, 10^6 903 to 28 and 1115 to 27.
-static bool one_block(const PagesArgs& a) {
-  return a.pages <= kSmallPages && (int64_t)a.batch * ((a.columns + 63) / 64) <= kSmallRows;
+static bool one_block(int64_t batch, int64_t columns, int64_t pages) {
+  return pages <= kSmallPages && batch * ((columns + 63) / 64) <= kSmallRows;
 }
 
 static int blocks_for(int64_t n, int each, int most) {
@@ -597,7 +597,8 @@ static int64_t pages_list(int64_t batch, int64_t columns, int64_t pages) {
 
 static int64_t pages_workspace(int64_t batch, int64_t columns, int64_t pages) {
   const int64_t copies = batch > pages / 2 ? batch : pages / 2;  // of a fork, and of a compaction
-  return 4 * (4 * batch + 2 * pages + pages_list(batch, columns, pages) + 3 * copies + 3 + kScanBlocks);
+  const int64_t sums = one_block(batch, columns, pages) ? 0 : 2 + kScanBlocks;
+  return 4 * (4 * batch + 2 * pages + pages_list(batch, columns, pages) + 3 * copies + 1 + sums);
 }
 
 static int check_state(const char* what, int batch, int columns, int pages, int page_size) {
@@ -625,7 +626,7 @@ static PagesArgs pages_args(const C& c) {
   a.rows = reinterpret_cast<int4*>(take(4 * (int64_t)c.batch));
   a.hold = take(c.pages), a.first = take(c.pages), a.free_pages = take(a.list);
   a.source = take(copies), a.target = take(copies), a.tokens = take(copies), a.copies = take(1);
-  a.needed = take(1), a.open = take(1), a.sums = take(kScanBlocks);
+  if (!one_block(c.batch, c.columns, c.pages)) a.needed = take(1), a.open = take(1), a.sums = take(kScanBlocks);
   return a;
 }
 
@@ -652,7 +653,7 @@ extern "C" int tt_cache_fork(const tt_cache_fork_pages* args, void* stream) {
   PagesArgs a = pages_args(c);
   a.parents = c.parents, a.counts = c.counts, a.new_lengths = c.new_lengths;
   static std::atomic<uint64_t> ready{0};  // devices whose limit of dynamic LDS is raised
-  if (one_block(a))
+  if (one_block(c.batch, c.columns, c.pages))
     TT_CHECK(launch_pages("cache_fork_kernel", cache_fork_kernel, 16 * c.batch + 8 * c.pages, a, ready, (hipStream_t)stream));
   else
     TT_CHECK(launch_large_fork(a, (hipStream_t)stream));
@@ -673,7 +674,7 @@ extern "C" int tt_cache_compact(const tt_cache_compact_pages* args, void* stream
              "cache_compact: null pointer, or table_row %lld", (long long)c.table_row);
   const PagesArgs a = pages_args(c);
   static std::atomic<uint64_t> ready{0};
-  if (one_block(a))
+  if (one_block(c.batch, c.columns, c.pages))
     TT_CHECK(launch_pages("cache_compact_kernel", cache_compact_kernel, 8 * c.pages, a, ready, (hipStream_t)stream));
   else
     TT_CHECK(launch_large_compact(a, (hipStream_t)stream));
