@@ -32,7 +32,7 @@
 // a tile, each for a head of its own, where heads lie side by side: pieces of 64, 128, 256 and 512 bytes a row are read at
 // 3.0, 5.5, 6.0 and 6.2 TB/s.  64 tokens over 8000 keys, 32 heads of 128 on 8, bf16: 195 us, 5.4 TB/s; over lengths of 67 to 8000
 // 107 us, 4.9; 64 over 4000 keys on 16 heads of 64 105 us, 5.0; 4 over 100000 on 64 heads of 128 on 8 154 us, 5.3.  8 chunks of
-// 512 over up to 4608 keys 196 us, 0.84 PFLOP/s (16 bits: 183; 32 of 300 vector instructions a tile widen, and 10 more find
+// 512 over up to 4608 keys 196 us, 0.84 PFLOP/s (16 bits: 183; 32 of 280 vector instructions a tile widen, and 10 more find
 // the scales).
 //
 // Per wave and tile: S^T = K Q^T with v_mfma_f32_32x32x16 (lane l holds row l % 32; of its 32 keys per block those
