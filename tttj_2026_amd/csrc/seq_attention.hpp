@@ -986,6 +986,7 @@ __global__ __launch_bounds__(64 * RW * KW * NH) __attribute__((amdgpu_waves_per_
         Bytes kx, vx;  // of the next tile; what held the scores has room for them
         if (widen) {
           wait_vmcnt<0>();
+          asm volatile("" ::: "memory");
           read_bytes(kx, k_bytes);
           read_bytes(vx, v_bytes);
         }
