@@ -484,6 +484,28 @@ def rotary_frequencies(dims: int, base: float = 10000.0, *, factor: float = 1.0,
     return (frequencies / factor).to(device)
 
 
+class _Rotary(torch.autograd.Function):
+    """``rotary`` of an x whose gradient is asked for: the result's gradient, turned back.  Rows outside every sequence are 0 in
+    a new tensor, and so is their gradient; in place they stay, and their gradient passes."""
+
+    @staticmethod
+    def forward(ctx, x, frequencies, positions, lengths, starts, interleaved, magnitude, transpose, in_place):
+        ctx.save_for_backward(frequencies, positions, lengths, starts)
+        ctx.how = interleaved, magnitude, transpose, in_place
+        if in_place:
+            ctx.mark_dirty(x)
+        out = x if in_place else x.new_zeros(x.shape) if starts is not None else None
+        return rotary(x, frequencies, positions, lengths=lengths, starts=starts, interleaved=interleaved,
+                      magnitude=magnitude, transpose=transpose, out=out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        interleaved, magnitude, transpose, in_place = ctx.how
+        if in_place:
+            grad = grad.clone(memory_format=torch.contiguous_format)
+        return _Rotary.apply(grad, *ctx.saved_tensors, interleaved, magnitude, not transpose, in_place), *[None] * 8
+
+
 def rotary(x: torch.Tensor, frequencies: torch.Tensor, positions: Optional[torch.Tensor] = None, *,
            lengths: Optional[torch.Tensor] = None, starts: Optional[torch.Tensor] = None, interleaved: bool = False,
            magnitude: float = 1.0, transpose: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -494,10 +516,15 @@ def rotary(x: torch.Tensor, frequencies: torch.Tensor, positions: Optional[torch
     others stay.  Positions are ``positions`` (int32 [T]), or those that ``cache_append`` gives new tokens for
     ``lengths`` and ``starts`` (there rows outside every sequence are left as they are in ``out``, arbitrary in a new
     tensor).  With ``transpose`` they are turned back: the gradient of a loss for x is ``rotary`` of its gradient for the
-    result with ``transpose=True``.
+    result with ``transpose=True``.  Where x requires a gradient, autograd is told so.
 
     Queries and keys that lie side by side in a projection's output are turned in one call, as heads of one tensor.
-    ``out`` is x itself (in place) or a tensor that overlaps nothing; features are adjacent in both, head_dim at most 256."""
+    ``out`` is x itself (in place) or a tensor that overlaps nothing, without gradients; features are adjacent in both,
+    head_dim at most 256."""
+    if torch.is_grad_enabled() and (x.requires_grad or out is not None and out.requires_grad):
+        if out is not None and out is not x:
+            raise ValueError("rotary into another tensor has no gradient: call it without out, or under torch.no_grad()")
+        return _Rotary.apply(x, frequencies, positions, lengths, starts, interleaved, magnitude, transpose, out is x)
     dtype, index = _typed(x, "x")
     shape = x.shape
     if len(shape) != 3 or shape[1] == 0:
