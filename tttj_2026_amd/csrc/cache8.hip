@@ -209,6 +209,15 @@ extern "C" int tt_cache_append8(const tt_cache_rows8* args, void* stream) {
   TT_CHECK(check_rows8("cache_append: k_cache", c.k_cache, c.kc_page, c.kc_row, c.kc_head));
   TT_CHECK(check_rows8("cache_append: v_cache", c.v_cache, c.vc_page, c.vc_row, c.vc_head));
   TT_CHECK(check_scales("cache_append", c));
+  TT_CHECK(check_apart("cache_append: k_cache", "pages", c.kc_page, c.pages));
+  TT_CHECK(check_apart("cache_append: v_cache", "pages", c.vc_page, c.pages));
+  TT_CHECK(check_apart("cache_append: k_cache", "rows", c.kc_row, c.page_size));
+  TT_CHECK(check_apart("cache_append: v_cache", "rows", c.vc_row, c.page_size));
+  TT_CHECK(check_apart("cache_append: k_cache", "heads", c.kc_head, c.kv_heads));
+  TT_CHECK(check_apart("cache_append: v_cache", "heads", c.vc_head, c.kv_heads));
+  TT_CHECK(check_apart("cache_append: scales", "pages", c.s_page, c.pages));
+  TT_CHECK(check_apart("cache_append: scales", "blocks", c.s_block, c.page_size / c.block));
+  TT_CHECK(check_apart("cache_append: scales", "heads", c.s_head, c.kv_heads));
   TT_REQUIRE(c.table_row >= 0, "cache_append: table_row %lld", (long long)c.table_row);
   Append8Args a{};
   a.k = static_cast<const uint16_t*>(c.k), a.v = static_cast<const uint16_t*>(c.v);

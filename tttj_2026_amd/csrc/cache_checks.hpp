@@ -65,6 +65,12 @@ int check_scales(const char* what, const C& c) {
   return TT_OK;
 }
 
+// What a call writes: `n` of them lie apart.
+inline int check_apart(const char* what, const char* of, int64_t stride, int64_t n) {
+  TT_REQUIRE(stride > 0 || n <= 1, "%s: %lld %s at one address", what, (long long)n, of);
+  return TT_OK;
+}
+
 }  // namespace tt
 
 #define TT_CHECK(call)            \
