@@ -329,7 +329,8 @@ int tt_cache_attention_fwd(const tt_cache_attention* args, void* stream);
  * in one call the bytes of either may stay.  A scale of 255 is no number: it stays, and the keys of its block count
  * as NaN in the attention, like those of a page outside the cache.
  *
- * Attention: K and V are widened to `dtype` (q's and out's): exact, but for products beyond its range.
+ * Attention: K and V are widened to `dtype` (q's and out's): exact, but for products beyond its range (infinities) and
+ * those that are subnormal in it (rounded to the nearest).
  * The workspace is that of tt_cache_attention8_workspace_bytes. */
 typedef struct {
   int64_t size;
@@ -399,7 +400,8 @@ typedef struct {
 int tt_cache_pages_workspace_bytes(int batch, int columns, int pages, int64_t* bytes);
 
 /* Row b becomes what row parents[b] was (NULL: itself; outside [0, batch): empty, which frees its pages), with
- * counts[b] (NULL: 0) more tokens, or fewer, from 0 to what the table holds.  Whole pages are shared.  A page that is
+ * counts[b] (NULL: 0) more tokens, or fewer, from 0 to what the table holds (a row that would pass that is cut there, and has
+ * no room for all of the new tokens: appending them would write over older ones).  Whole pages are shared.  A page that is
  * taken over in part, and so is about to be written, is kept by the first row that takes it so, unless a row
  * holds it whole or the program holds it; the others get copies of the rows of it that hold their tokens.  New pages are the
  * free ones of lowest number, row by row; where they run out, the table has -1. */

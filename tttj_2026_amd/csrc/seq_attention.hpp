@@ -32,8 +32,8 @@
 // a tile, each for a head of its own, where heads lie side by side: pieces of 64, 128, 256 and 512 bytes a row are read at
 // 3.0, 5.5, 6.0 and 6.2 TB/s.  64 tokens over 8000 keys, 32 heads of 128 on 8, bf16: 195 us, 5.4 TB/s; over lengths of 67 to 8000
 // 107 us, 4.9; 64 over 4000 keys on 16 heads of 64 105 us, 5.0; 4 over 100000 on 64 heads of 128 on 8 154 us, 5.3.  8 chunks of
-// 512 over up to 4608 keys 196 us, 0.84 PFLOP/s (16 bits: 183; 32 of 280 vector instructions a tile widen, and 10 more find
-// the scales).
+// 512 over up to 4608 keys 196 to 203 us, 0.84 to 0.81 PFLOP/s (16 bits: 183; 32 of 280 vector instructions a tile widen, and
+// 10 more find the scales).
 //
 // Per wave and tile: S^T = K Q^T with v_mfma_f32_32x32x16 (lane l holds row l % 32; of its 32 keys per block those
 // with bit 2 equal to l / 32), softmax with a running maximum and sum in fp32, O^T += V^T P^T.  K and V stay in the
@@ -210,7 +210,7 @@ __device__ __forceinline__ int vseg8(int row, int c) {
 
 // Tiles of T that are widened on their way into LDS: a lane writes two chunks, 2 c and 2 c + 1, and 8 lanes at a time 128
 // bytes without conflict if the even chunks of a row come first and the odd ones behind them (and with rows of 128 bytes,
-// halves of odd rows change places).  Reads as of the other tiles.  (8 chunks of 512: 197.6 -> 195.6 us.)
+// halves of odd rows change places).  Reads as of the other tiles.  (8 chunks of 512: 2 us of 198.)
 template <int HD>
 __device__ __forceinline__ int kswz_widened(int row, int c) {
   const int p = c >> 1 | (c & 1) << (HD == 128 ? 3 : 2);

@@ -337,15 +337,15 @@ def cache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     alignment and tokens less than 2^26 elements apart, e.g. both halves of one tensor, or a permuted
     [pages, kv_heads, page_size, head_dim]); page_size is a power of two from 16 on.  Position t of sequence b
     lies in page page_table[b, t // page_size] (int32 [B, n]) at t % page_size.  ``lengths`` (int32 [B]) counts the keys
-    of each sequence with the new ones: the n tokens of sequence b, rows starts[b] ... starts[b + 1] - 1 (or row b alone without ``starts``), take
-    positions lengths[b] - n ... lengths[b] - 1.  Tokens whose position is negative or beyond the table, or whose
-    page is no page of the cache, are not written.
+    of each sequence with the new ones: the n tokens of sequence b, rows starts[b] ... starts[b + 1] - 1 (or row b alone
+    without ``starts``), take positions lengths[b] - n ... lengths[b] - 1.  Tokens whose position is negative or beyond the
+    table, or whose page is no page of the cache, are not written.
 
     With ``k_scales`` and ``v_scales`` (float8_e8m0fnu [pages, page_size / block, kv_heads], block a power of two from
     16 on, both with the same strides) the cache is in 8 bits: k_cache and v_cache are float8_e4m3fn, and a value is the
-    product of both.  A block's scale is the smallest power of two that holds its tokens' largest finite magnitude.  Where
-    a new token is too large for the block that older ones of its sequence lie in, the scale grows and those are rounded
-    to it.  Infinities and NaN become NaN, head_dim is a multiple of 16, and two sequences may not write to one
+    product of both.  A block's scale is the smallest power of two that holds its tokens' largest finite magnitude, those
+    among them that were dropped since the block was begun.  Where a new token is too large for the block that older ones of
+    its sequence lie in, the scale grows and those are rounded to it.  Infinities and NaN become NaN, head_dim is a multiple of 16, and two sequences may not write to one
     block in one call."""
     if k_scales is not None or v_scales is not None:
         return _append8(k, v, k_cache, v_cache, page_table, lengths, starts, k_scales, v_scales)
@@ -407,7 +407,8 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     the work is split.  Keys in a page whose number is no page of the cache are not read and count as NaN.  ``out`` may
     not overlap the other tensors.
 
-    ``k_scales`` and ``v_scales`` as in ``cache_append``: the cache is in 8 bits, read as values of q's type."""
+    ``k_scales`` and ``v_scales`` as in ``cache_append``: the cache is in 8 bits, read as values of q's type (rounded where
+    subnormal in it, infinities past its largest)."""
     dtype, index = _typed(q, "q")
     q, (tokens, heads, hd), q_at, q_row, q_head = _rows(q, "q", dtype, index)
     shape = (*k_cache.shape[:3], hd)
@@ -649,6 +650,8 @@ def cache_fork(caches: Sequence[torch.Tensor], page_table: torch.Tensor, lengths
     Row b of the new ``page_table`` (int32 [B, n]) and ``lengths`` (int32 [B]) is what row parents[b] was (without
     ``parents``, int32 [B]: row b itself; a number outside 0 ... B - 1: an empty sequence, whose pages are given up), with
     counts[b] tokens more or fewer (``counts``, int32 [B]; none without it), so that ``cache_append`` finds room for them.
+    Lengths are cut to what a row of the table holds: for a row that would pass it, appending all of its new tokens would
+    write over older ones, so a program keeps to the table or makes it wider first.
     ``uses`` (int32 [pages]) counts the rows that hold each page, and holds that the program has on one besides (a prompt
     that is kept); pages with 0 are free.  Rows hold the pages of their lengths; what the table has behind those counts
     for nothing and is -1 in the new one.
@@ -682,7 +685,7 @@ def cache_compact(caches: Sequence[torch.Tensor], page_table: torch.Tensor, leng
 
     Of U used pages those numbered U and above go to the free numbers below U, both in rising order, in all ``caches``;
     what lies at and above U is free afterwards.  Other tables and lists of page numbers are the caller's to renumber:
-    page p is used if ``uses`` is not 0, and a page that moves keeps its count."""
+    page p is used if ``uses`` is above 0, and a page that moves keeps its count."""
     parts, count, pages, page_size, index = _parts(caches)
     page_table, lengths, uses, batch, columns, row = _state(page_table, lengths, uses, pages, index)
     work = uses.new_empty(_lib.cache_pages_workspace_bytes(batch, columns, pages), dtype=torch.uint8)
